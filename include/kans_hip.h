@@ -399,6 +399,27 @@ int kans_decode_set_weight_loads(int mode);
  * and test switch). */
 int kans_prefill_set_block_pairs(int on);
 
+/* ======================================================================= *
+ * The training step around the layers (no reference counterpart in this form): device pointers,
+ * work enqueued on `stream`.
+ * ======================================================================= */
+/* One AdamW step over n_tensors tensors of element type `dtype`:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),  all in fp32.
+ * params, grads, numel, blocks and steps are host arrays; tensor i has numel[i] consecutive elements, its
+ * states start at element 256 * blocks[i] of the state buffers (distinct tensors in distinct blocks) and
+ * t = steps[i] >= 1.  state_bits 32: exp_avg and exp_avg_sq are fp32.  state_bits 8: int8 and uint8 codes with
+ * one fp32 scale per block of 256 each, values s (q/127) |q/127| and s (q/255)^4; codes behind a
+ * tensor's last element must be 0.  16-bit tensors need `master` (fp32, same layout), whose rounding they become.
+ * State buffers are 16-byte aligned; tensors may have any alignment.  KANS_ERR_STATE on a capturing stream. */
+int kans_adamw_step(int dtype, int state_bits, int n_tensors, void* const* params, const void* const* grads,
+                    const long* numel, const long* blocks, const long* steps, void* exp_avg, void* exp_avg_sq,
+                    float* exp_avg_scale, float* exp_avg_sq_scale, float* master, double lr, double beta1, double beta2,
+                    double eps, double weight_decay, void* stream);
+/* fp32 values of `blocks` blocks of 8-bit states */
+int kans_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale,
+                      const float* exp_avg_sq_scale, float* avg_out, float* sq_out, long blocks, void* stream);
+
 /* Measured ceilings for the roofline report (no reference counterpart; measurement only).
  * kans_mfma_ceiling: TFLOP/s of back-to-back v_mfma_f32_32x32x16 (dtype DT_F16 / DT_BF16) on 16 A and
  * 16 B operand fragments given as host arrays [16][64 lanes][8 x 16-bit], at the fused block kernel's

@@ -17,21 +17,24 @@ from .quantization import (QuantizedWeight, TernaryQuantizedWeight, quantize, to
 __version__ = "0.6.0+mi355x"
 
 
+# What works on torch tensors and the module it is in: imported on first use so that `import metal_kans` does
+# not import torch; None without torch, as in the reference (metal_kans/__init__.py:34-38).
+_TORCH = {"TorchMetalKANLinear": "torch_module", "TorchMetalKAN": "torch_module", "TorchAdamW": "adamw"}
+
+
 def __getattr__(name):
-    # TorchMetalKANLinear / TorchMetalKAN (torch_module.py), imported on first use so that
-    # `import metal_kans` does not import torch; None without torch, as in the reference
-    # (metal_kans/__init__.py:34-38).
-    if name in ("TorchMetalKANLinear", "TorchMetalKAN"):
+    if name in _TORCH:
+        from importlib import import_module
         try:
-            from . import torch_module
+            import torch  # noqa: F401
         except ImportError:
             return None
-        return getattr(torch_module, name)
+        return getattr(import_module("." + _TORCH[name], __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 __all__ = [
     "set_async", "sync", "get_metal_bridge", "is_metal_available", "is_gpu_available",
     "ChebyKAN", "FastKAN", "BSplineKAN", "KAN", "MetalKAN", "GatedKAN",
     "QuantizedWeight", "TernaryQuantizedWeight", "quantize", "to_int8", "to_int4", "to_ternary",
-    "TorchMetalKANLinear", "TorchMetalKAN",
+    "TorchMetalKANLinear", "TorchMetalKAN", "TorchAdamW",
 ]

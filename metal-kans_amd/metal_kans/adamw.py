@@ -1,0 +1,274 @@
+"""AdamW over all tensors of a model at once, on the gfx950 kernel of ``kans_adamw_step``.
+
+``TorchAdamW`` is a ``torch.optim.Optimizer`` for parameters on the GPU: fp32, fp16 or bf16 (16-bit ones
+with an fp32 master in the state), the two moments in 32 bits or, with ``state_bits=8``, in 8.  One launch
+updates up to 96 tensors; the step is enqueued on torch's current stream.
+
+The states of a group's parameters of one dtype lie in one buffer per kind, each parameter's at a
+multiple of 256 elements in the order of the group; ``state[p]`` holds views of them, ``flat_state()`` the
+buffers.  Per parameter:
+
+* ``step`` (int) and ``exp_avg``, ``exp_avg_sq`` in the parameter's shape: fp32, or with ``state_bits=8``
+  int8 / uint8 codes with ``exp_avg_scale``, ``exp_avg_sq_scale`` (one fp32 each per 256 elements);
+  the values that codes stand for are ``scale * (q / 127) * |q / 127|`` and ``scale * (q / 255) ** 4``;
+* ``master`` (16-bit parameters): the fp32 value that the parameter is the rounding of.
+
+Gradients that are None leave their parameter alone.  A master follows its parameter only when it is
+made: after other changes to a 16-bit parameter (a loaded model), ``state.clear()`` starts anew.  A step on a
+capturing stream is refused (its bias corrections belong to that one step).
+"""
+from __future__ import annotations
+
+from array import array
+from typing import Dict, List
+
+import torch
+
+from . import device
+from ._engine import DT_BF16, DT_F16, DT_F32
+from .torch_module import _stream_of
+
+_DT = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
+BLOCK = 256  # elements that share a scale of the 8-bit states
+
+
+class _Arena:
+    """The states of one group's parameters of one dtype."""
+
+    def __init__(self, params: List[torch.Tensor], bits: int):
+        p0 = params[0]
+        self.params = params
+        self.bits = bits
+        self.dtype, self.device = p0.dtype, p0.device
+        self.numel = [p.numel() for p in params]
+        self.blocks = []
+        total = 0
+        for n in self.numel:
+            self.blocks.append(total)
+            total += (n + BLOCK - 1) // BLOCK
+        self.total = total
+        zeros = lambda n, dt: torch.zeros(n, dtype=dt, device=self.device)  # noqa: E731
+        f32 = torch.float32
+        self.flat: Dict[str, torch.Tensor] = {
+            "exp_avg": zeros(total * BLOCK, torch.int8 if bits == 8 else f32),
+            "exp_avg_sq": zeros(total * BLOCK, torch.uint8 if bits == 8 else f32)}
+        if bits == 8:
+            self.flat["exp_avg_scale"] = zeros(total, f32)
+            self.flat["exp_avg_sq_scale"] = zeros(total, f32)
+        if self.dtype != f32:
+            self.flat["master"] = zeros(total * BLOCK, f32)
+        self._numel = array("q", self.numel)
+        self._blocks = array("q", self.blocks)
+
+    def views(self, i: int) -> Dict[str, torch.Tensor]:
+        b, n, shape = self.blocks[i], self.numel[i], self.params[i].shape
+        out = {}
+        for name, t in self.flat.items():
+            if name.endswith("_scale"):
+                out[name] = t[b:b + (n + BLOCK - 1) // BLOCK]
+            else:
+                # in the parameter's own order of memory
+                out[name] = t[b * BLOCK:b * BLOCK + n].as_strided(shape, self.params[i].stride(), b * BLOCK)
+        return out
+
+    def start(self, i: int, state: dict) -> dict:
+        """The state of parameter i: zeros and its value, or what ``state`` holds."""
+        p = self.params[i]
+        views = self.views(i)
+        for name, v in views.items():
+            given = state.get(name)
+            if given is not None:
+                if given.shape != v.shape or (given.is_floating_point() != v.is_floating_point()):
+                    raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} is {given.dtype} "
+                                     f"{tuple(given.shape)}, expected {v.dtype} {tuple(v.shape)}")
+                v.copy_(given)
+            elif name == "master":
+                v.copy_(p.detach())
+            elif state:
+                raise ValueError(f"state {name!r} is missing (states in {self.bits} bits)")
+            else:
+                v.zero_()
+        return {"step": int(state.get("step", 0)), **views}
+
+
+def _dense(p: torch.Tensor) -> bool:
+    """Whether the elements fill p.numel() consecutive places (in any order of the dimensions)."""
+    if p.is_contiguous():
+        return True
+    at = 1
+    for size, stride in sorted(zip(p.shape, p.stride()), key=lambda v: v[1]):
+        if size != 1:
+            if stride != at:
+                return False
+            at *= size
+    return True
+
+
+class TorchAdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) on device tensors.
+
+    Args:
+        params: parameters or parameter groups (``lr``, ``betas``, ``eps``, ``weight_decay`` per group)
+        lr, betas, eps, weight_decay: as in the formula p = p (1 - lr wd) - lr m^ / (sqrt(v^) + eps)
+        state_bits: 32 or 8, the moments' width (for all groups)
+    """
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 state_bits: int = 32):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        self.state_bits = state_bits
+        self._arenas: Dict[int, List[_Arena]] = {}
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group) -> None:
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            b1, b2 = g["betas"]
+            if not (g["lr"] >= 0 and g["eps"] >= 0 and g["weight_decay"] >= 0):
+                raise ValueError("lr, eps and weight_decay must be >= 0")
+            if not (0 <= b1 < 1 and 0 <= b2 < 1):
+                raise ValueError(f"betas must be in [0, 1), got {g['betas']}")
+            for p in g["params"]:
+                if p.dtype not in _DT:
+                    raise TypeError(f"unsupported parameter dtype {p.dtype}")
+                if not _dense(p):
+                    raise ValueError("parameters must be dense (no gaps or overlaps in memory)")
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    # ---- states ----------------------------------------------------------------
+    def _group_arenas(self, gi: int) -> List[_Arena]:
+        arenas = self._arenas.get(gi)
+        if arenas is None:
+            kinds: Dict[tuple, List[torch.Tensor]] = {}
+            for p in self.param_groups[gi]["params"]:
+                if not p.is_cuda:
+                    raise ValueError("TorchAdamW takes parameters on the GPU")
+                kinds.setdefault((p.dtype, p.device), []).append(p)
+            arenas = []
+            for params in kinds.values():
+                a = _Arena(params, self.state_bits)
+                for i, p in enumerate(params):
+                    if self.state.get(p):
+                        self.state[p] = a.start(i, self.state[p])
+                arenas.append(a)
+            self._arenas[gi] = arenas
+        return arenas
+
+    def flat_state(self) -> List[Dict[str, torch.Tensor]]:
+        """The states as flat buffers, one dict for each parameter group and dtype: ``exp_avg`` and
+        ``exp_avg_sq`` in fp32 (the buffers themselves, or in 8 bits the values of the codes), ``master`` for
+        16-bit parameters, and ``params``.  A parameter's elements start at the sum of the sizes before it, each rounded
+        up to 256; what lies between is zero."""
+        out = []
+        for gi in range(len(self.param_groups)):
+            for a in self._group_arenas(gi):
+                flat = dict(a.flat)
+                if self.state_bits == 8:
+                    avg, sq = (torch.empty(a.total * BLOCK, device=a.device) for _ in range(2))
+                    stream = _stream_of(torch.cuda.current_stream(a.device))
+                    device.check(device.get_metal_bridge().kans_adamw_values(
+                        flat["exp_avg"].data_ptr(), flat["exp_avg_sq"].data_ptr(), flat.pop("exp_avg_scale").data_ptr(),
+                        flat.pop("exp_avg_sq_scale").data_ptr(), avg.data_ptr(), sq.data_ptr(), a.total, stream),
+                        "kans_adamw_values")
+                    flat["exp_avg"], flat["exp_avg_sq"] = avg, sq
+                flat["params"] = a.params
+                out.append(flat)
+        return out
+
+    def state_dict(self):
+        sd = super().state_dict()
+        sd["state_bits"] = self.state_bits
+        return sd
+
+    def load_state_dict(self, state_dict) -> None:
+        """As torch's, with the states kept in their own types; refuses states of the other width."""
+        bits = state_dict.get("state_bits", self.state_bits)
+        if bits != self.state_bits:
+            raise ValueError(f"the states are in {bits} bits, the optimizer's in {self.state_bits}")
+        groups = state_dict["param_groups"]
+        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
+            raise ValueError("the parameter groups differ in number or size")
+        state, arenas = dict(self.state), self._arenas
+        loaded = {}
+        for g, sg in zip(self.param_groups, groups):
+            for p, key in zip(g["params"], sg["params"]):
+                if state_dict["state"].get(key):
+                    loaded[p] = dict(state_dict["state"][key])
+        self.state.clear()
+        self.state.update(loaded)
+        self._arenas = {}
+        try:
+            for gi in range(len(self.param_groups)):
+                self._group_arenas(gi)
+        except Exception:
+            self.state.clear()
+            self.state.update(state)
+            self._arenas = arenas
+            raise
+        for g, sg in zip(self.param_groups, groups):
+            g.update({k: v for k, v in sg.items() if k != "params"})
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits}
+
+    def __setstate__(self, state) -> None:
+        super().__setstate__(state)
+        self._arenas = {}  # made anew around the states at the next step
+
+    # ---- step --------------------------------------------------------------------
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        lib = device.get_metal_bridge()
+        for gi, group in enumerate(self.param_groups):
+            for a in self._group_arenas(gi):
+                self._step_arena(lib, group, a)
+        return loss
+
+    def _step_arena(self, lib, group, a: _Arena) -> None:
+        ids, params, grads, steps, keep = [], [], [], [], []
+        for i, p in enumerate(a.params):
+            g = p.grad
+            if g is None:
+                continue
+            if g.is_sparse or g.dtype != a.dtype or g.device != a.device:
+                raise TypeError(f"gradients must be dense {a.dtype} tensors on {a.device}")
+            if p.dtype != a.dtype or p.device != a.device or p.numel() != a.numel[i]:
+                raise ValueError("a parameter's dtype, device or size changed under its optimizer")
+            if g.stride() != p.stride():  # (elements are paired by their place in memory)
+                g = torch.empty_like(p).copy_(g)
+            keep.append(g)
+            ids.append(i)
+            params.append(p.data_ptr())
+            grads.append(g.data_ptr())
+            st = self.state.get(p)
+            if not st:
+                st = self.state[p] = a.start(i, {})
+            steps.append(st["step"] + 1)
+        if not ids:
+            return
+        whole = len(ids) == len(a.params)
+        arrays = [array("Q", params), array("Q", grads),
+                  a._numel if whole else array("q", [a.numel[i] for i in ids]),
+                  a._blocks if whole else array("q", [a.blocks[i] for i in ids]), array("q", steps)]
+        at = [v.buffer_info()[0] for v in arrays]
+        f = a.flat
+        ptr = lambda name: f[name].data_ptr() if name in f else None  # noqa: E731
+        b1, b2 = group["betas"]
+        device.check(lib.kans_adamw_step(
+            _DT[a.dtype], a.bits, len(ids), *at, ptr("exp_avg"), ptr("exp_avg_sq"), ptr("exp_avg_scale"),
+            ptr("exp_avg_sq_scale"), ptr("master"), float(group["lr"]), float(b1), float(b2), float(group["eps"]),
+            float(group["weight_decay"]), _stream_of(torch.cuda.current_stream(a.device))), "kans_adamw_step")
+        changed = []
+        for i, t in zip(ids, steps):
+            p = a.params[i]
+            self.state[p]["step"] = t
+            changed.append(p)
+        torch.autograd.graph.increment_version(changed)

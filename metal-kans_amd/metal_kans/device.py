@@ -133,6 +133,10 @@ SIGNATURES = {
     "kans_decode_set_pre_basis": (c_int, [c_int]),
     "kans_decode_set_weight_loads": (c_int, [c_int]),
     "kans_prefill_set_block_pairs": (c_int, [c_int]),
+    # training step around the layers
+    "kans_adamw_step": (c_int, [c_int, c_int, c_int, P, P, P, P, P, P, P, P, P, P, c_double, c_double, c_double, c_double,
+                                c_double, P]),
+    "kans_adamw_values": (c_int, [P, P, P, P, P, P, c_long, P]),
     "kans_mfma_ceiling": (c_int, [c_int, P, P, c_int, P]),
     "kans_stream_ceiling": (c_int, [P, c_size_t, P]),
 }

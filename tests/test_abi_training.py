@@ -1,0 +1,36 @@
+"""Refusals of the training-step entry points that need no GPU: negative codes before any HIP call."""
+import ctypes
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from metal_kans import device
+    return device.load_library()
+
+
+def adamw(lib, **kw):
+    a = dict(dtype=0, bits=32, n=1, params=None, grads=None, numel=4, block=0, step=1, m=64, v=64, ms=None, vs=None,
+             master=None, lr=1e-3, b1=0.9, b2=0.999, eps=1e-8, wd=0.0)
+    a.update(kw)
+    V, L = ctypes.c_void_p, ctypes.c_long
+    one = lambda t, v: ctypes.cast((t * 1)(v), V)  # noqa: E731
+    return lib.kans_adamw_step(a["dtype"], a["bits"], a["n"], one(V, a["params"] or 0), one(V, a["grads"] or 0),
+                               one(L, a["numel"]), one(L, a["block"]), one(L, a["step"]), a["m"], a["v"], a["ms"], a["vs"],
+                               a["master"], a["lr"], a["b1"], a["b2"], a["eps"], a["wd"], None)
+
+
+def test_adamw_refusals(lib):
+    ok = dict(params=64, grads=64)
+    for bad in (dict(), dict(ok, dtype=3), dict(ok, bits=16), dict(ok, n=-1), dict(ok, numel=-1), dict(ok, block=-1),
+                dict(ok, step=0), dict(ok, m=None), dict(ok, m=65), dict(ok, bits=8), dict(ok, dtype=1),
+                dict(ok, lr=-1.0), dict(ok, lr=float("nan")), dict(ok, b1=1.0), dict(ok, b2=-0.1),
+                dict(ok, eps=float("inf")), dict(ok, wd=-1.0)):
+        assert adamw(lib, **bad) == -1, bad
+        assert lib.kans_last_error()
+    assert adamw(lib, **ok, numel=1 << 40) == -5
+    assert adamw(lib, n=0) == 0
+    assert lib.kans_adamw_values(None, None, None, None, None, None, 1, None) == -1
+    assert lib.kans_adamw_values(64, 64, 64, 64, 72, 64, 1, None) == -1
+    assert lib.kans_adamw_values(None, None, None, None, None, None, 0, None) == 0

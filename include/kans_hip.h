@@ -420,6 +420,28 @@ int kans_adamw_step(int dtype, int state_bits, int n_tensors, void* const* param
 int kans_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale,
                       const float* exp_avg_sq_scale, float* avg_out, float* sq_out, long blocks, void* stream);
 
+/* Norms before and after a block, fused with its gate and residual scale, over `rows` rows of D elements:
+ *   y = x + scale * gate * N(block) * post_w,  h = N(y) * pre_w,
+ *   N(a) = a / sqrt(mean(a^2) + eps) (kind 0) or (a - mean(a)) / sqrt(var(a) + eps) (kind 1).
+ * x and y are of res_dtype (`dtype` or KANS_DT_F32), everything else of `dtype`; all rows contiguous, any
+ * alignment.  gate has one row for each gate_group rows of x (1: its own for each, rows: one for all).  Null
+ * gate, post_w, pre_w: ones; null block: y = x (not written), h = N(x) * pre_w.  The scale is *scale_dev
+ * (fp32 on the device) or, where that is null, `scale`.  stats (null: not wanted): fp32 [rows][2 + 2 * kind]
+ * for the backward. */
+int kans_residual_norm_forward(int res_dtype, int dtype, int kind, const void* x, const void* block, const void* gate,
+                               long gate_group, const void* post_w, const void* pre_w, const float* scale_dev, double scale,
+                               double eps, void* y, void* h, float* stats, long rows, int D, void* stream);
+/* bytes of device memory that the backward works in (gate_group 0: no gate) */
+long kans_residual_norm_workspace(long rows, int D, long gate_group);
+/* Gradients from dy (res_dtype) and dh (dtype), either of which may be null (zero): dx in res_dtype, dscale one
+ * fp32, the others in `dtype` (dgate summed over the rows that share a gate row, or with dgate_f32 = 1, for
+ * gate_group 1, in fp32 for a caller that sums it further); null ones are not computed. */
+int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* x, const void* block, const void* gate,
+                                long gate_group, const void* post_w, const void* pre_w, const float* scale_dev, double scale,
+                                double eps, const float* stats, const void* dy, const void* dh, void* dx, void* dblock,
+                                void* dgate, int dgate_f32, void* dpost_w, void* dpre_w, float* dscale, long rows, int D,
+                                void* workspace, long workspace_bytes, void* stream);
+
 /* Measured ceilings for the roofline report (no reference counterpart; measurement only).
  * kans_mfma_ceiling: TFLOP/s of back-to-back v_mfma_f32_32x32x16 (dtype DT_F16 / DT_BF16) on 16 A and
  * 16 B operand fragments given as host arrays [16][64 lanes][8 x 16-bit], at the fused block kernel's

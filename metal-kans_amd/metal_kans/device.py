@@ -137,6 +137,11 @@ SIGNATURES = {
     "kans_adamw_step": (c_int, [c_int, c_int, c_int, P, P, P, P, P, P, P, P, P, P, c_double, c_double, c_double, c_double,
                                 c_double, P]),
     "kans_adamw_values": (c_int, [P, P, P, P, P, P, c_long, P]),
+    "kans_residual_norm_forward": (c_int, [c_int, c_int, c_int, P, P, P, c_long, P, P, P, c_double, c_double, P, P, P, c_long,
+                                           c_int, P]),
+    "kans_residual_norm_workspace": (c_long, [c_long, c_int, c_long]),
+    "kans_residual_norm_backward": (c_int, [c_int, c_int, c_int, P, P, P, c_long, P, P, P, c_double, c_double, P, P, P, P, P,
+                                            P, c_int, P, P, P, c_long, c_int, P, c_long, P]),
     "kans_mfma_ceiling": (c_int, [c_int, P, P, c_int, P]),
     "kans_stream_ceiling": (c_int, [P, c_size_t, P]),
 }

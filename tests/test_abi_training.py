@@ -34,3 +34,24 @@ def test_adamw_refusals(lib):
     assert lib.kans_adamw_values(None, None, None, None, None, None, 1, None) == -1
     assert lib.kans_adamw_values(64, 64, 64, 64, 72, 64, 1, None) == -1
     assert lib.kans_adamw_values(None, None, None, None, None, None, 0, None) == 0
+
+
+def test_residual_norm_refusals(lib):
+    def fwd(res=0, dt=0, kind=0, x=64, block=64, gate=None, group=4, post=None, eps=1e-6, y=64, h=64, rows=4, d=8):
+        return lib.kans_residual_norm_forward(res, dt, kind, x, block, gate, group, post, None, None, 1.0, eps, y, h, None,
+                                              rows, d, None)
+
+    def bwd(stats=64, gate=None, dgate=None, f32=0, ws=64, size=1 << 20, block=64, dblock=None):
+        return lib.kans_residual_norm_backward(0, 0, 0, 64, block, gate, 4, None, None, None, 1.0, 1e-6, stats, 64, 64, 64, dblock,
+                                               dgate, f32, None, None, None, 4, 8, ws, size, None)
+    for bad in (dict(res=1), dict(dt=3), dict(res=3), dict(res=2, dt=1), dict(kind=2), dict(x=None), dict(block=None, gate=64),
+                dict(block=None, post=64), dict(eps=-1.0), dict(eps=float("nan")), dict(y=None), dict(h=None), dict(rows=-1),
+                dict(d=0), dict(gate=64, group=3), dict(gate=64, group=0), dict(gate=64, group=8)):
+        assert fwd(**bad) == -1, bad
+    assert fwd(rows=1 << 22) == -5
+    assert fwd(rows=0, x=None) == 0
+    for bad in (dict(stats=None), dict(dgate=64), dict(ws=None), dict(size=8), dict(block=None, dblock=64),
+                dict(gate=64, dgate=64, f32=1)):
+        assert bwd(**bad) == -1, bad
+    assert lib.kans_residual_norm_workspace(0, 8, 0) == 0
+    assert lib.kans_residual_norm_workspace(4, 8, 0) >= 4 * (3 * 8 + 1)

@@ -14,8 +14,8 @@
 // writes y and h once; the backward reads x, block, dy, dh and writes dx and dblock.
 // It takes y from x and block again (fp32, never rounded) instead of reading the
 // stored one: the same bytes, and no rounding of y enters the gradients.  Rows
-// live in registers: a row belongs to TPR threads of IT vectors each, the statistics of
-// the forward are kept (fp32, 2 or 4 a row) so that the backward needs two row sums.
+// live in registers, 8 elements a thread; the forward's statistics are kept
+// (fp32, 2 or 4 a row) so that the backward needs two row sums.
 //
 // Sums over rows (weights, a shared gate, the scale): a workgroup takes a run
 // of rows that share their gate row, adds up in fp32 registers and writes one partial row; a
@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "kans_api_internal.h"
 
@@ -48,44 +49,89 @@ struct NormArgs {
   int want_scale, gate_f32;  // gate_f32: dgate of a gate row for each row in fp32
 };
 
-// Elements of a vector: 16 bytes of the block's type.
-template <typename TB> constexpr int vec_of() { return 16 / (int)sizeof(TB); }
+constexpr int V = 8;  // elements of a thread: one 16-byte access in 16 bits, two in fp32
 
-template <typename T, int V> struct Vec { T e[V]; };
+// V elements as they lie in memory (16-bit ones stay packed in their registers).
+template <typename T> struct Raw { unsigned w[V * sizeof(T) / 4]; };
 
-// V elements from p, of which `left` exist (the others 0).  Rows start at any element: the
-// device takes wide accesses at any address.
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_vec(const T* p, int left) {
-  Vec<T, V> v;
+template <typename T>
+__device__ __forceinline__ float get(const Raw<T>& r, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(r.w[e]);
+  else if constexpr (std::is_same_v<T, __bf16>) return __uint_as_float(e & 1 ? r.w[e / 2] & 0xffff0000u : r.w[e / 2] << 16);
+  else return (float)__builtin_bit_cast(_Float16, (unsigned short)(r.w[e / 2] >> (16 * (e & 1))));
+}
+
+// Makes the compiler take the packed values anew from here on, instead of keeping what it
+// has unpacked or computed from them before: a few instructions for many registers.
+template <typename T>
+__device__ __forceinline__ void repack(Raw<T>& r) {
+#pragma unroll
+  for (int i = 0; i < (int)(V * sizeof(T) / 4); ++i) asm volatile("" : "+v"(r.w[i]));
+}
+
+template <typename T>
+__device__ __forceinline__ Raw<T> fill_raw(float v) {
+  Raw<T> r;
+  const T t = from_f32<T>(v);
+#pragma unroll
+  for (int i = 0; i < (int)(V * sizeof(T) / 4); ++i) {
+    if constexpr (sizeof(T) == 4) r.w[i] = __builtin_bit_cast(unsigned, t);
+    else r.w[i] = __builtin_bit_cast(unsigned short, t) * 0x10001u;
+  }
+  return r;
+}
+
+// V elements from p, of which `left` exist (the others 0).  Rows start at any element: the device takes wide
+// accesses at any address.
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, int left) {
+  Raw<T> r;
   if (left >= V) {
-    __builtin_memcpy(&v, p, sizeof(v));
+    __builtin_memcpy(&r, p, sizeof(r));
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) r.w[e] = e < left ? ((const unsigned*)p)[e] : 0u;
   } else {
 #pragma unroll
-    for (int e = 0; e < V; ++e) v.e[e] = e < left ? p[e] : (T)0.0f;
+    for (int i = 0; i < V / 2; ++i) {
+      const unsigned short* q = (const unsigned short*)p;
+      r.w[i] = (2 * i < left ? q[2 * i] : 0u) | (2 * i + 1 < left ? (unsigned)q[2 * i + 1] << 16 : 0u);
+    }
   }
-  return v;
+  return r;
 }
-template <typename T, int V>
+template <typename T>
+__device__ __forceinline__ Raw<T> load_or_one(const T* p, long at, int left) {
+  return p ? load_raw(p + at, left) : fill_raw<T>(1.0f);
+}
+template <typename T>
 __device__ __forceinline__ void store_vec(T* p, int left, const float* o) {
-  Vec<T, V> v;
+  T v[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) v.e[e] = from_f32<T>(o[e]);
+  for (int e = 0; e < V; ++e) v[e] = from_f32<T>(o[e]);
   if (left >= V) {
-    __builtin_memcpy(p, &v, sizeof(v));
+    __builtin_memcpy(p, v, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
-      if (e < left) p[e] = v.e[e];
+      if (e < left) p[e] = v[e];
   }
 }
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_or_one(const T* p, long at, int left) {
-  if (p) return load_vec<T, V>(p + at, left);
-  Vec<T, V> v;
-#pragma unroll
-  for (int e = 0; e < V; ++e) v.e[e] = (T)1.0f;
-  return v;
+
+// The sum over a wave, in every lane: within 4, 8 and 16 lanes, then across the rows of 16.
+__device__ __forceinline__ float wave_sum(float v) {
+  auto step = [](float a, auto ctrl, auto rows) {
+    return a + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, a), decltype(ctrl)::value,
+                                                                      decltype(rows)::value, 0xf, false));
+  };
+  using std::integral_constant;
+  v = step(v, integral_constant<int, 0xb1>{}, integral_constant<int, 0xf>{});   // lane ^ 1
+  v = step(v, integral_constant<int, 0x4e>{}, integral_constant<int, 0xf>{});   // lane ^ 2
+  v = step(v, integral_constant<int, 0x141>{}, integral_constant<int, 0xf>{});  // mirrored in 8
+  v = step(v, integral_constant<int, 0x140>{}, integral_constant<int, 0xf>{});  // mirrored in 16
+  v = step(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // lane 15 of a row into the next
+  v = step(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // lane 31 into the upper half
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // Sums of a and b over the TPR threads of a row, in each of them.  `slot` (0 or 1)
@@ -93,13 +139,10 @@ __device__ __forceinline__ Vec<T, V> load_or_one(const T* p, long at, int left) 
 // call before from the writes of the next.
 template <int TPR>
 __device__ __forceinline__ void row_sum2(float& a, float& b, float (*lds)[2][16], int slot) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    a += __shfl_xor(a, d, 64);
-    b += __shfl_xor(b, d, 64);
-  }
+  a = wave_sum(a);
+  b = wave_sum(b);
   if constexpr (TPR > 64) {
-    const int wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6, first = threadIdx.x / TPR * (TPR / 64);
     if ((threadIdx.x & 63) == 0) {
       lds[slot][0][wave] = a;
       lds[slot][1][wave] = b;
@@ -108,101 +151,73 @@ __device__ __forceinline__ void row_sum2(float& a, float& b, float (*lds)[2][16]
     a = b = 0.0f;
 #pragma unroll
     for (int w = 0; w < TPR / 64; ++w) {
-      a += lds[slot][0][w];
-      b += lds[slot][1][w];
+      a += lds[slot][0][first + w];
+      b += lds[slot][1][first + w];
     }
   }
 }
 
-// Mean (layer) and reciprocal size of a row's values in v (zeros outside the row).
-template <bool kLayer, int TPR, int IT, int V>
-__device__ __forceinline__ void row_stats(const float (&v)[IT][V], int at0, int D, float eps, float (*lds)[2][16], int& slot,
+// Mean (layer) and reciprocal size of a row, of which this thread holds `left` elements in v (zeros behind them).
+template <bool kLayer, int TPR>
+__device__ __forceinline__ void row_stats(const float (&v)[V], int left, int D, float eps, float (*lds)[2][16], int& slot,
                                           float& mean, float& r) {
   float s = 0.0f, none = 0.0f;
   mean = 0.0f;
   if constexpr (kLayer) {
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) s += v[i][e];
+    for (int e = 0; e < V; ++e) s += v[e];
     row_sum2<TPR>(s, none, lds, slot);
     slot ^= 1;
     mean = s / (float)D;
     s = none = 0.0f;
   }
 #pragma unroll
-  for (int i = 0; i < IT; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float c = at0 + i * TPR * V + e < D ? v[i][e] - mean : 0.0f;
-      s += c * c;
-    }
+  for (int e = 0; e < V; ++e) {
+    const float c = e < left ? v[e] - mean : 0.0f;
+    s += c * c;
+  }
   row_sum2<TPR>(s, none, lds, slot);
   slot ^= 1;
   r = 1.0f / __builtin_sqrtf(s / (float)D + eps);
 }
 
-template <typename TX, typename TB, bool kLayer, int TPR, int IT>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_resnorm_fwd(const NormArgs A) {
-  constexpr int V = vec_of<TB>();
+// Threads of a workgroup, and the rows that it takes at a time.
+template <int TPR> constexpr int threads_of() { return TPR > 512 ? TPR : 512; }
+template <int TPR> constexpr int rows_of() { return threads_of<TPR>() / TPR; }
+
+template <typename TX, typename TB, bool kLayer, int TPR>
+__global__ __launch_bounds__(threads_of<TPR>()) void k_resnorm_fwd(const NormArgs A) {
   __shared__ float lds[2][2][16];
-  const int t = TPR == 64 ? threadIdx.x & 63 : threadIdx.x;
-  const long row = TPR == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x;
-  if (row >= A.rows) return;  // (TPR = 64 only, whose waves meet at no barrier)
-  const int D = A.D, at0 = t * V;
-  const long base = row * D;
-  float y[IT][V];
-  Vec<TX, V> x[IT];
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int at = at0 + i * TPR * V;
-    x[i] = load_vec<TX, V>((const TX*)A.x + base + at, D - at);
-  }
+  const long row = (long)blockIdx.x * rows_of<TPR>() + threadIdx.x / TPR;
+  const int at = threadIdx.x % TPR * V, D = A.D, left = row < A.rows ? D - at : 0;  // elements of this thread
+  const long base = row * D + at;
+  const Raw<TX> x = load_raw((const TX*)A.x + base, left);
   int slot = 0;
-  float mean_b = 0.0f, r_b = 0.0f;
+  float y[V], mean_b = 0.0f, r_b = 0.0f;
+  const Raw<TB> nw = load_or_one((const TB*)A.pre_w, at, left);
   if (A.block) {
-    Vec<TB, V> g[IT], pw[IT];
-    float b[IT][V];
-    const long grow = row / A.gate_group * D;
-#pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int at = at0 + i * TPR * V;
-      const Vec<TB, V> bv = load_vec<TB, V>((const TB*)A.block + base + at, D - at);
-      g[i] = load_or_one<TB, V>((const TB*)A.gate, grow + at, D - at);
-      pw[i] = load_or_one<TB, V>((const TB*)A.post_w, at, D - at);
-#pragma unroll
-      for (int e = 0; e < V; ++e) b[i][e] = to_f32(bv.e[e]);
-    }
+    const Raw<TB> bv = load_raw((const TB*)A.block + base, left);
+    const Raw<TB> g = load_or_one((const TB*)A.gate, row / A.gate_group * D + at, left);
+    const Raw<TB> pw = load_or_one((const TB*)A.post_w, at, left);
     const float scale = A.scale_dev ? *A.scale_dev : A.scale;
-    row_stats<kLayer, TPR, IT, V>(b, at0, D, A.eps, lds, slot, mean_b, r_b);
+    float b[V];
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int at = at0 + i * TPR * V;
+    for (int e = 0; e < V; ++e) b[e] = get(bv, e);
+    row_stats<kLayer, TPR>(b, left, D, A.eps, lds, slot, mean_b, r_b);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        y[i][e] = at + e < D ? to_f32(x[i].e[e]) + scale * to_f32(g[i].e[e]) * ((b[i][e] - mean_b) * r_b * to_f32(pw[i].e[e])) : 0.0f;
-      store_vec<TX, V>((TX*)A.y + base + at, D - at, y[i]);
-    }
+    for (int e = 0; e < V; ++e)
+      y[e] = e < left ? get(x, e) + scale * get(g, e) * ((b[e] - mean_b) * r_b * get(pw, e)) : 0.0f;
+    store_vec((TX*)A.y + base, left, y);
   } else {
 #pragma unroll
-    for (int i = 0; i < IT; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) y[i][e] = to_f32(x[i].e[e]);
+    for (int e = 0; e < V; ++e) y[e] = get(x, e);
   }
-  Vec<TB, V> nw[IT];
+  float mean_y, r_y, h[V];
+  row_stats<kLayer, TPR>(y, left, D, A.eps, lds, slot, mean_y, r_y);
 #pragma unroll
-  for (int i = 0; i < IT; ++i) nw[i] = load_or_one<TB, V>((const TB*)A.pre_w, at0 + i * TPR * V, D - at0 - i * TPR * V);
-  float mean_y, r_y;
-  row_stats<kLayer, TPR, IT, V>(y, at0, D, A.eps, lds, slot, mean_y, r_y);
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int at = at0 + i * TPR * V;
-    float h[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) h[e] = (y[i][e] - mean_y) * r_y * to_f32(nw[i].e[e]);
-    store_vec<TB, V>((TB*)A.h + base + at, D - at, h);
-  }
-  if (A.stats && t == 0) {
+  for (int e = 0; e < V; ++e) h[e] = (y[e] - mean_y) * r_y * get(nw, e);
+  store_vec((TB*)A.h + base, left, h);
+  if (A.stats && at == 0 && row < A.rows) {
     float* s = A.stats + row * (kLayer ? 4 : 2);
     s[0] = r_b;
     s[1] = r_y;
@@ -214,177 +229,149 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_resnorm_fwd(const Nor
 }
 
 // What the backward reads of one row.
-template <typename TX, typename TB, int IT>
+template <typename TX, typename TB>
 struct RowIn {
-  static constexpr int V = vec_of<TB>();
-  Vec<TX, V> x[IT], dy[IT];
-  Vec<TB, V> b[IT], dh[IT], g[IT];
+  Raw<TX> x, dy;
+  Raw<TB> b, dh, g;
   float r_b, r_y, mean_b, mean_y;
 };
 
-template <typename TX, typename TB, bool kLayer, int TPR, int IT>
-__device__ __forceinline__ void load_row(RowIn<TX, TB, IT>& in, const NormArgs& A, long row, int at0, bool gate_rows) {
-  constexpr int V = vec_of<TB>();
-  const long base = row * A.D;
-#pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int at = at0 + i * TPR * V, left = A.D - at;
-    in.x[i] = load_vec<TX, V>((const TX*)A.x + base + at, left);
-    if (A.dy) in.dy[i] = load_vec<TX, V>((const TX*)A.dy + base + at, left);
-    if (A.dh) in.dh[i] = load_vec<TB, V>((const TB*)A.dh + base + at, left);
-    if (A.block) in.b[i] = load_vec<TB, V>((const TB*)A.block + base + at, left);
-    if (gate_rows) in.g[i] = load_vec<TB, V>((const TB*)A.gate + base + at, left);
-  }
+// (a row that is not there: zeros, which add nothing to any sum)
+template <typename TX, typename TB, bool kLayer>
+__device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, long row, bool there, int at, bool gate_rows) {
+  const long base = row * A.D + at;
+  const int left = there ? A.D - at : 0;
+  in.x = load_raw((const TX*)A.x + base, left);
+  in.dy = load_raw((const TX*)A.dy + base, A.dy ? left : 0);
+  in.dh = load_raw((const TB*)A.dh + base, A.dh ? left : 0);
+  in.b = load_raw((const TB*)A.block + base, A.block ? left : 0);
+  if (gate_rows) in.g = load_raw((const TB*)A.gate + base, left);
   const float* s = A.stats + row * (kLayer ? 4 : 2);
-  in.r_b = s[0];
-  in.r_y = s[1];
-  in.mean_b = kLayer ? s[2] : 0.0f;
-  in.mean_y = kLayer ? s[3] : 0.0f;
+  in.r_b = there ? s[0] : 0.0f;
+  in.r_y = there ? s[1] : 0.0f;
+  in.mean_b = kLayer && there ? s[2] : 0.0f;
+  in.mean_y = kLayer && there ? s[3] : 0.0f;
 }
 
-// One workgroup takes the rows of a chunk, four at a time where a wave holds a row (TPR = 64), else one
-// after the other with the next row's loads in flight.
-template <typename TX, typename TB, bool kLayer, int TPR, int IT>
-__global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void k_resnorm_bwd(const NormArgs A) {
-  constexpr int V = vec_of<TB>();
-  constexpr int ROWS = TPR == 64 ? 4 : 1;
+// One workgroup takes the rows of a run, rows_of<TPR>() at a time, with the next ones' loads in flight (at
+// 1024 threads the 128 registers that a thread may have do not hold them too).  Two workgroups a CU, with
+// up to 256 registers: held to 128 the kernel spills, and 16384 x 4096 bf16 take 600 us instead of 170.
+template <typename TX, typename TB, bool kLayer, int TPR>
+__global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnorm_bwd(const NormArgs A) {
+  constexpr int ROWS = rows_of<TPR>();
   __shared__ float lds[2][2][16];
-  __shared__ float sums[TPR == 64 ? IT * V * 64 : 1];
-  const int t = TPR == 64 ? threadIdx.x & 63 : threadIdx.x, sub = TPR == 64 ? threadIdx.x >> 6 : 0;
-  const int D = A.D, at0 = t * V;
+  __shared__ float sums[ROWS > 1 ? TPR * V : 1];
+  const int at = threadIdx.x % TPR * V, sub = threadIdx.x / TPR;
+  const int D = A.D, left = D - at;
   const long chunk = blockIdx.x, group = chunk / A.chunks_per_group;
   const long first = group * A.span + (chunk - group * A.chunks_per_group) * A.per_chunk;
   const long end = min(min(first + A.per_chunk, (group + 1) * A.span), A.rows);
   const bool gate_rows = A.gate && A.gate_group == 1;
   const float scale = A.scale_dev ? *A.scale_dev : A.scale;
-  Vec<TB, V> pw[IT], nw[IT];
-  RowIn<TX, TB, IT> next;
+  Raw<TB> pw = load_or_one((const TB*)A.post_w, at, left), nw = load_or_one((const TB*)A.pre_w, at, left);
+  RowIn<TX, TB> next;
+  next.g = load_or_one((const TB*)A.gate, group * D + at, gate_rows ? 0 : left);
+  float s_pre[V], s_post[V], s_gate[V], s_scale = 0.0f;
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
-    const int at = at0 + i * TPR * V;
-    pw[i] = load_or_one<TB, V>((const TB*)A.post_w, at, D - at);
-    nw[i] = load_or_one<TB, V>((const TB*)A.pre_w, at, D - at);
-    next.g[i] = load_or_one<TB, V>((const TB*)A.gate, group * D + at, gate_rows ? 0 : D - at);
+  for (int e = 0; e < V; ++e) s_pre[e] = s_post[e] = s_gate[e] = 0.0f;
+  const float inv_d = 1.0f / (float)D;
+  constexpr bool kAhead = TPR <= 512;
+  if (kAhead) load_row<TX, TB, kLayer>(next, A, first + sub, first + sub < end, at, gate_rows);
+  for (long row0 = first; row0 < end; row0 += ROWS) {
+    const long row = row0 + sub;
+    if (!kAhead) load_row<TX, TB, kLayer>(next, A, row, row < end, at, gate_rows);
+    RowIn<TX, TB> in = next;
+    if (kAhead && row0 + ROWS < end) load_row<TX, TB, kLayer>(next, A, row + ROWS, row + ROWS < end, at, gate_rows);
+    const long base = row * D + at;
+    const int out = row < end ? left : 0;
+    auto bn = [&](int e) { return e < left ? (get(in.b, e) - in.mean_b) * in.r_b : 0.0f; };
+    auto yn = [&](int e) {
+      const float y = get(in.x, e) + scale * get(in.g, e) * (bn(e) * get(pw, e));
+      return e < left ? (y - in.mean_y) * in.r_y : 0.0f;
+    };
+    float t[V], sa = 0.0f, sb = 0.0f;
+    repack(pw);
+    repack(nw);
+    repack(in.g);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      next.dy[i].e[e] = (TX)0.0f;
-      next.dh[i].e[e] = (TB)0.0f;
-      next.b[i].e[e] = (TB)0.0f;
+      const float dh = get(in.dh, e), q = get(nw, e) * dh, n = yn(e);
+      s_pre[e] += dh * n;
+      sa += q * n;
+      sb += q;
     }
-  }
-  float s_pre[IT][V], s_post[IT][V], s_gate[IT][V], s_scale = 0.0f;
-#pragma unroll
-  for (int i = 0; i < IT; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) s_pre[i][e] = s_post[i][e] = s_gate[i][e] = 0.0f;
-  const float inv_d = 1.0f / (float)D;
-  if (first + sub < end) load_row<TX, TB, kLayer, TPR, IT>(next, A, first + sub, at0, gate_rows);
-  for (long row = first + sub; row < end; row += ROWS) {
-    const RowIn<TX, TB, IT> in = next;
-    if (row + ROWS < end) load_row<TX, TB, kLayer, TPR, IT>(next, A, row + ROWS, at0, gate_rows);
-    const long base = row * D;
-    float tt[IT][V], bn[IT][V], yn[IT][V];
-    float sa = 0.0f, sb = 0.0f;
-#pragma unroll
-    for (int i = 0; i < IT; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const bool ok = at0 + i * TPR * V + e < D;
-        bn[i][e] = ok ? (to_f32(in.b[i].e[e]) - in.mean_b) * in.r_b : 0.0f;
-        const float y = to_f32(in.x[i].e[e]) + scale * to_f32(in.g[i].e[e]) * (bn[i][e] * to_f32(pw[i].e[e]));
-        yn[i][e] = ok ? (y - in.mean_y) * in.r_y : 0.0f;
-        const float dh = to_f32(in.dh[i].e[e]), q = to_f32(nw[i].e[e]) * dh;
-        s_pre[i][e] += dh * yn[i][e];
-        sa += q * yn[i][e];
-        sb += q;
-      }
     row_sum2<TPR>(sa, sb, lds, 0);
     sa *= inv_d;
     sb = kLayer ? sb * inv_d : 0.0f;
-    float pa = 0.0f, pb = 0.0f;
+    float pa = 0.0f, pb = 0.0f, dg[V];
+    repack(in.x);
+    repack(in.b);
+    repack(in.dh);
+    repack(in.g);
+    repack(pw);
+    repack(nw);
 #pragma unroll
-    for (int i = 0; i < IT; ++i) {
-      const int at = at0 + i * TPR * V;
-      float dg[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float q = to_f32(nw[i].e[e]) * to_f32(in.dh[i].e[e]);
-        const float T = to_f32(in.dy[i].e[e]) + in.r_y * (q - yn[i][e] * sa - sb);
-        tt[i][e] = T;
-        const float g = to_f32(in.g[i].e[e]), u = bn[i][e] * to_f32(pw[i].e[e]);
-        dg[e] = scale * T * u;
-        const float du = scale * g * T;
-        s_gate[i][e] += dg[e];
-        s_scale += at + e < D ? T * (g * u) : 0.0f;
-        s_post[i][e] += du * bn[i][e];
-        const float p = du * to_f32(pw[i].e[e]);
-        pa += p * bn[i][e];
-        pb += at + e < D ? p : 0.0f;
-      }
-      if (A.dx) store_vec<TX, V>((TX*)A.dx + base + at, D - at, tt[i]);
-      if (gate_rows && A.dgate) {
-        if (A.gate_f32) store_vec<float, V>((float*)A.dgate + base + at, D - at, dg);
-        else store_vec<TB, V>((TB*)A.dgate + base + at, D - at, dg);
-      }
+    for (int e = 0; e < V; ++e) {
+      const float q = get(nw, e) * get(in.dh, e), g = get(in.g, e), b = bn(e), u = b * get(pw, e);
+      t[e] = get(in.dy, e) + in.r_y * (q - yn(e) * sa - sb);
+      dg[e] = scale * t[e] * u;
+      s_gate[e] += dg[e];
+      s_scale += e < left ? t[e] * (g * u) : 0.0f;
+      const float du = scale * g * t[e], p = du * get(pw, e);
+      s_post[e] += du * b;
+      pa += p * b;
+      pb += e < left ? p : 0.0f;
     }
-    if (A.block) {
-      row_sum2<TPR>(pa, pb, lds, 1);
+    if (A.dx) store_vec((TX*)A.dx + base, out, t);
+    if (gate_rows && A.dgate) {
+      if (A.gate_f32) store_vec((float*)A.dgate + base, out, dg);
+      else store_vec((TB*)A.dgate + base, out, dg);
+    }
+    row_sum2<TPR>(pa, pb, lds, 1);
+    if (A.dblock) {
       pa *= inv_d;
       pb = kLayer ? pb * inv_d : 0.0f;
-      if (A.dblock) {
+      float db[V];
+      repack(in.b);
+      repack(in.g);
+      repack(pw);
 #pragma unroll
-        for (int i = 0; i < IT; ++i) {
-          const int at = at0 + i * TPR * V;
-          float db[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float p = scale * to_f32(in.g[i].e[e]) * tt[i][e] * to_f32(pw[i].e[e]);
-            db[e] = in.r_b * (p - bn[i][e] * pa - pb);
-          }
-          store_vec<TB, V>((TB*)A.dblock + base + at, D - at, db);
-        }
+      for (int e = 0; e < V; ++e) {
+        const float p = scale * get(in.g, e) * t[e] * get(pw, e);
+        db[e] = in.r_b * (p - bn(e) * pa - pb);
       }
-    } else if constexpr (TPR > 64) {
-      __syncthreads();  // the barrier of the second sum (row_sum2)
+      store_vec((TB*)A.dblock + base, out, db);
     }
   }
-  // the chunk's partial rows
+  // the run's partial rows; where several rows go at a time, those of the same columns one after the other
   float* part = A.part + chunk * A.parts * D;
-  auto put = [&](int at_part, const float(&s)[IT][V]) {
+  auto put = [&](int at_part, const float(&s)[V]) {
     if (at_part < 0) return;
     float* o = part + (long)at_part * D;
-    if constexpr (TPR == 64) {
-      // the four waves one after the other, into one row of LDS
-      for (int w = 0; w < 4; ++w) {
+    if constexpr (ROWS == 1) {
+      store_vec(o + at, left, s);
+    } else {
+      for (int w = 0; w < ROWS; ++w) {
         if (sub == w) {
 #pragma unroll
-          for (int i = 0; i < IT; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-              float* c = &sums[(i * V + e) * 64 + t];
-              *c = w == 0 ? s[i][e] : *c + s[i][e];
-            }
+          for (int e = 0; e < V; ++e) {
+            float* c = &sums[e * TPR + threadIdx.x % TPR];
+            *c = w == 0 ? s[e] : *c + s[e];
+          }
         }
         __syncthreads();
       }
-      for (int j = threadIdx.x; j < D; j += 256) {
-        const int i = j / (64 * V), l = (j / V) & 63, e = j % V;
-        o[j] = sums[(i * V + e) * 64 + l];
-      }
+      for (int j = threadIdx.x; j < D; j += threads_of<TPR>()) o[j] = sums[j % V * TPR + j / V];
       __syncthreads();
-    } else {
-#pragma unroll
-      for (int i = 0; i < IT; ++i) store_vec<float, V>(o + at0 + i * TPR * V, D - at0 - i * TPR * V, s[i]);
     }
   };
   put(A.at_pre, s_pre);
   put(A.at_post, s_post);
   put(A.at_gate, s_gate);
   if (A.want_scale) {
-    constexpr int NT = TPR == 64 ? 256 : TPR;
     float none = 0.0f;
     __syncthreads();
-    row_sum2<NT>(s_scale, none, lds, 0);
+    row_sum2<threads_of<TPR>()>(s_scale, none, lds, 0);
     if (threadIdx.x == 0) A.part_scale[chunk] = s_scale;
   }
 }
@@ -532,6 +519,7 @@ __global__ __launch_bounds__(1024) void k_resnorm_reduce(const ReduceArgs A) {
     const long c0 = g >= 0 ? g * A.chunks_per_group : 0, c1 = g >= 0 ? c0 + A.chunks_per_group : A.chunks;
     float s = 0.0f;
     if (col < A.D)
+#pragma unroll 8
       for (long c = c0 + run; c < c1; c += 16) s += A.part[(c * A.parts + which) * A.D + col];
     lds[run][lane] = s;
     __syncthreads();
@@ -558,35 +546,40 @@ __global__ __launch_bounds__(1024) void k_resnorm_reduce(const ReduceArgs A) {
 }
 
 // ---- launches ---------------------------------------------------------------------------------------
-// Threads a row and vectors a thread: a wave for the rows that it holds in two vectors a lane (no barriers), else the
-// fewest threads that hold the row in at most two.
+// Calls go(threads a row) with the fewest threads that hold a row, or 0 where no workgroup does.
+template <typename F>
+void by_width(int D, F go) {
+  const int vecs = (D + V - 1) / V;
+  if (vecs <= 64) go(std::integral_constant<int, 64>{});
+  else if (vecs <= 128) go(std::integral_constant<int, 128>{});
+  else if (vecs <= 256) go(std::integral_constant<int, 256>{});
+  else if (vecs <= 512) go(std::integral_constant<int, 512>{});
+  else if (vecs <= 1024) go(std::integral_constant<int, 1024>{});
+  else go(std::integral_constant<int, 0>{});
+}
+
 template <typename TX, typename TB, bool kLayer>
 hipError_t launch_fwd(const NormArgs& A, hipStream_t st) {
-  constexpr int V = vec_of<TB>();
-  const int vecs = (A.D + V - 1) / V;
-  const dim3 rows((unsigned)A.rows), four((unsigned)((A.rows + 3) / 4));
-  if (vecs <= 64) hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, 64, 1>), four, dim3(256), 0, st, A);
-  else if (vecs <= 128) hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, 64, 2>), four, dim3(256), 0, st, A);
-  else if (vecs <= 256) hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, 256, 1>), rows, dim3(256), 0, st, A);
-  else if (vecs <= 512) hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, 256, 2>), rows, dim3(256), 0, st, A);
-  else if (vecs <= 1024) hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, 512, 2>), rows, dim3(512), 0, st, A);
-  else if (vecs <= 2048) hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, 1024, 2>), rows, dim3(1024), 0, st, A);
-  else hipLaunchKernelGGL((k_resnorm_wide_fwd<TX, TB, kLayer>), rows, dim3(kWide), 0, st, A);
+  by_width(A.D, [&](auto width) {
+    constexpr int TPR = decltype(width)::value;
+    if constexpr (TPR == 0)
+      hipLaunchKernelGGL((k_resnorm_wide_fwd<TX, TB, kLayer>), dim3((unsigned)A.rows), dim3(kWide), 0, st, A);
+    else
+      hipLaunchKernelGGL((k_resnorm_fwd<TX, TB, kLayer, TPR>), dim3((unsigned)((A.rows + rows_of<TPR>() - 1) / rows_of<TPR>())),
+                         dim3(threads_of<TPR>()), 0, st, A);
+  });
   return hipGetLastError();
 }
 
 template <typename TX, typename TB, bool kLayer>
 hipError_t launch_bwd(const NormArgs& A, long chunks, hipStream_t st) {
-  constexpr int V = vec_of<TB>();
-  const int vecs = (A.D + V - 1) / V;
-  const dim3 grid((unsigned)chunks);
-  if (vecs <= 64) hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, 64, 1>), grid, dim3(256), 0, st, A);
-  else if (vecs <= 128) hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, 64, 2>), grid, dim3(256), 0, st, A);
-  else if (vecs <= 256) hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, 256, 1>), grid, dim3(256), 0, st, A);
-  else if (vecs <= 512) hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, 256, 2>), grid, dim3(256), 0, st, A);
-  else if (vecs <= 1024) hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, 512, 2>), grid, dim3(512), 0, st, A);
-  else if (vecs <= 2048) hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, 1024, 2>), grid, dim3(1024), 0, st, A);
-  else hipLaunchKernelGGL((k_resnorm_wide_bwd<TX, TB, kLayer>), grid, dim3(kWide), 0, st, A);
+  by_width(A.D, [&](auto width) {
+    constexpr int TPR = decltype(width)::value;
+    if constexpr (TPR == 0)
+      hipLaunchKernelGGL((k_resnorm_wide_bwd<TX, TB, kLayer>), dim3((unsigned)chunks), dim3(kWide), 0, st, A);
+    else
+      hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, TPR>), dim3((unsigned)chunks), dim3(threads_of<TPR>()), 0, st, A);
+  });
   return hipGetLastError();
 }
 

@@ -26,7 +26,7 @@ import torch
 
 from . import device
 from ._engine import DT_BF16, DT_F16, DT_F32
-from .torch_module import _stream_of
+from .torch_module import _current_stream
 
 _DT = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
 BLOCK = 256  # elements that share a scale of the 8-bit states
@@ -169,7 +169,7 @@ class TorchAdamW(torch.optim.Optimizer):
                 flat = dict(a.flat)
                 if self.state_bits == 8:
                     avg, sq = (torch.empty(a.total * BLOCK, device=a.device) for _ in range(2))
-                    stream = _stream_of(torch.cuda.current_stream(a.device))
+                    stream = _current_stream(a.device)
                     device.check(device.get_metal_bridge().kans_adamw_values(
                         flat["exp_avg"].data_ptr(), flat["exp_avg_sq"].data_ptr(), flat.pop("exp_avg_scale").data_ptr(),
                         flat.pop("exp_avg_sq_scale").data_ptr(), avg.data_ptr(), sq.data_ptr(), a.total, stream),
@@ -265,7 +265,7 @@ class TorchAdamW(torch.optim.Optimizer):
         device.check(lib.kans_adamw_step(
             _DT[a.dtype], a.bits, len(ids), *at, ptr("exp_avg"), ptr("exp_avg_sq"), ptr("exp_avg_scale"),
             ptr("exp_avg_sq_scale"), ptr("master"), float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-            float(group["weight_decay"]), _stream_of(torch.cuda.current_stream(a.device))), "kans_adamw_step")
+            float(group["weight_decay"]), _current_stream(a.device)), "kans_adamw_step")
         changed = []
         for i, t in zip(ids, steps):
             p = a.params[i]

@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 
 from . import device
 from ._engine import DT_BF16, DT_F16, DT_F32
-from .torch_module import _stream_of
+from .torch_module import _current_stream
 
 _DT = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
 _KINDS = {"rms": 0, "layer": 1}
@@ -39,7 +39,7 @@ def _forward(x, block, gate, post, pre, scale, group, kind, eps, dt, want_stats)
     device.check(device.get_metal_bridge().kans_residual_norm_forward(
         _DT[x.dtype], _DT[dt], kind, x.data_ptr(), _ptr(block), _ptr(gate), group, _ptr(post), _ptr(pre), _ptr(dev),
         0.0 if dev is not None else scale, eps, _ptr(y if block is not None else None), h.data_ptr(), _ptr(stats), rows, d,
-        _stream_of(torch.cuda.current_stream(x.device))), "kans_residual_norm_forward")
+        _current_stream(x.device)), "kans_residual_norm_forward")
     return y, h, stats
 
 
@@ -88,7 +88,7 @@ class _ResidualNorm(torch.autograd.Function):
             _DT[x.dtype], _DT[dt], kind, x.data_ptr(), _ptr(block), _ptr(gate), group, _ptr(post), _ptr(pre), _ptr(dev),
             scale, eps, stats.data_ptr(), _ptr(dy), _ptr(dh), _ptr(dx), _ptr(db), _ptr(dg),
             int(wide), _ptr(dpost), _ptr(dpre), _ptr(ds), rows, d, ws.data_ptr(), size,
-            _stream_of(torch.cuda.current_stream(x.device))), "kans_residual_norm_backward")
+            _current_stream(x.device)), "kans_residual_norm_backward")
         if wide:
             dg = dg.sum_to_size(ctx.gate_shape).to(dt)
         return dx, db, dg, dpost, dpre, ds, None, None, None, None
@@ -111,6 +111,26 @@ def _gate_rows(gate: torch.Tensor, x: torch.Tensor):
                 group *= size
             return gate.contiguous(), group
     return gate, 0
+
+
+def _refuse(x, block, gate, scale, post_weight, pre_weight, dt) -> None:
+    d = x.shape[-1]
+    if dt not in _DT or x.dtype not in (dt, torch.float32):
+        raise TypeError(f"x is {x.dtype} and the block {dt}; x must be fp32 or the block's fp32, fp16 or bf16")
+    for name, t in (("block", block), ("gate", gate), ("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if t is not None and t.dtype != dt:
+            raise TypeError(f"{name} is {t.dtype}, expected {dt}")
+    if isinstance(scale, torch.Tensor) and (scale.numel() != 1 or scale.dtype != torch.float32):
+        raise TypeError("a tensor scale is one fp32 element")
+    for name, t in (("x", x), ("block", block), ("gate", gate), ("post_weight", post_weight), ("pre_weight", pre_weight),
+                    ("scale", scale)):
+        if isinstance(t, torch.Tensor) and (not t.is_cuda or t.device != x.device):
+            raise ValueError(f"{name} is on {t.device}; residual_norm takes tensors on one GPU")
+    if block is not None and block.shape != x.shape:
+        raise ValueError(f"block is {tuple(block.shape)}, x {tuple(x.shape)}")
+    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
+        if w is not None and tuple(w.shape) != (d,):
+            raise ValueError(f"{name} is {tuple(w.shape)}, expected ({d},)")
 
 
 def residual_norm(x: torch.Tensor, block: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
@@ -140,33 +160,27 @@ def residual_norm(x: torch.Tensor, block: Optional[torch.Tensor] = None, gate: O
         raise ValueError(f"eps must be finite and >= 0, got {eps}")
     d = x.shape[-1]
     dt = block.dtype if block is not None else pre_weight.dtype if pre_weight is not None else x.dtype
-    if dt not in _DT or x.dtype not in (dt, torch.float32):
-        raise TypeError(f"x is {x.dtype} and the block {dt}; x must be fp32 or the block's fp32, fp16 or bf16")
-    for name, t in (("block", block), ("gate", gate), ("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if t is not None and t.dtype != dt:
-            raise TypeError(f"{name} is {t.dtype}, expected {dt}")
-    if isinstance(scale, torch.Tensor):
-        if scale.numel() != 1 or scale.dtype != torch.float32:
-            raise TypeError("a tensor scale is one fp32 element")
-    else:
+    if not isinstance(scale, torch.Tensor):
         scale = float(scale)
-    for name, t in (("x", x), ("block", block), ("gate", gate), ("post_weight", post_weight), ("pre_weight", pre_weight),
-                    ("scale", scale if isinstance(scale, torch.Tensor) else None)):
-        if t is not None and (not t.is_cuda or t.device != x.device):
-            raise ValueError(f"{name} is on {t.device}; residual_norm takes tensors on one GPU")
-    if block is not None and block.shape != x.shape:
-        raise ValueError(f"block is {tuple(block.shape)}, x {tuple(x.shape)}")
-    for name, w in (("post_weight", post_weight), ("pre_weight", pre_weight)):
-        if w is not None and tuple(w.shape) != (d,):
-            raise ValueError(f"{name} is {tuple(w.shape)}, expected ({d},)")
+    # (the tests of a call that passes, quickly; a call that does not is told why)
+    gpu, vec = x.get_device(), x.shape[-1:]
+    if not (dt in _DT and gpu >= 0 and (x.dtype is dt or x.dtype is torch.float32)
+            and (block is None or (block.shape == x.shape and block.dtype is dt and block.get_device() == gpu))
+            and (gate is None or (gate.dtype is dt and gate.get_device() == gpu))
+            and (post_weight is None or (post_weight.shape == vec and post_weight.dtype is dt and post_weight.get_device() == gpu))
+            and (pre_weight is None or (pre_weight.shape == vec and pre_weight.dtype is dt and pre_weight.get_device() == gpu))
+            and (type(scale) is float or (scale.numel() == 1 and scale.dtype is torch.float32 and scale.get_device() == gpu))):
+        _refuse(x, block, gate, scale, post_weight, pre_weight, dt)
     rows = x.numel() // d
     group = max(rows, 1)
     if gate is not None:
         gate, group = _gate_rows(gate, x)
     xc = x.contiguous()
-    block, post, pre = (None if t is None else t.contiguous() for t in (block, post_weight, pre_weight))
+    block = block.contiguous() if block is not None else None
+    post = post_weight.contiguous() if post_weight is not None else None
+    pre = pre_weight.contiguous() if pre_weight is not None else None
     inputs = (xc, block, gate, post, pre, scale)
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs if isinstance(t, torch.Tensor)):
         y, h = _ResidualNorm.apply(*inputs, group, _KINDS[kind], float(eps), dt)
     else:
         if group == 0:

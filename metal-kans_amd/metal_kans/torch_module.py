@@ -69,6 +69,18 @@ def _stream_of(s: torch.cuda.Stream) -> int:
     return h or _LEGACY_STREAM
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _current_stream(dev: torch.device) -> int:
+    """The library's handle of torch's current stream on a GPU: without a stream object (2 us) where the library
+    knows it already."""
+    h = _raw_stream(dev.index) if _raw_stream is not None and dev.index is not None else -1
+    if h in _kept:
+        return h or _LEGACY_STREAM
+    return _stream_of(torch.cuda.current_stream(dev))
+
+
 class _KANFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, base_weight, bias, module):

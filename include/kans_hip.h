@@ -442,6 +442,24 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
                                 void* dgate, int dgate_f32, void* dpost_w, void* dpre_w, float* dscale, long rows, int D,
                                 void* workspace, long workspace_bytes, void* stream);
 
+/* Softmax cross entropy of a linear head, without its logits: with l = H W^T (H [N][D], W [V][D] of `dtype`, rows
+ * contiguous) and loss[n] = log sum_v exp l[n][v] - l[n][target[n]] in fp32,
+ *   reduction 0: loss[N] (0 in ignored rows), 1: their mean over the rows that are not ignored (NaN if there
+ *   are none), 2: their sum.
+ * Rows whose target is ignore_index take part in nothing, whatever H holds there; another target outside
+ * [0, V) makes its row's loss NaN.  `state` (int32, 4 + 3 N) is filled for the backward.  The workspace
+ * (device memory, 16-byte aligned) has kans_linear_xent_workspace bytes, which is negative for refused sizes: N up to
+ * 2^22, D to 2^16, V to 2^24. */
+long kans_linear_xent_workspace(int dtype, int N, int D, int V, int backward);
+int kans_linear_xent_forward(int dtype, const void* H, const void* W, const int64_t* target, int N, int D, int V,
+                             int64_t ignore_index, int reduction, float* loss, int* state, void* workspace,
+                             long workspace_bytes, void* stream);
+/* dH [N][D] and dW [V][D] of `dtype` (null: not computed) from grad, d(result): fp32, [N] for reduction 0, else
+ * one; zeros in dH's ignored rows. */
+int kans_linear_xent_backward(int dtype, const void* H, const void* W, const int64_t* target, int N, int D, int V,
+                              int64_t ignore_index, int reduction, const int* state, const float* grad, void* dH, void* dW,
+                              void* workspace, long workspace_bytes, void* stream);
+
 /* Measured ceilings for the roofline report (no reference counterpart; measurement only).
  * kans_mfma_ceiling: TFLOP/s of back-to-back v_mfma_f32_32x32x16 (dtype DT_F16 / DT_BF16) on 16 A and
  * 16 B operand fragments given as host arrays [16][64 lanes][8 x 16-bit], at the fused block kernel's

@@ -34,8 +34,8 @@ __device__ __forceinline__ int xcd_remap(int id, int total) {
 // GM m-tiles x all n-tiles, m fastest, so the 1/8 of the grid one XCD owns is a
 // GM x (n_tiles/8)-ish block: its workgroups share input rows (x) and weight
 // N-tiles (W') in that XCD's L2.
+template <int GM = 16>
 __device__ __forceinline__ void tile_of(int lin, int m_tiles, int n_tiles, int& m_tile, int& n_tile) {
-  constexpr int GM = 16;
   const int group = lin / (GM * n_tiles);
   const int first_m = group * GM;
   const int gm = min(GM, m_tiles - first_m);

@@ -1,0 +1,710 @@
+// Kernels and launches of the cross entropy for one element type TO (see kans_xent.h).
+//
+// The logits are computed twice: for the sums of the softmax, and again in the backward, a piece of the vocabulary
+// at a time, where the epilogue turns them into G.  Only G of one piece is ever in memory (16-bit, or three
+// bf16 terms for fp32; at most kXentPiece elements), in both orders, and goes into the two products behind it.
+// 8 N D V operations in all against the 6 N D V of a program that keeps the logits: the price of
+// not writing and reading N V of them.
+//
+// G is stored as (p - [v = t]) rho_n up_of<T>() with |rho_n| <= 1 (the row's share of the largest |c_n|; 1 where
+// all rows have the same); the factor common to all rows comes in at the end, in fp32.  So fp16's smallest
+// number stands for p = 2^-38, and p below fp32's normal numbers stays a normal one (the matrix pipe may drop
+// others).  Rounding G to the inputs' type is an error of half a step of that type in each
+// term of a sum whose result is rounded to that type too.
+#pragma once
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "kans_xent.h"
+#include "kans_xent_gemm.h"
+
+namespace kans {
+namespace {
+
+constexpr long kXentPiece = 1L << 27;  // elements of G in memory at a time
+constexpr long kXentHeadPiece = 1L << 28;  // elements of the head that are laid out anew at a time
+constexpr int kPad = 256;              // compact rows and vocabulary of a piece are padded to this
+constexpr float kNoLogit = -__builtin_inff();
+
+template <typename TO> struct XentTypes { typedef TO T; static constexpr int TERMS = 1; };
+template <> struct XentTypes<float> { typedef __bf16 T; static constexpr int TERMS = 3; };
+
+template <typename T> __host__ __device__ constexpr float up_of() { return std::is_same_v<T, _Float16> ? 0x1p14f : 0x1p32f; }
+
+enum XentEpilogue { XE_STATS, XE_GRAD, XE_DW, XE_DH };
+
+struct XentArgs {
+  GemmOperand A, B;
+  int m_tiles, n_tiles;
+  int steps, steps_per_split;  // of k; XE_DW: bounded by the compact rows as well
+  const int* state;
+  int N, V;                    // rows of the call; vocabulary (XE_STATS, XE_GRAD: entries of this piece)
+  int v0;                      // first entry of the piece
+  float2* part;                // XE_STATS: [m tile][Np] largest logit and sum of exp
+  float* picked;               // XE_STATS: [N] the target's logit
+  long Np, Vp;
+  const float* rho;            // XE_GRAD: per compact row, or null (1)
+  char *g, *gt;                // XE_GRAD: panels [v / kStep][Np] and [n / kStep][Vp]; either may be null
+  const float* alpha;          // XE_DW: factor
+  void* out;                   // XE_DW: dW of the piece [V][D]
+  int D;
+  float* acc;                  // XE_DH: [split][Np][Dq] fp32
+  long Dq;
+  int add;                     // XE_DH: add to acc
+};
+
+// up exp(x) for a power of two up: exp2 of the rounded product, and (kExact) what the rounding left as a factor.  exp2
+// drops results below 2^-126; with up > 1 those are taken times up at once.
+template <bool kExact>
+__device__ __forceinline__ float exp_of(float x, float up = 1.0f, float log_up = 0.0f) {
+  const float h = x * kLog2e;
+  const bool small = log_up != 0.0f && h < -126.0f;
+  float e = __builtin_amdgcn_exp2f(small ? h + log_up : h) * (small ? 1.0f : up);
+  if (kExact) {
+    const float l = __builtin_fmaf(x, 1.925963033500e-8f, __builtin_fmaf(x, kLog2e, -h));  // log2(e) - kLog2e
+    if (h > -200.0f) e = __builtin_fmaf(e, l * 0.6931471805599453f, e);  // (x = -inf has no rest)
+  }
+  return e;
+}
+
+// Four consecutive elements of G: 16-bit, or their three terms `term` bytes apart.
+template <typename T, int TERMS>
+__device__ __forceinline__ void store_g(char* p, int term, const float* v) {
+  if constexpr (TERMS == 1) {
+    struct alignas(8) { T e[4]; } q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q.e[e] = from_f32<T>(v[e]);
+    *(uint2*)p = __builtin_bit_cast(uint2, q);
+  } else {
+    float w[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
+    const Split8 s = split8(w);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) *(uint2*)(p + t * term) = make_uint2(s.t[t].x, s.t[t].y);
+  }
+}
+template <typename T, int TERMS>
+__device__ __forceinline__ void store_g1(char* p, int term, float v) {
+  if constexpr (TERMS == 1) {
+    *(T*)p = from_f32<T>(v);
+  } else {
+    const __bf16 h = (__bf16)v;
+    const float r = v - (float)h;
+    const __bf16 m = (__bf16)r;
+    *(__bf16*)p = h;
+    *(__bf16*)(p + term) = m;
+    *(__bf16*)(p + 2 * term) = (__bf16)(r - (float)m);
+  }
+}
+
+template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N>
+__global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentArgs A) {
+  typedef typename XentTypes<TO>::T T;
+  constexpr int TERMS = XentTypes<TO>::TERMS;
+  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N>;
+  using Step = StepOf<TERMS>;
+  constexpr int MB = Tile::MB, NB = Tile::NB;
+  __shared__ alignas(16) char st0[Tile::STAGE];
+  __shared__ alignas(16) char st1[Tile::STAGE];
+  int mt, nt;
+  tile_of<8>(xcd_remap(blockIdx.x, A.m_tiles * A.n_tiles), A.m_tiles, A.n_tiles, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN;
+  const int count = A.state[0];  // compact rows
+  // (G of the rows that fill up the last step of k is written too: zeros)
+  if (EPI != XE_DW && n0 >= (EPI == XE_GRAD ? (count + 63) / 64 * 64 : count)) return;
+  int first = 0, steps = A.steps;
+  if (EPI == XE_DW) steps = min(steps, (count + Step::kStep - 1) / Step::kStep);
+  if (EPI == XE_DH) {
+    first = blockIdx.y * A.steps_per_split;
+    steps = min(A.steps_per_split, steps - first);
+  }
+  floatx16 acc[MB][NB];
+  Tile::run(A.A, A.B, m0, n0, first, steps, st0, st1, acc);
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / WAVES_N, wn = wave % WAVES_N, col = lane & 31, half = lane >> 5;
+  // acc[i][j][r] is C[mrow(i, r)][ncol(j)]
+  auto mrow = [&](int i, int r) { return m0 + (wm * MB + i) * 32 + 8 * (r / 4) + 4 * half + r % 4; };
+  auto ncol = [&](int j) { return n0 + (wn * NB + j) * 32 + col; };
+
+  if constexpr (EPI == XE_STATS) {
+    float2* join = (float2*)st0;  // [WAVES_M][BN]
+    const bool edge = m0 + BM > A.V;
+    const int* target = A.state + kXentHead + A.N;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int n = ncol(j);
+      const int t = n < count ? target[n] - A.v0 - (m0 + wm * MB * 32) : -1;  // among this wave's entries
+      float top = kNoLogit, sum = 0.0f, own = 0.0f;
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (mrow(i, r) >= A.V) acc[i][j][r] = kNoLogit;
+      }
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float at = top == kNoLogit ? 0.0f : top;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum += exp_of<TERMS == 3>(acc[i][j][r] - at);
+      sum += __shfl_xor(sum, 32, 64);
+      if (t >= 0 && t < MB * 32 && ((t >> 2) & 1) == half) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (t == i * 32 + 8 * (r / 4) + 4 * half + r % 4) own = acc[i][j][r];
+        A.picked[n] = own;
+      }
+      if (half == 0) join[wm * BN + (wn * NB + j) * 32 + col] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < BN; c += Tile::THREADS) {
+      float2 s = join[c];
+#pragma unroll
+      for (int w = 1; w < WAVES_M; ++w) {
+        const float2 o = join[w * BN + c];
+        const float top = fmaxf(s.x, o.x), at = top == kNoLogit ? 0.0f : top;
+        s.y = s.y * exp_of<TERMS == 3>(s.x - at) + o.y * exp_of<TERMS == 3>(o.x - at);
+        s.x = top;
+      }
+      A.part[(long)mt * A.Np + n0 + c] = s;
+    }
+  } else if constexpr (EPI == XE_GRAD) {
+    constexpr float kUp = up_of<TO>(), kLogUp = std::is_same_v<TO, _Float16> ? 14.0f : 32.0f;
+    const int* target = A.state + kXentHead + A.N;
+    const float* lse = (const float*)(target + A.N);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int n = ncol(j);
+      const bool there = n < count;
+      const float at = there ? lse[n] : 0.0f, rho = there && A.rho ? A.rho[n] : 1.0f;
+      const int t = there ? target[n] - A.v0 : -1;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int m = mrow(i, 4 * q);
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float p = exp_of<TERMS == 3>(acc[i][j][4 * q + e] - at, kUp, kLogUp) - (m + e == t ? kUp : 0.0f);
+            v[e] = there && m + e < A.V ? p * rho : 0.0f;
+          }
+          constexpr int K = Step::kStep;
+          if (A.g) store_g<T, TERMS>(A.g + ((long)(m / K) * A.Np + n) * Step::row_bytes + m % K * 2, K * 2, v);
+          if (A.gt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              store_g1<T, TERMS>(A.gt + ((long)(n / K) * A.Vp + m + e) * Step::row_bytes + n % K * 2, K * 2, v[e]);
+          }
+        }
+    }
+  } else if constexpr (EPI == XE_DW) {
+    const float alpha = *A.alpha;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int v = ncol(j);
+      if (v >= A.V) continue;
+      TO* o = (TO*)A.out + (long)v * A.D;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = mrow(i, 4 * q);
+          struct alignas(4 * sizeof(TO)) { TO e[4]; } x;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x.e[e] = from_f32<TO>(acc[i][j][4 * q + e] * alpha);
+          if (d + 4 <= A.D) {
+            __builtin_memcpy(o + d, &x, sizeof(x));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d + e < A.D) o[d + e] = x.e[e];
+          }
+        }
+    }
+  } else {
+    float* base = A.acc + (long)blockIdx.y * A.Np * A.Dq;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      float* o = base + (long)ncol(j) * A.Dq;
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int d = mrow(i, 4 * q);
+          if (d >= A.Dq) continue;
+          float4 x = make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+          if (A.add) {
+            const float4 y = *(const float4*)(o + d);
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+          }
+          *(float4*)(o + d) = x;
+        }
+    }
+  }
+}
+
+// ---- operands ---------------------------------------------------------------------------------------
+// 8 elements of a row of D from element `at`, 0 behind its end.
+template <typename TO>
+__device__ __forceinline__ void row8(const TO* p, int at, int D, float* v) {
+  if (at + 8 <= D) {
+    TO e[8];
+    __builtin_memcpy(e, p + at, sizeof(e));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = at + i < D ? to_f32(p[at + i]) : 0.0f;
+  }
+}
+template <typename T, int TERMS>
+__device__ __forceinline__ void store8(char* p, int term, const float* v) {
+  if constexpr (TERMS == 1) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    uint4 u;
+    __builtin_memcpy(&u, e, 16);
+    *(uint4*)p = u;
+  } else {
+    const Split8 s = split8(v);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) *(uint4*)(p + t * term) = s.t[t];
+  }
+}
+
+// Panels [step of D][R rows][kStep] of `rows` rows of a matrix [.][D], padded with zeros.  With `state`
+// the rows are the compact ones (`rows` bounds their number) and rows behind the last 256 that hold one stay as they are.
+template <typename TO>
+__global__ __launch_bounds__(256) void k_xent_pack(const TO* __restrict__ src, const int* __restrict__ state, int rows, int D,
+                                                   char* __restrict__ dst, int R, int steps) {
+  typedef typename XentTypes<TO>::T T;
+  constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep, C = K / 8;
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const int chunk = (int)(i % C);
+  const long rs = i / C;
+  const int row = (int)(rs % R), step = (int)(rs / R);
+  if (step >= steps) return;
+  if (state) {
+    rows = min(rows, state[0]);
+    if (row >= (rows + kPad - 1) / kPad * kPad) return;
+  }
+  float v[8];
+  if (row < rows) {
+    row8(src + (long)(state ? state[kXentHead + row] : row) * D, step * K + chunk * 8, D, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  }
+  store8<T, TERMS>(dst + ((long)step * R + row) * StepOf<TERMS>::row_bytes + chunk * 16, K * 2, v);
+}
+
+// Panels [step of the rows][R][kStep] of the transpose: 64 rows x 64 columns a workgroup, by way of LDS.
+template <typename TO>
+__global__ __launch_bounds__(256) void k_xent_pack_t(const TO* __restrict__ src, const int* __restrict__ state, int rows, int D,
+                                                     char* __restrict__ dst, int R) {
+  typedef typename XentTypes<TO>::T T;
+  constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
+  __shared__ float tile[64][65];
+  const int d0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+  if (state) {
+    rows = min(rows, state[0]);
+    if (r0 >= (rows + kPad - 1) / kPad * kPad) return;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = threadIdx.x / 8 + i * 32, c = threadIdx.x % 8 * 8;
+    float v[8];
+    if (r0 + r < rows) {
+      row8(src + (long)(state ? state[kXentHead + r0 + r] : r0 + r) * D, d0 + c, D, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[r][c + e] = v[e];
+  }
+  __syncthreads();
+  const int d = threadIdx.x / 4;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (threadIdx.x % 4 * 2 + i) * 8;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = tile[r + e][d];
+    store8<T, TERMS>(dst + ((long)((r0 + r) / K) * R + d0 + d) * StepOf<TERMS>::row_bytes + r % K * 2, K * 2, v);
+  }
+}
+
+// ---- the ends ------------------------------------------------------------------------------------------
+// Numbers the rows that count, in their order, and clears what the products may not write.
+__global__ __launch_bounds__(1024) void k_xent_rows(const int64_t* __restrict__ target, int N, int V, int64_t ignore,
+                                                    int* __restrict__ state, float* __restrict__ picked,
+                                                    float* __restrict__ loss) {
+  __shared__ int waves[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int base = 0;
+  for (int r0 = 0; r0 < N; r0 += 1024) {
+    const int r = r0 + threadIdx.x;
+    const int64_t t = r < N ? target[r] : ignore;
+    const bool in = r < N && t != ignore;
+    const unsigned long long mask = __builtin_amdgcn_ballot_w64(in);
+    if (lane == 0) waves[wave] = __builtin_popcountll(mask);
+    __syncthreads();
+    int at = base + __builtin_popcountll(mask & ((1ull << lane) - 1));
+    for (int w = 0; w < 16; ++w) {
+      at += w < wave ? waves[w] : 0;
+      base += waves[w];
+    }
+    if (in) {
+      state[kXentHead + at] = r;
+      state[kXentHead + N + at] = t >= 0 && t < V ? (int)t : -1;
+    }
+    if (r < N) {
+      picked[r] = __builtin_nanf("");  // of a target outside the vocabulary
+      loss[r] = 0.0f;                  // of an ignored row
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) state[0] = base;
+}
+
+// Joins the tiles' sums: 64 rows a workgroup, 16 runs of tiles.
+template <bool kExact>
+__global__ __launch_bounds__(1024) void k_xent_loss(const float2* __restrict__ part, int tiles, long Np, int N,
+                                                    int* __restrict__ state, const float* __restrict__ picked,
+                                                    float* __restrict__ loss) {
+  __shared__ float2 join[16][64];
+  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
+  const int n = blockIdx.x * 64 + lane, count = state[0];
+  if ((int)blockIdx.x * 64 >= count) return;
+  float top = kNoLogit, sum = 0.0f;
+  auto add = [&](float2 o) {
+    const float both = fmaxf(top, o.x), at = both == kNoLogit ? 0.0f : both;
+    sum = sum * exp_of<kExact>(top - at) + o.y * exp_of<kExact>(o.x - at);
+    top = both;
+  };
+#pragma unroll 4
+  for (int t = run; t < tiles; t += 16) add(part[(long)t * Np + n]);
+  join[run][lane] = make_float2(top, sum);
+  __syncthreads();
+  if (run != 0 || n >= count) return;
+  for (int r = 1; r < 16; ++r) add(join[r][lane]);
+  const bool known = state[kXentHead + N + n] >= 0;
+  const float lse = known ? top + __builtin_logf(sum) : __builtin_nanf("");
+  ((float*)state)[kXentHead + 2 * N + n] = lse;
+  loss[state[kXentHead + n]] = lse - picked[n];
+}
+
+// The sum of the rows' losses, or their mean over the rows that count.
+__global__ __launch_bounds__(1024) void k_xent_sum(const float* __restrict__ rows, int N, const int* __restrict__ state, int mean,
+                                                   float* __restrict__ out) {
+  __shared__ float join[1024];
+  float s = 0.0f;
+  for (int r = threadIdx.x; r < N; r += 1024) s += rows[r];
+  join[threadIdx.x] = s;
+  __syncthreads();
+  for (int d = 512; d > 0; d >>= 1) {
+    if ((int)threadIdx.x < d) join[threadIdx.x] += join[threadIdx.x + d];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *out = mean ? join[0] / (float)state[0] : join[0];
+}
+
+// The factor common to all rows of G (up: the scale that G is stored with) and each row's share of it.
+__global__ __launch_bounds__(1024) void k_xent_scale(const float* __restrict__ grad, int reduction, const int* __restrict__ state,
+                                                     float up, float* __restrict__ alpha, float* __restrict__ rho) {
+  __shared__ float join[1024];
+  const int count = state[0];
+  if (reduction != 0) {
+    if (threadIdx.x == 0) *alpha = count == 0 ? 0.0f : (reduction == 1 ? *grad / (float)count : *grad) / up;
+    return;
+  }
+  float top = 0.0f;
+  bool bad = false;
+  for (int n = threadIdx.x; n < count; n += 1024) {
+    const float g = __builtin_fabsf(grad[state[kXentHead + n]]);
+    bad |= !(g < __builtin_inff());
+    top = fmaxf(top, g);
+  }
+  join[threadIdx.x] = bad ? __builtin_inff() : top;
+  __syncthreads();
+  for (int d = 512; d > 0; d >>= 1) {
+    if ((int)threadIdx.x < d) join[threadIdx.x] = fmaxf(join[threadIdx.x], join[threadIdx.x + d]);
+    __syncthreads();
+  }
+  // (an infinite or NaN gradient: as it is, without a common factor)
+  top = join[0];
+  const float by = top > 0.0f && top < __builtin_inff() ? top : 1.0f;
+  if (threadIdx.x == 0) *alpha = by / up;
+  for (int n = threadIdx.x; n < count; n += 1024) rho[n] = grad[state[kXentHead + n]] / by;
+}
+
+// dH: the splits' sums times alpha in the rows' own places, zeros for the ignored rows.
+template <typename TO>
+__global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, int splits, long Np, long Dq, int D,
+                                                 const int* __restrict__ state, const int64_t* __restrict__ target,
+                                                 int64_t ignore, const float* __restrict__ alpha, TO* __restrict__ dH) {
+  const int row = blockIdx.x;
+  if (target[row] == ignore)
+    for (int d = threadIdx.x; d < D; d += 256) dH[(long)row * D + d] = (TO)0.0f;
+  if (row >= state[0]) return;
+  const float a = *alpha;
+  TO* o = dH + (long)state[kXentHead + row] * D;
+  for (int d = threadIdx.x * 4; d < D; d += 1024) {
+    float4 s = *(const float4*)(acc + (long)row * Dq + d);
+    for (int k = 1; k < splits; ++k) {
+      const float4 x = *(const float4*)(acc + ((long)k * Np + row) * Dq + d);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
+    }
+    const float v[4] = {s.x * a, s.y * a, s.z * a, s.w * a};
+    TO e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_f32<TO>(v[i]);
+    if (d + 4 <= D) {
+      __builtin_memcpy(o + d, e, sizeof(e));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (d + i < D) o[d + i] = e[i];
+    }
+  }
+}
+
+// ---- plans ----------------------------------------------------------------------------------------------
+inline long up_to(long v, long m) { return (v + m - 1) / m * m; }
+
+// Tiles of a product: the large one where its tiles fill most of the CUs, else the small one; few rows get a narrow one.
+enum { TILE_LARGE, TILE_SMALL, TILE_NARROW };
+template <typename TO> struct Tiles;
+template <> struct Tiles<float> { static constexpr int large_m = 256, large_n = 128, narrow_n = 64; };
+template <> struct Tiles<_Float16> { static constexpr int large_m = 256, large_n = 256, narrow_n = 32; };
+template <> struct Tiles<__bf16> { static constexpr int large_m = 256, large_n = 256, narrow_n = 32; };
+
+template <typename TO>
+int tile_for(long m, long n, bool narrow) {
+  if (narrow && n <= Tiles<TO>::narrow_n) return TILE_NARROW;
+  const long large = (m + Tiles<TO>::large_m - 1) / Tiles<TO>::large_m * ((n + Tiles<TO>::large_n - 1) / Tiles<TO>::large_n);
+  return large >= 192 ? TILE_LARGE : TILE_SMALL;
+}
+
+template <typename TO>
+struct XentPlan {
+  static constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
+  static constexpr long ROW = StepOf<TERMS>::row_bytes;
+  long Np, Dk, Dr, Dq;     // padded rows; D in whole steps (of k), of panel rows, of fp32 quads
+  int d_steps;
+  bool pack_w;             // W goes through panels
+  long piece, pieces;      // vocabulary of a piece (a multiple of kPad) and how many
+  int stats_tile, dh_splits;
+  // offsets into the workspace
+  size_t h, w, part, picked, rows, ht, wt, g, gt, acc, alpha, rho, bytes;
+};
+
+template <typename TO>
+XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
+  XentPlan<TO> p{};
+  typedef XentPlan<TO> P;
+  p.Np = up_to(N, kPad);
+  p.Dk = up_to(D, P::K);
+  p.d_steps = (int)(p.Dk / P::K);
+  p.Dr = up_to(D, 64);
+  p.Dq = up_to(D, 4);
+  // rows of whole steps of 16-byte chunks are read as they are
+  p.pack_w = P::TERMS == 3 || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
+  const long all = up_to(V, kPad);
+  p.piece = std::max<long>(kPad, std::min({all, kXentPiece / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
+  if (!backward && !p.pack_w) p.piece = all;
+  p.pieces = (V + p.piece - 1) / p.piece;
+  p.stats_tile = tile_for<TO>(p.piece, N, true);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  p.h = take((size_t)p.d_steps * p.Np * P::ROW);
+  p.w = p.pack_w ? take((size_t)p.d_steps * p.piece * P::ROW) : 0;
+  if (!backward) {
+    const int bm = p.stats_tile == TILE_SMALL ? 128 : 256;
+    p.part = take((size_t)((V + bm - 1) / bm + p.pieces) * p.Np * sizeof(float2));
+    p.picked = take((size_t)N * 4);
+    p.rows = take((size_t)N * 4);
+  } else {
+    // dH of few tiles is split over the vocabulary, whole pieces at a time going into each split's own sums
+    const long tiles = (p.Dr + 127) / 128 * ((N + 127) / 128);
+    p.dh_splits = (int)std::max<long>(1, std::min<long>({512 / std::max<long>(1, tiles), p.piece / P::K / 8, 32}));
+    if (tile_for<TO>(D, N, false) == TILE_LARGE) p.dh_splits = 1;
+    p.ht = take((size_t)p.Np / P::K * p.Dr * P::ROW);
+    p.wt = take((size_t)p.piece / P::K * p.Dr * P::ROW);
+    p.g = take((size_t)p.piece / P::K * p.Np * P::ROW);
+    p.gt = take((size_t)p.Np / P::K * p.piece * P::ROW);
+    p.acc = take((size_t)p.dh_splits * p.Np * p.Dq * 4);
+    p.alpha = take(4);
+    p.rho = take((size_t)N * 4);
+  }
+  p.bytes = at;
+  return p;
+}
+
+template <typename TO, int EPI>
+hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStream_t st) {
+  auto go = [&](auto bm, auto bn, auto wm, auto wn) {
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+    A.m_tiles = (int)((m + BM - 1) / BM);
+    A.n_tiles = (int)((n + BN - 1) / BN);
+    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN>), dim3((unsigned)((long)A.m_tiles * A.n_tiles), splits),
+                       dim3(WM * WN * 64), 0, st, A);
+    return hipGetLastError();
+  };
+  using std::integral_constant;
+  typedef integral_constant<int, 2> c2;
+  typedef integral_constant<int, 4> c4;
+  typedef integral_constant<int, 128> c128;
+  typedef integral_constant<int, 256> c256;
+  if constexpr (EPI == XE_STATS || EPI == XE_GRAD)
+    if (tile == TILE_NARROW) return go(c256{}, integral_constant<int, Tiles<TO>::narrow_n>{}, c4{}, integral_constant<int, 1>{});
+  if (tile == TILE_SMALL) return go(c128{}, c128{}, c2{}, c2{});
+  if constexpr (sizeof(TO) == 4) return go(c256{}, c128{}, c4{}, c2{});
+  else return go(c256{}, c256{}, c2{}, c4{});
+}
+
+template <typename TO>
+hipError_t pack(const TO* src, const int* state, int rows, int D, char* dst, int R, int steps, hipStream_t st) {
+  const long threads = (long)steps * R * (XentPlan<TO>::K / 8);
+  hipLaunchKernelGGL((k_xent_pack<TO>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, src, state, rows, D, dst, R,
+                     steps);
+  return hipGetLastError();
+}
+
+template <typename TO>
+hipError_t pack_t(const TO* src, const int* state, int rows, long padded, int D, char* dst, int R, hipStream_t st) {
+  hipLaunchKernelGGL((k_xent_pack_t<TO>), dim3((unsigned)((D + 63) / 64), (unsigned)(padded / 64)), dim3(256), 0, st, src, state,
+                     rows, D, dst, R);
+  return hipGetLastError();
+}
+
+#define XENT_TRY(expr)                  \
+  do {                                  \
+    const hipError_t _e = (expr);       \
+    if (_e != hipSuccess) return _e;    \
+  } while (0)
+
+// A's operand of the products with the head: entries [v0, v0 + rows) of W, through panels where it must.
+template <typename TO>
+hipError_t head_operand(const XentPlan<TO>& p, const XentCall& c, long v0, int rows, GemmOperand* A, hipStream_t st) {
+  typedef XentPlan<TO> P;
+  const TO* w = (const TO*)c.W + v0 * c.D;
+  if (!p.pack_w) {
+    *A = {w, (long)c.D * (long)sizeof(TO), P::ROW, rows};
+    return hipSuccess;
+  }
+  *A = {c.ws + p.w, P::ROW, p.piece * P::ROW, (int)p.piece};
+  return pack<TO>(w, nullptr, rows, c.D, c.ws + p.w, (int)p.piece, p.d_steps, st);
+}
+
+}  // namespace
+
+template <typename TO>
+size_t xent_workspace(int N, int D, int V, bool backward) {
+  // (W's address decides whether it is packed: the larger plan)
+  const size_t a = plan_xent<TO>(N, D, V, nullptr, backward).bytes;
+  return std::max(a, plan_xent<TO>(N, D, V, (const void*)1, backward).bytes);
+}
+
+template <typename TO>
+hipError_t xent_forward(const XentCall& c, hipStream_t st) {
+  typedef XentPlan<TO> P;
+  const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, false);
+  float* rows = c.reduction ? (float*)(c.ws + p.rows) : c.loss;
+  float* picked = (float*)(c.ws + p.picked);
+  hipLaunchKernelGGL(k_xent_rows, dim3(1), dim3(1024), 0, st, c.target, c.N, c.V, c.ignore, c.state, picked, rows);
+  XENT_TRY(hipGetLastError());
+  XENT_TRY(pack<TO>((const TO*)c.H, c.state, c.N, c.D, c.ws + p.h, (int)p.Np, p.d_steps, st));
+  const int bm = p.stats_tile == TILE_SMALL ? 128 : 256;
+  long tiles = 0;
+  for (long v0 = 0; v0 < c.V; v0 += p.piece) {
+    const int n = (int)std::min<long>(p.piece, c.V - v0);
+    XentArgs A{};
+    XENT_TRY(head_operand<TO>(p, c, v0, n, &A.A, st));
+    A.B = {c.ws + p.h, P::ROW, p.Np * P::ROW, (int)p.Np};
+    A.steps = p.d_steps;
+    A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0;
+    A.part = (float2*)(c.ws + p.part) + tiles * p.Np;
+    A.picked = picked; A.Np = p.Np;
+    XENT_TRY((launch_gemm<TO, XE_STATS>(A, n, c.N, p.stats_tile, 1, st)));
+    tiles += (n + bm - 1) / bm;
+  }
+  hipLaunchKernelGGL((k_xent_loss<P::TERMS == 3>), dim3((c.N + 63) / 64), dim3(1024), 0, st, (const float2*)(c.ws + p.part),
+                     (int)tiles, p.Np, c.N, c.state, picked, rows);
+  XENT_TRY(hipGetLastError());
+  if (c.reduction) {
+    hipLaunchKernelGGL(k_xent_sum, dim3(1), dim3(1024), 0, st, rows, c.N, c.state, c.reduction == 1, c.loss);
+    XENT_TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+template <typename TO>
+hipError_t xent_backward(const XentCall& c, hipStream_t st) {
+  typedef XentPlan<TO> P;
+  const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, true);
+  constexpr float up = up_of<TO>();
+  float *alpha = (float*)(c.ws + p.alpha), *rho = (float*)(c.ws + p.rho);
+  hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(1024), 0, st, c.grad, c.reduction, c.state, up, alpha, rho);
+  XENT_TRY(hipGetLastError());
+  XENT_TRY(pack<TO>((const TO*)c.H, c.state, c.N, c.D, c.ws + p.h, (int)p.Np, p.d_steps, st));
+  if (c.dW) XENT_TRY(pack_t<TO>((const TO*)c.H, c.state, c.N, p.Np, c.D, c.ws + p.ht, (int)p.Dr, st));
+  for (long v0 = 0; v0 < c.V; v0 += p.piece) {
+    const int n = (int)std::min<long>(p.piece, c.V - v0);
+    const int n_steps = (int)(up_to(n, P::K) / P::K);
+    XentArgs A{};
+    XENT_TRY(head_operand<TO>(p, c, v0, n, &A.A, st));
+    A.B = {c.ws + p.h, P::ROW, p.Np * P::ROW, (int)p.Np};
+    A.steps = p.d_steps;
+    A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0; A.D = c.D;
+    A.Np = p.Np; A.Vp = p.piece;
+    A.rho = c.reduction ? nullptr : rho;
+    A.g = c.dH ? c.ws + p.g : nullptr;
+    A.gt = c.dW ? c.ws + p.gt : nullptr;
+    // (every entry of the padded piece is written: tiles of 256 or 128 entries and rows)
+    XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile_for<TO>(n, c.N, true), 1, st)));
+    A.alpha = alpha;
+    if (c.dW) {
+      XentArgs B = A;
+      B.A = {c.ws + p.ht, P::ROW, p.Dr * P::ROW, (int)p.Dr};
+      B.B = {c.ws + p.gt, P::ROW, p.piece * P::ROW, (int)p.piece};
+      B.steps = (int)(p.Np / P::K);
+      B.out = (TO*)c.dW + v0 * c.D;
+      XENT_TRY((launch_gemm<TO, XE_DW>(B, c.D, n, tile_for<TO>(c.D, n, false), 1, st)));
+    }
+    if (c.dH) {
+      XENT_TRY(pack_t<TO>((const TO*)c.W + v0 * c.D, nullptr, n, up_to(n, 64), c.D, c.ws + p.wt, (int)p.Dr, st));
+      XentArgs B = A;
+      B.A = {c.ws + p.wt, P::ROW, p.Dr * P::ROW, (int)p.Dr};
+      B.B = {c.ws + p.g, P::ROW, p.Np * P::ROW, (int)p.Np};
+      B.steps = n_steps;
+      B.steps_per_split = (int)((p.piece / P::K + p.dh_splits - 1) / p.dh_splits);
+      B.acc = (float*)(c.ws + p.acc); B.Dq = p.Dq;
+      B.add = v0 > 0;
+      XENT_TRY((launch_gemm<TO, XE_DH>(B, c.D, c.N, tile_for<TO>(c.D, c.N, false), p.dh_splits, st)));
+    }
+  }
+  if (c.dH) {
+    hipLaunchKernelGGL((k_xent_dh<TO>), dim3(c.N), dim3(256), 0, st, (const float*)(c.ws + p.acc), p.dh_splits, p.Np, p.Dq, c.D,
+                       c.state, c.target, c.ignore, alpha, (TO*)c.dH);
+    XENT_TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+}  // namespace kans

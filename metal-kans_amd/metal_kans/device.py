@@ -142,6 +142,9 @@ SIGNATURES = {
     "kans_residual_norm_workspace": (c_long, [c_long, c_int, c_long]),
     "kans_residual_norm_backward": (c_int, [c_int, c_int, c_int, P, P, P, c_long, P, P, P, c_double, c_double, P, P, P, P, P,
                                             P, c_int, P, P, P, c_long, c_int, P, c_long, P]),
+    "kans_linear_xent_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int]),
+    "kans_linear_xent_forward": (c_int, [c_int, P, P, P, c_int, c_int, c_int, c_longlong, c_int, P, P, P, c_long, P]),
+    "kans_linear_xent_backward": (c_int, [c_int, P, P, P, c_int, c_int, c_int, c_longlong, c_int, P, P, P, P, P, c_long, P]),
     "kans_mfma_ceiling": (c_int, [c_int, P, P, c_int, P]),
     "kans_stream_ceiling": (c_int, [P, c_size_t, P]),
 }

@@ -55,3 +55,24 @@ def test_residual_norm_refusals(lib):
         assert bwd(**bad) == -1, bad
     assert lib.kans_residual_norm_workspace(0, 8, 0) == 0
     assert lib.kans_residual_norm_workspace(4, 8, 0) >= 4 * (3 * 8 + 1)
+
+
+def test_linear_xent_refusals(lib):
+    def fwd(dt=0, h=64, w=64, t=64, n=4, d=8, v=10, red=1, loss=64, state=64, ws=64, size=1 << 40):
+        return lib.kans_linear_xent_forward(dt, h, w, t, n, d, v, -100, red, loss, state, ws, size, None)
+
+    def bwd(grad=64, dh=64, ws=64, size=1 << 40, n=4):
+        return lib.kans_linear_xent_backward(0, 64, 64, 64, n, 8, 10, -100, 1, 64, grad, dh, None, ws, size, None)
+    for bad in (dict(dt=3), dict(h=None), dict(w=None), dict(t=None), dict(t=68), dict(n=-1), dict(d=0), dict(v=0), dict(red=3),
+                dict(loss=None), dict(state=None), dict(state=66), dict(ws=None), dict(ws=72), dict(size=8)):
+        assert fwd(**bad) == -1, bad
+    for big in (dict(n=(1 << 22) + 1), dict(d=(1 << 16) + 1), dict(v=(1 << 24) + 1)):
+        assert fwd(**big) == -5, big
+    assert fwd(n=0) == 0 and bwd(n=0) == 0 and bwd(dh=None) == 0
+    for bad in (dict(grad=None), dict(ws=None), dict(size=8)):
+        assert bwd(**bad) == -1, bad
+    assert lib.kans_linear_xent_workspace(0, 0, 8, 10, 1) == 0
+    assert lib.kans_linear_xent_workspace(0, 4, 8, 1 << 25, 1) == -5
+    assert lib.kans_linear_xent_workspace(3, 4, 8, 10, 1) == -1
+    # no more than a piece of the vocabulary is ever held: below the logits' size
+    assert lib.kans_linear_xent_workspace(2, 16384, 4096, 131072, 0) < 16384 * 131072

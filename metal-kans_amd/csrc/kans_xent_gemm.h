@@ -8,8 +8,9 @@
 //
 // A workgroup of WAVES_M x WAVES_N waves holds a BM x BN tile.  A step's rows go from memory to LDS by DMA
 // (buffer loads, 16 bytes a lane) into one of two stages; the barrier that opens stage s + 1 stands before
-// the last part of step s, whose operands are in registers by then: the DMA of step s + 2 starts there, and the
-// first operands of step s + 1 are read while the matrix pipe works on the last of step s.  The two stages are
+// the last part of step s, whose operands are in registers by then: the first operands of step s + 1 are read
+// while the matrix pipe works on it.  The DMA of step s + 2 goes out in that part and the next one, one
+// instruction between a few products: all of them at once fill the memory pipe's queue, and the waves stand there.  The two stages are
 // separate arrays and the step loop is unrolled by two, so that the compiler sees that reads of one do not
 // depend on the DMA into the other.
 //
@@ -81,17 +82,26 @@ struct GemmTile {
     const char* pb = (const char*)B.p + (long)b0 * B.row_stride + (long)first * B.step_stride;
     // (buffer loads, not global ones: behind a global load to LDS the compiler waits for every LDS read
     // where it could wait for the older ones)
-    auto dma = [&](int s, char* st) {
-      const auto ra = resource(pa + (long)s * A.step_stride), rb = resource(pb + (long)s * B.step_stride);
-#pragma unroll
-      for (int i = 0; i < DMA_A; ++i)
+    struct Source {
+      __amdgpu_buffer_rsrc_t a, b;
+    };
+    auto source = [&](int s) {
+      return Source{resource(pa + (long)s * A.step_stride), resource(pb + (long)s * B.step_stride)};
+    };
+    auto dma1 = [&](const Source& o, char* st, int i) {  // the i-th of this wave's DMAs of a step
+      if (i < DMA_A)
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            ra, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16, off_a[i], 0, 0, 0);
-#pragma unroll
-      for (int i = 0; i < DMA_B; ++i)
+            o.a, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16, off_a[i < DMA_A ? i : 0], 0, 0, 0);
+      else
         __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rb, (__attribute__((address_space(3))) void*)(st + BM * Step::row_bytes + (i * WAVES + wave) * 1024), 16, off_b[i],
-            0, 0, 0);
+            o.b, (__attribute__((address_space(3))) void*)(st + BM * Step::row_bytes + ((i - DMA_A) * WAVES + wave) * 1024), 16,
+            off_b[i < DMA_A ? 0 : i - DMA_A], 0, 0, 0);
+    };
+    constexpr int DMAS = DMA_A + DMA_B, EACH = (DMAS + 2 * MB - 1) / (2 * MB);  // behind each of 2 MB rows of blocks
+    auto dma = [&](int s, char* st, int from, int to) {
+      const Source o = source(s);
+#pragma unroll
+      for (int i = from; i < to; ++i) dma1(o, st, i);
     };
     const int row = lane & 31, half = lane >> 5;
     auto read = [&](const char* st, int r, int part, int term) {
@@ -108,15 +118,30 @@ struct GemmTile {
         for (int j = 0; j < NB; ++j) fb[j][t] = read(st + BM * Step::row_bytes, (wn * NB + j) * 32 + row, part, t);
       }
     };
-    auto multiply = [&](const frag (&fa)[MB][TERMS], const frag (&fb)[NB][TERMS]) {
+    // the products of one part; between(i) comes before those of the i-th row of blocks
+    auto multiply = [&](const frag (&fa)[MB][TERMS], const frag (&fb)[NB][TERMS], auto between) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+      for (int i = 0; i < MB; ++i) {
+        between(i);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           if constexpr (TERMS == 3) acc[i][j] = mma_split(fa[i], fb[j], acc[i][j]);
           else acc[i][j] = Mfma<T>::mma(fa[i][0], fb[j][0], acc[i][j]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+      }
     };
+    auto dma_between = [&](bool on, int s, char* st, int from) {
+      const Source o = source(s);
+      return [=](int i) {
+        if (!on) return;
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+          if (from + i * EACH + e < DMAS) dma1(o, st, from + i * EACH + e);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+    };
+    auto nothing = [](int) {};
     constexpr int P = Step::parts;
     static_assert(P % 2 == 0, "the fragment buffers alternate");
     // step s from `cur`; `next`: another one follows (in `nxt`), `ahead`: and one behind it
@@ -125,21 +150,19 @@ struct GemmTile {
       for (int p = 0; p + 1 < P; ++p) {
         fetch(cur, p + 1, a[(p + 1) & 1], b[(p + 1) & 1]);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(a[p & 1], b[p & 1]);
-        __builtin_amdgcn_sched_barrier(0);
+        if (p == 0) multiply(a[0], b[0], dma_between(next, s + 1, nxt, MB * EACH));
+        else multiply(a[p & 1], b[p & 1], nothing);
       }
       if (next) {
         __syncthreads();  // every wave has read `cur`, and `nxt` has landed
-        if (ahead) dma(s + 2, cur);
         fetch(nxt, 0, a[0], b[0]);
         __builtin_amdgcn_sched_barrier(0);
       }
-      multiply(a[1], b[1]);
-      __builtin_amdgcn_sched_barrier(0);
+      multiply(a[1], b[1], dma_between(ahead, s + 2, cur, 0));
     };
-    dma(0, st0);
+    dma(0, st0, 0, DMAS);
     __syncthreads();
-    if (steps > 1) dma(1, st1);
+    if (steps > 1) dma(1, st1, 0, min(MB * EACH, DMAS));
     fetch(st0, 0, a[0], b[0]);
     int s = 0;
 #pragma unroll 1

@@ -32,12 +32,12 @@ template <> struct XentTypes<float> { typedef __bf16 T; static constexpr int TER
 
 template <typename T> __host__ __device__ constexpr float up_of() { return std::is_same_v<T, _Float16> ? 0x1p14f : 0x1p32f; }
 
-enum XentEpilogue { XE_STATS, XE_GRAD, XE_DW, XE_DH };
+enum XentEpilogue { XE_STATS, XE_GRAD, XE_DW, XE_DW_SPLIT, XE_DH };
 
 struct XentArgs {
   GemmOperand A, B;
   int m_tiles, n_tiles;
-  int steps, steps_per_split;  // of k; XE_DW: bounded by the compact rows as well
+  int steps, steps_per_split;  // of k; products over the rows: bounded by the compact rows as well
   const int* state;
   int N, V;                    // rows of the call; vocabulary (XE_STATS, XE_GRAD: entries of this piece)
   int v0;                      // first entry of the piece
@@ -49,52 +49,69 @@ struct XentArgs {
   const float* alpha;          // XE_DW: factor
   void* out;                   // XE_DW: dW of the piece [V][D]
   int D;
-  float* acc;                  // XE_DH: [split][Np][Dq] fp32
+  float* acc;                  // XE_DH: [split][Np][Dq] fp32; XE_DW_SPLIT: [split][Vp][Dq]
   long Dq;
   int add;                     // XE_DH: add to acc
 };
 
-// up exp(x) for a power of two up: exp2 of the rounded product, and (kExact) what the rounding left as a factor.  exp2
-// drops results below 2^-126; with up > 1 those are taken times up at once.
+// exp(x): exp2 of the rounded product, and (kExact) what the rounding left as a factor.
+constexpr float kLog2eRest = 1.925963033500e-8f;  // log2(e) - kLog2e
 template <bool kExact>
-__device__ __forceinline__ float exp_of(float x, float up = 1.0f, float log_up = 0.0f) {
+__device__ __forceinline__ float exp_of(float x) {
   const float h = x * kLog2e;
-  const bool small = log_up != 0.0f && h < -126.0f;
-  float e = __builtin_amdgcn_exp2f(small ? h + log_up : h) * (small ? 1.0f : up);
-  if (kExact) {
-    const float l = __builtin_fmaf(x, 1.925963033500e-8f, __builtin_fmaf(x, kLog2e, -h));  // log2(e) - kLog2e
-    if (h > -200.0f) e = __builtin_fmaf(e, l * 0.6931471805599453f, e);  // (x = -inf has no rest)
-  }
-  return e;
+  const float e = __builtin_amdgcn_exp2f(h);
+  if (!kExact) return e;
+  const float l = __builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, -h));
+  return h > -126.0f ? __builtin_fmaf(e, l * 0.6931471805599453f, e) : e;
 }
 
-// Four consecutive elements of G: 16-bit, or their three terms `term` bytes apart.
+// 2^log_up exp(x - at), for x - at <= 0 or so, as a function of x.  The power of two goes into the exponent, so
+// that results below 2^-126, which exp2 drops, are there.  16-bit G: one fma and exp2; the rounding of `at` and of the
+// exponent is 2^-18 of the result, far below the 2^-9 and 2^-12 of G.  fp32: what the roundings left as a factor.
+template <bool kExact>
+struct ExpUp {
+  float at, log_up;
+  __device__ __forceinline__ ExpUp(float at_, float log_up_, bool there)
+      : at(there ? (kExact ? at_ : log_up_ - at_ * kLog2e) : (kExact ? __builtin_inff() : -__builtin_inff())), log_up(log_up_) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    if (!kExact) return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, at));
+    x -= at;
+    x = x < -160.0f ? -160.0f : x;  // 0 all the same (-inf would leave a NaN as its rest); a NaN stays
+    const float h = __builtin_fmaf(x, kLog2e, log_up), e = __builtin_amdgcn_exp2f(h);
+    const float l = __builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, log_up - h));
+    return __builtin_fmaf(e, l * 0.6931471805599453f, e);
+  }
+};
+
+// 8 values as packed 16-bit pairs, or as those of their three terms.
 template <typename T, int TERMS>
-__device__ __forceinline__ void store_g(char* p, int term, const float* v) {
+__device__ __forceinline__ void pack8(const float* v, uint4 (&d)[TERMS]) {
   if constexpr (TERMS == 1) {
-    struct alignas(8) { T e[4]; } q;
+    T e[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) q.e[e] = from_f32<T>(v[e]);
-    *(uint2*)p = __builtin_bit_cast(uint2, q);
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    __builtin_memcpy(&d[0], e, 16);
   } else {
-    float w[8] = {v[0], v[1], v[2], v[3], 0.0f, 0.0f, 0.0f, 0.0f};
-    const Split8 s = split8(w);
+    const Split8 s = split8_bounded(v);  // (|v| <= 2^32, or NaN)
 #pragma unroll
-    for (int t = 0; t < 3; ++t) *(uint2*)(p + t * term) = make_uint2(s.t[t].x, s.t[t].y);
+    for (int t = 0; t < 3; ++t) d[t] = s.t[t];
   }
 }
-template <typename T, int TERMS>
-__device__ __forceinline__ void store_g1(char* p, int term, float v) {
-  if constexpr (TERMS == 1) {
-    *(T*)p = from_f32<T>(v);
-  } else {
-    const __bf16 h = (__bf16)v;
-    const float r = v - (float)h;
-    const __bf16 m = (__bf16)r;
-    *(__bf16*)p = h;
-    *(__bf16*)(p + term) = m;
-    *(__bf16*)(p + 2 * term) = (__bf16)(r - (float)m);
-  }
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+
+// A quad of lanes (columns n .. n + 3) with four 16-bit rows each, transposed: lane l of the quad gets the four columns
+// of row 2 (l & 1) + (l >> 1).
+__device__ __forceinline__ uint2 quad_transpose(unsigned r01, unsigned r23, int lane) {
+  const bool odd = lane & 1, two = lane & 2;
+  const unsigned other = dpp<0xb1>(odd ? r01 : r23), own = odd ? r23 : r01;  // lane ^ 1
+  const unsigned lo = odd ? other : own, hi = odd ? own : other;
+  const unsigned a = __builtin_amdgcn_perm(hi, lo, 0x05040100), b = __builtin_amdgcn_perm(hi, lo, 0x07060302);
+  const unsigned far = dpp<0x4e>(two ? a : b);  // lane ^ 2
+  return two ? make_uint2(far, b) : make_uint2(a, far);
 }
 
 template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N>
@@ -111,10 +128,11 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   const int m0 = mt * BM, n0 = nt * BN;
   const int count = A.state[0];  // compact rows
   // (G of the rows that fill up the last step of k is written too: zeros)
-  if (EPI != XE_DW && n0 >= (EPI == XE_GRAD ? (count + 63) / 64 * 64 : count)) return;
+  constexpr bool kOverRows = EPI == XE_DW || EPI == XE_DW_SPLIT;
+  if (!kOverRows && n0 >= (EPI == XE_GRAD ? (count + 63) / 64 * 64 : count)) return;
   int first = 0, steps = A.steps;
-  if (EPI == XE_DW) steps = min(steps, (count + Step::kStep - 1) / Step::kStep);
-  if (EPI == XE_DH) {
+  if (kOverRows) steps = min(steps, (count + Step::kStep - 1) / Step::kStep);
+  if (EPI == XE_DH || EPI == XE_DW_SPLIT) {
     first = blockIdx.y * A.steps_per_split;
     steps = min(A.steps_per_split, steps - first);
   }
@@ -178,31 +196,59 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     }
   } else if constexpr (EPI == XE_GRAD) {
     constexpr float kUp = up_of<TO>(), kLogUp = std::is_same_v<TO, _Float16> ? 14.0f : 32.0f;
+    constexpr int K = Step::kStep;
     const int* target = A.state + kXentHead + A.N;
     const float* lse = (const float*)(target + A.N);
+    if (m0 + BM > A.V) {
+#pragma unroll
+      for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (mrow(i, r) >= A.V) acc[i][j][r] = kNoLogit;
+    }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int n = ncol(j);
       const bool there = n < count;
-      const float at = there ? lse[n] : 0.0f, rho = there && A.rho ? A.rho[n] : 1.0f;
+      const ExpUp<TERMS == 3> exp_up(there ? lse[n] : 0.0f, kLogUp, there);
+      const float rho = there && A.rho ? A.rho[n] : 1.0f;
       const int t = there ? target[n] - A.v0 : -1;
 #pragma unroll
       for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int m = mrow(i, 4 * q);
-          float v[4];
+        for (int q = 0; q < 4; q += 2) {
+          const int m = mrow(i, 4 * q);  // values 0 .. 3 are its rows, 4 .. 7 those 8 further on
+          float v[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float p = exp_of<TERMS == 3>(acc[i][j][4 * q + e] - at, kUp, kLogUp) - (m + e == t ? kUp : 0.0f);
-            v[e] = there && m + e < A.V ? p * rho : 0.0f;
+          for (int e = 0; e < 8; ++e) v[e] = exp_up(acc[i][j][4 * q + e]) * rho;
+          const int own = t - m;
+          if (__builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4))) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= own == e % 4 + e / 4 * 8 ? kUp * rho : 0.0f;
           }
-          constexpr int K = Step::kStep;
-          if (A.g) store_g<T, TERMS>(A.g + ((long)(m / K) * A.Np + n) * Step::row_bytes + m % K * 2, K * 2, v);
-          if (A.gt) {
+          uint4 d[TERMS];
+          pack8<T, TERMS>(v, d);
+          if (A.g) {
+            // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
+            const int m8 = m - 4 * half + 8 * half;
+            char* o = A.g + ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              store_g1<T, TERMS>(A.gt + ((long)(n / K) * A.Vp + m + e) * Step::row_bytes + n % K * 2, K * 2, v[e]);
+            for (int c = 0; c < TERMS; ++c) {
+              const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
+              const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
+              *(uint4*)(o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+            }
+          }
+          if (A.gt) {
+            const int mt4 = m + 2 * (lane & 1) + (lane >> 1 & 1), n4 = n - (lane & 3);
+            char* o = A.gt + ((long)(n / K) * A.Vp + mt4) * Step::row_bytes + n4 % K * 2;
+#pragma unroll
+            for (int c = 0; c < TERMS; ++c) {
+              *(uint2*)(o + c * K * 2) = quad_transpose(d[c].x, d[c].y, lane);
+              *(uint2*)(o + c * K * 2 + 8 * Step::row_bytes) = quad_transpose(d[c].z, d[c].w, lane);
+            }
           }
         }
     }
@@ -231,7 +277,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
         }
     }
   } else {
-    float* base = A.acc + (long)blockIdx.y * A.Np * A.Dq;
+    float* base = A.acc + (long)blockIdx.y * (EPI == XE_DH ? A.Np : A.Vp) * A.Dq;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       float* o = base + (long)ncol(j) * A.Dq;
@@ -449,24 +495,16 @@ __global__ __launch_bounds__(1024) void k_xent_scale(const float* __restrict__ g
   for (int n = threadIdx.x; n < count; n += 1024) rho[n] = grad[state[kXentHead + n]] / by;
 }
 
-// dH: the splits' sums times alpha in the rows' own places, zeros for the ignored rows.
+// The splits' sums of one row times alpha, in the inputs' type.
 template <typename TO>
-__global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, int splits, long Np, long Dq, int D,
-                                                 const int* __restrict__ state, const int64_t* __restrict__ target,
-                                                 int64_t ignore, const float* __restrict__ alpha, TO* __restrict__ dH) {
-  const int row = blockIdx.x;
-  if (target[row] == ignore)
-    for (int d = threadIdx.x; d < D; d += 256) dH[(long)row * D + d] = (TO)0.0f;
-  if (row >= state[0]) return;
-  const float a = *alpha;
-  TO* o = dH + (long)state[kXentHead + row] * D;
+__device__ __forceinline__ void finish_row(const float* acc, int splits, long stride, int D, float alpha, TO* o) {
   for (int d = threadIdx.x * 4; d < D; d += 1024) {
-    float4 s = *(const float4*)(acc + (long)row * Dq + d);
+    float4 s = *(const float4*)(acc + d);
     for (int k = 1; k < splits; ++k) {
-      const float4 x = *(const float4*)(acc + ((long)k * Np + row) * Dq + d);
+      const float4 x = *(const float4*)(acc + k * stride + d);
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
-    const float v[4] = {s.x * a, s.y * a, s.z * a, s.w * a};
+    const float v[4] = {s.x * alpha, s.y * alpha, s.z * alpha, s.w * alpha};
     TO e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = from_f32<TO>(v[i]);
@@ -480,21 +518,69 @@ __global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, 
   }
 }
 
+// dH: compact rows into their own places, zeros for the ignored rows.
+template <typename TO>
+__global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, int splits, long Np, long Dq, int D,
+                                                 const int* __restrict__ state, const int64_t* __restrict__ target,
+                                                 int64_t ignore, const float* __restrict__ alpha, TO* __restrict__ dH) {
+  const int row = blockIdx.x;
+  if (target[row] == ignore)
+    for (int d = threadIdx.x; d < D; d += 256) dH[(long)row * D + d] = (TO)0.0f;
+  if (row >= state[0]) return;
+  finish_row(acc + row * Dq, splits, Np * Dq, D, *alpha, dH + (long)state[kXentHead + row] * D);
+}
+
+template <typename TO>
+__global__ __launch_bounds__(256) void k_xent_dw(const float* __restrict__ acc, int splits, long Vp, long Dq, int D,
+                                                 const float* __restrict__ alpha, TO* __restrict__ dW) {
+  finish_row(acc + (long)blockIdx.x * Dq, splits, Vp * Dq, D, *alpha, dW + (long)blockIdx.x * D);
+}
+
 // ---- plans ----------------------------------------------------------------------------------------------
 inline long up_to(long v, long m) { return (v + m - 1) / m * m; }
 
-// Tiles of a product: the large one where its tiles fill most of the CUs, else the small one; few rows get a narrow one.
+// Tiles of a product: the large one or the small one (128 x 128); few rows get a narrow one.
 enum { TILE_LARGE, TILE_SMALL, TILE_NARROW };
 template <typename TO> struct Tiles;
-template <> struct Tiles<float> { static constexpr int large_m = 256, large_n = 128, narrow_n = 64; };
-template <> struct Tiles<_Float16> { static constexpr int large_m = 256, large_n = 256, narrow_n = 32; };
-template <> struct Tiles<__bf16> { static constexpr int large_m = 256, large_n = 256, narrow_n = 32; };
+// small_cost: time of a step of as many small tiles as a CU holds, in steps of a large tile.  Measured: 16-bit tiles
+// of 128 x 128, two a CU, reach 3/4 of the rate of one of 256 x 256; fp32 (98 KB of LDS, one a CU) 2/3 of that of 256 x 128.
+template <> struct Tiles<float> {
+  static constexpr int large_m = 256, large_n = 128, narrow_n = 64, small_per_cu = 1;
+  static constexpr double small_cost = 0.7;
+};
+template <> struct Tiles<_Float16> {
+  static constexpr int large_m = 256, large_n = 256, narrow_n = 32, small_per_cu = 2;
+  static constexpr double small_cost = 0.65;
+};
+template <> struct Tiles<__bf16> : Tiles<_Float16> {};
 
+struct SplitTile {
+  int tile, splits;
+};
+// The tile, and the splits of the `steps` steps of k (up to max_splits, none below 4 steps), that take the
+// least time by this estimate: rounds of workgroups over the 256 CUs times the steps of one, and about 6 steps' time for
+// the beginning and the end of each (a split's sums are written and read again: as long once more).
 template <typename TO>
-int tile_for(long m, long n, bool narrow) {
-  if (narrow && n <= Tiles<TO>::narrow_n) return TILE_NARROW;
-  const long large = (m + Tiles<TO>::large_m - 1) / Tiles<TO>::large_m * ((n + Tiles<TO>::large_n - 1) / Tiles<TO>::large_n);
-  return large >= 192 ? TILE_LARGE : TILE_SMALL;
+SplitTile split_tile(long m, long n, long steps, int max_splits) {
+  SplitTile best{TILE_LARGE, 1};
+  double least = 1e300;
+  for (int tile : {TILE_LARGE, TILE_SMALL}) {
+    const long bm = tile == TILE_LARGE ? Tiles<TO>::large_m : 128, bn = tile == TILE_LARGE ? Tiles<TO>::large_n : 128;
+    const long tiles = (m + bm - 1) / bm * ((n + bn - 1) / bn), slots = 256 * (tile == TILE_LARGE ? 1 : Tiles<TO>::small_per_cu);
+    for (int s = 1; s <= max_splits && (s == 1 || steps / s >= 4); ++s) {
+      const double rounds = (double)((tiles * s + slots - 1) / slots);
+      const double time = rounds * (double)((steps + s - 1) / s + (s > 1 ? 12 : 6)) * (tile == TILE_LARGE ? 1.0 : Tiles<TO>::small_cost);
+      if (time < least) {
+        least = time;
+        best = {tile, s};
+      }
+    }
+  }
+  return best;
+}
+template <typename TO>
+int tile_for(long m, long n, long steps) {
+  return n <= Tiles<TO>::narrow_n ? (int)TILE_NARROW : split_tile<TO>(m, n, steps, 1).tile;
 }
 
 template <typename TO>
@@ -505,9 +591,10 @@ struct XentPlan {
   int d_steps;
   bool pack_w;             // W goes through panels
   long piece, pieces;      // vocabulary of a piece (a multiple of kPad) and how many
-  int stats_tile, dh_splits;
+  int stats_tile;
+  SplitTile dh, dw;        // dw in splits only where the vocabulary is one piece
   // offsets into the workspace
-  size_t h, w, part, picked, rows, ht, wt, g, gt, acc, alpha, rho, bytes;
+  size_t h, w, part, picked, rows, ht, wt, g, gt, acc, acc_w, alpha, rho, bytes;
 };
 
 template <typename TO>
@@ -525,7 +612,8 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   p.piece = std::max<long>(kPad, std::min({all, kXentPiece / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
   if (!backward && !p.pack_w) p.piece = all;
   p.pieces = (V + p.piece - 1) / p.piece;
-  p.stats_tile = tile_for<TO>(p.piece, N, true);
+  p.piece = up_to((V + p.pieces - 1) / p.pieces, kPad);
+  p.stats_tile = tile_for<TO>(std::min<long>(V, p.piece), N, p.d_steps);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
@@ -540,15 +628,14 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
     p.picked = take((size_t)N * 4);
     p.rows = take((size_t)N * 4);
   } else {
-    // dH of few tiles is split over the vocabulary, whole pieces at a time going into each split's own sums
-    const long tiles = (p.Dr + 127) / 128 * ((N + 127) / 128);
-    p.dh_splits = (int)std::max<long>(1, std::min<long>({512 / std::max<long>(1, tiles), p.piece / P::K / 8, 32}));
-    if (tile_for<TO>(D, N, false) == TILE_LARGE) p.dh_splits = 1;
+    p.dh = split_tile<TO>(D, N, std::min<long>(V, p.piece) / P::K, 32);
+    p.dw = split_tile<TO>(D, std::min<long>(V, p.piece), p.Np / P::K, p.pieces > 1 ? 1 : 32);
     p.ht = take((size_t)p.Np / P::K * p.Dr * P::ROW);
     p.wt = take((size_t)p.piece / P::K * p.Dr * P::ROW);
     p.g = take((size_t)p.piece / P::K * p.Np * P::ROW);
     p.gt = take((size_t)p.Np / P::K * p.piece * P::ROW);
-    p.acc = take((size_t)p.dh_splits * p.Np * p.Dq * 4);
+    p.acc = take((size_t)p.dh.splits * p.Np * p.Dq * 4);
+    p.acc_w = p.dw.splits > 1 ? take((size_t)p.dw.splits * p.piece * p.Dq * 4) : 0;
     p.alpha = take(4);
     p.rho = take((size_t)N * 4);
   }
@@ -677,7 +764,7 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     A.g = c.dH ? c.ws + p.g : nullptr;
     A.gt = c.dW ? c.ws + p.gt : nullptr;
     // (every entry of the padded piece is written: tiles of 256 or 128 entries and rows)
-    XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile_for<TO>(n, c.N, true), 1, st)));
+    XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile_for<TO>(n, c.N, p.d_steps), 1, st)));
     A.alpha = alpha;
     if (c.dW) {
       XentArgs B = A;
@@ -685,7 +772,15 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
       B.B = {c.ws + p.gt, P::ROW, p.piece * P::ROW, (int)p.piece};
       B.steps = (int)(p.Np / P::K);
       B.out = (TO*)c.dW + v0 * c.D;
-      XENT_TRY((launch_gemm<TO, XE_DW>(B, c.D, n, tile_for<TO>(c.D, n, false), 1, st)));
+      if (p.dw.splits == 1) {
+        XENT_TRY((launch_gemm<TO, XE_DW>(B, c.D, n, p.dw.tile, 1, st)));
+      } else {
+        B.acc = (float*)(c.ws + p.acc_w); B.Dq = p.Dq;
+        B.steps_per_split = (B.steps + p.dw.splits - 1) / p.dw.splits;
+        XENT_TRY((launch_gemm<TO, XE_DW_SPLIT>(B, c.D, n, p.dw.tile, p.dw.splits, st)));
+        hipLaunchKernelGGL((k_xent_dw<TO>), dim3(n), dim3(256), 0, st, B.acc, p.dw.splits, p.piece, p.Dq, c.D, alpha, (TO*)c.dW);
+        XENT_TRY(hipGetLastError());
+      }
     }
     if (c.dH) {
       XENT_TRY(pack_t<TO>((const TO*)c.W + v0 * c.D, nullptr, n, up_to(n, 64), c.D, c.ws + p.wt, (int)p.Dr, st));
@@ -693,14 +788,14 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
       B.A = {c.ws + p.wt, P::ROW, p.Dr * P::ROW, (int)p.Dr};
       B.B = {c.ws + p.g, P::ROW, p.Np * P::ROW, (int)p.Np};
       B.steps = n_steps;
-      B.steps_per_split = (int)((p.piece / P::K + p.dh_splits - 1) / p.dh_splits);
+      B.steps_per_split = (n_steps + p.dh.splits - 1) / p.dh.splits;
       B.acc = (float*)(c.ws + p.acc); B.Dq = p.Dq;
       B.add = v0 > 0;
-      XENT_TRY((launch_gemm<TO, XE_DH>(B, c.D, c.N, tile_for<TO>(c.D, c.N, false), p.dh_splits, st)));
+      XENT_TRY((launch_gemm<TO, XE_DH>(B, c.D, c.N, p.dh.tile, p.dh.splits, st)));
     }
   }
   if (c.dH) {
-    hipLaunchKernelGGL((k_xent_dh<TO>), dim3(c.N), dim3(256), 0, st, (const float*)(c.ws + p.acc), p.dh_splits, p.Np, p.Dq, c.D,
+    hipLaunchKernelGGL((k_xent_dh<TO>), dim3(c.N), dim3(256), 0, st, (const float*)(c.ws + p.acc), p.dh.splits, p.Np, p.Dq, c.D,
                        c.state, c.target, c.ignore, alpha, (TO*)c.dH);
     XENT_TRY(hipGetLastError());
   }

@@ -328,42 +328,42 @@ __device__ __forceinline__ void store8(char* p, int term, const float* v) {
   }
 }
 
-// Panels [step of D][R rows][kStep] of `rows` rows of a matrix [.][D], padded with zeros.  With `state`
-// the rows are the compact ones (`rows` bounds their number) and rows behind the last 256 that hold one stay as they are.
-template <typename TO>
-__global__ __launch_bounds__(256) void k_xent_pack(const TO* __restrict__ src, const int* __restrict__ state, int rows, int D,
-                                                   char* __restrict__ dst, int R, int steps) {
-  typedef typename XentTypes<TO>::T T;
-  constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep, C = K / 8;
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  const int chunk = (int)(i % C);
-  const long rs = i / C;
-  const int row = (int)(rs % R), step = (int)(rs / R);
-  if (step >= steps) return;
-  if (state) {
-    rows = min(rows, state[0]);
-    if (row >= (rows + kPad - 1) / kPad * kPad) return;
-  }
-  float v[8];
-  if (row < rows) {
-    row8(src + (long)(state ? state[kXentHead + row] : row) * D, step * K + chunk * 8, D, v);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-  }
-  store8<T, TERMS>(dst + ((long)step * R + row) * StepOf<TERMS>::row_bytes + chunk * 16, K * 2, v);
-}
+// A matrix [.][D] laid out for the products: panels [step of D][R][kStep] of its rows (dst), and panels
+// [step of the rows][Rt][kStep] of its columns (dst_t); either may be null.  `padded` rows (a multiple of 64) are
+// written, zeros behind the last.  With `state` the rows are the compact ones (`rows` bounds their number) and
+// rows behind the last kPad that hold one stay as they are.
+struct XentLayout {
+  const void* src;
+  const int* state;
+  int rows, padded, D, steps, R, Rt;
+  char *dst, *dst_t;
+  int blocks;  // tiles of 64 x 64
+};
 
-// Panels [step of the rows][R][kStep] of the transpose: 64 rows x 64 columns a workgroup, by way of LDS.
+// What the products need before they start, in one launch: block 0 numbers the rows, the next one makes the
+// common factor of G, the others lay out H and a piece of W.
+struct XentBegin {
+  XentLayout m[2];
+  int number_rows, make_scale;
+  const int64_t* target;
+  int N, V;
+  int64_t ignore;
+  int* state;
+  float *picked, *loss;        // cleared with the numbering: what the products may not write
+  const float* grad;
+  int reduction;
+  float up;
+  float *alpha, *rho;
+};
+
 template <typename TO>
-__global__ __launch_bounds__(256) void k_xent_pack_t(const TO* __restrict__ src, const int* __restrict__ state, int rows, int D,
-                                                     char* __restrict__ dst, int R) {
+__device__ __forceinline__ void lay_out(const XentLayout& L, int block, float (*tile)[65]) {
   typedef typename XentTypes<TO>::T T;
   constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
-  __shared__ float tile[64][65];
-  const int d0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-  if (state) {
-    rows = min(rows, state[0]);
+  const int across = (L.D + 63) / 64, r0 = block / across * 64, d0 = block % across * 64;
+  int rows = L.rows;
+  if (L.state) {
+    rows = min(rows, L.state[0]);
     if (r0 >= (rows + kPad - 1) / kPad * kPad) return;
   }
 #pragma unroll
@@ -371,14 +371,20 @@ __global__ __launch_bounds__(256) void k_xent_pack_t(const TO* __restrict__ src,
     const int r = threadIdx.x / 8 + i * 32, c = threadIdx.x % 8 * 8;
     float v[8];
     if (r0 + r < rows) {
-      row8(src + (long)(state ? state[kXentHead + r0 + r] : r0 + r) * D, d0 + c, D, v);
+      row8((const TO*)L.src + (long)(L.state ? L.state[kXentHead + r0 + r] : r0 + r) * L.D, d0 + c, L.D, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.0f;
     }
+    const int step = (d0 + c) / K;
+    if (L.dst && step < L.steps)
+      store8<T, TERMS>(L.dst + ((long)step * L.R + r0 + r) * StepOf<TERMS>::row_bytes + (d0 + c) % K * 2, K * 2, v);
+    if (L.dst_t) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) tile[r][c + e] = v[e];
+      for (int e = 0; e < 8; ++e) tile[r][c + e] = v[e];
+    }
   }
+  if (!L.dst_t) return;
   __syncthreads();
   const int d = threadIdx.x / 4;
 #pragma unroll
@@ -387,74 +393,93 @@ __global__ __launch_bounds__(256) void k_xent_pack_t(const TO* __restrict__ src,
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = tile[r + e][d];
-    store8<T, TERMS>(dst + ((long)((r0 + r) / K) * R + d0 + d) * StepOf<TERMS>::row_bytes + r % K * 2, K * 2, v);
+    store8<T, TERMS>(L.dst_t + ((long)((r0 + r) / K) * L.Rt + d0 + d) * StepOf<TERMS>::row_bytes + r % K * 2, K * 2, v);
   }
 }
 
-// ---- the ends ------------------------------------------------------------------------------------------
-// Numbers the rows that count, in their order, and clears what the products may not write.
-__global__ __launch_bounds__(1024) void k_xent_rows(const int64_t* __restrict__ target, int N, int V, int64_t ignore,
-                                                    int* __restrict__ state, float* __restrict__ picked,
-                                                    float* __restrict__ loss) {
-  __shared__ int waves[16];
+// Numbers the rows that count, in their order, four to a thread.
+__device__ __forceinline__ void number_rows(const XentBegin& A, int* waves) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
-  for (int r0 = 0; r0 < N; r0 += 1024) {
-    const int r = r0 + threadIdx.x;
-    const int64_t t = r < N ? target[r] : ignore;
-    const bool in = r < N && t != ignore;
-    const unsigned long long mask = __builtin_amdgcn_ballot_w64(in);
-    if (lane == 0) waves[wave] = __builtin_popcountll(mask);
+  for (int r0 = 0; r0 < A.N; r0 += 1024) {
+    const int r = r0 + threadIdx.x * 4;
+    int64_t t[4];
+    bool in[4];
+    int at = 0, all = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      t[e] = r + e < A.N ? A.target[r + e] : A.ignore;
+      in[e] = t[e] != A.ignore;
+      const unsigned long long mask = __builtin_amdgcn_ballot_w64(in[e]);
+      at += __builtin_popcountll(mask & ((1ull << lane) - 1));
+      all += __builtin_popcountll(mask);
+    }
+    if (lane == 0) waves[wave] = all;
     __syncthreads();
-    int at = base + __builtin_popcountll(mask & ((1ull << lane) - 1));
-    for (int w = 0; w < 16; ++w) {
+    at += base;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
       at += w < wave ? waves[w] : 0;
       base += waves[w];
     }
-    if (in) {
-      state[kXentHead + at] = r;
-      state[kXentHead + N + at] = t >= 0 && t < V ? (int)t : -1;
-    }
-    if (r < N) {
-      picked[r] = __builtin_nanf("");  // of a target outside the vocabulary
-      loss[r] = 0.0f;                  // of an ignored row
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (in[e]) {
+        A.state[kXentHead + at] = r + e;
+        A.state[kXentHead + A.N + at] = t[e] >= 0 && t[e] < A.V ? (int)t[e] : -1;
+        ++at;
+      }
+      if (r + e < A.N) {
+        A.picked[r + e] = __builtin_nanf("");  // of a target outside the vocabulary
+        A.loss[r + e] = 0.0f;                  // of an ignored row
+      }
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) state[0] = base;
+  if (threadIdx.x == 0) A.state[0] = base;
 }
 
-// Joins the tiles' sums: 64 rows a workgroup, 16 runs of tiles.
-template <bool kExact>
-__global__ __launch_bounds__(1024) void k_xent_loss(const float2* __restrict__ part, int tiles, long Np, int N,
-                                                    int* __restrict__ state, const float* __restrict__ picked,
-                                                    float* __restrict__ loss) {
-  __shared__ float2 join[16][64];
-  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
-  const int n = blockIdx.x * 64 + lane, count = state[0];
-  if ((int)blockIdx.x * 64 >= count) return;
-  float top = kNoLogit, sum = 0.0f;
-  auto add = [&](float2 o) {
-    const float both = fmaxf(top, o.x), at = both == kNoLogit ? 0.0f : both;
-    sum = sum * exp_of<kExact>(top - at) + o.y * exp_of<kExact>(o.x - at);
-    top = both;
-  };
-#pragma unroll 4
-  for (int t = run; t < tiles; t += 16) add(part[(long)t * Np + n]);
-  join[run][lane] = make_float2(top, sum);
+// The factor common to all rows of G (up: the scale that G is stored with) and each row's share of it.
+__device__ __forceinline__ void make_scale(const XentBegin& A, float* join) {
+  const int count = A.state[0];
+  if (A.reduction != 0) {
+    if (threadIdx.x == 0) *A.alpha = count == 0 ? 0.0f : (A.reduction == 1 ? *A.grad / (float)count : *A.grad) / A.up;
+    return;
+  }
+  float top = 0.0f;
+  bool bad = false;
+  for (int n = threadIdx.x; n < count; n += 256) {
+    const float g = __builtin_fabsf(A.grad[A.state[kXentHead + n]]);
+    bad |= !(g < __builtin_inff());
+    top = fmaxf(top, g);
+  }
+  join[threadIdx.x] = bad ? __builtin_inff() : top;
   __syncthreads();
-  if (run != 0 || n >= count) return;
-  for (int r = 1; r < 16; ++r) add(join[r][lane]);
-  const bool known = state[kXentHead + N + n] >= 0;
-  const float lse = known ? top + __builtin_logf(sum) : __builtin_nanf("");
-  ((float*)state)[kXentHead + 2 * N + n] = lse;
-  loss[state[kXentHead + n]] = lse - picked[n];
+  for (int d = 128; d > 0; d >>= 1) {
+    if ((int)threadIdx.x < d) join[threadIdx.x] = fmaxf(join[threadIdx.x], join[threadIdx.x + d]);
+    __syncthreads();
+  }
+  // (an infinite or NaN gradient: as it is, without a common factor)
+  top = join[0];
+  const float by = top > 0.0f && top < __builtin_inff() ? top : 1.0f;
+  if (threadIdx.x == 0) *A.alpha = by / A.up;
+  for (int n = threadIdx.x; n < count; n += 256) A.rho[n] = A.grad[A.state[kXentHead + n]] / by;
 }
 
-// The sum of the rows' losses, or their mean over the rows that count.
-__global__ __launch_bounds__(1024) void k_xent_sum(const float* __restrict__ rows, int N, const int* __restrict__ state, int mean,
-                                                   float* __restrict__ out) {
-  __shared__ float join[1024];
+template <typename TO>
+__global__ __launch_bounds__(256) void k_xent_begin(const XentBegin A) {
+  __shared__ float tile[64][65];
+  int block = blockIdx.x;
+  if (A.number_rows && block-- == 0) return number_rows(A, (int*)tile);
+  if (A.make_scale && block-- == 0) return make_scale(A, &tile[0][0]);
+  const bool second = block >= A.m[0].blocks;
+  lay_out<TO>(A.m[second], second ? block - A.m[0].blocks : block, tile);
+}
+
+// ---- the ends ------------------------------------------------------------------------------------------
+// Joins the tiles' sums: 64 rows at a time, 16 runs of tiles.  With `out` (one workgroup): the sum of the rows'
+// losses, or their mean over the rows that count.
+__device__ __forceinline__ void sum_rows(const float* rows, int N, int count, int mean, float* join, float* out) {
   float s = 0.0f;
   for (int r = threadIdx.x; r < N; r += 1024) s += rows[r];
   join[threadIdx.x] = s;
@@ -463,36 +488,42 @@ __global__ __launch_bounds__(1024) void k_xent_sum(const float* __restrict__ row
     if ((int)threadIdx.x < d) join[threadIdx.x] += join[threadIdx.x + d];
     __syncthreads();
   }
-  if (threadIdx.x == 0) *out = mean ? join[0] / (float)state[0] : join[0];
+  if (threadIdx.x == 0) *out = mean ? join[0] / (float)count : join[0];
 }
 
-// The factor common to all rows of G (up: the scale that G is stored with) and each row's share of it.
-__global__ __launch_bounds__(1024) void k_xent_scale(const float* __restrict__ grad, int reduction, const int* __restrict__ state,
-                                                     float up, float* __restrict__ alpha, float* __restrict__ rho) {
-  __shared__ float join[1024];
-  const int count = state[0];
-  if (reduction != 0) {
-    if (threadIdx.x == 0) *alpha = count == 0 ? 0.0f : (reduction == 1 ? *grad / (float)count : *grad) / up;
-    return;
-  }
-  float top = 0.0f;
-  bool bad = false;
-  for (int n = threadIdx.x; n < count; n += 1024) {
-    const float g = __builtin_fabsf(grad[state[kXentHead + n]]);
-    bad |= !(g < __builtin_inff());
-    top = fmaxf(top, g);
-  }
-  join[threadIdx.x] = bad ? __builtin_inff() : top;
-  __syncthreads();
-  for (int d = 512; d > 0; d >>= 1) {
-    if ((int)threadIdx.x < d) join[threadIdx.x] = fmaxf(join[threadIdx.x], join[threadIdx.x + d]);
+template <bool kExact>
+__global__ __launch_bounds__(1024) void k_xent_loss(const float2* __restrict__ part, int tiles, long Np, int N, int* state,
+                                                    const float* __restrict__ picked, float* loss, int mean, float* out) {
+  __shared__ float2 join[16][64];
+  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, count = state[0];
+  for (int n0 = blockIdx.x * 64; n0 < count; n0 += gridDim.x * 64) {
+    const int n = n0 + lane;
+    float top = kNoLogit, sum = 0.0f;
+    auto add = [&](float2 o) {
+      const float both = fmaxf(top, o.x), at = both == kNoLogit ? 0.0f : both;
+      sum = sum * exp_of<kExact>(top - at) + o.y * exp_of<kExact>(o.x - at);
+      top = both;
+    };
+#pragma unroll 4
+    for (int t = run; t < tiles; t += 16) add(part[(long)t * Np + n]);
+    join[run][lane] = make_float2(top, sum);
+    __syncthreads();
+    if (run == 0 && n < count) {
+      for (int r = 1; r < 16; ++r) add(join[r][lane]);
+      const bool known = state[kXentHead + N + n] >= 0;
+      const float lse = known ? top + __builtin_logf(sum) : __builtin_nanf("");
+      ((float*)state)[kXentHead + 2 * N + n] = lse;
+      loss[state[kXentHead + n]] = lse - picked[n];
+    }
     __syncthreads();
   }
-  // (an infinite or NaN gradient: as it is, without a common factor)
-  top = join[0];
-  const float by = top > 0.0f && top < __builtin_inff() ? top : 1.0f;
-  if (threadIdx.x == 0) *alpha = by / up;
-  for (int n = threadIdx.x; n < count; n += 1024) rho[n] = grad[state[kXentHead + n]] / by;
+  if (out) sum_rows(loss, N, count, mean, (float*)join, out);
+}
+
+__global__ __launch_bounds__(1024) void k_xent_sum(const float* __restrict__ rows, int N, const int* __restrict__ state, int mean,
+                                                   float* __restrict__ out) {
+  __shared__ float join[1024];
+  sum_rows(rows, N, state[0], mean, join, out);
 }
 
 // The splits' sums of one row times alpha, in the inputs' type.
@@ -539,18 +570,22 @@ __global__ __launch_bounds__(256) void k_xent_dw(const float* __restrict__ acc, 
 // ---- plans ----------------------------------------------------------------------------------------------
 inline long up_to(long v, long m) { return (v + m - 1) / m * m; }
 
-// Tiles of a product: the large one or the small one (128 x 128); few rows get a narrow one.
-enum { TILE_LARGE, TILE_SMALL, TILE_NARROW };
+// Tiles of a product: the large one, the small one (128 x 128) or the tiny one (64 x 64); few rows get a narrow one.
+enum { TILE_LARGE, TILE_SMALL, TILE_TINY, TILE_NARROW };
+constexpr int tile_rows(int tile) { return tile == TILE_SMALL ? 128 : tile == TILE_TINY ? 64 : 256; }
 template <typename TO> struct Tiles;
-// small_cost: time of a step of as many small tiles as a CU holds, in steps of a large tile.  Measured: 16-bit tiles
-// of 128 x 128, two a CU, reach 3/4 of the rate of one of 256 x 256; fp32 (98 KB of LDS, one a CU) 2/3 of that of 256 x 128.
+// per_cu, cost: small and tiny tiles that a CU holds at a time, and the time of a step of that many, in steps of a
+// large tile.  Measured: 16-bit tiles of 128 x 128, two a CU, reach 3/4 of the rate of one of 256 x 256; fp32 (98 KB of
+// LDS, one a CU) 2/3 of that of 256 x 128.  Tiny tiles read LDS twice as often a product, at about half the rate.
 template <> struct Tiles<float> {
-  static constexpr int large_m = 256, large_n = 128, narrow_n = 64, small_per_cu = 1;
-  static constexpr double small_cost = 0.7;
+  static constexpr int large_m = 256, large_n = 128, narrow_n = 64;
+  static constexpr int per_cu[3] = {1, 1, 3};
+  static constexpr double cost[3] = {1.0, 0.7, 0.6};
 };
 template <> struct Tiles<_Float16> {
-  static constexpr int large_m = 256, large_n = 256, narrow_n = 32, small_per_cu = 2;
-  static constexpr double small_cost = 0.65;
+  static constexpr int large_m = 256, large_n = 256, narrow_n = 32;
+  static constexpr int per_cu[3] = {1, 2, 5};
+  static constexpr double cost[3] = {1.0, 0.65, 0.7};
 };
 template <> struct Tiles<__bf16> : Tiles<_Float16> {};
 
@@ -564,12 +599,14 @@ template <typename TO>
 SplitTile split_tile(long m, long n, long steps, int max_splits) {
   SplitTile best{TILE_LARGE, 1};
   double least = 1e300;
-  for (int tile : {TILE_LARGE, TILE_SMALL}) {
-    const long bm = tile == TILE_LARGE ? Tiles<TO>::large_m : 128, bn = tile == TILE_LARGE ? Tiles<TO>::large_n : 128;
-    const long tiles = (m + bm - 1) / bm * ((n + bn - 1) / bn), slots = 256 * (tile == TILE_LARGE ? 1 : Tiles<TO>::small_per_cu);
+  for (int tile : {TILE_LARGE, TILE_SMALL, TILE_TINY}) {
+    const long bm = tile_rows(tile), bn = tile == TILE_LARGE ? Tiles<TO>::large_n : bm;
+    const long tiles = (m + bm - 1) / bm * ((n + bn - 1) / bn), slots = 256 * Tiles<TO>::per_cu[tile];
     for (int s = 1; s <= max_splits && (s == 1 || steps / s >= 4); ++s) {
-      const double rounds = (double)((tiles * s + slots - 1) / slots);
-      const double time = rounds * (double)((steps + s - 1) / s + (s > 1 ? 12 : 6)) * (tile == TILE_LARGE ? 1.0 : Tiles<TO>::small_cost);
+      // (the tiles of a CU share it: a round that leaves each with one of several takes that share of the time)
+      const double full = (double)(tiles * s) / (double)slots, fit = Tiles<TO>::per_cu[tile];
+      const double rounds = full > 1.0 ? std::ceil(full) : std::ceil(full * fit) / fit;
+      const double time = rounds * Tiles<TO>::cost[tile] * (double)((steps + s - 1) / s + (s > 1 ? 12 : 6));
       if (time < least) {
         least = time;
         best = {tile, s};
@@ -623,7 +660,7 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   p.h = take((size_t)p.d_steps * p.Np * P::ROW);
   p.w = p.pack_w ? take((size_t)p.d_steps * p.piece * P::ROW) : 0;
   if (!backward) {
-    const int bm = p.stats_tile == TILE_SMALL ? 128 : 256;
+    const int bm = tile_rows(p.stats_tile);
     p.part = take((size_t)((V + bm - 1) / bm + p.pieces) * p.Np * sizeof(float2));
     p.picked = take((size_t)N * 4);
     p.rows = take((size_t)N * 4);
@@ -661,23 +698,9 @@ hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStre
   if constexpr (EPI == XE_STATS || EPI == XE_GRAD)
     if (tile == TILE_NARROW) return go(c256{}, integral_constant<int, Tiles<TO>::narrow_n>{}, c4{}, integral_constant<int, 1>{});
   if (tile == TILE_SMALL) return go(c128{}, c128{}, c2{}, c2{});
+  if (tile == TILE_TINY) return go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, c2{}, c2{});
   if constexpr (sizeof(TO) == 4) return go(c256{}, c128{}, c4{}, c2{});
   else return go(c256{}, c256{}, c2{}, c4{});
-}
-
-template <typename TO>
-hipError_t pack(const TO* src, const int* state, int rows, int D, char* dst, int R, int steps, hipStream_t st) {
-  const long threads = (long)steps * R * (XentPlan<TO>::K / 8);
-  hipLaunchKernelGGL((k_xent_pack<TO>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, src, state, rows, D, dst, R,
-                     steps);
-  return hipGetLastError();
-}
-
-template <typename TO>
-hipError_t pack_t(const TO* src, const int* state, int rows, long padded, int D, char* dst, int R, hipStream_t st) {
-  hipLaunchKernelGGL((k_xent_pack_t<TO>), dim3((unsigned)((D + 63) / 64), (unsigned)(padded / 64)), dim3(256), 0, st, src, state,
-                     rows, D, dst, R);
-  return hipGetLastError();
 }
 
 #define XENT_TRY(expr)                  \
@@ -686,17 +709,42 @@ hipError_t pack_t(const TO* src, const int* state, int rows, long padded, int D,
     if (_e != hipSuccess) return _e;    \
   } while (0)
 
-// A's operand of the products with the head: entries [v0, v0 + rows) of W, through panels where it must.
+// Layout of H's compact rows.
 template <typename TO>
-hipError_t head_operand(const XentPlan<TO>& p, const XentCall& c, long v0, int rows, GemmOperand* A, hipStream_t st) {
+XentLayout hidden_layout(const XentPlan<TO>& p, const XentCall& c, bool rows, bool columns) {
+  XentLayout L{c.H, c.state, c.N, (int)p.Np, c.D, p.d_steps, (int)p.Np, (int)p.Dr, nullptr, nullptr, 0};
+  L.dst = rows ? c.ws + p.h : nullptr;
+  L.dst_t = columns ? c.ws + p.ht : nullptr;
+  L.blocks = (int)(p.Np / 64 * ((c.D + 63) / 64));
+  return L;
+}
+
+// Layout of the entries [v0, v0 + n) of W (none where they are read as they are and their columns are not asked for).
+template <typename TO>
+XentLayout head_layout(const XentPlan<TO>& p, const XentCall& c, long v0, int n, bool columns) {
+  // (the products read whole tiles of panels: padded like the piece)
+  const int padded = (int)up_to(n, p.pack_w ? kPad : 64);
+  XentLayout L{(const TO*)c.W + v0 * c.D, nullptr, n, padded, c.D, p.d_steps, (int)p.piece, (int)p.Dr, nullptr, nullptr, 0};
+  L.dst = p.pack_w ? c.ws + p.w : nullptr;
+  L.dst_t = columns ? c.ws + p.wt : nullptr;
+  L.blocks = L.dst || L.dst_t ? padded / 64 * ((c.D + 63) / 64) : 0;
+  return L;
+}
+
+// Those entries as an operand of the products with H.
+template <typename TO>
+GemmOperand head_operand(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
   typedef XentPlan<TO> P;
-  const TO* w = (const TO*)c.W + v0 * c.D;
-  if (!p.pack_w) {
-    *A = {w, (long)c.D * (long)sizeof(TO), P::ROW, rows};
-    return hipSuccess;
-  }
-  *A = {c.ws + p.w, P::ROW, p.piece * P::ROW, (int)p.piece};
-  return pack<TO>(w, nullptr, rows, c.D, c.ws + p.w, (int)p.piece, p.d_steps, st);
+  if (p.pack_w) return {c.ws + p.w, P::ROW, p.piece * P::ROW, (int)up_to(n, kPad)};
+  return {(const TO*)c.W + v0 * c.D, (long)c.D * (long)sizeof(TO), P::ROW, n};
+}
+
+template <typename TO>
+hipError_t launch_begin(const XentBegin& A, hipStream_t st) {
+  const unsigned blocks = (unsigned)(A.m[0].blocks + A.m[1].blocks + (A.number_rows != 0) + (A.make_scale != 0));
+  if (blocks == 0) return hipSuccess;
+  hipLaunchKernelGGL((k_xent_begin<TO>), dim3(blocks), dim3(256), 0, st, A);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -714,15 +762,24 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
   const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, false);
   float* rows = c.reduction ? (float*)(c.ws + p.rows) : c.loss;
   float* picked = (float*)(c.ws + p.picked);
-  hipLaunchKernelGGL(k_xent_rows, dim3(1), dim3(1024), 0, st, c.target, c.N, c.V, c.ignore, c.state, picked, rows);
-  XENT_TRY(hipGetLastError());
-  XENT_TRY(pack<TO>((const TO*)c.H, c.state, c.N, c.D, c.ws + p.h, (int)p.Np, p.d_steps, st));
-  const int bm = p.stats_tile == TILE_SMALL ? 128 : 256;
+  const int bm = tile_rows(p.stats_tile);
   long tiles = 0;
   for (long v0 = 0; v0 < c.V; v0 += p.piece) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
+    XentBegin F{};
+    F.m[0] = head_layout<TO>(p, c, v0, n, false);
+    if (v0 == 0) {
+      F.number_rows = 1;
+      F.target = c.target; F.N = c.N; F.V = c.V; F.ignore = c.ignore; F.state = c.state; F.picked = picked; F.loss = rows;
+    }
+    XENT_TRY(launch_begin<TO>(F, st));
+    if (v0 == 0) {
+      XentBegin H{};
+      H.m[0] = hidden_layout<TO>(p, c, true, false);
+      XENT_TRY(launch_begin<TO>(H, st));
+    }
     XentArgs A{};
-    XENT_TRY(head_operand<TO>(p, c, v0, n, &A.A, st));
+    A.A = head_operand<TO>(p, c, v0, n);
     A.B = {c.ws + p.h, P::ROW, p.Np * P::ROW, (int)p.Np};
     A.steps = p.d_steps;
     A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0;
@@ -731,10 +788,13 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
     XENT_TRY((launch_gemm<TO, XE_STATS>(A, n, c.N, p.stats_tile, 1, st)));
     tiles += (n + bm - 1) / bm;
   }
-  hipLaunchKernelGGL((k_xent_loss<P::TERMS == 3>), dim3((c.N + 63) / 64), dim3(1024), 0, st, (const float2*)(c.ws + p.part),
-                     (int)tiles, p.Np, c.N, c.state, picked, rows);
+  // few rows: their losses and the sum of them in one workgroup
+  const bool once = c.reduction && c.N <= 256;
+  hipLaunchKernelGGL((k_xent_loss<P::TERMS == 3>), dim3(once ? 1 : (c.N + 63) / 64), dim3(1024), 0, st,
+                     (const float2*)(c.ws + p.part), (int)tiles, p.Np, c.N, c.state, picked, rows, c.reduction == 1,
+                     once ? c.loss : nullptr);
   XENT_TRY(hipGetLastError());
-  if (c.reduction) {
+  if (c.reduction && !once) {
     hipLaunchKernelGGL(k_xent_sum, dim3(1), dim3(1024), 0, st, rows, c.N, c.state, c.reduction == 1, c.loss);
     XENT_TRY(hipGetLastError());
   }
@@ -745,17 +805,20 @@ template <typename TO>
 hipError_t xent_backward(const XentCall& c, hipStream_t st) {
   typedef XentPlan<TO> P;
   const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, true);
-  constexpr float up = up_of<TO>();
   float *alpha = (float*)(c.ws + p.alpha), *rho = (float*)(c.ws + p.rho);
-  hipLaunchKernelGGL(k_xent_scale, dim3(1), dim3(1024), 0, st, c.grad, c.reduction, c.state, up, alpha, rho);
-  XENT_TRY(hipGetLastError());
-  XENT_TRY(pack<TO>((const TO*)c.H, c.state, c.N, c.D, c.ws + p.h, (int)p.Np, p.d_steps, st));
-  if (c.dW) XENT_TRY(pack_t<TO>((const TO*)c.H, c.state, c.N, p.Np, c.D, c.ws + p.ht, (int)p.Dr, st));
   for (long v0 = 0; v0 < c.V; v0 += p.piece) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
     const int n_steps = (int)(up_to(n, P::K) / P::K);
+    XentBegin F{};
+    F.m[0] = head_layout<TO>(p, c, v0, n, c.dH != nullptr);
+    if (v0 == 0) {
+      F.m[1] = hidden_layout<TO>(p, c, true, c.dW != nullptr);
+      F.make_scale = 1;
+      F.state = c.state; F.grad = c.grad; F.reduction = c.reduction; F.up = up_of<TO>(); F.alpha = alpha; F.rho = rho;
+    }
+    XENT_TRY(launch_begin<TO>(F, st));
     XentArgs A{};
-    XENT_TRY(head_operand<TO>(p, c, v0, n, &A.A, st));
+    A.A = head_operand<TO>(p, c, v0, n);
     A.B = {c.ws + p.h, P::ROW, p.Np * P::ROW, (int)p.Np};
     A.steps = p.d_steps;
     A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0; A.D = c.D;
@@ -783,7 +846,6 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
       }
     }
     if (c.dH) {
-      XENT_TRY(pack_t<TO>((const TO*)c.W + v0 * c.D, nullptr, n, up_to(n, 64), c.D, c.ws + p.wt, (int)p.Dr, st));
       XentArgs B = A;
       B.A = {c.ws + p.wt, P::ROW, p.Dr * P::ROW, (int)p.Dr};
       B.B = {c.ws + p.g, P::ROW, p.Np * P::ROW, (int)p.Np};

@@ -7,17 +7,17 @@
 // bf16 terms of kans_split.h, [row][term][32] in a step, and take six MFMAs a product.
 //
 // A workgroup of WAVES_M x WAVES_N waves holds a BM x BN tile.  A step's rows go from memory to LDS by DMA
-// (buffer loads, 16 bytes a lane) into one of two stages; the barrier that opens stage s + 1 stands before
-// the last part of step s, whose operands are in registers by then: the first operands of step s + 1 are read
-// while the matrix pipe works on it.  The DMA of step s + 2 goes out in that part and the next one, one
-// instruction between a few products: all of them at once fill the memory pipe's queue, and the waves stand there.  The two stages are
-// separate arrays and the step loop is unrolled by two, so that the compiler sees that reads of one do not
-// depend on the DMA into the other.
+// (buffer loads, 16 bytes a lane) into one of two stages, or of three for A (A_STAGES).  The barrier that opens step
+// s + 1 stands before the last part of step s, whose operands are in registers by then: the first operands of step
+// s + 1 are read while the matrix pipe works on it.  The DMAs into the stages that step s has left go out in that
+// part and the next one, a few between the products of each row of blocks: all of them at once fill the memory pipe's queue,
+// and the waves stand there.  The stages are separate arrays and the step loop is unrolled until they repeat,
+// so that the compiler sees that reads of one do not depend on the DMA into another.
 //
 // LDS rows are 128 (or, with three terms, 192) bytes, so a column of 16-byte chunks would meet the same banks in
 // every second (fourth) row: chunk c of row r lies in slot c ^ ((r >> 1) & 7) (c ^ ((r >> 2) & 3)), which
-// spreads 16 rows over all 64 banks.  The DMA writes LDS in lane order, so it is the source address that is permuted,
-// inside one row's step.
+// spreads 16 rows over all 64 banks (no conflict counted).  The DMA writes LDS in lane order, so it is the source
+// address that is permuted, inside one row's step.
 #pragma once
 #include "kans_split.h"
 #include "kans_tile.h"
@@ -40,24 +40,28 @@ template <int TERMS> struct StepOf {
   }
 };
 
-template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N>
+template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES>
 struct GemmTile {
   using Step = StepOf<TERMS>;
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
   static constexpr int MB = BM / WAVES_M / 32, NB = BN / WAVES_N / 32;  // 32 x 32 blocks of a wave
-  static constexpr int STAGE = (BM + BN) * Step::row_bytes;
-  static constexpr int DMA_A = BM * Step::row_bytes / 1024 / WAVES, DMA_B = BN * Step::row_bytes / 1024 / WAVES;
-  static_assert(DMA_A * 1024 * WAVES == BM * Step::row_bytes && DMA_B * 1024 * WAVES == BN * Step::row_bytes, "whole DMAs");
+  static constexpr int STAGE_A = BM * Step::row_bytes, STAGE_B = BN * Step::row_bytes;  // bytes of a stage
+  static constexpr int DMA_A = STAGE_A / 1024 / WAVES, DMA_B = STAGE_B / 1024 / WAVES;  // of a wave
+  static_assert(DMA_A * 1024 * WAVES == STAGE_A && DMA_B * 1024 * WAVES == STAGE_B, "whole DMAs");
+  static_assert(A_STAGES == 2 || (A_STAGES == 3 && DMA_A < 16), "stages of A");
   typedef typename Mfma<T>::frag frag;
 
-  // A raw buffer from p on: 32-bit offsets, not bounded (the operands' rows are: GemmOperand).
+  // A raw buffer from p on: 32-bit offsets, not bounded (the operands' rows are: GemmOperand).  Buffer loads, not
+  // global ones: behind a global load to LDS the compiler waits for every LDS read where it could wait for the
+  // older ones.
   static __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const char* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, 0xffffffffu, 0x00027000);
   }
 
   // acc = the tile at (m0, n0) over `steps` steps from step `first`.
   static __device__ __forceinline__ void run(const GemmOperand& A, const GemmOperand& B, int m0, int n0, int first, int steps,
-                                             char* st0, char* st1, floatx16 (&acc)[MB][NB]) {
+                                             char* a_st0, char* a_st1, char* a_st2, char* b_st0, char* b_st1,
+                                             floatx16 (&acc)[MB][NB]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WAVES_N, wn = wave % WAVES_N;
 #pragma unroll
@@ -80,28 +84,13 @@ struct GemmTile {
     for (int i = 0; i < DMA_B; ++i) off_b[i] = place((i * WAVES + wave) * 64 + lane, n0, b0, B);
     const char* pa = (const char*)A.p + (long)a0 * A.row_stride + (long)first * A.step_stride;
     const char* pb = (const char*)B.p + (long)b0 * B.row_stride + (long)first * B.step_stride;
-    // (buffer loads, not global ones: behind a global load to LDS the compiler waits for every LDS read
-    // where it could wait for the older ones)
-    struct Source {
-      __amdgpu_buffer_rsrc_t a, b;
+    auto dma_a = [&](const __amdgpu_buffer_rsrc_t& o, char* st, int i) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(o, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16,
+                                               off_a[i], 0, 0, 0);
     };
-    auto source = [&](int s) {
-      return Source{resource(pa + (long)s * A.step_stride), resource(pb + (long)s * B.step_stride)};
-    };
-    auto dma1 = [&](const Source& o, char* st, int i) {  // the i-th of this wave's DMAs of a step
-      if (i < DMA_A)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            o.a, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16, off_a[i < DMA_A ? i : 0], 0, 0, 0);
-      else
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            o.b, (__attribute__((address_space(3))) void*)(st + BM * Step::row_bytes + ((i - DMA_A) * WAVES + wave) * 1024), 16,
-            off_b[i < DMA_A ? 0 : i - DMA_A], 0, 0, 0);
-    };
-    constexpr int DMAS = DMA_A + DMA_B, EACH = (DMAS + 2 * MB - 1) / (2 * MB);  // behind each of 2 MB rows of blocks
-    auto dma = [&](int s, char* st, int from, int to) {
-      const Source o = source(s);
-#pragma unroll
-      for (int i = from; i < to; ++i) dma1(o, st, i);
+    auto dma_b = [&](const __amdgpu_buffer_rsrc_t& o, char* st, int i) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(o, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16,
+                                               off_b[i], 0, 0, 0);
     };
     const int row = lane & 31, half = lane >> 5;
     auto read = [&](const char* st, int r, int part, int term) {
@@ -109,14 +98,15 @@ struct GemmTile {
       return *(const frag*)(st + r * Step::row_bytes + slot * 16);
     };
     frag a[2][MB][TERMS], b[2][NB][TERMS];
-    auto fetch = [&](const char* st, int part, frag (&fa)[MB][TERMS], frag (&fb)[NB][TERMS]) {
+    auto fetch = [&](const char* sa, const char* sb, int part, frag (&fa)[MB][TERMS], frag (&fb)[NB][TERMS]) {
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) fa[i][t] = read(st, (wm * MB + i) * 32 + row, part, t);
+        for (int i = 0; i < MB; ++i) fa[i][t] = read(sa, (wm * MB + i) * 32 + row, part, t);
 #pragma unroll
-        for (int j = 0; j < NB; ++j) fb[j][t] = read(st + BM * Step::row_bytes, (wn * NB + j) * 32 + row, part, t);
+        for (int j = 0; j < NB; ++j) fb[j][t] = read(sb, (wn * NB + j) * 32 + row, part, t);
       }
+      __builtin_amdgcn_sched_barrier(0);
     };
     // the products of one part; between(i) comes before those of the i-th row of blocks
     auto multiply = [&](const frag (&fa)[MB][TERMS], const frag (&fb)[NB][TERMS], auto between) {
@@ -131,50 +121,84 @@ struct GemmTile {
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    auto dma_between = [&](bool on, int s, char* st, int from) {
-      const Source o = source(s);
+    // The DMAs that go out behind the barrier of step s: B of step s + 2, then A of step s + A_STAGES (so that those
+    // which the next barrier need not wait for are the last); EACH of them before each of 2 MB rows of blocks.
+    // `all`: both steps exist.
+    constexpr int DMAS = DMA_A + DMA_B, EACH = (DMAS + 2 * MB - 1) / (2 * MB);
+    auto dma_between = [&](int s, char* sa, char* sb, int from, bool all) {
+      const auto ra = resource(pa + (long)(s + A_STAGES) * A.step_stride), rb = resource(pb + (long)(s + 2) * B.step_stride);
+      const bool on_a = all || s + A_STAGES < steps, on_b = all || s + 2 < steps;
       return [=](int i) {
-        if (!on) return;
 #pragma unroll
-        for (int e = 0; e < EACH; ++e)
-          if (from + i * EACH + e < DMAS) dma1(o, st, from + i * EACH + e);
+        for (int e = 0; e < EACH; ++e) {
+          const int k = from + i * EACH + e;
+          if (k < DMA_B) {
+            if (on_b) dma_b(rb, sb, k < DMA_B ? k : 0);
+          } else if (k < DMAS) {
+            if (on_a) dma_a(ra, sa, k < DMAS ? k - DMA_B : 0);
+          }
+        }
         __builtin_amdgcn_sched_barrier(0);
       };
     };
     auto nothing = [](int) {};
+    // What this wave has read and asked for is there, but for the newest DMAs of A (of the step after the next) where
+    // they have gone out; then all waves meet.
+    auto meet = [&](bool newest_a_out) {
+      asm volatile("" ::: "memory");
+      if (A_STAGES == 3 && newest_a_out) __builtin_amdgcn_s_waitcnt(0x70 | DMA_A);  // vmcnt(DMA_A) lgkmcnt(0)
+      else __builtin_amdgcn_s_waitcnt(0x70);                                        // vmcnt(0) lgkmcnt(0)
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
     constexpr int P = Step::parts;
     static_assert(P % 2 == 0, "the fragment buffers alternate");
-    // step s from `cur`; `next`: another one follows (in `nxt`), `ahead`: and one behind it
-    auto step = [&](int s, char* cur, char* nxt, bool next, bool ahead) {
+    // step s from (a_cur, b_cur); the next one is in (a_nxt, b_nxt), the one before was in (a_old, b_nxt)
+    auto step = [&](int s, char* a_old, char* a_cur, char* a_nxt, char* b_cur, char* b_nxt, bool all) {
 #pragma unroll
       for (int p = 0; p + 1 < P; ++p) {
-        fetch(cur, p + 1, a[(p + 1) & 1], b[(p + 1) & 1]);
-        __builtin_amdgcn_sched_barrier(0);
-        if (p == 0) multiply(a[0], b[0], dma_between(next, s + 1, nxt, MB * EACH));
+        fetch(a_cur, b_cur, p + 1, a[(p + 1) & 1], b[(p + 1) & 1]);
+        if (p == 0) multiply(a[0], b[0], dma_between(s - 1, a_old, b_nxt, MB * EACH, all));
         else multiply(a[p & 1], b[p & 1], nothing);
       }
-      if (next) {
-        __syncthreads();  // every wave has read `cur`, and `nxt` has landed
-        fetch(nxt, 0, a[0], b[0]);
-        __builtin_amdgcn_sched_barrier(0);
+      if (all || s + 1 < steps) {
+        meet(all || s + 2 < steps);  // every wave has read step s, and step s + 1 has landed
+        fetch(a_nxt, b_nxt, 0, a[0], b[0]);
       }
-      multiply(a[1], b[1], dma_between(ahead, s + 2, cur, 0));
+      multiply(a[1], b[1], dma_between(s, a_cur, b_cur, 0, all));
     };
-    dma(0, st0, 0, DMAS);
-    __syncthreads();
-    if (steps > 1) dma(1, st1, 0, min(MB * EACH, DMAS));
-    fetch(st0, 0, a[0], b[0]);
+    // step 0, and what would have gone out behind the steps before it
+    {
+      const auto ra = resource(pa), rb = resource(pb), ra1 = resource(pa + A.step_stride);
+#pragma unroll
+      for (int i = 0; i < DMA_A; ++i) dma_a(ra, a_st0, i);
+#pragma unroll
+      for (int i = 0; i < DMA_B; ++i) dma_b(rb, b_st0, i);
+      if (A_STAGES == 3 && steps > 1) {
+#pragma unroll
+        for (int i = 0; i < DMA_A; ++i) dma_a(ra1, a_st1, i);
+      }
+      meet(steps > 1);
+      const auto first_half = dma_between(-1, A_STAGES == 3 ? a_st2 : a_st1, b_st1, 0, false);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) first_half(i);
+      fetch(a_st0, b_st0, 0, a[0], b[0]);
+    }
+    constexpr int ROUND = A_STAGES == 3 ? 6 : 2;  // steps until the stages repeat
+    char* const as[3] = {a_st0, a_st1, a_st2};
+    char* const bs[2] = {b_st0, b_st1};
+    auto round = [&](int s, bool all) {
+      static_for<0, ROUND>([&](auto k) {
+        constexpr int i = decltype(k)::value;
+        if (all || s + i < steps)
+          step(s + i, as[(i + A_STAGES - 1) % A_STAGES], as[i % A_STAGES], as[(i + 1) % A_STAGES], bs[i % 2], bs[(i + 1) % 2], all);
+      });
+    };
     int s = 0;
 #pragma unroll 1
-    for (; s + 3 < steps; s += 2) {
-      step(s, st0, st1, true, true);
-      step(s + 1, st1, st0, true, true);
-    }
+    for (; s + ROUND + A_STAGES - 1 < steps; s += ROUND) round(s, true);
 #pragma unroll 1
-    for (; s < steps; s += 2) {  // the last one to three
-      step(s, st0, st1, s + 1 < steps, s + 2 < steps);
-      if (s + 1 < steps) step(s + 1, st1, st0, s + 2 < steps, false);
-    }
+    for (; s < steps; s += ROUND) round(s, false);
     __syncthreads();  // the stages are free for the epilogue
   }
 };

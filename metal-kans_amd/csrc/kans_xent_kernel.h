@@ -118,11 +118,13 @@ template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentArgs A) {
   typedef typename XentTypes<TO>::T T;
   constexpr int TERMS = XentTypes<TO>::TERMS;
-  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N>;
+  // a third stage of A where the tile has a CU's LDS for itself and it still fits (160 KB)
+  constexpr int A_STAGES = TERMS == 1 && BM == 256 && BN == 256 ? 3 : 2;
+  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES>;
   using Step = StepOf<TERMS>;
   constexpr int MB = Tile::MB, NB = Tile::NB;
-  __shared__ alignas(16) char st0[Tile::STAGE];
-  __shared__ alignas(16) char st1[Tile::STAGE];
+  __shared__ alignas(16) char a_st0[Tile::STAGE_A], a_st1[Tile::STAGE_A], a_st2[A_STAGES == 3 ? Tile::STAGE_A : 16];
+  __shared__ alignas(16) char b_st0[Tile::STAGE_B], b_st1[Tile::STAGE_B];
   int mt, nt;
   tile_of<8>(xcd_remap(blockIdx.x, A.m_tiles * A.n_tiles), A.m_tiles, A.n_tiles, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN;
@@ -137,7 +139,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     steps = min(A.steps_per_split, steps - first);
   }
   floatx16 acc[MB][NB];
-  Tile::run(A.A, A.B, m0, n0, first, steps, st0, st1, acc);
+  Tile::run(A.A, A.B, m0, n0, first, steps, a_st0, a_st1, a_st2, b_st0, b_st1, acc);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N, col = lane & 31, half = lane >> 5;
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   auto ncol = [&](int j) { return n0 + (wn * NB + j) * 32 + col; };
 
   if constexpr (EPI == XE_STATS) {
-    float2* join = (float2*)st0;  // [WAVES_M][BN]
+    float2* join = (float2*)a_st0;  // [WAVES_M][BN]
     const bool edge = m0 + BM > A.V;
     const int* target = A.state + kXentHead + A.N;
 #pragma unroll

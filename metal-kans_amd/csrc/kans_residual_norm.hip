@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "kans_api_internal.h"
+#include "kans_wave.h"
 
 namespace kans {
 namespace {
@@ -116,22 +117,6 @@ __device__ __forceinline__ void store_vec(T* p, int left, const float* o) {
     for (int e = 0; e < V; ++e)
       if (e < left) p[e] = v[e];
   }
-}
-
-// The sum over a wave, in every lane: within 4, 8 and 16 lanes, then across the rows of 16.
-__device__ __forceinline__ float wave_sum(float v) {
-  auto step = [](float a, auto ctrl, auto rows) {
-    return a + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, a), decltype(ctrl)::value,
-                                                                      decltype(rows)::value, 0xf, false));
-  };
-  using std::integral_constant;
-  v = step(v, integral_constant<int, 0xb1>{}, integral_constant<int, 0xf>{});   // lane ^ 1
-  v = step(v, integral_constant<int, 0x4e>{}, integral_constant<int, 0xf>{});   // lane ^ 2
-  v = step(v, integral_constant<int, 0x141>{}, integral_constant<int, 0xf>{});  // mirrored in 8
-  v = step(v, integral_constant<int, 0x140>{}, integral_constant<int, 0xf>{});  // mirrored in 16
-  v = step(v, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});  // lane 15 of a row into the next
-  v = step(v, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});  // lane 31 into the upper half
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // Sums of a and b over the TPR threads of a row, in each of them.  `slot` (0 or 1)

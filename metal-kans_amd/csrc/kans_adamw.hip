@@ -254,20 +254,23 @@ int kans_adamw_step(int dtype, int state_bits, int n_tensors, void* const* param
   if (state_bits != 8 && state_bits != 32) return kans_fail(KANS_ERR_ARG, "state_bits=%d, must be 8 or 32", state_bits);
   if (n_tensors < 0) return kans_fail(KANS_ERR_ARG, "n_tensors=%d", n_tensors);
   if (n_tensors == 0) return 0;
-  if (!params || !grads || !numel || !blocks || !steps || !exp_avg || !exp_avg_sq)
-    return kans_fail(KANS_ERR_ARG, "null tensor table or state");
-  if (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) return kans_fail(KANS_ERR_ARG, "8-bit states need their scales");
-  if (dtype != DT_F32 && !master) return kans_fail(KANS_ERR_ARG, "16-bit parameters need their fp32 masters");
-  if (((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq | (uintptr_t)master) & 15)
-    return kans_fail(KANS_ERR_ARG, "states must be 16-byte aligned");
+  if (!params || !grads || !numel || !blocks || !steps) return kans_fail(KANS_ERR_ARG, "null tensor table");
   if (!rate(lr) || !rate(eps) || !rate(weight_decay) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
     return kans_fail(KANS_ERR_ARG, "lr, eps and weight_decay must be finite and >= 0, the betas in [0, 1)");
+  bool any = false;
   for (int i = 0; i < n_tensors; ++i) {
     if (numel[i] < 0 || blocks[i] < 0 || steps[i] < 1 || (numel[i] > 0 && (!params[i] || !grads[i])))
       return kans_fail(KANS_ERR_ARG, "tensor %d: null pointer, negative size or block, or step %ld < 1", i, steps[i]);
     if (numel[i] > kAdamMaxGrid * kAdamTile || blocks[i] > 0xffffffffL)
       return kans_fail(KANS_ERR_UNSUPPORTED, "tensor %d: %ld elements at block %ld exceed one launch", i, numel[i], blocks[i]);
+    any |= numel[i] > 0;
   }
+  if (!any) return 0;
+  if (!exp_avg || !exp_avg_sq) return kans_fail(KANS_ERR_ARG, "null state");
+  if (state_bits == 8 && (!exp_avg_scale || !exp_avg_sq_scale)) return kans_fail(KANS_ERR_ARG, "8-bit states need their scales");
+  if (dtype != DT_F32 && !master) return kans_fail(KANS_ERR_ARG, "16-bit parameters need their fp32 masters");
+  if (((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq | (uintptr_t)master) & 15)
+    return kans_fail(KANS_ERR_ARG, "states must be 16-byte aligned");
   std::lock_guard<std::mutex> lk(kans_mutex());
   int rc = kans_ensure_init();
   if (rc) return rc;

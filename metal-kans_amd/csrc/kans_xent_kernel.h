@@ -649,7 +649,8 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   p.pack_w = P::TERMS == 3 || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
   const long all = up_to(V, kPad);
   p.piece = std::max<long>(kPad, std::min({all, kXentPiece / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
-  if (!backward && !p.pack_w) p.piece = all;
+  // (in one piece where nothing of it is laid out; a grid holds fewer than 2^32 threads, 2^-7 of the logits)
+  if (!backward && !p.pack_w) p.piece = std::max<long>(kPad, std::min(all, (1L << 37) / p.Np / kPad * kPad));
   p.pieces = (V + p.piece - 1) / p.piece;
   p.piece = up_to((V + p.pieces - 1) / p.pieces, kPad);
   p.stats_tile = tile_for<TO>(std::min<long>(V, p.piece), N, p.d_steps);

@@ -238,7 +238,7 @@ class TorchAdamW(torch.optim.Optimizer):
             g = p.grad
             if g is None:
                 continue
-            if g.is_sparse or g.dtype != a.dtype or g.device != a.device:
+            if g.layout is not torch.strided or g.dtype != a.dtype or g.device != a.device:
                 raise TypeError(f"gradients must be dense {a.dtype} tensors on {a.device}")
             if p.dtype != a.dtype or p.device != a.device or p.numel() != a.numel[i]:
                 raise ValueError("a parameter's dtype, device or size changed under its optimizer")

@@ -30,6 +30,7 @@ def test_adamw_refusals(lib):
         assert adamw(lib, **bad) == -1, bad
         assert lib.kans_last_error()
     assert adamw(lib, **ok, numel=1 << 40) == -5
+    assert adamw(lib, numel=0, m=None, v=None) == 0
     assert adamw(lib, n=0) == 0
     assert lib.kans_adamw_values(None, None, None, None, None, None, 1, None) == -1
     assert lib.kans_adamw_values(64, 64, 64, 64, 72, 64, 1, None) == -1

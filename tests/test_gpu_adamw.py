@@ -321,6 +321,14 @@ def test_refusals(cuda):
     cpu[0].grad = torch.zeros(4)
     with pytest.raises(ValueError):
         mk.TorchAdamW(cpu).step()
+    empty = torch.nn.Parameter(torch.zeros(0, 3, device="cuda"))
+    empty.grad = torch.zeros_like(empty)
+    for bits in (8, 32):
+        mk.TorchAdamW([empty], state_bits=bits).step()
+    p[0].grad = torch.sparse_coo_tensor([[1]], [1.0], (4,), device="cuda")
+    with pytest.raises(TypeError):
+        mk.TorchAdamW(p).step()
+    p[0].grad = None
     opt = mk.TorchAdamW(p)
     opt.step()                     # no gradient anywhere: nothing to do
     assert not opt.state.get(p[0])

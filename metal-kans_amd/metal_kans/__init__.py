@@ -3,8 +3,9 @@
 Drop-in for the hot-path surface of Shuril/metal-kans (metal_kans/__init__.py:6-40):
 Chebyshev / Gaussian-RBF / cubic B-spline layers, the multi-layer container, the
 GatedKAN block, INT8 / INT4 / ternary weight quantization, the Chebyshev layer
-backward and the torch modules.  Optimizers, pruning, symbolic export and the
-other KAN families are outside this build's scope.
+backward and the torch modules.  Around them, on torch tensors, the rest of a training
+step: ``residual_norm``, ``linear_cross_entropy`` and ``TorchAdamW``.  The reference's NumPy
+optimizers, pruning, symbolic export and the other KAN families are outside this build's scope.
 """
 from .device import get_metal_bridge, is_gpu_available, is_metal_available, set_async, sync
 from .cheby_kan import ChebyKAN

@@ -449,7 +449,7 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
  * Rows whose target is ignore_index take part in nothing, whatever H holds there; another target outside
  * [0, V) makes its row's loss NaN.  `state` (int32, 4 + 3 N) is filled for the backward.  The workspace
  * (device memory, 16-byte aligned) has kans_linear_xent_workspace bytes, which is negative for refused sizes: N up to
- * 2^22, D to 2^16, V to 2^24. */
+ * 2^21, D to 2^16, V to 2^24. */
 long kans_linear_xent_workspace(int dtype, int N, int D, int V, int backward);
 int kans_linear_xent_forward(int dtype, const void* H, const void* W, const int64_t* target, int N, int D, int V,
                              int64_t ignore_index, int reduction, float* loss, int* state, void* workspace,

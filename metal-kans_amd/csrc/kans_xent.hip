@@ -14,8 +14,8 @@ int check_xent(int dtype, const void* H, const void* W, const void* target, int 
   if (N > 0 && (!H || !W || !target || !state)) return kans_fail(KANS_ERR_ARG, "null hidden, weight, target or state");
   if (((uintptr_t)target & 7) || ((uintptr_t)state & 3)) return kans_fail(KANS_ERR_ARG, "misaligned target or state");
   // 32-bit places inside a tile and in a panel's grid
-  if (N > (1 << 22) || V > (1 << 24) || D > (1 << 16))
-    return kans_fail(KANS_ERR_UNSUPPORTED, "N=%d D=%d V=%d, at most 2^22, 2^16 and 2^24", N, D, V);
+  if (N > (1 << 21) || V > (1 << 24) || D > (1 << 16))
+    return kans_fail(KANS_ERR_UNSUPPORTED, "N=%d D=%d V=%d, at most 2^21, 2^16 and 2^24", N, D, V);
   return 0;
 }
 

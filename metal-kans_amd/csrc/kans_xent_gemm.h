@@ -1,10 +1,14 @@
 // Matrix product of the cross entropy kernels (kans_xent.hip): C[m][n] = sum_k A[m][k] B[n][k] on the 16-bit
 // matrix cores, with the epilogue taking the tile from the accumulators.
 //
-// Operands are rows of k in steps of kStep elements: step s of row r is `row_bytes` consecutive bytes at
-// base + r * row_stride + s * step_stride.  That covers a row-major matrix (step_stride = row_bytes) and panels
-// [step][row][kStep], whose tile of a step is one contiguous run.  fp32 operands (TERMS = 3) are the three
-// bf16 terms of kans_split.h, [row][term][32] in a step, and take six MFMAs a product.
+// k goes in steps of kStep.  An operand lies in memory either way:
+//   row after row: step s of row r is `row_bytes` consecutive bytes at base + r * row_stride + s * step_stride;
+//   column after column (COLUMNS): row_bytes of kStep consecutive rows r = b kStep .. at one k are at
+//   base + b * block_stride + k * row_stride.
+// Both cover a row-major matrix (as itself or as its transpose) and panels [step][row][kStep] of one, whose rows of a
+// step are one contiguous run; the second reads its operands from LDS transposed (ds_read_b64_tr_b16).  So one layout of a
+// matrix serves the products along either dimension.  fp32 operands (TERMS = 3) are the three bf16 terms of
+// kans_split.h, [term][32] in a step, and take six MFMAs a product.
 //
 // A workgroup of WAVES_M x WAVES_N waves holds a BM x BN tile.  A step's rows go from memory to LDS by DMA
 // (buffer loads, 16 bytes a lane) into one of two stages, or of three for A (A_STAGES).  The barrier that opens step
@@ -15,9 +19,10 @@
 // so that the compiler sees that reads of one do not depend on the DMA into another.
 //
 // LDS rows are 128 (or, with three terms, 192) bytes, so a column of 16-byte chunks would meet the same banks in
-// every second (fourth) row: chunk c of row r lies in slot c ^ ((r >> 1) & 7) (c ^ ((r >> 2) & 3)), which
-// spreads 16 rows over all 64 banks (no conflict counted).  The DMA writes LDS in lane order, so it is the source
-// address that is permuted, inside one row's step.
+// every second (fourth) row: chunk c of row r lies in slot c ^ reversed 3 bits of (r >> 1) (c ^ ((r >> 2) & 3)), which
+// spreads 16 rows over all 64 banks, and four rows of 32 bytes, as the transposed reads take them, too (no
+// conflict counted).  The DMA writes LDS in lane order, so it is the source address that is permuted, inside one row's
+// step.
 #pragma once
 #include "kans_split.h"
 #include "kans_tile.h"
@@ -26,8 +31,10 @@ namespace kans {
 
 struct GemmOperand {
   const void* p;
-  long row_stride, step_stride;  // bytes
-  int rows;                      // rows that exist; those of a tile behind them repeat the last
+  long row_stride, step_stride;  // bytes (step_stride: from a step of k to the next)
+  int rows;                      // rows that exist (COLUMNS: blocks of them); those of a tile behind them repeat the last
+  long block_stride;             // COLUMNS
+  long bytes;                    // COLUMNS: zeros are read from base + bytes on (0: everything that is read exists)
 };
 
 template <int TERMS> struct StepOf {
@@ -36,11 +43,11 @@ template <int TERMS> struct StepOf {
   static constexpr int chunks = row_bytes / 16;
   static constexpr int parts = kStep / 16;                        // MFMA depths of a step
   static __device__ __forceinline__ int slot(int row, int chunk) {
-    return TERMS == 1 ? chunk ^ ((row >> 1) & 7) : chunk ^ ((row >> 2) & 3);
+    return TERMS == 1 ? chunk ^ ((row >> 3 & 1) | (row >> 1 & 2) | (row << 1 & 4)) : chunk ^ ((row >> 2) & 3);
   }
 };
 
-template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES>
+template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES, bool A_COLUMNS, bool B_COLUMNS>
 struct GemmTile {
   using Step = StepOf<TERMS>;
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
@@ -51,11 +58,16 @@ struct GemmTile {
   static_assert(A_STAGES == 2 || (A_STAGES == 3 && DMA_A < 16), "stages of A");
   typedef typename Mfma<T>::frag frag;
 
-  // A raw buffer from p on: 32-bit offsets, not bounded (the operands' rows are: GemmOperand).  Buffer loads, not
-  // global ones: behind a global load to LDS the compiler waits for every LDS read where it could wait for the
-  // older ones.
-  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const char* p) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, 0xffffffffu, 0x00027000);
+  // A raw buffer from p on, 32-bit offsets, zeros behind `records` bytes.  Buffer loads, not global ones: behind a
+  // global load to LDS the compiler waits for every LDS read where it could wait for the older ones.
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t resource(const char* p, unsigned records) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(p), 0, (int)records, 0x00027000);
+  }
+  template <bool COLUMNS>
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const GemmOperand& o, const char* p, int s, int first) {
+    const unsigned records =
+        COLUMNS && o.bytes ? (unsigned)(o.bytes - (long)(first + s) * o.step_stride - (p - (const char*)o.p)) : 0xffffffffu;
+    return resource(p + (long)(first + s) * o.step_stride, records);
   }
 
   // acc = the tile at (m0, n0) over `steps` steps from step `first`.
@@ -71,19 +83,31 @@ struct GemmTile {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     if (steps <= 0) return;
-    // this lane's places in the tile's rows
+    // the tile's first row, and this lane's places in its rows
     unsigned off_a[DMA_A], off_b[DMA_B];
-    const int a0 = min(m0, A.rows - 1), b0 = min(n0, B.rows - 1);
-    auto place = [&](int q, int tile0, int row0, const GemmOperand& o) {
-      const int row = q / Step::chunks, chunk = Step::slot(row, q - row * Step::chunks);
-      return (unsigned)(min(tile0 + row, o.rows - 1) - row0) * (unsigned)o.row_stride + chunk * 16;
+    constexpr int KS = Step::kStep;
+    auto start = [&](const GemmOperand& o, int tile0, auto columns) {
+      if constexpr (decltype(columns)::value) return (const char*)o.p + (long)min(tile0 / KS, o.rows - 1) * o.block_stride;
+      else return (const char*)o.p + (long)min(tile0, o.rows - 1) * o.row_stride;
     };
+    auto place = [&](int q, int tile0, const GemmOperand& o, auto columns) {
+      const int row = q / Step::chunks, chunk = Step::slot(row, q - row * Step::chunks);
+      if constexpr (decltype(columns)::value) {
+        const int b0 = min(tile0 / KS, o.rows - 1), block = min(tile0 / KS + row / KS, o.rows - 1) - b0;
+        return (unsigned)block * (unsigned)o.block_stride + (unsigned)(row % KS) * (unsigned)o.row_stride + chunk * 16;
+      } else {
+        return (unsigned)(min(tile0 + row, o.rows - 1) - min(tile0, o.rows - 1)) * (unsigned)o.row_stride + chunk * 16;
+      }
+    };
+    constexpr std::integral_constant<bool, A_COLUMNS> a_columns{};
+    constexpr std::integral_constant<bool, B_COLUMNS> b_columns{};
 #pragma unroll
-    for (int i = 0; i < DMA_A; ++i) off_a[i] = place((i * WAVES + wave) * 64 + lane, m0, a0, A);
+    for (int i = 0; i < DMA_A; ++i) off_a[i] = place((i * WAVES + wave) * 64 + lane, m0, A, a_columns);
 #pragma unroll
-    for (int i = 0; i < DMA_B; ++i) off_b[i] = place((i * WAVES + wave) * 64 + lane, n0, b0, B);
-    const char* pa = (const char*)A.p + (long)a0 * A.row_stride + (long)first * A.step_stride;
-    const char* pb = (const char*)B.p + (long)b0 * B.row_stride + (long)first * B.step_stride;
+    for (int i = 0; i < DMA_B; ++i) off_b[i] = place((i * WAVES + wave) * 64 + lane, n0, B, b_columns);
+    const char *pa = start(A, m0, a_columns), *pb = start(B, n0, b_columns);
+    auto source_a = [&](int s) { return source<A_COLUMNS>(A, pa, s, first); };
+    auto source_b = [&](int s) { return source<B_COLUMNS>(B, pb, s, first); };
     auto dma_a = [&](const __amdgpu_buffer_rsrc_t& o, char* st, int i) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(o, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16,
                                                off_a[i], 0, 0, 0);
@@ -93,18 +117,59 @@ struct GemmTile {
                                                off_b[i], 0, 0, 0);
     };
     const int row = lane & 31, half = lane >> 5;
-    auto read = [&](const char* st, int r, int part, int term) {
-      const int slot = Step::slot(r, term * (Step::kStep / 8) + part * 2 + half);
+    // operand of the 32 rows from 32 * block of a stage, at one part of the step
+    auto read_rows = [&](const char* st, int block, int part, int term) {
+      const int r = block * 32 + row, slot = Step::slot(r, term * (KS / 8) + part * 2 + half);
       return *(const frag*)(st + r * Step::row_bytes + slot * 16);
+    };
+    // Groups of 16 lanes take four k of 16 rows: a lane reads four rows' values at one k and gets four k of one row.  Its
+    // place, by the block's half of a 128-byte row and the four k of eight:
+    int place_t[TERMS == 1 ? 2 : 1][2];
+    if constexpr (A_COLUMNS || B_COLUMNS) {
+      const int in16 = lane & 15, rows16 = lane >> 4 & 1;
+#pragma unroll
+      for (int q = 0; q < (TERMS == 1 ? 2 : 1); ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int k = half * 8 + h * 4 + in16 / 4;
+          place_t[q][h] = k * Step::row_bytes + Step::slot(k, q * 4 + rows16 * 2 + in16 % 4 / 2) * 16 + in16 % 2 * 8;
+        }
+    }
+    auto read_columns = [&](const char* st, const int (&at)[TERMS == 1 ? 2 : 1][2], int block, int part, int term) {
+      typedef short short4_t __attribute__((ext_vector_type(4)));
+      struct { short4_t v[2]; } f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        f.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) short4_t*)(st + (block * 32 / KS * KS + part * 16) * Step::row_bytes + term * 64 +
+                                                          at[TERMS == 1 ? block % 2 : 0][h]));
+      return __builtin_bit_cast(frag, f);
     };
     frag a[2][MB][TERMS], b[2][NB][TERMS];
     auto fetch = [&](const char* sa, const char* sb, int part, frag (&fa)[MB][TERMS], frag (&fb)[NB][TERMS]) {
+      int at[TERMS == 1 ? 2 : 1][2];
+      if constexpr (A_COLUMNS || B_COLUMNS) {
+        // (taken anew each time: the compiler would keep every sum of a place and a stage in a register of its own)
+#pragma unroll
+        for (int q = 0; q < (TERMS == 1 ? 2 : 1); ++q)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            at[q][h] = place_t[q][h];
+            asm volatile("" : "+v"(at[q][h]));
+          }
+      }
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
-        for (int i = 0; i < MB; ++i) fa[i][t] = read(sa, (wm * MB + i) * 32 + row, part, t);
+        for (int i = 0; i < MB; ++i) {
+          if constexpr (A_COLUMNS) fa[i][t] = read_columns(sa, at, wm * MB + i, part, t);
+          else fa[i][t] = read_rows(sa, wm * MB + i, part, t);
+        }
 #pragma unroll
-        for (int j = 0; j < NB; ++j) fb[j][t] = read(sb, (wn * NB + j) * 32 + row, part, t);
+        for (int j = 0; j < NB; ++j) {
+          if constexpr (B_COLUMNS) fb[j][t] = read_columns(sb, at, wn * NB + j, part, t);
+          else fb[j][t] = read_rows(sb, wn * NB + j, part, t);
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     };
@@ -126,7 +191,7 @@ struct GemmTile {
     // `all`: both steps exist.
     constexpr int DMAS = DMA_A + DMA_B, EACH = (DMAS + 2 * MB - 1) / (2 * MB);
     auto dma_between = [&](int s, char* sa, char* sb, int from, bool all) {
-      const auto ra = resource(pa + (long)(s + A_STAGES) * A.step_stride), rb = resource(pb + (long)(s + 2) * B.step_stride);
+      const auto ra = source_a(s + A_STAGES), rb = source_b(s + 2);
       const bool on_a = all || s + A_STAGES < steps, on_b = all || s + 2 < steps;
       return [=](int i) {
 #pragma unroll
@@ -169,7 +234,7 @@ struct GemmTile {
     };
     // step 0, and what would have gone out behind the steps before it
     {
-      const auto ra = resource(pa), rb = resource(pb), ra1 = resource(pa + A.step_stride);
+      const auto ra = source_a(0), rb = source_b(0), ra1 = source_a(1);
 #pragma unroll
       for (int i = 0; i < DMA_A; ++i) dma_a(ra, a_st0, i);
 #pragma unroll

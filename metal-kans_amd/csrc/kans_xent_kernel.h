@@ -2,7 +2,8 @@
 //
 // The logits are computed twice: for the sums of the softmax, and again in the backward, a piece of the vocabulary
 // at a time, where the epilogue turns them into G.  Only G of one piece is ever in memory (16-bit, or three
-// bf16 terms for fp32; at most kXentPiece elements), in both orders, and goes into the two products behind it.
+// bf16 terms for fp32; at most kXentPiece elements) and goes into the two products behind it.  H, G and a head whose rows are not whole steps
+// lie in panels that serve the products along either of their dimensions; another head is read as it is.
 // 8 N D V operations in all against the 6 N D V of a program that keeps the logits: the price of
 // not writing and reading N V of them.
 //
@@ -45,7 +46,7 @@ struct XentArgs {
   float* picked;               // XE_STATS: [N] the target's logit
   long Np, Vp;
   const float* rho;            // XE_GRAD: per compact row, or null (1)
-  char *g, *gt;                // XE_GRAD: panels [v / kStep][Np] and [n / kStep][Vp]; either may be null
+  char* g;                     // XE_GRAD: panels [v / kStep][Np][kStep]
   const float* alpha;          // XE_DW: factor
   void* out;                   // XE_DW: dW of the piece [V][D]
   int D;
@@ -98,22 +99,6 @@ __device__ __forceinline__ void pack8(const float* v, uint4 (&d)[TERMS]) {
   }
 }
 
-template <int CTRL>
-__device__ __forceinline__ unsigned dpp(unsigned v) {
-  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
-}
-
-// A quad of lanes (columns n .. n + 3) with four 16-bit rows each, transposed: lane l of the quad gets the four columns
-// of row 2 (l & 1) + (l >> 1).
-__device__ __forceinline__ uint2 quad_transpose(unsigned r01, unsigned r23, int lane) {
-  const bool odd = lane & 1, two = lane & 2;
-  const unsigned other = dpp<0xb1>(odd ? r01 : r23), own = odd ? r23 : r01;  // lane ^ 1
-  const unsigned lo = odd ? other : own, hi = odd ? own : other;
-  const unsigned a = __builtin_amdgcn_perm(hi, lo, 0x05040100), b = __builtin_amdgcn_perm(hi, lo, 0x07060302);
-  const unsigned far = dpp<0x4e>(two ? a : b);  // lane ^ 2
-  return two ? make_uint2(far, b) : make_uint2(a, far);
-}
-
 // The products.  8192 x 4096 x 65536 bf16, 256 x 256 tiles (four pieces in the backward):
 //   XE_STATS 3.25 ms (1.35 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 4 x 0.93 ms (1.18: its
 //   stores, 268 MB in each of two orders), XE_DW 4 x 0.83 and XE_DH 4 x 0.83 ms (1.32).
@@ -125,7 +110,9 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   constexpr int TERMS = XentTypes<TO>::TERMS;
   // a third stage of A where the tile has a CU's LDS for itself and it still fits (160 KB)
   constexpr int A_STAGES = TERMS == 1 && BM == 256 && BN == 256 ? 3 : 2;
-  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES>;
+  // dW = G^T H and dH = G W run along the rows of their operands: H and G, or W
+  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES, EPI != XE_STATS && EPI != XE_GRAD,
+                        EPI == XE_DW || EPI == XE_DW_SPLIT>;
   using Step = StepOf<TERMS>;
   constexpr int MB = Tile::MB, NB = Tile::NB;
   __shared__ alignas(16) char a_st0[Tile::STAGE_A], a_st1[Tile::STAGE_A], a_st2[A_STAGES == 3 ? Tile::STAGE_A : 16];
@@ -237,25 +224,14 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
           }
           uint4 d[TERMS];
           pack8<T, TERMS>(v, d);
-          if (A.g) {
-            // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
-            const int m8 = m - 4 * half + 8 * half;
-            char* o = A.g + ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
+          // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
+          const int m8 = m - 4 * half + 8 * half;
+          char* o = A.g + ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
 #pragma unroll
-            for (int c = 0; c < TERMS; ++c) {
-              const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
-              const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
-              *(uint4*)(o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
-            }
-          }
-          if (A.gt) {
-            const int mt4 = m + 2 * (lane & 1) + (lane >> 1 & 1), n4 = n - (lane & 3);
-            char* o = A.gt + ((long)(n / K) * A.Vp + mt4) * Step::row_bytes + n4 % K * 2;
-#pragma unroll
-            for (int c = 0; c < TERMS; ++c) {
-              *(uint2*)(o + c * K * 2) = quad_transpose(d[c].x, d[c].y, lane);
-              *(uint2*)(o + c * K * 2 + 8 * Step::row_bytes) = quad_transpose(d[c].z, d[c].w, lane);
-            }
+          for (int c = 0; c < TERMS; ++c) {
+            const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
+            *(uint4*)(o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
           }
         }
     }
@@ -335,16 +311,15 @@ __device__ __forceinline__ void store8(char* p, int term, const float* v) {
   }
 }
 
-// A matrix [.][D] laid out for the products: panels [step of D][R][kStep] of its rows (dst), and panels
-// [step of the rows][Rt][kStep] of its columns (dst_t); either may be null.  `padded` rows (a multiple of 64) are
-// written, zeros behind the last.  With `state` the rows are the compact ones (`rows` bounds their number) and
-// rows behind the last kPad that hold one stay as they are.
+// A matrix [.][D] laid out for the products: panels [step of D][R][kStep] of its rows.  `padded` rows (a multiple
+// of 64) are written, zeros behind the last.  With `state` the rows are the compact ones (`rows` bounds their number)
+// and rows behind the last kPad that hold one stay as they are.
 struct XentLayout {
   const void* src;
   const int* state;
-  int rows, padded, D, steps, R, Rt;
-  char *dst, *dst_t;
-  int blocks;  // tiles of 64 x 64
+  int rows, padded, D, steps, R;
+  char* dst;
+  int blocks;  // of 64 rows x 64 elements
 };
 
 // What the products need before they start, in one launch: block 0 numbers the rows, the next one makes the
@@ -364,7 +339,7 @@ struct XentBegin {
 };
 
 template <typename TO>
-__device__ __forceinline__ void lay_out(const XentLayout& L, int block, float (*tile)[65]) {
+__device__ __forceinline__ void lay_out(const XentLayout& L, int block) {
   typedef typename XentTypes<TO>::T T;
   constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
   const int across = (L.D + 63) / 64, r0 = block / across * 64, d0 = block % across * 64;
@@ -375,32 +350,16 @@ __device__ __forceinline__ void lay_out(const XentLayout& L, int block, float (*
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = threadIdx.x / 8 + i * 32, c = threadIdx.x % 8 * 8;
+    const int r = r0 + threadIdx.x / 8 + i * 32, c = d0 + threadIdx.x % 8 * 8, step = c / K;
+    if (step >= L.steps) return;
     float v[8];
-    if (r0 + r < rows) {
-      row8((const TO*)L.src + (long)(L.state ? L.state[kXentHead + r0 + r] : r0 + r) * L.D, d0 + c, L.D, v);
+    if (r < rows) {
+      row8((const TO*)L.src + (long)(L.state ? L.state[kXentHead + r] : r) * L.D, c, L.D, v);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = 0.0f;
     }
-    const int step = (d0 + c) / K;
-    if (L.dst && step < L.steps)
-      store8<T, TERMS>(L.dst + ((long)step * L.R + r0 + r) * StepOf<TERMS>::row_bytes + (d0 + c) % K * 2, K * 2, v);
-    if (L.dst_t) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) tile[r][c + e] = v[e];
-    }
-  }
-  if (!L.dst_t) return;
-  __syncthreads();
-  const int d = threadIdx.x / 4;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (threadIdx.x % 4 * 2 + i) * 8;
-    float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = tile[r + e][d];
-    store8<T, TERMS>(L.dst_t + ((long)((r0 + r) / K) * L.Rt + d0 + d) * StepOf<TERMS>::row_bytes + r % K * 2, K * 2, v);
+    store8<T, TERMS>(L.dst + ((long)step * L.R + r) * StepOf<TERMS>::row_bytes + c % K * 2, K * 2, v);
   }
 }
 
@@ -473,16 +432,14 @@ __device__ __forceinline__ void make_scale(const XentBegin& A, float* join) {
   for (int n = threadIdx.x; n < count; n += 256) A.rho[n] = A.grad[A.state[kXentHead + n]] / by;
 }
 
-// 16384 x 4096 entries of a bf16 head and 8192 rows into both orders: 46 us (540 MB at the most, bound by HBM and the
-// LDS transposes).
 template <typename TO>
 __global__ __launch_bounds__(256) void k_xent_begin(const XentBegin A) {
-  __shared__ float tile[64][65];
+  __shared__ float join[256];
   int block = blockIdx.x;
-  if (A.number_rows && block-- == 0) return number_rows(A, (int*)tile);
-  if (A.make_scale && block-- == 0) return make_scale(A, &tile[0][0]);
+  if (A.number_rows && block-- == 0) return number_rows(A, (int*)join);
+  if (A.make_scale && block-- == 0) return make_scale(A, join);
   const bool second = block >= A.m[0].blocks;
-  lay_out<TO>(A.m[second], second ? block - A.m[0].blocks : block, tile);
+  lay_out<TO>(A.m[second], second ? block - A.m[0].blocks : block);
 }
 
 // ---- the ends ------------------------------------------------------------------------------------------
@@ -633,14 +590,14 @@ template <typename TO>
 struct XentPlan {
   static constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
   static constexpr long ROW = StepOf<TERMS>::row_bytes;
-  long Np, Dk, Dr, Dq;     // padded rows; D in whole steps (of k), of panel rows, of fp32 quads
+  long Np, Dk, Dq;         // padded rows; D in whole steps, in fp32 quads
   int d_steps;
   bool pack_w;             // W goes through panels
   long piece, pieces;      // vocabulary of a piece (a multiple of kPad) and how many
   int stats_tile;
   SplitTile dh, dw;        // dw in splits only where the vocabulary is one piece
   // offsets into the workspace
-  size_t h, w, part, picked, rows, ht, wt, g, gt, acc, acc_w, alpha, rho, bytes;
+  size_t h, w, part, picked, rows, g, acc, acc_w, alpha, rho, bytes;
 };
 
 template <typename TO>
@@ -650,7 +607,6 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   p.Np = up_to(N, kPad);
   p.Dk = up_to(D, P::K);
   p.d_steps = (int)(p.Dk / P::K);
-  p.Dr = up_to(D, 64);
   p.Dq = up_to(D, 4);
   // rows of whole steps of 16-byte chunks are read as they are
   p.pack_w = P::TERMS == 3 || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
@@ -677,10 +633,7 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   } else {
     p.dh = split_tile<TO>(D, N, std::min<long>(V, p.piece) / P::K, 32);
     p.dw = split_tile<TO>(D, std::min<long>(V, p.piece), p.Np / P::K, p.pieces > 1 ? 1 : 32);
-    p.ht = take((size_t)p.Np / P::K * p.Dr * P::ROW);
-    p.wt = take((size_t)p.piece / P::K * p.Dr * P::ROW);
     p.g = take((size_t)p.piece / P::K * p.Np * P::ROW);
-    p.gt = take((size_t)p.Np / P::K * p.piece * P::ROW);
     p.acc = take((size_t)p.dh.splits * p.Np * p.Dq * 4);
     p.acc_w = p.dw.splits > 1 ? take((size_t)p.dw.splits * p.piece * p.Dq * 4) : 0;
     p.alpha = take(4);
@@ -721,32 +674,40 @@ hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStre
 
 // Layout of H's compact rows.
 template <typename TO>
-XentLayout hidden_layout(const XentPlan<TO>& p, const XentCall& c, bool rows, bool columns) {
-  XentLayout L{c.H, c.state, c.N, (int)p.Np, c.D, p.d_steps, (int)p.Np, (int)p.Dr, nullptr, nullptr, 0};
-  L.dst = rows ? c.ws + p.h : nullptr;
-  L.dst_t = columns ? c.ws + p.ht : nullptr;
-  L.blocks = (int)(p.Np / 64 * ((c.D + 63) / 64));
-  return L;
+XentLayout hidden_layout(const XentPlan<TO>& p, const XentCall& c) {
+  return {c.H, c.state, c.N, (int)p.Np, c.D, p.d_steps, (int)p.Np, c.ws + p.h, (int)(p.Np / 64 * ((c.D + 63) / 64))};
 }
 
-// Layout of the entries [v0, v0 + n) of W (none where they are read as they are and their columns are not asked for).
+// Layout of the entries [v0, v0 + n) of W; none where W is read as it is.
 template <typename TO>
-XentLayout head_layout(const XentPlan<TO>& p, const XentCall& c, long v0, int n, bool columns) {
-  // (the products read whole tiles of panels: padded like the piece)
-  const int padded = (int)up_to(n, p.pack_w ? kPad : 64);
-  XentLayout L{(const TO*)c.W + v0 * c.D, nullptr, n, padded, c.D, p.d_steps, (int)p.piece, (int)p.Dr, nullptr, nullptr, 0};
-  L.dst = p.pack_w ? c.ws + p.w : nullptr;
-  L.dst_t = columns ? c.ws + p.wt : nullptr;
-  L.blocks = L.dst || L.dst_t ? padded / 64 * ((c.D + 63) / 64) : 0;
-  return L;
+XentLayout head_layout(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
+  if (!p.pack_w) return {};
+  const int padded = (int)up_to(n, kPad);  // (the products read whole tiles of panels)
+  return {(const TO*)c.W + v0 * c.D, nullptr, n, padded, c.D, p.d_steps, (int)p.piece, c.ws + p.w,
+          padded / 64 * ((c.D + 63) / 64)};
 }
 
-// Those entries as an operand of the products with H.
+// H's compact rows, G's and entries of W as operands: row after row, or column after column.
 template <typename TO>
-GemmOperand head_operand(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
-  typedef XentPlan<TO> P;
-  if (p.pack_w) return {c.ws + p.w, P::ROW, p.piece * P::ROW, (int)up_to(n, kPad)};
-  return {(const TO*)c.W + v0 * c.D, (long)c.D * (long)sizeof(TO), P::ROW, n};
+GemmOperand panel_rows(const char* p, long R, int rows) {
+  constexpr long ROW = XentPlan<TO>::ROW;
+  return {p, ROW, R * ROW, rows, 0, 0};
+}
+template <typename TO>
+GemmOperand panel_columns(const char* p, long R, int blocks) {
+  constexpr long ROW = XentPlan<TO>::ROW;
+  return {p, ROW, XentPlan<TO>::K * ROW, blocks, R * ROW, 0};
+}
+template <typename TO>
+GemmOperand head_rows(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
+  if (p.pack_w) return panel_rows<TO>(c.ws + p.w, p.piece, (int)up_to(n, kPad));
+  return {(const TO*)c.W + v0 * c.D, (long)c.D * (long)sizeof(TO), XentPlan<TO>::ROW, n, 0, 0};
+}
+template <typename TO>
+GemmOperand head_columns(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
+  if (p.pack_w) return panel_columns<TO>(c.ws + p.w, p.piece, p.d_steps);
+  const long row = (long)c.D * (long)sizeof(TO);
+  return {(const TO*)c.W + v0 * c.D, row, XentPlan<TO>::K * row, p.d_steps, XentPlan<TO>::ROW, n * row};
 }
 
 template <typename TO>
@@ -777,7 +738,7 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
   for (long v0 = 0; v0 < c.V; v0 += p.piece) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
     XentBegin F{};
-    F.m[0] = head_layout<TO>(p, c, v0, n, false);
+    F.m[0] = head_layout<TO>(p, c, v0, n);
     if (v0 == 0) {
       F.number_rows = 1;
       F.target = c.target; F.N = c.N; F.V = c.V; F.ignore = c.ignore; F.state = c.state; F.picked = picked; F.loss = rows;
@@ -785,12 +746,12 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
     XENT_TRY(launch_begin<TO>(F, st));
     if (v0 == 0) {
       XentBegin H{};
-      H.m[0] = hidden_layout<TO>(p, c, true, false);
+      H.m[0] = hidden_layout<TO>(p, c);
       XENT_TRY(launch_begin<TO>(H, st));
     }
     XentArgs A{};
-    A.A = head_operand<TO>(p, c, v0, n);
-    A.B = {c.ws + p.h, P::ROW, p.Np * P::ROW, (int)p.Np};
+    A.A = head_rows<TO>(p, c, v0, n);
+    A.B = panel_rows<TO>(c.ws + p.h, p.Np, (int)p.Np);
     A.steps = p.d_steps;
     A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0;
     A.part = (float2*)(c.ws + p.part) + tiles * p.Np;
@@ -820,29 +781,28 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
     const int n_steps = (int)(up_to(n, P::K) / P::K);
     XentBegin F{};
-    F.m[0] = head_layout<TO>(p, c, v0, n, c.dH != nullptr);
+    F.m[0] = head_layout<TO>(p, c, v0, n);
     if (v0 == 0) {
-      F.m[1] = hidden_layout<TO>(p, c, true, c.dW != nullptr);
+      F.m[1] = hidden_layout<TO>(p, c);
       F.make_scale = 1;
       F.state = c.state; F.grad = c.grad; F.reduction = c.reduction; F.up = up_of<TO>(); F.alpha = alpha; F.rho = rho;
     }
     XENT_TRY(launch_begin<TO>(F, st));
     XentArgs A{};
-    A.A = head_operand<TO>(p, c, v0, n);
-    A.B = {c.ws + p.h, P::ROW, p.Np * P::ROW, (int)p.Np};
+    A.A = head_rows<TO>(p, c, v0, n);
+    A.B = panel_rows<TO>(c.ws + p.h, p.Np, (int)p.Np);
     A.steps = p.d_steps;
     A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0; A.D = c.D;
     A.Np = p.Np; A.Vp = p.piece;
     A.rho = c.reduction ? nullptr : rho;
-    A.g = c.dH ? c.ws + p.g : nullptr;
-    A.gt = c.dW ? c.ws + p.gt : nullptr;
+    A.g = c.ws + p.g;
     // (every entry of the padded piece is written: tiles of 256 or 128 entries and rows)
     XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile_for<TO>(n, c.N, p.d_steps), 1, st)));
     A.alpha = alpha;
     if (c.dW) {
       XentArgs B = A;
-      B.A = {c.ws + p.ht, P::ROW, p.Dr * P::ROW, (int)p.Dr};
-      B.B = {c.ws + p.gt, P::ROW, p.piece * P::ROW, (int)p.piece};
+      B.A = panel_columns<TO>(c.ws + p.h, p.Np, p.d_steps);
+      B.B = panel_columns<TO>(c.ws + p.g, p.Np, (int)(up_to(n, kPad) / P::K));
       B.steps = (int)(p.Np / P::K);
       B.out = (TO*)c.dW + v0 * c.D;
       if (p.dw.splits == 1) {
@@ -857,8 +817,8 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     }
     if (c.dH) {
       XentArgs B = A;
-      B.A = {c.ws + p.wt, P::ROW, p.Dr * P::ROW, (int)p.Dr};
-      B.B = {c.ws + p.g, P::ROW, p.Np * P::ROW, (int)p.Np};
+      B.A = head_columns<TO>(p, c, v0, n);
+      B.B = panel_rows<TO>(c.ws + p.g, p.Np, (int)p.Np);
       B.steps = n_steps;
       B.steps_per_split = (n_steps + p.dh.splits - 1) / p.dh.splits;
       B.acc = (float*)(c.ws + p.acc); B.Dq = p.Dq;

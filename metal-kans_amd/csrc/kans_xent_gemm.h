@@ -12,8 +12,8 @@
 //
 // A workgroup of WAVES_M x WAVES_N waves holds a BM x BN tile.  A step's rows go from memory to LDS by DMA
 // (buffer loads, 16 bytes a lane) into one of two stages, or of three for A (A_STAGES).  The barrier that opens step
-// s + 1 stands before the last part of step s, whose operands are in registers by then: the first operands of step
-// s + 1 are read while the matrix pipe works on it.  The DMAs into the stages that step s has left go out in that
+// s + 1 stands before the last part of step s, whose operands are in registers by then; a part's operands are read
+// between the products of the part before it.  The DMAs into the stages that step s has left go out in that
 // part and the next one, a few between the products of each row of blocks: all of them at once fill the memory pipe's queue,
 // and the waves stand there.  The stages are separate arrays and the step loop is unrolled until they repeat,
 // so that the compiler sees that reads of one do not depend on the DMA into another.
@@ -123,68 +123,65 @@ struct GemmTile {
       return *(const frag*)(st + r * Step::row_bytes + slot * 16);
     };
     // Groups of 16 lanes take four k of 16 rows: a lane reads four rows' values at one k and gets four k of one row.  Its
-    // place, by the block's half of a 128-byte row and the four k of eight:
-    int place_t[TERMS == 1 ? 2 : 1][2];
+    // places in this wave's blocks, by the block's half of a 128-byte row (16-bit: two blocks share one) and the four k of
+    // eight; everything else is a constant distance from them.
+    constexpr int HALVES = TERMS == 1 ? 2 : 1;
+    static_assert(TERMS == 3 || ((MB % 2 == 0 || MB == 1) && (NB % 2 == 0 || NB == 1)), "a wave's blocks are whole pairs, or one");
+    int at_a[HALVES][2], at_b[HALVES][2];
     if constexpr (A_COLUMNS || B_COLUMNS) {
       const int in16 = lane & 15, rows16 = lane >> 4 & 1;
+      auto place_columns = [&](int w, int blocks, int q, int h) {  // of wave row or column w with so many blocks
+        const int k = half * 8 + h * 4 + in16 / 4, pair = TERMS == 3 ? 0 : blocks == 1 ? w & 1 : q;
+        const int first = TERMS == 3 ? w * blocks * 32 : w * blocks / 2 * 64;
+        return (first + k) * Step::row_bytes + Step::slot(k, pair * 4 + rows16 * 2 + in16 % 4 / 2) * 16 + in16 % 2 * 8;
+      };
 #pragma unroll
-      for (int q = 0; q < (TERMS == 1 ? 2 : 1); ++q)
+      for (int q = 0; q < HALVES; ++q)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int k = half * 8 + h * 4 + in16 / 4;
-          place_t[q][h] = k * Step::row_bytes + Step::slot(k, q * 4 + rows16 * 2 + in16 % 4 / 2) * 16 + in16 % 2 * 8;
+          at_a[q][h] = place_columns(wm, MB, q, h);
+          at_b[q][h] = place_columns(wn, NB, q, h);
         }
     }
-    auto read_columns = [&](const char* st, const int (&at)[TERMS == 1 ? 2 : 1][2], int block, int part, int term) {
+    auto read_columns = [&](const char* st, const int (&at)[HALVES][2], int block, int part, int term) {
       typedef short short4_t __attribute__((ext_vector_type(4)));
       struct { short4_t v[2]; } f;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        f.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) short4_t*)(st + (block * 32 / KS * KS + part * 16) * Step::row_bytes + term * 64 +
-                                                          at[TERMS == 1 ? block % 2 : 0][h]));
+        f.v[h] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(
+            st + (block * 32 / KS * KS + part * 16) * Step::row_bytes + term * 64 + at[block % HALVES][h]));
       return __builtin_bit_cast(frag, f);
     };
     frag a[2][MB][TERMS], b[2][NB][TERMS];
-    auto fetch = [&](const char* sa, const char* sb, int part, frag (&fa)[MB][TERMS], frag (&fb)[NB][TERMS]) {
-      int at[TERMS == 1 ? 2 : 1][2];
-      if constexpr (A_COLUMNS || B_COLUMNS) {
-        // (taken anew each time: the compiler would keep every sum of a place and a stage in a register of its own)
-#pragma unroll
-        for (int q = 0; q < (TERMS == 1 ? 2 : 1); ++q)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            at[q][h] = place_t[q][h];
-            asm volatile("" : "+v"(at[q][h]));
-          }
-      }
+    // The operands of one part in MB pieces: A's i-th block and its share of B's.
+    auto fetch = [&](const char* sa, const char* sb, int part, frag (&fa)[MB][TERMS], frag (&fb)[NB][TERMS], int i) {
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) {
+        if constexpr (A_COLUMNS) fa[i][t] = read_columns(sa, at_a, i, part, t);
+        else fa[i][t] = read_rows(sa, wm * MB + i, part, t);
 #pragma unroll
-        for (int i = 0; i < MB; ++i) {
-          if constexpr (A_COLUMNS) fa[i][t] = read_columns(sa, at, wm * MB + i, part, t);
-          else fa[i][t] = read_rows(sa, wm * MB + i, part, t);
-        }
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          if constexpr (B_COLUMNS) fb[j][t] = read_columns(sb, at, wn * NB + j, part, t);
-          else fb[j][t] = read_rows(sb, wn * NB + j, part, t);
-        }
+        for (int j = 0; j < NB; ++j)
+          if (j % MB == i) {
+            if constexpr (B_COLUMNS) fb[j][t] = read_columns(sb, at_b, j, part, t);
+            else fb[j][t] = read_rows(sb, wn * NB + j, part, t);
+          }
       }
-      __builtin_amdgcn_sched_barrier(0);
     };
-    // the products of one part; between(i) comes before those of the i-th row of blocks
+    // The products of one part.  between(i) goes out behind the first of the i-th row of blocks: what it issues is
+    // hidden by the matrix pipe (all of the next part's reads before the first product cost a tenth of dW's time).
     auto multiply = [&](const frag (&fa)[MB][TERMS], const frag (&fb)[NB][TERMS], auto between) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i) {
-        between(i);
+      for (int i = 0; i < MB; ++i)
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           if constexpr (TERMS == 3) acc[i][j] = mma_split(fa[i], fb[j], acc[i][j]);
           else acc[i][j] = Mfma<T>::mma(fa[i][0], fb[j][0], acc[i][j]);
+          if (j == 0) {
+            __builtin_amdgcn_sched_barrier(0);
+            between(i);
+          }
+          if (j == 0 || j == NB - 1) __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
-      }
     };
     // The DMAs that go out behind the barrier of step s: B of step s + 2, then A of step s + A_STAGES (so that those
     // which the next barrier need not wait for are the last); EACH of them before each of 2 MB rows of blocks.
@@ -203,10 +200,8 @@ struct GemmTile {
             if (on_a) dma_a(ra, sa, k < DMAS ? k - DMA_B : 0);
           }
         }
-        __builtin_amdgcn_sched_barrier(0);
       };
     };
-    auto nothing = [](int) {};
     // What this wave has read and asked for is there, but for the newest DMAs of A (of the step after the next) where
     // they have gone out; then all waves meet.
     auto meet = [&](bool newest_a_out) {
@@ -222,15 +217,25 @@ struct GemmTile {
     auto step = [&](int s, char* a_old, char* a_cur, char* a_nxt, char* b_cur, char* b_nxt, bool all) {
 #pragma unroll
       for (int p = 0; p + 1 < P; ++p) {
-        fetch(a_cur, b_cur, p + 1, a[(p + 1) & 1], b[(p + 1) & 1]);
-        if (p == 0) multiply(a[0], b[0], dma_between(s - 1, a_old, b_nxt, MB * EACH, all));
-        else multiply(a[p & 1], b[p & 1], nothing);
+        auto& fa = a[(p + 1) & 1];
+        auto& fb = b[(p + 1) & 1];
+        if (p == 0) {
+          const auto dma = dma_between(s - 1, a_old, b_nxt, MB * EACH, all);
+          multiply(a[0], b[0], [&](int i) {
+            fetch(a_cur, b_cur, p + 1, fa, fb, i);
+            dma(i);
+          });
+        } else {
+          multiply(a[p & 1], b[p & 1], [&](int i) { fetch(a_cur, b_cur, p + 1, fa, fb, i); });
+        }
       }
-      if (all || s + 1 < steps) {
-        meet(all || s + 2 < steps);  // every wave has read step s, and step s + 1 has landed
-        fetch(a_nxt, b_nxt, 0, a[0], b[0]);
-      }
-      multiply(a[1], b[1], dma_between(s, a_cur, b_cur, 0, all));
+      const bool next = all || s + 1 < steps;
+      if (next) meet(all || s + 2 < steps);  // every wave has read step s, and step s + 1 has landed
+      const auto dma = dma_between(s, a_cur, b_cur, 0, all);
+      multiply(a[1], b[1], [&](int i) {
+        if (next) fetch(a_nxt, b_nxt, 0, a[0], b[0], i);
+        dma(i);
+      });
     };
     // step 0, and what would have gone out behind the steps before it
     {
@@ -246,8 +251,10 @@ struct GemmTile {
       meet(steps > 1);
       const auto first_half = dma_between(-1, A_STAGES == 3 ? a_st2 : a_st1, b_st1, 0, false);
 #pragma unroll
-      for (int i = 0; i < MB; ++i) first_half(i);
-      fetch(a_st0, b_st0, 0, a[0], b[0]);
+      for (int i = 0; i < MB; ++i) {
+        fetch(a_st0, b_st0, 0, a[0], b[0], i);
+        first_half(i);
+      }
     }
     constexpr int ROUND = A_STAGES == 3 ? 6 : 2;  // steps until the stages repeat
     char* const as[3] = {a_st0, a_st1, a_st2};

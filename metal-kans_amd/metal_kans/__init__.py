@@ -31,7 +31,9 @@ def __getattr__(name):
             import torch  # noqa: F401
         except ImportError:
             return None
-        return getattr(import_module("." + _TORCH[name], __name__), name)
+        # (kept: the module's own name from here on, without this function's few microseconds at each use)
+        value = globals()[name] = getattr(import_module("." + _TORCH[name], __name__), name)
+        return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 __all__ = [

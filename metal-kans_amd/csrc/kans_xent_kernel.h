@@ -38,7 +38,8 @@ enum XentEpilogue { XE_STATS, XE_GRAD, XE_DW, XE_DW_SPLIT, XE_DH };
 struct XentArgs {
   GemmOperand A, B;
   int m_tiles, n_tiles;
-  int steps, steps_per_split;  // of k; products over the rows: bounded by the compact rows as well
+  int steps;                   // of k; products over the rows: bounded by the compact rows as well
+  int splits, most_splits;     // of k, as the grid has them; most that XE_DH makes of it
   const int* state;
   int N, V;                    // rows of the call; vocabulary (XE_STATS, XE_GRAD: entries of this piece)
   int v0;                      // first entry of the piece
@@ -50,7 +51,7 @@ struct XentArgs {
   const float* alpha;          // XE_DW: factor
   void* out;                   // XE_DW: dW of the piece [V][D]
   int D;
-  float* acc;                  // XE_DH: [split][Np][Dq] fp32; XE_DW_SPLIT: [split][Vp][Dq]
+  float* acc;                  // XE_DH: [split][rows of its tiles][Dq] fp32; XE_DW_SPLIT: [split][Vp][Dq]
   long Dq;
   int add;                     // XE_DH: add to acc
 };
@@ -99,6 +100,17 @@ __device__ __forceinline__ void pack8(const float* v, uint4 (&d)[TERMS]) {
   }
 }
 
+// How dH's products are shared out: a call's rows are known to the device alone, so the grid is made for all of
+// them (`n_tiles` tiles of bn columns, `splits` of k), and the workgroups of tiles without a row that counts go to more splits of
+// the others.
+struct XentShare {
+  int n_tiles, splits;
+};
+__device__ __forceinline__ XentShare share_of(int count, int bn, int n_tiles, int splits, int most) {
+  const int there = min((count + bn - 1) / bn, n_tiles);
+  return {there, min(n_tiles * splits / max(there, 1), most)};
+}
+
 // The products.  8192 x 4096 x 65536 bf16, 256 x 256 tiles (four pieces in the backward):
 //   XE_STATS 3.25 ms (1.35 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 4 x 0.93 ms (1.18: its
 //   stores, 268 MB in each of two orders), XE_DW 4 x 0.83 and XE_DH 4 x 0.83 ms (1.32).
@@ -117,18 +129,30 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   constexpr int MB = Tile::MB, NB = Tile::NB;
   __shared__ alignas(16) char a_st0[Tile::STAGE_A], a_st1[Tile::STAGE_A], a_st2[A_STAGES == 3 ? Tile::STAGE_A : 16];
   __shared__ alignas(16) char b_st0[Tile::STAGE_B], b_st1[Tile::STAGE_B];
-  int mt, nt;
-  tile_of<8>(xcd_remap(blockIdx.x, A.m_tiles * A.n_tiles), A.m_tiles, A.n_tiles, mt, nt);
-  const int m0 = mt * BM, n0 = nt * BN;
   const int count = A.state[0];  // compact rows
-  // (G of the rows that fill up the last step of k is written too: zeros)
   constexpr bool kOverRows = EPI == XE_DW || EPI == XE_DW_SPLIT;
+  int id = blockIdx.x, n_tiles = A.n_tiles, split = 0, splits = A.splits;
+  if constexpr (EPI == XE_DH) {
+    const XentShare share = share_of(count, BN, A.n_tiles, A.splits, A.most_splits);
+    n_tiles = share.n_tiles;
+    splits = share.splits;
+    split = id / max(A.m_tiles * n_tiles, 1);
+    id -= split * A.m_tiles * n_tiles;
+    if (split >= splits) return;
+  } else if constexpr (EPI == XE_DW_SPLIT) {
+    split = blockIdx.y;
+  }
+  int mt, nt;
+  tile_of<8>(xcd_remap(id, A.m_tiles * n_tiles), A.m_tiles, n_tiles, mt, nt);
+  const int m0 = mt * BM, n0 = nt * BN;
+  // (G of the rows that fill up the last step of k is written too: zeros)
   if (!kOverRows && n0 >= (EPI == XE_GRAD ? (count + 63) / 64 * 64 : count)) return;
   int first = 0, steps = A.steps;
   if (kOverRows) steps = min(steps, (count + Step::kStep - 1) / Step::kStep);
   if (EPI == XE_DH || EPI == XE_DW_SPLIT) {
-    first = blockIdx.y * A.steps_per_split;
-    steps = min(A.steps_per_split, steps - first);
+    const int each = (steps + splits - 1) / splits;
+    first = split * each;
+    steps = min(each, steps - first);
   }
   floatx16 acc[MB][NB];
   Tile::run(A.A, A.B, m0, n0, first, steps, a_st0, a_st1, a_st2, b_st0, b_st1, acc);
@@ -260,7 +284,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
         }
     }
   } else {
-    float* base = A.acc + (long)blockIdx.y * (EPI == XE_DH ? A.Np : A.Vp) * A.Dq;
+    float* base = A.acc + (long)split * (EPI == XE_DH ? n_tiles * BN : A.Vp) * A.Dq;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       float* o = base + (long)ncol(j) * A.Dq;
@@ -517,14 +541,16 @@ __device__ __forceinline__ void finish_row(const float* acc, int splits, long st
 
 // dH: compact rows into their own places, zeros for the ignored rows.
 template <typename TO>
-__global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, int splits, long Np, long Dq, int D,
+__global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, int bn, int n_tiles, int splits, int most, long Dq, int D,
                                                  const int* __restrict__ state, const int64_t* __restrict__ target,
                                                  int64_t ignore, const float* __restrict__ alpha, TO* __restrict__ dH) {
   const int row = blockIdx.x;
   if (target[row] == ignore)
     for (int d = threadIdx.x; d < D; d += 256) dH[(long)row * D + d] = (TO)0.0f;
-  if (row >= state[0]) return;
-  finish_row(acc + row * Dq, splits, Np * Dq, D, *alpha, dH + (long)state[kXentHead + row] * D);
+  const int count = state[0];
+  if (row >= count) return;
+  const XentShare share = share_of(count, bn, n_tiles, splits, most);
+  finish_row(acc + row * Dq, share.splits, (long)share.n_tiles * bn * Dq, D, *alpha, dH + (long)state[kXentHead + row] * D);
 }
 
 template <typename TO>
@@ -555,6 +581,11 @@ template <> struct Tiles<_Float16> {
 };
 template <> struct Tiles<__bf16> : Tiles<_Float16> {};
 
+template <typename TO>
+constexpr int tile_columns(int tile) {
+  return tile == TILE_LARGE ? Tiles<TO>::large_n : tile == TILE_NARROW ? Tiles<TO>::narrow_n : tile_rows(tile);
+}
+
 struct SplitTile {
   int tile, splits;
 };
@@ -566,7 +597,7 @@ SplitTile split_tile(long m, long n, long steps, int max_splits) {
   SplitTile best{TILE_LARGE, 1};
   double least = 1e300;
   for (int tile : {TILE_LARGE, TILE_SMALL, TILE_TINY}) {
-    const long bm = tile_rows(tile), bn = tile == TILE_LARGE ? Tiles<TO>::large_n : bm;
+    const long bm = tile_rows(tile), bn = tile_columns<TO>(tile);
     const long tiles = (m + bm - 1) / bm * ((n + bn - 1) / bn), slots = 256 * Tiles<TO>::per_cu[tile];
     for (int s = 1; s <= max_splits && (s == 1 || steps / s >= 4); ++s) {
       // (the tiles of a CU share it: a round that leaves each with one of several takes that share of the time)
@@ -596,6 +627,7 @@ struct XentPlan {
   long piece, pieces;      // vocabulary of a piece (a multiple of kPad) and how many
   int stats_tile;
   SplitTile dh, dw;        // dw in splits only where the vocabulary is one piece
+  int dh_most;             // splits of dh where rows are ignored (share_of)
   // offsets into the workspace
   size_t h, w, part, picked, rows, g, acc, acc_w, alpha, rho, bytes;
 };
@@ -632,6 +664,7 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
     p.rows = take((size_t)N * 4);
   } else {
     p.dh = split_tile<TO>(D, N, std::min<long>(V, p.piece) / P::K, 32);
+    p.dh_most = std::max<int>(p.dh.splits, (int)(std::min<long>(V, p.piece) / P::K / 8));
     p.dw = split_tile<TO>(D, std::min<long>(V, p.piece), p.Np / P::K, p.pieces > 1 ? 1 : 32);
     p.g = take((size_t)p.piece / P::K * p.Np * P::ROW);
     p.acc = take((size_t)p.dh.splits * p.Np * p.Dq * 4);
@@ -649,7 +682,10 @@ hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStre
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
     A.m_tiles = (int)((m + BM - 1) / BM);
     A.n_tiles = (int)((n + BN - 1) / BN);
-    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN>), dim3((unsigned)((long)A.m_tiles * A.n_tiles), splits),
+    A.splits = splits;
+    const long tiles = (long)A.m_tiles * A.n_tiles;
+    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN>),
+                       EPI == XE_DH ? dim3((unsigned)(tiles * splits)) : dim3((unsigned)tiles, splits),
                        dim3(WM * WN * 64), 0, st, A);
     return hipGetLastError();
   };
@@ -809,7 +845,6 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
         XENT_TRY((launch_gemm<TO, XE_DW>(B, c.D, n, p.dw.tile, 1, st)));
       } else {
         B.acc = (float*)(c.ws + p.acc_w); B.Dq = p.Dq;
-        B.steps_per_split = (B.steps + p.dw.splits - 1) / p.dw.splits;
         XENT_TRY((launch_gemm<TO, XE_DW_SPLIT>(B, c.D, n, p.dw.tile, p.dw.splits, st)));
         hipLaunchKernelGGL((k_xent_dw<TO>), dim3(n), dim3(256), 0, st, B.acc, p.dw.splits, p.piece, p.Dq, c.D, alpha, (TO*)c.dW);
         XENT_TRY(hipGetLastError());
@@ -820,15 +855,16 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
       B.A = head_columns<TO>(p, c, v0, n);
       B.B = panel_rows<TO>(c.ws + p.g, p.Np, (int)p.Np);
       B.steps = n_steps;
-      B.steps_per_split = (n_steps + p.dh.splits - 1) / p.dh.splits;
+      B.most_splits = p.dh_most;
       B.acc = (float*)(c.ws + p.acc); B.Dq = p.Dq;
       B.add = v0 > 0;
       XENT_TRY((launch_gemm<TO, XE_DH>(B, c.D, c.N, p.dh.tile, p.dh.splits, st)));
     }
   }
   if (c.dH) {
-    hipLaunchKernelGGL((k_xent_dh<TO>), dim3(c.N), dim3(256), 0, st, (const float*)(c.ws + p.acc), p.dh.splits, p.Np, p.Dq, c.D,
-                       c.state, c.target, c.ignore, alpha, (TO*)c.dH);
+    const int dh_columns = tile_columns<TO>(p.dh.tile);
+    hipLaunchKernelGGL((k_xent_dh<TO>), dim3(c.N), dim3(256), 0, st, (const float*)(c.ws + p.acc), dh_columns, (c.N + dh_columns - 1) / dh_columns,
+                       p.dh.splits, p.dh_most, p.Dq, c.D, c.state, c.target, c.ignore, alpha, (TO*)c.dH);
     XENT_TRY(hipGetLastError());
   }
   return hipSuccess;

@@ -117,6 +117,28 @@ def test_vocabulary_in_pieces(cuda, dt):
     check(mk, h, w, t, dt, "none", gen)
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("n,d,v", [(8180, 72, 33001),     # more than 2^28 logits
+                                   (5, 4099, 70001)])     # a head of more than 2^28 values, laid out anew
+def test_large_vocabulary_in_pieces(cuda, n, d, v, dt):
+    import metal_kans as mk
+    h, w, t, gen = data(n, d, v, dt, 4, ignored=0.2)
+    last = torch.arange(v - 11, v + 39, device="cuda").clamp_max(v - 1)[-min(n, 50):]
+    t[:len(last)] = last
+    check(mk, h, w, t, dt, "none", gen)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d,v,ignored", [(2100, 800, 9001, 0.9),    # dH's workgroups of rows that do not count
+                                           (1300, 300, 20011, 0.5),   # go to more splits of the others
+                                           (1000, 2050, 300, 0.97)])
+def test_work_shared_out_by_the_rows_that_count(cuda, n, d, v, ignored, dt):
+    import metal_kans as mk
+    h, w, t, gen = data(n, d, v, dt, 5, ignored=ignored)
+    t[1] = 0
+    check(mk, h, w, t, dt, "mean", gen)
+
+
 @pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("ignored", [0.1, 0.5, 0.97])
 def test_ignored_rows_take_part_in_nothing(cuda, ignored, dt):

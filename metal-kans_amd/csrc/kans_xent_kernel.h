@@ -23,7 +23,7 @@
 namespace kans {
 namespace {
 
-constexpr long kXentPiece = 1L << 27;  // elements of G in memory at a time
+constexpr long kXentPiece = 1L << 28;  // elements of G in memory at a time (2^27: 10 % slower at 3001 x 777 x 50021, 1 % at 8192 x 4096 x 65536)
 constexpr long kXentHeadPiece = 1L << 28;  // elements of the head that are laid out anew at a time
 constexpr int kPad = 256;              // compact rows and vocabulary of a piece are padded to this
 constexpr float kNoLogit = -__builtin_inff();

@@ -70,8 +70,10 @@ struct GemmTile {
     return resource(p + (long)(first + s) * o.step_stride, records);
   }
 
-  // acc = the tile at (m0, n0) over `steps` steps from step `first`.
-  static __device__ __forceinline__ void run(const GemmOperand& A, const GemmOperand& B, int m0, int n0, int first, int steps,
+  // acc = the tile at (m0, n0) over `steps` steps from step `first`; zeros in the waves whose rows of A or B are all
+  // behind the first `rows_m` or `rows_n`.
+  static __device__ __forceinline__ void run(const GemmOperand& A, const GemmOperand& B, int m0, int n0, int rows_m, int rows_n,
+                                             int first, int steps,
                                              char* a_st0, char* a_st1, char* a_st2, char* b_st0, char* b_st1,
                                              floatx16 (&acc)[MB][NB]) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -259,6 +261,29 @@ struct GemmTile {
     constexpr int ROUND = A_STAGES == 3 ? 6 : 2;  // steps until the stages repeat
     char* const as[3] = {a_st0, a_st1, a_st2};
     char* const bs[2] = {b_st0, b_st1};
+    if (m0 + wm * MB * 32 >= rows_m || n0 + wn * NB * 32 >= rows_n) {
+      // nothing to multiply: this wave's DMAs and barriers, in the same order
+      char *old = a_st2, *cur = a_st0, *nxt = a_st1, *b_cur = b_st0, *b_nxt = b_st1;
+      if (A_STAGES == 2) old = a_st1;
+#pragma unroll 1
+      for (int s = 0; s < steps; ++s) {
+        const auto second_half = dma_between(s - 1, old, b_nxt, MB * EACH, false);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) second_half(i);
+        if (s + 1 < steps) meet(s + 2 < steps);
+        const auto first_half = dma_between(s, cur, b_cur, 0, false);
+#pragma unroll
+        for (int i = 0; i < MB; ++i) first_half(i);
+        char *const a_third = old, *const b_first = b_cur;
+        old = cur;
+        cur = nxt;
+        nxt = A_STAGES == 3 ? a_third : old;
+        b_cur = b_nxt;
+        b_nxt = b_first;
+      }
+      __syncthreads();
+      return;
+    }
     auto round = [&](int s, bool all) {
       static_for<0, ROUND>([&](auto k) {
         constexpr int i = decltype(k)::value;

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   __shared__ alignas(16) char a_st0[Tile::STAGE_A], a_st1[Tile::STAGE_A], a_st2[A_STAGES == 3 ? Tile::STAGE_A : 16];
   __shared__ alignas(16) char b_st0[Tile::STAGE_B], b_st1[Tile::STAGE_B];
   const int count = A.state[0];  // compact rows
-  constexpr bool kOverRows = EPI == XE_DW || EPI == XE_DW_SPLIT;
+  constexpr bool kOverRows = EPI == XE_DW || EPI == XE_DW_SPLIT, kOverD = kOverRows || EPI == XE_DH;  // k; m
   int id = blockIdx.x, n_tiles = A.n_tiles, split = 0, splits = A.splits;
   if constexpr (EPI == XE_DH) {
     const XentShare share = share_of(count, BN, A.n_tiles, A.splits, A.most_splits);
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     steps = min(each, steps - first);
   }
   floatx16 acc[MB][NB];
-  Tile::run(A.A, A.B, m0, n0, first, steps, a_st0, a_st1, a_st2, b_st0, b_st1, acc);
+  Tile::run(A.A, A.B, m0, n0, kOverD ? A.D : A.V, kOverRows ? A.V : count, first, steps, a_st0, a_st1, a_st2, b_st0, b_st1, acc);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N, col = lane & 31, half = lane >> 5;

@@ -337,17 +337,21 @@ __device__ __forceinline__ void store8(char* p, int term, const float* v) {
 
 // A matrix [.][D] laid out for the products: panels [step of D][R][kStep] of its rows.  `padded` rows (a multiple
 // of 64) are written, zeros behind the last.  With `state` the rows are the compact ones (`rows` bounds their number)
-// and rows behind the last kPad that hold one stay as they are.
+// and rows behind the last kPad that hold one stay as they are; with `numbered` too, but each workgroup numbers them for
+// itself.
 struct XentLayout {
   const void* src;
   const int* state;
+  int numbered;
   int rows, padded, D, steps, R;
   char* dst;
   int blocks;  // of 64 rows x 64 elements
 };
 
 // What the products need before they start, in one launch: block 0 numbers the rows, the next one makes the
-// common factor of G, the others lay out H and a piece of W.
+// common factor of G, the others lay out H and a piece of W.  H's compact rows wait for their numbers: more than
+// kSelfNumbered rows of a forward are laid out by a launch of their own.
+constexpr int kSelfNumbered = 1024;  // rows that a workgroup numbers in one go
 struct XentBegin {
   XentLayout m[2];
   int number_rows, make_scale;
@@ -362,36 +366,13 @@ struct XentBegin {
   float *alpha, *rho;
 };
 
-template <typename TO>
-__device__ __forceinline__ void lay_out(const XentLayout& L, int block) {
-  typedef typename XentTypes<TO>::T T;
-  constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
-  const int across = (L.D + 63) / 64, r0 = block / across * 64, d0 = block % across * 64;
-  int rows = L.rows;
-  if (L.state) {
-    rows = min(rows, L.state[0]);
-    if (r0 >= (rows + kPad - 1) / kPad * kPad) return;
-  }
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = r0 + threadIdx.x / 8 + i * 32, c = d0 + threadIdx.x % 8 * 8, step = c / K;
-    if (step >= L.steps) return;
-    float v[8];
-    if (r < rows) {
-      row8((const TO*)L.src + (long)(L.state ? L.state[kXentHead + r] : r) * L.D, c, L.D, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    }
-    store8<T, TERMS>(L.dst + ((long)step * L.R + r) * StepOf<TERMS>::row_bytes + c % K * 2, K * 2, v);
-  }
-}
-
-// Numbers the rows that count, in their order, four to a thread.
-__device__ __forceinline__ void number_rows(const XentBegin& A, int* waves) {
+// Numbers the rows that count, in their order, four to a thread: per row its target and whether it counts, and its number;
+// how many there are.
+template <typename F>
+__device__ __forceinline__ int number_rows(const XentBegin& A, int* waves, const F& each) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int base = 0;
-  for (int r0 = 0; r0 < A.N; r0 += 1024) {
+  for (int r0 = 0; r0 < A.N; r0 += kSelfNumbered) {
     const int r = r0 + threadIdx.x * 4;
     int64_t t[4];
     bool in[4];
@@ -414,19 +395,53 @@ __device__ __forceinline__ void number_rows(const XentBegin& A, int* waves) {
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (in[e]) {
-        A.state[kXentHead + at] = r + e;
-        A.state[kXentHead + A.N + at] = t[e] >= 0 && t[e] < A.V ? (int)t[e] : -1;
-        ++at;
-      }
-      if (r + e < A.N) {
-        A.picked[r + e] = __builtin_nanf("");  // of a target outside the vocabulary
-        A.loss[r + e] = 0.0f;                  // of an ignored row
-      }
+      if (r + e < A.N) each(r + e, t[e], in[e], at);
+      at += in[e];
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) A.state[0] = base;
+  return base;
+}
+__device__ __forceinline__ void keep_numbers(const XentBegin& A, int* waves) {
+  const int count = number_rows(A, waves, [&](int r, int64_t t, bool in, int at) {
+    if (in) {
+      A.state[kXentHead + at] = r;
+      A.state[kXentHead + A.N + at] = t >= 0 && t < A.V ? (int)t : -1;
+    }
+    A.picked[r] = __builtin_nanf("");  // of a target outside the vocabulary
+    A.loss[r] = 0.0f;                  // of an ignored row
+  });
+  if (threadIdx.x == 0) A.state[0] = count;
+}
+
+template <typename TO>
+__device__ __forceinline__ void lay_out(const XentBegin& A, const XentLayout& L, int block, int* waves, int* row_of) {
+  typedef typename XentTypes<TO>::T T;
+  constexpr int TERMS = XentTypes<TO>::TERMS, K = StepOf<TERMS>::kStep;
+  const int across = (L.D + 63) / 64, r0 = block / across * 64, d0 = block % across * 64;
+  int rows = L.rows;
+  if (L.numbered) {
+    rows = number_rows(A, waves, [&](int r, int64_t, bool in, int at) {
+      if (in && at >= r0 && at < r0 + 64) row_of[at - r0] = r;
+    });
+  } else if (L.state) {
+    rows = min(rows, L.state[0]);
+  }
+  if ((L.numbered || L.state) && r0 >= (rows + kPad - 1) / kPad * kPad) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = r0 + threadIdx.x / 8 + i * 32, c = d0 + threadIdx.x % 8 * 8, step = c / K;
+    if (step >= L.steps) return;
+    float v[8];
+    if (r < rows) {
+      const int from = L.numbered ? row_of[r - r0] : L.state ? L.state[kXentHead + r] : r;
+      row8((const TO*)L.src + (long)from * L.D, c, L.D, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+    }
+    store8<T, TERMS>(L.dst + ((long)step * L.R + r) * StepOf<TERMS>::row_bytes + c % K * 2, K * 2, v);
+  }
 }
 
 // The factor common to all rows of G (up: the scale that G is stored with) and each row's share of it.
@@ -460,10 +475,10 @@ template <typename TO>
 __global__ __launch_bounds__(256) void k_xent_begin(const XentBegin A) {
   __shared__ float join[256];
   int block = blockIdx.x;
-  if (A.number_rows && block-- == 0) return number_rows(A, (int*)join);
+  if (A.number_rows && block-- == 0) return keep_numbers(A, (int*)join);
   if (A.make_scale && block-- == 0) return make_scale(A, join);
   const bool second = block >= A.m[0].blocks;
-  lay_out<TO>(A.m[second], second ? block - A.m[0].blocks : block);
+  lay_out<TO>(A, A.m[second], second ? block - A.m[0].blocks : block, (int*)join, (int*)join + 64);
 }
 
 // ---- the ends ------------------------------------------------------------------------------------------
@@ -711,7 +726,7 @@ hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStre
 // Layout of H's compact rows.
 template <typename TO>
 XentLayout hidden_layout(const XentPlan<TO>& p, const XentCall& c) {
-  return {c.H, c.state, c.N, (int)p.Np, c.D, p.d_steps, (int)p.Np, c.ws + p.h, (int)(p.Np / 64 * ((c.D + 63) / 64))};
+  return {c.H, c.state, 0, c.N, (int)p.Np, c.D, p.d_steps, (int)p.Np, c.ws + p.h, (int)(p.Np / 64 * ((c.D + 63) / 64))};
 }
 
 // Layout of the entries [v0, v0 + n) of W; none where W is read as it is.
@@ -719,7 +734,7 @@ template <typename TO>
 XentLayout head_layout(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
   if (!p.pack_w) return {};
   const int padded = (int)up_to(n, kPad);  // (the products read whole tiles of panels)
-  return {(const TO*)c.W + v0 * c.D, nullptr, n, padded, c.D, p.d_steps, (int)p.piece, c.ws + p.w,
+  return {(const TO*)c.W + v0 * c.D, nullptr, 0, n, padded, c.D, p.d_steps, (int)p.piece, c.ws + p.w,
           padded / 64 * ((c.D + 63) / 64)};
 }
 
@@ -775,12 +790,17 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
     XentBegin F{};
     F.m[0] = head_layout<TO>(p, c, v0, n);
+    const bool numbered = c.N <= kSelfNumbered;
     if (v0 == 0) {
       F.number_rows = 1;
+      if (numbered) {
+        F.m[1] = hidden_layout<TO>(p, c);
+        F.m[1].numbered = 1;
+      }
       F.target = c.target; F.N = c.N; F.V = c.V; F.ignore = c.ignore; F.state = c.state; F.picked = picked; F.loss = rows;
     }
     XENT_TRY(launch_begin<TO>(F, st));
-    if (v0 == 0) {
+    if (v0 == 0 && !numbered) {
       XentBegin H{};
       H.m[0] = hidden_layout<TO>(p, c);
       XENT_TRY(launch_begin<TO>(H, st));

@@ -105,13 +105,20 @@ template <typename T>
 __device__ __forceinline__ Raw<T> load_or_one(const T* p, long at, int left) {
   return p ? load_raw(p + at, left) : fill_raw<T>(1.0f);
 }
+// Results leave nontemporal: lines that are written whole need not be read or kept.  y and h of 2048 x 4096 bf16: 12.1 us
+// (plain stores 16.4), of 16384 x 4096: 80 (112); with an operation behind them that reads both: 23.5 (26.5) and 161 (185).
+// (Nontemporal loads as well: 14.7 and 94 us, as what a caller has just written is no longer found in a cache.)
+template <typename T> using Wide = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, int left, const float* o) {
   T v[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) v[e] = from_f32<T>(o[e]);
   if (left >= V) {
-    __builtin_memcpy(p, v, sizeof(v));
+    Wide<T> w[sizeof(v) / 16];
+    __builtin_memcpy(w, v, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(v) / 16); ++i) __builtin_nontemporal_store(w[i], (Wide<T>*)p + i);
   } else {
 #pragma unroll
     for (int e = 0; e < V; ++e)
@@ -170,7 +177,7 @@ __device__ __forceinline__ void row_stats(const float (&v)[V], int left, int D, 
 template <int TPR> constexpr int threads_of() { return TPR > 512 ? TPR : 512; }
 template <int TPR> constexpr int rows_of() { return threads_of<TPR>() / TPR; }
 
-// Bound by HBM: 16384 x 4096 bf16 (537 MB) in 115 - 126 us, 4.3 - 4.7 TB/s (a copy reaches 4.8).  One row's worth of threads
+// Bound by HBM: 16384 x 4096 bf16 (537 MB) in 80 us where the inputs are partly in a cache (6.7 TB/s), 90 - 105 cold.  One row's worth of threads
 // a row with 8 elements each: two vectors a thread (half the threads) took 137 us.  A single row of 4096 is 8 waves and two
 // barriers; its call is bound by the launch.
 template <typename TX, typename TB, bool kLayer, int TPR>

@@ -82,10 +82,10 @@ __device__ __forceinline__ Raw<T> fill_raw(float v) {
   return r;
 }
 
-// V elements from p, of which `left` exist (the others 0).  Rows start at any element: the device takes wide
-// accesses at any address.
+// V elements of a row of D from p on, of which `left` exist (maybe none), 0 for the others.  Rows start at any element:
+// the device takes wide accesses at any address.
 template <typename T>
-__device__ __forceinline__ Raw<T> load_raw(const T* p, int left) {
+__device__ __forceinline__ Raw<T> load_part(const T* p, int left) {
   Raw<T> r;
   if (left >= V) {
     __builtin_memcpy(&r, p, sizeof(r));
@@ -101,9 +101,41 @@ __device__ __forceinline__ Raw<T> load_raw(const T* p, int left) {
   }
   return r;
 }
+// The same in two steps: load_raw asks for the values, settle makes them usable.  In 16 bits the narrow loads at the end of
+// a row are put together at once, which waits for them, and with them for all loads that are under way.  So there (kShift) a
+// thread at the end of the row reads its last V elements instead, in the one access that all make, and settle moves them to
+// their places: 30000 x 2047 bf16, forward 143 -> 94 us, both directions 589 -> 309; 10000 x 7000: 125 -> 122, 443 -> 360.  (fp32,
+// with nothing to put together, is 5 - 10 % slower so.)  `here` elements exist from p on, `left` of them count: all, or
+// none in a row that is not there (p is then another row's).
+template <typename T> constexpr bool shifts() { return sizeof(T) == 2; }
+template <bool kShift, typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* p, int here, int left, int D) {
+  if constexpr (!kShift) return load_part(p, left);
+  if (D < V) return load_part(p, here);
+  Raw<T> r;
+  __builtin_memcpy(&r, p - max(V - here, 0), sizeof(r));
+  return r;
+}
+template <bool kShift, typename T>
+__device__ __forceinline__ void settle(Raw<T>& r, int left, int D) {
+  if constexpr (kShift) {
+    const int back = min(max(V - left, 0), V);
+    if (!__builtin_amdgcn_ballot_w64(back != 0)) return;
+    if (D >= V) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) r.w[i] = back & 1 ? r.w[i] >> 16 | (i + 1 < V / 2 ? r.w[i + 1] << 16 : 0u) : r.w[i];
+#pragma unroll
+      for (int by = 1; by < V / 2; by *= 2)
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) r.w[i] = back & 2 * by ? (i + by < V / 2 ? r.w[i + by] : 0u) : r.w[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) r.w[i] = back == V ? 0u : r.w[i];
+  }
+}
 template <typename T>
 __device__ __forceinline__ Raw<T> load_or_one(const T* p, long at, int left) {
-  return p ? load_raw(p + at, left) : fill_raw<T>(1.0f);
+  return p ? load_part(p + at, left) : fill_raw<T>(1.0f);
 }
 // Results leave nontemporal: lines that are written whole need not be read or kept.  y and h of 2048 x 4096 bf16: 12.1 us
 // (plain stores 16.4), of 16384 x 4096: 80 (112); with an operation behind them that reads both: 23.5 (26.5) and 161 (185).
@@ -184,16 +216,23 @@ template <typename TX, typename TB, bool kLayer, int TPR>
 __global__ __launch_bounds__(threads_of<TPR>()) void k_resnorm_fwd(const NormArgs A) {
   __shared__ float lds[2][2][16];
   const long row = (long)blockIdx.x * rows_of<TPR>() + threadIdx.x / TPR;
-  const int at = threadIdx.x % TPR * V, D = A.D, left = row < A.rows ? D - at : 0;  // elements of this thread
-  const long base = row * D + at;
-  const Raw<TX> x = load_raw((const TX*)A.x + base, left);
+  const int at = threadIdx.x % TPR * V, D = A.D, here = D - at, left = row < A.rows ? here : 0;  // elements of this thread
+  const long there = min(row, A.rows - 1), base = there * D + at;  // (a row that is not there reads the last)
+  constexpr bool kx = shifts<TX>(), kb = shifts<TB>();
+  Raw<TX> x = load_raw<kx>((const TX*)A.x + base, here, left, D);
   int slot = 0;
   float y[V], mean_b = 0.0f, r_b = 0.0f;
-  const Raw<TB> nw = load_or_one((const TB*)A.pre_w, at, left);
+  auto load_or_one = [&](const void* p, long from) {
+    return p ? load_raw<kb>((const TB*)p + from, here, left, D) : fill_raw<TB>(1.0f);
+  };
+  Raw<TB> nw = load_or_one(A.pre_w, at);
   if (A.block) {
-    const Raw<TB> bv = load_raw((const TB*)A.block + base, left);
-    const Raw<TB> g = load_or_one((const TB*)A.gate, row / A.gate_group * D + at, left);
-    const Raw<TB> pw = load_or_one((const TB*)A.post_w, at, left);
+    Raw<TB> bv = load_raw<kb>((const TB*)A.block + base, here, left, D);
+    Raw<TB> g = load_or_one(A.gate, there / A.gate_group * D + at), pw = load_or_one(A.post_w, at);
+    settle<kb>(bv, left, D);
+    settle<kx>(x, left, D);
+    settle<kb>(g, left, D);
+    settle<kb>(pw, left, D);
     const float scale = A.scale_dev ? *A.scale_dev : A.scale;
     float b[V];
 #pragma unroll
@@ -204,9 +243,11 @@ __global__ __launch_bounds__(threads_of<TPR>()) void k_resnorm_fwd(const NormArg
       y[e] = e < left ? get(x, e) + scale * get(g, e) * ((b[e] - mean_b) * r_b * get(pw, e)) : 0.0f;
     store_vec((TX*)A.y + base, left, y);
   } else {
+    settle<kx>(x, left, D);
 #pragma unroll
     for (int e = 0; e < V; ++e) y[e] = get(x, e);
   }
+  settle<kb>(nw, left, D);
   float mean_y, r_y, h[V];
   row_stats<kLayer, TPR>(y, left, D, A.eps, lds, slot, mean_y, r_y);
 #pragma unroll
@@ -231,16 +272,19 @@ struct RowIn {
   float r_b, r_y, mean_b, mean_y;
 };
 
-// (a row that is not there: zeros, which add nothing to any sum)
+// Asks for row `row`; one behind `last` is not there, and its values are zeros, which add nothing to any sum.
 template <typename TX, typename TB, bool kLayer>
-__device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, long row, bool there, int at, bool gate_rows) {
-  const long base = row * A.D + at;
-  const int left = there ? A.D - at : 0;
-  in.x = load_raw((const TX*)A.x + base, left);
-  in.dy = load_raw((const TX*)A.dy + base, A.dy ? left : 0);
-  in.dh = load_raw((const TB*)A.dh + base, A.dh ? left : 0);
-  in.b = load_raw((const TB*)A.block + base, A.block ? left : 0);
-  if (gate_rows) in.g = load_raw((const TB*)A.gate + base, left);
+__device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, long row, long last, int at, bool gate_rows) {
+  constexpr bool kx = shifts<TX>(), kb = shifts<TB>();
+  const bool there = row <= last;
+  const int D = A.D, here = D - at, left = there ? here : 0;
+  row = min(row, last);
+  const long base = row * D + at;
+  in.x = load_raw<kx>((const TX*)A.x + base, here, left, D);
+  if (A.dy) in.dy = load_raw<kx>((const TX*)A.dy + base, here, left, D);
+  if (A.dh) in.dh = load_raw<kb>((const TB*)A.dh + base, here, left, D);
+  if (A.block) in.b = load_raw<kb>((const TB*)A.block + base, here, left, D);
+  if (gate_rows) in.g = load_raw<kb>((const TB*)A.gate + base, here, left, D);
   const float* s = A.stats + row * (kLayer ? 4 : 2);
   in.r_b = there ? s[0] : 0.0f;
   in.r_y = there ? s[1] : 0.0f;
@@ -250,13 +294,15 @@ __device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, l
 
 // One workgroup takes the rows of a run, rows_of<TPR>() at a time, with the next ones' loads in flight (at
 // 1024 threads the 128 registers that a thread may have do not hold them too).  Two workgroups a CU, with
-// up to 256 registers: held to 128 the kernel spills, and 16384 x 4096 bf16 (805 MB) take 600 us instead of 170 - 200
-// (4.0 - 4.7 TB/s).
+// up to 256 registers: held to 128 the kernel spills, and 16384 x 4096 bf16 (805 MB) take 600 us instead of 155 - 190
+// (4.2 - 5.2 TB/s).
 template <typename TX, typename TB, bool kLayer, int TPR>
 __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnorm_bwd(const NormArgs A) {
   constexpr int ROWS = rows_of<TPR>();
   __shared__ float lds[2][2][16];
+  constexpr bool kAhead = TPR <= 512;
   __shared__ float sums[ROWS > 1 ? TPR * V : 1];
+  __shared__ float4 kept[kAhead ? 1 : 3 * V / 4 * TPR];
   const int at = threadIdx.x % TPR * V, sub = threadIdx.x / TPR;
   const int D = A.D, left = D - at;
   const long chunk = blockIdx.x, group = chunk / A.chunks_per_group;
@@ -265,37 +311,66 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
   const bool gate_rows = A.gate && A.gate_group == 1;
   const float scale = A.scale_dev ? *A.scale_dev : A.scale;
   Raw<TB> pw = load_or_one((const TB*)A.post_w, at, left), nw = load_or_one((const TB*)A.pre_w, at, left);
-  RowIn<TX, TB> next;
-  next.g = load_or_one((const TB*)A.gate, group * D + at, gate_rows ? 0 : left);
-  float s_pre[V], s_post[V], s_gate[V], s_scale = 0.0f;
+  RowIn<TX, TB> next{};
+  if (!gate_rows) next.g = load_or_one((const TB*)A.gate, group * D + at, left);
+  // sums of this thread's columns over the run's rows: pre_w, post_w, gate.  At 1024 threads a row they lie in LDS, each
+  // thread its own, so that the rest fits in 128 registers: 8192 x 8192 bf16, both directions, 382 -> 301 us, fp32 780 -> 573.
+  float s[kAhead ? 3 : 1][V], s_scale = 0.0f;
+  auto kept_at = [&](int k, int i) { return &kept[(k * (V / 4) + i) * TPR + threadIdx.x]; };
+  auto add_up = [&](int k, const float(&v)[V]) {
+    if constexpr (kAhead) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) s_pre[e] = s_post[e] = s_gate[e] = 0.0f;
+      for (int e = 0; e < V; ++e) s[k][e] += v[e];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) {
+        float4 o = *kept_at(k, i);
+        o.x += v[4 * i]; o.y += v[4 * i + 1]; o.z += v[4 * i + 2]; o.w += v[4 * i + 3];
+        *kept_at(k, i) = o;
+      }
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[k][e] = 0.0f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) *kept_at(k, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
   const float inv_d = 1.0f / (float)D;
-  constexpr bool kAhead = TPR <= 512;
-  if (kAhead) load_row<TX, TB, kLayer>(next, A, first + sub, first + sub < end, at, gate_rows);
+  if (kAhead) load_row<TX, TB, kLayer>(next, A, first + sub, end - 1, at, gate_rows);
   for (long row0 = first; row0 < end; row0 += ROWS) {
     const long row = row0 + sub;
-    if (!kAhead) load_row<TX, TB, kLayer>(next, A, row, row < end, at, gate_rows);
+    if (!kAhead) load_row<TX, TB, kLayer>(next, A, row, end - 1, at, gate_rows);
     RowIn<TX, TB> in = next;
-    if (kAhead && row0 + ROWS < end) load_row<TX, TB, kLayer>(next, A, row + ROWS, row + ROWS < end, at, gate_rows);
+    if (kAhead && row0 + ROWS < end) load_row<TX, TB, kLayer>(next, A, row + ROWS, end - 1, at, gate_rows);
     const long base = row * D + at;
     const int out = row < end ? left : 0;
+    constexpr bool kx = shifts<TX>(), kb = shifts<TB>();
+    settle<kx>(in.x, out, D);
+    settle<kx>(in.dy, out, D);
+    settle<kb>(in.dh, out, D);
+    settle<kb>(in.b, out, D);
+    if (gate_rows) settle<kb>(in.g, out, D);
     auto bn = [&](int e) { return e < left ? (get(in.b, e) - in.mean_b) * in.r_b : 0.0f; };
     auto yn = [&](int e) {
       const float y = get(in.x, e) + scale * get(in.g, e) * (bn(e) * get(pw, e));
       return e < left ? (y - in.mean_y) * in.r_y : 0.0f;
     };
-    float t[V], sa = 0.0f, sb = 0.0f;
+    float t[V], add[V], sa = 0.0f, sb = 0.0f;
     repack(pw);
     repack(nw);
     repack(in.g);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float dh = get(in.dh, e), q = get(nw, e) * dh, n = yn(e);
-      s_pre[e] += dh * n;
+      add[e] = dh * n;
       sa += q * n;
       sb += q;
     }
+    add_up(0, add);
     row_sum2<TPR>(sa, sb, lds, 0);
     sa *= inv_d;
     sb = kLayer ? sb * inv_d : 0.0f;
@@ -311,13 +386,14 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
       const float q = get(nw, e) * get(in.dh, e), g = get(in.g, e), b = bn(e), u = b * get(pw, e);
       t[e] = get(in.dy, e) + in.r_y * (q - yn(e) * sa - sb);
       dg[e] = scale * t[e] * u;
-      s_gate[e] += dg[e];
       s_scale += e < left ? t[e] * (g * u) : 0.0f;
       const float du = scale * g * t[e], p = du * get(pw, e);
-      s_post[e] += du * b;
+      add[e] = du * b;
       pa += p * b;
       pb += e < left ? p : 0.0f;
     }
+    add_up(1, add);
+    add_up(2, dg);
     if (A.dx) store_vec((TX*)A.dx + base, out, t);
     if (gate_rows && A.dgate) {
       if (A.gate_f32) store_vec((float*)A.dgate + base, out, dg);
@@ -341,18 +417,23 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
   }
   // the run's partial rows; where several rows go at a time, those of the same columns one after the other
   float* part = A.part + chunk * A.parts * D;
-  auto put = [&](int at_part, const float(&s)[V]) {
+  auto put = [&](int at_part, int k) {
     if (at_part < 0) return;
     float* o = part + (long)at_part * D;
-    if constexpr (ROWS == 1) {
-      store_vec(o + at, left, s);
+    if constexpr (!kAhead) {
+      float v[V];
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) __builtin_memcpy(v + 4 * i, kept_at(k, i), 16);
+      store_vec(o + at, left, v);
+    } else if constexpr (ROWS == 1) {
+      store_vec(o + at, left, s[k]);
     } else {
       for (int w = 0; w < ROWS; ++w) {
         if (sub == w) {
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             float* c = &sums[e * TPR + threadIdx.x % TPR];
-            *c = w == 0 ? s[e] : *c + s[e];
+            *c = w == 0 ? s[k][e] : *c + s[k][e];
           }
         }
         __syncthreads();
@@ -361,9 +442,9 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
       __syncthreads();
     }
   };
-  put(A.at_pre, s_pre);
-  put(A.at_post, s_post);
-  put(A.at_gate, s_gate);
+  put(A.at_pre, 0);
+  put(A.at_post, 1);
+  put(A.at_gate, 2);
   if (A.want_scale) {
     float none = 0.0f;
     __syncthreads();

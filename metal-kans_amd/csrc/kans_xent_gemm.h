@@ -47,7 +47,7 @@ template <int TERMS> struct StepOf {
   }
 };
 
-template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES, bool A_COLUMNS, bool B_COLUMNS>
+template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES, bool A_COLUMNS, bool B_COLUMNS, bool A_ONCE>
 struct GemmTile {
   using Step = StepOf<TERMS>;
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
@@ -110,9 +110,10 @@ struct GemmTile {
     const char *pa = start(A, m0, a_columns), *pb = start(B, n0, b_columns);
     auto source_a = [&](int s) { return source<A_COLUMNS>(A, pa, s, first); };
     auto source_b = [&](int s) { return source<B_COLUMNS>(B, pb, s, first); };
+    // (A_ONCE: no other tile reads A's rows, so they need not stay in a cache: nontemporal)
     auto dma_a = [&](const __amdgpu_buffer_rsrc_t& o, char* st, int i) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(o, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16,
-                                               off_a[i], 0, 0, 0);
+                                               off_a[i], 0, 0, A_ONCE ? 2 : 0);
     };
     auto dma_b = [&](const __amdgpu_buffer_rsrc_t& o, char* st, int i) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(o, (__attribute__((address_space(3))) void*)(st + (i * WAVES + wave) * 1024), 16,

@@ -116,7 +116,7 @@ __device__ __forceinline__ XentShare share_of(int count, int bn, int n_tiles, in
 //   stores, 268 MB in each of two orders), XE_DW 4 x 0.83 and XE_DH 4 x 0.83 ms (1.32).
 // The matrix pipe is busy three quarters of the cycles at the 1.65 GHz that its power leaves; LDS reads meet no
 // bank conflict.  4096 (3700 count) x 1024 x 32768 fp32, 256 x 128: 1.19, 1.41, 1.07 and 1.20 ms (1.25 PFLOP/s of bf16 products).
-template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N>
+template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N, bool A_ONCE = false>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentArgs A) {
   typedef typename XentTypes<TO>::T T;
   constexpr int TERMS = XentTypes<TO>::TERMS;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   constexpr int A_STAGES = TERMS == 1 && BM == 256 && BN == 256 ? 3 : 2;
   // dW = G^T H and dH = G W run along the rows of their operands: H and G, or W
   using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES, EPI != XE_STATS && EPI != XE_GRAD,
-                        EPI == XE_DW || EPI == XE_DW_SPLIT>;
+                        EPI == XE_DW || EPI == XE_DW_SPLIT, A_ONCE>;
   using Step = StepOf<TERMS>;
   constexpr int MB = Tile::MB, NB = Tile::NB;
   __shared__ alignas(16) char a_st0[Tile::STAGE_A], a_st1[Tile::STAGE_A], a_st2[A_STAGES == 3 ? Tile::STAGE_A : 16];
@@ -693,28 +693,39 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
 
 template <typename TO, int EPI>
 hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStream_t st) {
-  auto go = [&](auto bm, auto bn, auto wm, auto wn) {
+  auto go = [&](auto bm, auto bn, auto wm, auto wn, auto once) {
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
     A.m_tiles = (int)((m + BM - 1) / BM);
     A.n_tiles = (int)((n + BN - 1) / BN);
     A.splits = splits;
     const long tiles = (long)A.m_tiles * A.n_tiles;
-    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN>),
+    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN, decltype(once)::value>),
                        EPI == XE_DH ? dim3((unsigned)(tiles * splits)) : dim3((unsigned)tiles, splits),
                        dim3(WM * WN * 64), 0, st, A);
     return hipGetLastError();
   };
   using std::integral_constant;
+  typedef integral_constant<int, 1> c1;
   typedef integral_constant<int, 2> c2;
   typedef integral_constant<int, 4> c4;
   typedef integral_constant<int, 128> c128;
   typedef integral_constant<int, 256> c256;
+  constexpr std::false_type again{};
   if constexpr (EPI == XE_STATS || EPI == XE_GRAD)
-    if (tile == TILE_NARROW) return go(c256{}, integral_constant<int, Tiles<TO>::narrow_n>{}, c4{}, integral_constant<int, 1>{});
-  if (tile == TILE_SMALL) return go(c128{}, c128{}, c2{}, c2{});
-  if (tile == TILE_TINY) return go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, c2{}, c2{});
-  if constexpr (sizeof(TO) == 4) return go(c256{}, c128{}, c4{}, c2{});
-  else return go(c256{}, c256{}, c2{}, c4{});
+    if (tile == TILE_NARROW) {
+      // One tile of rows reads the head's entries once.  The forward does so nontemporal where the caches (256 MB) will not hold
+      // the most of the head until its next pass: 16 x 4096 x 131072 bf16 (1.1 GB) 193.8 -> 175.1 us, a step of 20 rows (820 MB)
+      // 1052 -> 1013, (410 MB) 533 -> 528; 30 x 1024 x 130000 (266 MB) 333, and 344 so.  (The backward's products read it twice more:
+      // nontemporal there too 1025 and 544.)
+      constexpr integral_constant<int, Tiles<TO>::narrow_n> narrow{};
+      if (EPI == XE_STATS && (double)m * A.steps * StepOf<XentTypes<TO>::TERMS>::row_bytes > 350e6)
+        return go(c256{}, narrow, c4{}, c1{}, std::true_type{});
+      return go(c256{}, narrow, c4{}, c1{}, again);
+    }
+  if (tile == TILE_SMALL) return go(c128{}, c128{}, c2{}, c2{}, again);
+  if (tile == TILE_TINY) return go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, c2{}, c2{}, again);
+  if constexpr (sizeof(TO) == 4) return go(c256{}, c128{}, c4{}, c2{}, again);
+  else return go(c256{}, c256{}, c2{}, c4{}, again);
 }
 
 #define XENT_TRY(expr)                  \

@@ -226,9 +226,11 @@ __global__ __launch_bounds__(256) void k_adamw_values(const unsigned* mc, const 
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < quads; i += (long)gridDim.x * 256) {
     const float s = ms[i / 64], r = vs[i / 64];
     const unsigned a = mc[i], b = vc[i];
-    m[i] = make_float4(avg_value((signed char)a, s), avg_value((signed char)(a >> 8), s),
-                       avg_value((signed char)(a >> 16), s), avg_value((signed char)(a >> 24), s));
-    v[i] = make_float4(sq_value(b & 255, r), sq_value((b >> 8) & 255, r), sq_value((b >> 16) & 255, r), sq_value(b >> 24, r));
+    const float mv[4] = {avg_value((signed char)a, s), avg_value((signed char)(a >> 8), s),
+                         avg_value((signed char)(a >> 16), s), avg_value((signed char)(a >> 24), s)};
+    const float vv[4] = {sq_value(b & 255, r), sq_value((b >> 8) & 255, r), sq_value((b >> 16) & 255, r), sq_value(b >> 24, r)};
+    store4((float*)(m + i), 4, true, mv);
+    store4((float*)(v + i), 4, true, vv);
   }
 }
 

@@ -1,4 +1,4 @@
-"""The compiled autograd functions of ``csrc/kans_torch.cpp``, bound to the library that ``device`` loaded."""
+"""The compiled torch operators of ``csrc/kans_torch.cpp``, bound to the library that ``device`` loaded."""
 from __future__ import annotations
 
 import ctypes
@@ -9,7 +9,7 @@ from . import device
 
 _FUNCTIONS = ("kans_last_error", "kans_stream_keep", "kans_residual_norm_forward", "kans_residual_norm_workspace",
               "kans_residual_norm_backward", "kans_linear_xent_workspace", "kans_linear_xent_forward",
-              "kans_linear_xent_backward")
+              "kans_linear_xent_backward", "kans_adamw_step")
 _module = None
 
 

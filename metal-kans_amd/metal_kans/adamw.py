@@ -26,6 +26,7 @@ import torch
 
 from . import device
 from ._engine import DT_BF16, DT_F16, DT_F32
+from ._torch_ops import load
 from .torch_module import _current_stream
 
 _DT = {torch.float32: DT_F32, torch.float16: DT_F16, torch.bfloat16: DT_BF16}
@@ -57,8 +58,7 @@ class _Arena:
             self.flat["exp_avg_sq_scale"] = zeros(total, f32)
         if self.dtype != f32:
             self.flat["master"] = zeros(total * BLOCK, f32)
-        self._numel = array("q", self.numel)
-        self._blocks = array("q", self.blocks)
+        self.numel_q, self.blocks_q = array("q", self.numel), array("q", self.blocks)
 
     def views(self, i: int) -> Dict[str, torch.Tensor]:
         b, n, shape = self.blocks[i], self.numel[i], self.params[i].shape
@@ -226,49 +226,9 @@ class TorchAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        lib = device.get_metal_bridge()
         for gi, group in enumerate(self.param_groups):
+            lr, (b1, b2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
             for a in self._group_arenas(gi):
-                self._step_arena(lib, group, a)
+                load().adamw_step(self.state, a.params, a.numel_q, a.blocks_q, a.flat, _DT[a.dtype], a.bits,
+                                  lambda i, a=a: self.state.__setitem__(a.params[i], a.start(i, {})), lr, b1, b2, eps, decay)
         return loss
-
-    def _step_arena(self, lib, group, a: _Arena) -> None:
-        ids, params, grads, steps, keep = [], [], [], [], []
-        for i, p in enumerate(a.params):
-            g = p.grad
-            if g is None:
-                continue
-            if g.layout is not torch.strided or g.dtype != a.dtype or g.device != a.device:
-                raise TypeError(f"gradients must be dense {a.dtype} tensors on {a.device}")
-            if p.dtype != a.dtype or p.device != a.device or p.numel() != a.numel[i]:
-                raise ValueError("a parameter's dtype, device or size changed under its optimizer")
-            if g.stride() != p.stride():  # (elements are paired by their place in memory)
-                g = torch.empty_like(p).copy_(g)
-            keep.append(g)
-            ids.append(i)
-            params.append(p.data_ptr())
-            grads.append(g.data_ptr())
-            st = self.state.get(p)
-            if not st:
-                st = self.state[p] = a.start(i, {})
-            steps.append(st["step"] + 1)
-        if not ids:
-            return
-        whole = len(ids) == len(a.params)
-        arrays = [array("Q", params), array("Q", grads),
-                  a._numel if whole else array("q", [a.numel[i] for i in ids]),
-                  a._blocks if whole else array("q", [a.blocks[i] for i in ids]), array("q", steps)]
-        at = [v.buffer_info()[0] for v in arrays]
-        f = a.flat
-        ptr = lambda name: f[name].data_ptr() if name in f else None  # noqa: E731
-        b1, b2 = group["betas"]
-        device.check(lib.kans_adamw_step(
-            _DT[a.dtype], a.bits, len(ids), *at, ptr("exp_avg"), ptr("exp_avg_sq"), ptr("exp_avg_scale"),
-            ptr("exp_avg_sq_scale"), ptr("master"), float(group["lr"]), float(b1), float(b2), float(group["eps"]),
-            float(group["weight_decay"]), _current_stream(a.device)), "kans_adamw_step")
-        changed = []
-        for i, t in zip(ids, steps):
-            p = a.params[i]
-            self.state[p]["step"] = t
-            changed.append(p)
-        torch.autograd.graph.increment_version(changed)

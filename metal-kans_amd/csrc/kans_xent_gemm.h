@@ -8,7 +8,8 @@
 // Both cover a row-major matrix (as itself or as its transpose) and panels [step][row][kStep] of one, whose rows of a
 // step are one contiguous run; the second reads its operands from LDS transposed (ds_read_b64_tr_b16).  So one layout of a
 // matrix serves the products along either dimension.  fp32 operands (TERMS = 3) are the three bf16 terms of
-// kans_split.h, [term][32] in a step, and take six MFMAs a product.
+// kans_split.h, [term][32] in a step, and take six MFMAs a product; A's may lie in memory as they are (A_RAW, rows of whole
+// steps of 32), and are split on their way from LDS to the products.
 //
 // A workgroup of WAVES_M x WAVES_N waves holds a BM x BN tile.  A step's rows go from memory to LDS by DMA
 // (buffer loads, 16 bytes a lane) into one of two stages, or of three for A (A_STAGES).  The barrier that opens step
@@ -47,12 +48,15 @@ template <int TERMS> struct StepOf {
   }
 };
 
-template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES, bool A_COLUMNS, bool B_COLUMNS, bool A_ONCE>
+template <typename T, int TERMS, int BM, int BN, int WAVES_M, int WAVES_N, int A_STAGES, bool A_COLUMNS, bool B_COLUMNS, bool A_ONCE,
+          bool A_RAW>
 struct GemmTile {
+  static_assert(!A_RAW || (TERMS == 3 && !A_COLUMNS), "raw fp32 rows of A");
   using Step = StepOf<TERMS>;
+  using LinesA = StepOf<A_RAW ? 1 : TERMS>;  // a step's rows of A in LDS: raw ones are 128 bytes, as 16-bit ones are
   static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = WAVES * 64;
   static constexpr int MB = BM / WAVES_M / 32, NB = BN / WAVES_N / 32;  // 32 x 32 blocks of a wave
-  static constexpr int STAGE_A = BM * Step::row_bytes, STAGE_B = BN * Step::row_bytes;  // bytes of a stage
+  static constexpr int STAGE_A = BM * LinesA::row_bytes, STAGE_B = BN * Step::row_bytes;  // bytes of a stage
   static constexpr int DMA_A = STAGE_A / 1024 / WAVES, DMA_B = STAGE_B / 1024 / WAVES;  // of a wave
   static_assert(DMA_A * 1024 * WAVES == STAGE_A && DMA_B * 1024 * WAVES == STAGE_B, "whole DMAs");
   static_assert(A_STAGES == 2 || (A_STAGES == 3 && DMA_A < 16), "stages of A");
@@ -92,8 +96,9 @@ struct GemmTile {
       if constexpr (decltype(columns)::value) return (const char*)o.p + (long)min(tile0 / KS, o.rows - 1) * o.block_stride;
       else return (const char*)o.p + (long)min(tile0, o.rows - 1) * o.row_stride;
     };
-    auto place = [&](int q, int tile0, const GemmOperand& o, auto columns) {
-      const int row = q / Step::chunks, chunk = Step::slot(row, q - row * Step::chunks);
+    auto place = [&](int q, int tile0, const GemmOperand& o, auto columns, auto lines) {
+      using L = decltype(lines);
+      const int row = q / L::chunks, chunk = L::slot(row, q - row * L::chunks);
       if constexpr (decltype(columns)::value) {
         const int b0 = min(tile0 / KS, o.rows - 1), block = min(tile0 / KS + row / KS, o.rows - 1) - b0;
         return (unsigned)block * (unsigned)o.block_stride + (unsigned)(row % KS) * (unsigned)o.row_stride + chunk * 16;
@@ -104,9 +109,9 @@ struct GemmTile {
     constexpr std::integral_constant<bool, A_COLUMNS> a_columns{};
     constexpr std::integral_constant<bool, B_COLUMNS> b_columns{};
 #pragma unroll
-    for (int i = 0; i < DMA_A; ++i) off_a[i] = place((i * WAVES + wave) * 64 + lane, m0, A, a_columns);
+    for (int i = 0; i < DMA_A; ++i) off_a[i] = place((i * WAVES + wave) * 64 + lane, m0, A, a_columns, LinesA{});
 #pragma unroll
-    for (int i = 0; i < DMA_B; ++i) off_b[i] = place((i * WAVES + wave) * 64 + lane, n0, B, b_columns);
+    for (int i = 0; i < DMA_B; ++i) off_b[i] = place((i * WAVES + wave) * 64 + lane, n0, B, b_columns, Step{});
     const char *pa = start(A, m0, a_columns), *pb = start(B, n0, b_columns);
     auto source_a = [&](int s) { return source<A_COLUMNS>(A, pa, s, first); };
     auto source_b = [&](int s) { return source<B_COLUMNS>(B, pb, s, first); };
@@ -155,12 +160,26 @@ struct GemmTile {
             st + (block * 32 / KS * KS + part * 16) * Step::row_bytes + term * 64 + at[block % HALVES][h]));
       return __builtin_bit_cast(frag, f);
     };
+    // raw rows: eight fp32 values, made into their terms before the products
+    struct Raw8 { float4 v[2]; };
+    auto read_raw = [&](const char* st, int block, int part) {
+      const int r = block * 32 + row, chunk = part * 4 + half * 2;
+      Raw8 f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) f.v[h] = *(const float4*)(st + r * LinesA::row_bytes + LinesA::slot(r, chunk + h) * 16);
+      return f;
+    };
+    Raw8 raw[2][A_RAW ? MB : 1];
     frag a[2][MB][TERMS], b[2][NB][TERMS];
     // The operands of one part in MB pieces: A's i-th block and its share of B's.
-    auto fetch = [&](const char* sa, const char* sb, int part, frag (&fa)[MB][TERMS], frag (&fb)[NB][TERMS], int i) {
+    auto fetch = [&](const char* sa, const char* sb, int part, int to, int i) {
+      auto& fa = a[to];
+      auto& fb = b[to];
+      if constexpr (A_RAW) raw[to][i] = read_raw(sa, wm * MB + i, part);
 #pragma unroll
       for (int t = 0; t < TERMS; ++t) {
-        if constexpr (A_COLUMNS) fa[i][t] = read_columns(sa, at_a, i, part, t);
+        if constexpr (A_RAW) {
+        } else if constexpr (A_COLUMNS) fa[i][t] = read_columns(sa, at_a, i, part, t);
         else fa[i][t] = read_rows(sa, wm * MB + i, part, t);
 #pragma unroll
         for (int j = 0; j < NB; ++j)
@@ -172,9 +191,18 @@ struct GemmTile {
     };
     // The products of one part.  between(i) goes out behind the first of the i-th row of blocks: what it issues is
     // hidden by the matrix pipe (all of the next part's reads before the first product cost a tenth of dW's time).
-    auto multiply = [&](const frag (&fa)[MB][TERMS], const frag (&fb)[NB][TERMS], auto between) {
+    auto multiply = [&](int from, auto between) {
+      auto& fa = a[from];
+      const auto& fb = b[from];
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+      for (int i = 0; i < MB; ++i) {
+        if constexpr (A_RAW) {
+          float v[8];
+          __builtin_memcpy(v, &raw[from][i], sizeof(v));
+          const Split8 s = split8(v);
+#pragma unroll
+          for (int t = 0; t < TERMS; ++t) fa[i][t] = __builtin_bit_cast(frag, s.t[t]);
+        }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
           if constexpr (TERMS == 3) acc[i][j] = mma_split(fa[i], fb[j], acc[i][j]);
@@ -185,6 +213,7 @@ struct GemmTile {
           }
           if (j == 0 || j == NB - 1) __builtin_amdgcn_sched_barrier(0);
         }
+      }
     };
     // The DMAs that go out behind the barrier of step s: B of step s + 2, then A of step s + A_STAGES (so that those
     // which the next barrier need not wait for are the last); EACH of them before each of 2 MB rows of blocks.
@@ -220,23 +249,21 @@ struct GemmTile {
     auto step = [&](int s, char* a_old, char* a_cur, char* a_nxt, char* b_cur, char* b_nxt, bool all) {
 #pragma unroll
       for (int p = 0; p + 1 < P; ++p) {
-        auto& fa = a[(p + 1) & 1];
-        auto& fb = b[(p + 1) & 1];
         if (p == 0) {
           const auto dma = dma_between(s - 1, a_old, b_nxt, MB * EACH, all);
-          multiply(a[0], b[0], [&](int i) {
-            fetch(a_cur, b_cur, p + 1, fa, fb, i);
+          multiply(0, [&](int i) {
+            fetch(a_cur, b_cur, p + 1, 1, i);
             dma(i);
           });
         } else {
-          multiply(a[p & 1], b[p & 1], [&](int i) { fetch(a_cur, b_cur, p + 1, fa, fb, i); });
+          multiply(p & 1, [&](int i) { fetch(a_cur, b_cur, p + 1, (p + 1) & 1, i); });
         }
       }
       const bool next = all || s + 1 < steps;
       if (next) meet(all || s + 2 < steps);  // every wave has read step s, and step s + 1 has landed
       const auto dma = dma_between(s, a_cur, b_cur, 0, all);
-      multiply(a[1], b[1], [&](int i) {
-        if (next) fetch(a_nxt, b_nxt, 0, a[0], b[0], i);
+      multiply(1, [&](int i) {
+        if (next) fetch(a_nxt, b_nxt, 0, 0, i);
         dma(i);
       });
     };
@@ -255,7 +282,7 @@ struct GemmTile {
       const auto first_half = dma_between(-1, A_STAGES == 3 ? a_st2 : a_st1, b_st1, 0, false);
 #pragma unroll
       for (int i = 0; i < MB; ++i) {
-        fetch(a_st0, b_st0, 0, a[0], b[0], i);
+        fetch(a_st0, b_st0, 0, 0, i);
         first_half(i);
       }
     }

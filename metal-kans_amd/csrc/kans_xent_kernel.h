@@ -38,6 +38,7 @@ enum XentEpilogue { XE_STATS, XE_GRAD, XE_DW, XE_DW_SPLIT, XE_DH };
 struct XentArgs {
   GemmOperand A, B;
   int m_tiles, n_tiles;
+  int raw;                     // (host) narrow tiles of fp32: A is raw rows
   int steps;                   // of k; products over the rows: bounded by the compact rows as well
   int splits, most_splits;     // of k, as the grid has them; most that XE_DH makes of it
   const int* state;
@@ -116,15 +117,15 @@ __device__ __forceinline__ XentShare share_of(int count, int bn, int n_tiles, in
 //   stores, 268 MB in each of two orders), XE_DW 4 x 0.83 and XE_DH 4 x 0.83 ms (1.32).
 // The matrix pipe is busy three quarters of the cycles at the 1.65 GHz that its power leaves; LDS reads meet no
 // bank conflict.  4096 (3700 count) x 1024 x 32768 fp32, 256 x 128: 1.19, 1.41, 1.07 and 1.20 ms (1.25 PFLOP/s of bf16 products).
-template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N, bool A_ONCE = false>
+template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N, bool A_ONCE = false, bool A_RAW = false>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentArgs A) {
   typedef typename XentTypes<TO>::T T;
   constexpr int TERMS = XentTypes<TO>::TERMS;
   // a third stage of A where the tile has a CU's LDS for itself and it still fits (160 KB)
-  constexpr int A_STAGES = TERMS == 1 && BM == 256 && BN == 256 ? 3 : 2;
+  constexpr int A_STAGES = (TERMS == 1 && BM == 256 && BN == 256) || A_RAW ? 3 : 2;
   // dW = G^T H and dH = G W run along the rows of their operands: H and G, or W
   using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES, EPI != XE_STATS && EPI != XE_GRAD,
-                        EPI == XE_DW || EPI == XE_DW_SPLIT, A_ONCE>;
+                        EPI == XE_DW || EPI == XE_DW_SPLIT, A_ONCE, A_RAW>;
   using Step = StepOf<TERMS>;
   constexpr int MB = Tile::MB, NB = Tile::NB;
   __shared__ alignas(16) char a_st0[Tile::STAGE_A], a_st1[Tile::STAGE_A], a_st2[A_STAGES == 3 ? Tile::STAGE_A : 16];
@@ -579,26 +580,31 @@ inline long up_to(long v, long m) { return (v + m - 1) / m * m; }
 
 // Tiles of a product: the large one, the small one (128 x 128) or the tiny one (64 x 64); few rows get a narrow one.
 enum { TILE_LARGE, TILE_SMALL, TILE_TINY, TILE_NARROW };
-constexpr int tile_rows(int tile) { return tile == TILE_SMALL ? 128 : tile == TILE_TINY ? 64 : 256; }
 template <typename TO> struct Tiles;
 // per_cu, cost: small and tiny tiles that a CU holds at a time, and the time of a step of that many, in steps of a
 // large tile.  Measured: 16-bit tiles of 128 x 128, two a CU, reach 3/4 of the rate of one of 256 x 256; fp32 (98 KB of
 // LDS, one a CU) 2/3 of that of 256 x 128.  Tiny tiles read LDS twice as often a product, at about half the rate.
+// Narrow tiles have 128 entries of the head, so that a CU holds two or three: with 256, 16 x 4096 x 32000 bf16 took 73 us
+// instead of 49 (125 tiles for 256 CUs), 24 x 800 x 77870 fp32 89 instead of 69.
 template <> struct Tiles<float> {
-  static constexpr int large_m = 256, large_n = 128, narrow_n = 64;
+  static constexpr int large_m = 256, large_n = 128, narrow_m = 128, narrow_n = 64;
   static constexpr int per_cu[3] = {1, 1, 3};
   static constexpr double cost[3] = {1.0, 0.7, 0.6};
 };
 template <> struct Tiles<_Float16> {
-  static constexpr int large_m = 256, large_n = 256, narrow_n = 32;
+  static constexpr int large_m = 256, large_n = 256, narrow_m = 128, narrow_n = 32;
   static constexpr int per_cu[3] = {1, 2, 5};
   static constexpr double cost[3] = {1.0, 0.65, 0.7};
 };
 template <> struct Tiles<__bf16> : Tiles<_Float16> {};
 
 template <typename TO>
+constexpr int tile_rows(int tile) {
+  return tile == TILE_SMALL ? 128 : tile == TILE_TINY ? 64 : tile == TILE_NARROW ? Tiles<TO>::narrow_m : 256;
+}
+template <typename TO>
 constexpr int tile_columns(int tile) {
-  return tile == TILE_LARGE ? Tiles<TO>::large_n : tile == TILE_NARROW ? Tiles<TO>::narrow_n : tile_rows(tile);
+  return tile == TILE_LARGE ? Tiles<TO>::large_n : tile == TILE_NARROW ? Tiles<TO>::narrow_n : tile_rows<TO>(tile);
 }
 
 struct SplitTile {
@@ -612,7 +618,7 @@ SplitTile split_tile(long m, long n, long steps, int max_splits) {
   SplitTile best{TILE_LARGE, 1};
   double least = 1e300;
   for (int tile : {TILE_LARGE, TILE_SMALL, TILE_TINY}) {
-    const long bm = tile_rows(tile), bn = tile_columns<TO>(tile);
+    const long bm = tile_rows<TO>(tile), bn = tile_columns<TO>(tile);
     const long tiles = (m + bm - 1) / bm * ((n + bn - 1) / bn), slots = 256 * Tiles<TO>::per_cu[tile];
     for (int s = 1; s <= max_splits && (s == 1 || steps / s >= 4); ++s) {
       // (the tiles of a CU share it: a round that leaves each with one of several takes that share of the time)
@@ -655,8 +661,9 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   p.Dk = up_to(D, P::K);
   p.d_steps = (int)(p.Dk / P::K);
   p.Dq = up_to(D, 4);
-  // rows of whole steps of 16-byte chunks are read as they are
-  p.pack_w = P::TERMS == 3 || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
+  // rows of whole steps of 16-byte chunks are read as they are; fp32 ones by the forward of few rows, which is bound by
+  // reading them (24 x 800 x 77870, 249 MB: 69 us, with panels 191)
+  p.pack_w = (P::TERMS == 3 && (backward || N > Tiles<TO>::narrow_n)) || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
   const long all = up_to(V, kPad);
   p.piece = std::max<long>(kPad, std::min({all, kXentPiece / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
   // (in one piece where nothing of it is laid out; a grid holds fewer than 2^32 threads, 2^-7 of the logits)
@@ -673,7 +680,7 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   p.h = take((size_t)p.d_steps * p.Np * P::ROW);
   p.w = p.pack_w ? take((size_t)p.d_steps * p.piece * P::ROW) : 0;
   if (!backward) {
-    const int bm = tile_rows(p.stats_tile);
+    const int bm = tile_rows<TO>(p.stats_tile);
     p.part = take((size_t)((V + bm - 1) / bm + p.pieces) * p.Np * sizeof(float2));
     p.picked = take((size_t)N * 4);
     p.rows = take((size_t)N * 4);
@@ -693,13 +700,13 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
 
 template <typename TO, int EPI>
 hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStream_t st) {
-  auto go = [&](auto bm, auto bn, auto wm, auto wn, auto once) {
+  auto go = [&](auto bm, auto bn, auto wm, auto wn, auto once, auto raw) {
     constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
     A.m_tiles = (int)((m + BM - 1) / BM);
     A.n_tiles = (int)((n + BN - 1) / BN);
     A.splits = splits;
     const long tiles = (long)A.m_tiles * A.n_tiles;
-    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN, decltype(once)::value>),
+    hipLaunchKernelGGL((k_xent_gemm<TO, EPI, BM, BN, WM, WN, decltype(once)::value, decltype(raw)::value>),
                        EPI == XE_DH ? dim3((unsigned)(tiles * splits)) : dim3((unsigned)tiles, splits),
                        dim3(WM * WN * 64), 0, st, A);
     return hipGetLastError();
@@ -710,22 +717,28 @@ hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStre
   typedef integral_constant<int, 4> c4;
   typedef integral_constant<int, 128> c128;
   typedef integral_constant<int, 256> c256;
-  constexpr std::false_type again{};
+  constexpr std::false_type no{};
   if constexpr (EPI == XE_STATS || EPI == XE_GRAD)
     if (tile == TILE_NARROW) {
       // One tile of rows reads the head's entries once.  The forward does so nontemporal where the caches (256 MB) will not hold
       // the most of the head until its next pass: 16 x 4096 x 131072 bf16 (1.1 GB) 193.8 -> 175.1 us, a step of 20 rows (820 MB)
       // 1052 -> 1013, (410 MB) 533 -> 528; 30 x 1024 x 130000 (266 MB) 333, and 344 so.  (The backward's products read it twice more:
       // nontemporal there too 1025 and 544.)
+      constexpr integral_constant<int, Tiles<TO>::narrow_m> tall{};
       constexpr integral_constant<int, Tiles<TO>::narrow_n> narrow{};
-      if (EPI == XE_STATS && (double)m * A.steps * StepOf<XentTypes<TO>::TERMS>::row_bytes > 350e6)
-        return go(c256{}, narrow, c4{}, c1{}, std::true_type{});
-      return go(c256{}, narrow, c4{}, c1{}, again);
+      constexpr std::true_type yes{};
+      if constexpr (EPI == XE_STATS) {
+        const bool once = (double)m * A.steps * (A.raw ? 128 : StepOf<XentTypes<TO>::TERMS>::row_bytes) > 350e6;
+        if constexpr (XentTypes<TO>::TERMS == 3)
+          if (A.raw) return once ? go(tall, narrow, c4{}, c1{}, yes, yes) : go(tall, narrow, c4{}, c1{}, no, yes);
+        if (once) return go(tall, narrow, c4{}, c1{}, yes, no);
+      }
+      return go(tall, narrow, c4{}, c1{}, no, no);
     }
-  if (tile == TILE_SMALL) return go(c128{}, c128{}, c2{}, c2{}, again);
-  if (tile == TILE_TINY) return go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, c2{}, c2{}, again);
-  if constexpr (sizeof(TO) == 4) return go(c256{}, c128{}, c4{}, c2{}, again);
-  else return go(c256{}, c256{}, c2{}, c4{}, again);
+  if (tile == TILE_SMALL) return go(c128{}, c128{}, c2{}, c2{}, no, no);
+  if (tile == TILE_TINY) return go(integral_constant<int, 64>{}, integral_constant<int, 64>{}, c2{}, c2{}, no, no);
+  if constexpr (sizeof(TO) == 4) return go(c256{}, c128{}, c4{}, c2{}, no, no);
+  else return go(c256{}, c256{}, c2{}, c4{}, no, no);
 }
 
 #define XENT_TRY(expr)                  \
@@ -763,7 +776,7 @@ GemmOperand panel_columns(const char* p, long R, int blocks) {
 template <typename TO>
 GemmOperand head_rows(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
   if (p.pack_w) return panel_rows<TO>(c.ws + p.w, p.piece, (int)up_to(n, kPad));
-  return {(const TO*)c.W + v0 * c.D, (long)c.D * (long)sizeof(TO), XentPlan<TO>::ROW, n, 0, 0};
+  return {(const TO*)c.W + v0 * c.D, (long)c.D * (long)sizeof(TO), XentPlan<TO>::K * (long)sizeof(TO), n, 0, 0};
 }
 template <typename TO>
 GemmOperand head_columns(const XentPlan<TO>& p, const XentCall& c, long v0, int n) {
@@ -795,7 +808,7 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
   const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, false);
   float* rows = c.reduction ? (float*)(c.ws + p.rows) : c.loss;
   float* picked = (float*)(c.ws + p.picked);
-  const int bm = tile_rows(p.stats_tile);
+  const int bm = tile_rows<TO>(p.stats_tile);
   long tiles = 0;
   for (long v0 = 0; v0 < c.V; v0 += p.piece) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
@@ -818,6 +831,7 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
     }
     XentArgs A{};
     A.A = head_rows<TO>(p, c, v0, n);
+    A.raw = !p.pack_w;
     A.B = panel_rows<TO>(c.ws + p.h, p.Np, (int)p.Np);
     A.steps = p.d_steps;
     A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0;

@@ -117,6 +117,20 @@ def test_vocabulary_in_pieces(cuda, dt):
     check(mk, h, w, t, dt, "none", gen)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d,v", [(1, 32, 1), (3, 96, 129), (31, 64, 127), (32, 128, 4097), (33, 32, 300), (64, 160, 20001),
+                                   (65, 64, 1000), (2, 1024, 700), (24, 30, 1000), (4, 4096, 24000)])
+def test_few_rows(cuda, n, d, v, dt):
+    """Heads read as they are, in fp32 too, and the borders of the tiles that do it; a head of no aligned rows."""
+    import metal_kans as mk
+    h, w, t, gen = data(n, d, v, dt, n * v)
+    check(mk, h, w, t, dt, "none", gen)
+    shifted = torch.empty(v * d + 1, dtype=w.dtype, device="cuda")[1:].view(v, d).copy_(w)
+    with torch.no_grad():
+        a, b = (mk.linear_cross_entropy(h, x, t, reduction="none") for x in (w, shifted))
+    assert (a - b).abs().max() <= 1e-4 * (1 + a.abs().max())
+
+
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("n,d,v", [(8180, 72, 33001),     # more than 2^28 logits
                                    (5, 4099, 70001)])     # a head of more than 2^28 values, laid out anew

@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kAdamThreads) void k_adamw(const AdamwBatch A) {
   }
 }
 
-// The values of 8-bit states: a wave takes one block, 4 elements a lane (97 M of each moment, 970 MB: 170 us, 5.7 TB/s).
+// The values of 8-bit states: a wave takes one block, 4 elements a lane (97 M of each moment, 970 MB: 170 - 190 us).
 __global__ __launch_bounds__(256) void k_adamw_values(const unsigned* mc, const unsigned* vc, const float* ms,
                                                       const float* vs, float4* m, float4* v, long quads) {
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < quads; i += (long)gridDim.x * 256) {

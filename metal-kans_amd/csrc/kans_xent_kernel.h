@@ -2,8 +2,9 @@
 //
 // The logits are computed twice: for the sums of the softmax, and again in the backward, a piece of the vocabulary
 // at a time, where the epilogue turns them into G.  Only G of one piece is ever in memory (16-bit, or three
-// bf16 terms for fp32; at most kXentPiece elements) and goes into the two products behind it.  H, G and a head whose rows are not whole steps
-// lie in panels that serve the products along either of their dimensions; another head is read as it is.
+// bf16 terms for fp32; at most kXentPiece elements) and goes into the two products behind it.  H, G and a head whose
+// rows are not whole steps lie in panels that serve the products along either of their dimensions; another head is
+// read as it is.
 // 8 N D V operations in all against the 6 N D V of a program that keeps the logits: the price of
 // not writing and reading N V of them.
 //
@@ -112,11 +113,13 @@ __device__ __forceinline__ XentShare share_of(int count, int bn, int n_tiles, in
   return {there, min(n_tiles * splits / max(there, 1), most)};
 }
 
-// The products.  8192 x 4096 x 65536 bf16, 256 x 256 tiles (four pieces in the backward):
-//   XE_STATS 3.25 ms (1.35 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 4 x 0.93 ms (1.18: its
-//   stores, 268 MB in each of two orders), XE_DW 4 x 0.83 and XE_DH 4 x 0.83 ms (1.32).
-// The matrix pipe is busy three quarters of the cycles at the 1.65 GHz that its power leaves; LDS reads meet no
-// bank conflict.  4096 (3700 count) x 1024 x 32768 fp32, 256 x 128: 1.19, 1.41, 1.07 and 1.20 ms (1.25 PFLOP/s of bf16 products).
+// The products.  8192 x 4096 x 65536 bf16, 256 x 256 tiles (two pieces in the backward):
+//   XE_STATS 3.2 ms (1.37 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 2 x 1.68, XE_DW 2 x 1.69,
+//   XE_DH 2 x 1.62 ms (1.30 - 1.36).
+// The matrix pipe is busy 78 - 84 % of the cycles at the 1.55 GHz that its power leaves; LDS reads meet no
+// bank conflict.  4096 (3686 count) x 1024 x 32768 fp32, 256 x 128: 1.11, 1.18, 1.09 and 1.13 ms (1.25 - 1.36 PFLOP/s of bf16
+// products).  Short sums leave the tiles' beginnings and ends (7 us of 27 at 13 steps of 64): 3001 (2251 count) x 777 x 50021 fp16
+// 0.20, 0.22, 0.28 and 0.21 ms (0.62 - 0.86).
 template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N, bool A_ONCE = false, bool A_RAW = false>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentArgs A) {
   typedef typename XentTypes<TO>::T T;

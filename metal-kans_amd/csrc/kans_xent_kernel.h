@@ -70,8 +70,8 @@ __device__ __forceinline__ float exp_of(float x) {
 }
 
 // 2^log_up exp(x - at), for x - at <= 0 or so, as a function of x.  The power of two goes into the exponent, so
-// that results below 2^-126, which exp2 drops, are there.  16-bit G: one fma and exp2; the rounding of `at` and of the
-// exponent is 2^-18 of the result, far below the 2^-9 and 2^-12 of G.  fp32: what the roundings left as a factor.
+// that results below 2^-126, which exp2 drops, are there.  16-bit G, |at| < 2^8: one fma and exp2; the rounding of `at` and of
+// the exponent is 2^-15 of the result at most, below the 2^-9 and 2^-12 of G.  kExact: what the roundings left as a factor.
 template <bool kExact>
 struct ExpUp {
   float at, log_up;
@@ -86,6 +86,9 @@ struct ExpUp {
     return __builtin_fmaf(e, l * 0.6931471805599453f, e);
   }
 };
+
+// Whether some lane's `at` is too large for the short forms, which round at log2(e): below, that is 2^-16 at most in an exponent.
+__device__ __forceinline__ bool far(float at) { return __builtin_amdgcn_ballot_w64(!(__builtin_fabsf(at) < 0x1p8f)) != 0; }
 
 // 8 values as packed 16-bit pairs, or as those of their three terms.
 template <typename T, int TERMS>
@@ -189,10 +192,20 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
         for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const float at = top == kNoLogit ? 0.0f : top;
+      if (TERMS == 3 || far(at)) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sum += exp_of<TERMS == 3>(acc[i][j][r] - at);
+          for (int r = 0; r < 16; ++r) sum += exp_of<TERMS == 3>(acc[i][j][r] - at);
+      } else {
+        // one fma and exp2 a logit; what the rounding of at log2(e) adds to every exponent is taken out of the sum
+        const float at2 = at * kLog2e;
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -at2));
+        sum *= __builtin_amdgcn_exp2f(-__builtin_fmaf(at, kLog2e, -at2));
+      }
       sum += __shfl_xor(sum, 32, 64);
       if (t >= 0 && t < MB * 32 && ((t >> 2) & 1) == half) {
 #pragma unroll
@@ -234,34 +247,37 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     for (int j = 0; j < NB; ++j) {
       const int n = ncol(j);
       const bool there = n < count;
-      const ExpUp<TERMS == 3> exp_up(there ? lse[n] : 0.0f, kLogUp, there);
-      const float rho = there && A.rho ? A.rho[n] : 1.0f;
+      const float at = there ? lse[n] : 0.0f, rho = there && A.rho ? A.rho[n] : 1.0f;
       const int t = there ? target[n] - A.v0 : -1;
+      auto write = [&](const auto& exp_up) {
 #pragma unroll
-      for (int i = 0; i < MB; ++i)
+        for (int i = 0; i < MB; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-          const int m = mrow(i, 4 * q);  // values 0 .. 3 are its rows, 4 .. 7 those 8 further on
-          float v[8];
+          for (int q = 0; q < 4; q += 2) {
+            const int m = mrow(i, 4 * q);  // values 0 .. 3 are its rows, 4 .. 7 those 8 further on
+            float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = exp_up(acc[i][j][4 * q + e]) * rho;
-          const int own = t - m;
-          if (__builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4))) {
+            for (int e = 0; e < 8; ++e) v[e] = exp_up(acc[i][j][4 * q + e]) * rho;
+            const int own = t - m;
+            if (__builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4))) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] -= own == e % 4 + e / 4 * 8 ? kUp * rho : 0.0f;
+              for (int e = 0; e < 8; ++e) v[e] -= own == e % 4 + e / 4 * 8 ? kUp * rho : 0.0f;
+            }
+            uint4 d[TERMS];
+            pack8<T, TERMS>(v, d);
+            // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
+            const int m8 = m - 4 * half + 8 * half;
+            char* o = A.g + ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
+#pragma unroll
+            for (int c = 0; c < TERMS; ++c) {
+              const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
+              const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
+              *(uint4*)(o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+            }
           }
-          uint4 d[TERMS];
-          pack8<T, TERMS>(v, d);
-          // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
-          const int m8 = m - 4 * half + 8 * half;
-          char* o = A.g + ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
-#pragma unroll
-          for (int c = 0; c < TERMS; ++c) {
-            const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
-            *(uint4*)(o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
-          }
-        }
+      };
+      if (TERMS == 3 || far(at)) write(ExpUp<true>(at, kLogUp, there));
+      else write(ExpUp<false>(at, kLogUp, there));
     }
   } else if constexpr (EPI == XE_DW) {
     const float alpha = *A.alpha;

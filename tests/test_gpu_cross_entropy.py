@@ -132,6 +132,28 @@ def test_few_rows(cuda, n, d, v, dt):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_logits_near_the_largest_number(cuda, dt, sign):
+    """One logit stands out by more than any exponential's range, near fp32's largest number or far below all zeros."""
+    import metal_kans as mk
+    h = torch.tensor([[1.5 * 2.0 ** 63], [1.0]], device="cuda").to(DT[dt]).requires_grad_(True)
+    w = torch.full((300, 1), sign * 2.0 ** 63, device="cuda")
+    w[7] = w[7] * (1.25 if sign > 0 else 0.75)                          # logits sign 1.5 2^126, 1.875 2^126 or -1.125 2^126
+    w = w.to(DT[dt]).requires_grad_(True)
+    for target, p_target in ((7, 1.0), (8, 0.0)):
+        loss = mk.linear_cross_entropy(h, w, torch.full((2,), target, device="cuda"), reduction="none")
+        top, own = (h.detach().double() @ w.detach().double().t()).amax(1), (h.detach().double() * w.detach().double()[target, 0])[:, 0]
+        assert ((loss.detach().double() - (top - own)).abs() <= 2 * U * top.abs() + 1e-3).all()
+        dh, dw = torch.autograd.grad(loss, (h, w), torch.tensor([1.0, 0.0], device="cuda"))
+        want = w.detach().double()[7, 0] - w.detach().double()[target, 0]   # (p - y) W with p = 1 at 7
+        assert (dh[0, 0].double() - want).abs() <= 4 * T[dt] * w.detach().double()[7, 0].abs() and dh[1, 0] == 0
+        g = torch.zeros(300, dtype=torch.float64, device="cuda")
+        g[7] += 1
+        g[target] -= 1
+        assert ((dw[:, 0].double() - g * h.detach().double()[0, 0]).abs() <= 4 * T[dt] * h.detach().double()[0, 0].abs() * (g != 0)).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
 @pytest.mark.parametrize("n,d,v", [(8180, 72, 33001),     # more than 2^28 logits
                                    (5, 4099, 70001)])     # a head of more than 2^28 values, laid out anew
 def test_large_vocabulary_in_pieces(cuda, n, d, v, dt):

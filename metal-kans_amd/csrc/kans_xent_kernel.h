@@ -116,6 +116,12 @@ __device__ __forceinline__ XentShare share_of(int count, int bn, int n_tiles, in
   return {there, min(n_tiles * splits / max(there, 1), most)};
 }
 
+// Tile of a workgroup: consecutive ones go to the 8 XCDs in turn, and each XCD gets a run of the tiles.
+__device__ __forceinline__ int xcd_tile(int id, int tiles) {
+  const int xcd = id & 7;
+  return xcd * (tiles >> 3) + min(xcd, tiles & 7) + (id >> 3);
+}
+
 // The products.  8192 x 4096 x 65536 bf16, 256 x 256 tiles (two pieces in the backward):
 //   XE_STATS 3.2 ms (1.37 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 2 x 1.68, XE_DW 2 x 1.69,
 //   XE_DH 2 x 1.62 ms (1.30 - 1.36).
@@ -148,12 +154,14 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     if (split >= splits) return;
   } else if constexpr (EPI == XE_DW_SPLIT) {
     split = blockIdx.y;
+  } else if constexpr (!kOverRows) {
+    // (G of the rows that fill up the last step of k is written too: zeros)
+    n_tiles = min(n_tiles, ((EPI == XE_GRAD ? (count + 63) / 64 * 64 : count) + BN - 1) / BN);
   }
+  if (id >= A.m_tiles * n_tiles) return;
   int mt, nt;
-  tile_of<8>(xcd_remap(id, A.m_tiles * n_tiles), A.m_tiles, n_tiles, mt, nt);
+  tile_of<8>(xcd_tile(id, A.m_tiles * n_tiles), A.m_tiles, n_tiles, mt, nt);
   const int m0 = mt * BM, n0 = nt * BN;
-  // (G of the rows that fill up the last step of k is written too: zeros)
-  if (!kOverRows && n0 >= (EPI == XE_GRAD ? (count + 63) / 64 * 64 : count)) return;
   int first = 0, steps = A.steps;
   if (kOverRows) steps = min(steps, (count + Step::kStep - 1) / Step::kStep);
   if (EPI == XE_DH || EPI == XE_DW_SPLIT) {

@@ -564,8 +564,20 @@ __global__ __launch_bounds__(1024) void k_xent_loss(const float2* __restrict__ p
       sum = sum * exp_of<kExact>(top - at) + o.y * exp_of<kExact>(o.x - at);
       top = both;
     };
-#pragma unroll 4
-    for (int t = run; t < tiles; t += 16) add(part[(long)t * Np + n]);
+    // eight tiles at a time, their largest logit first: the exponentials do not wait for one another
+    for (int t0 = run; t0 < tiles; t0 += 128) {
+      float2 o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = t0 + 16 * i < tiles ? part[(long)(t0 + 16 * i) * Np + n] : make_float2(kNoLogit, 0.0f);
+      float both = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) both = fmaxf(both, o[i].x);
+      const float at = both == kNoLogit ? 0.0f : both;
+      sum *= exp_of<kExact>(top - at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += o[i].y * exp_of<kExact>(o[i].x - at);
+      top = both;
+    }
     join[run][lane] = make_float2(top, sum);
     __syncthreads();
     if (run == 0 && n < count) {

@@ -13,7 +13,8 @@ buffers.  Per parameter:
   the values that codes stand for are ``scale * (q / 127) * |q / 127|`` and ``scale * (q / 255) ** 4``;
 * ``master`` (16-bit parameters): the fp32 value that the parameter is the rounding of.
 
-Gradients that are None leave their parameter alone.  A master follows its parameter only when it is
+Gradients that are None leave their parameter alone.  Parameters are dense in memory, in any order of their dimensions;
+fp32 states follow a parameter into another order, 8-bit ones refuse it (``state.clear()`` starts anew).  A master follows its parameter only when it is
 made: after other changes to a 16-bit parameter (a loaded model), ``state.clear()`` starts anew.  A step on a
 capturing stream is refused (its bias corrections belong to that one step).
 """
@@ -72,23 +73,43 @@ class _Arena:
         return out
 
     def start(self, i: int, state: dict) -> dict:
-        """The state of parameter i: zeros and its value, or what ``state`` holds."""
+        """The state of parameter i in its present order of memory: zeros and its value, or what ``state`` holds."""
         p = self.params[i]
+        if not _dense(p):
+            raise ValueError(_NOT_DENSE)
         views = self.views(i)
+        given = {name: state.get(name) for name in views}
         for name, v in views.items():
-            given = state.get(name)
-            if given is not None:
-                if given.shape != v.shape or (given.is_floating_point() != v.is_floating_point()):
-                    raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} is {given.dtype} "
-                                     f"{tuple(given.shape)}, expected {v.dtype} {tuple(v.shape)}")
-                v.copy_(given)
+            g = given[name]
+            if g is None:
+                if state and name != "master":
+                    raise ValueError(f"state {name!r} is missing (states in {self.bits} bits)")
+                continue
+            if g.shape != v.shape or (g.is_floating_point() != v.is_floating_point()):
+                raise ValueError(f"state {name!r} of a parameter of shape {tuple(p.shape)} is {g.dtype} "
+                                 f"{tuple(g.shape)}, expected {v.dtype} {tuple(v.shape)}")
+            # (blocks of elements in this order share a scale)
+            if not g.is_floating_point() and _order(g) != _order(v):
+                raise ValueError(f"8-bit state {name!r} has strides {g.stride()}, its parameter {v.stride()}: codes belong to one "
+                                 "order of memory")
+            if g.device == v.device and g.untyped_storage().data_ptr() == v.untyped_storage().data_ptr():
+                given[name] = g.clone()  # the places that are written below, maybe in another order
+        for name, v in views.items():
+            if given[name] is not None:
+                v.copy_(given[name])
             elif name == "master":
                 v.copy_(p.detach())
-            elif state:
-                raise ValueError(f"state {name!r} is missing (states in {self.bits} bits)")
             else:
                 v.zero_()
         return {"step": int(state.get("step", 0)), **views}
+
+
+_NOT_DENSE = "parameters must be dense (no gaps or overlaps in memory)"
+
+
+def _order(t: torch.Tensor) -> tuple:
+    """The dimensions as they lie in memory, the slowest first."""
+    return tuple(sorted((i for i in range(t.dim()) if t.shape[i] > 1), key=lambda i: -t.stride(i)))
 
 
 def _dense(p: torch.Tensor) -> bool:
@@ -134,7 +155,7 @@ class TorchAdamW(torch.optim.Optimizer):
                 if p.dtype not in _DT:
                     raise TypeError(f"unsupported parameter dtype {p.dtype}")
                 if not _dense(p):
-                    raise ValueError("parameters must be dense (no gaps or overlaps in memory)")
+                    raise ValueError(_NOT_DENSE)
         except Exception:
             self.param_groups.pop()
             raise
@@ -230,5 +251,8 @@ class TorchAdamW(torch.optim.Optimizer):
             lr, (b1, b2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
             for a in self._group_arenas(gi):
                 load().adamw_step(self.state, a.params, a.numel_q, a.blocks_q, a.flat, _DT[a.dtype], a.bits,
-                                  lambda i, a=a: self.state.__setitem__(a.params[i], a.start(i, {})), lr, b1, b2, eps, decay)
+                                  lambda i, a=a: self._start(a, i), lr, b1, b2, eps, decay)
         return loss
+
+    def _start(self, a: _Arena, i: int) -> None:
+        self.state[a.params[i]] = a.start(i, self.state.get(a.params[i], {}))

@@ -332,3 +332,81 @@ def test_refusals(cuda):
     opt = mk.TorchAdamW(p)
     opt.step()                     # no gradient anywhere: nothing to do
     assert not opt.state.get(p[0])
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_parameter_in_another_order(cuda, dt):
+    """A parameter whose elements are put in another order between steps (a change of memory format) keeps its states."""
+    import metal_kans as mk
+    a, b = make([(30, 50), (2, 3, 4, 5)], DT[dt], 10), make([(30, 50), (2, 3, 4, 5)], DT[dt], 10)
+    one, two = mk.TorchAdamW(a, lr=0.1), mk.TorchAdamW(b, lr=0.1)
+    for i in range(4):
+        one.step()
+        two.step()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q), i
+            for name, s in one.state[p].items():
+                assert torch.equal(s, two.state[q][name]) if isinstance(s, torch.Tensor) else s == two.state[q][name]
+        if i == 0:
+            b[0].data = b[0].data.t().contiguous().t()
+            b[1].data = b[1].data.contiguous(memory_format=torch.channels_last)
+        elif i == 1:
+            b[0].grad = b[0].grad.t().contiguous().t()
+        elif i == 2:
+            b[0].data, b[1].data = b[0].data.contiguous(), b[1].data.permute(3, 0, 2, 1).contiguous().permute(1, 3, 2, 0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_parameter_with_gaps_after_a_step(cuda, bits):
+    """Elements that do not lie side by side any more are refused, and nothing is written."""
+    import metal_kans as mk
+    for started in (False, True):
+        p = make([(6, 40)], torch.float32, 11)
+        opt = mk.TorchAdamW(p, lr=0.1, state_bits=bits)
+        if started:
+            opt.step()
+        states = {n: s.clone() for n, s in opt.state[p[0]].items() if isinstance(s, torch.Tensor)} if started else {}
+        big = torch.full((6, 64), 3.0, device="cuda")
+        for view in (big[:, :40], big.view(-1)[:1].expand(6, 40), big[:, 4:44]):
+            p[0].data = view
+            with pytest.raises(ValueError, match="dense"):
+                opt.step()
+        assert (big == 3.0).all() and len(opt.state.get(p[0], {})) == (len(states) + 1 if started else 0)
+        for n, s in states.items():
+            assert torch.equal(opt.state[p[0]][n], s)
+        p[0].data = torch.zeros(40, 6, device="cuda")    # as many elements in another shape
+        if started:
+            with pytest.raises(ValueError):
+                opt.step()
+        p[0].data = torch.zeros(6, 40, device="cuda")
+        p[0].grad = torch.ones(6, 40, device="cuda")
+        opt.step()
+        assert opt.state[p[0]]["step"] == (2 if started else 1)
+
+
+def test_8_bit_states_belong_to_an_order(cuda):
+    """The scales are those of blocks in the parameter's order of memory: in another one the codes mean nothing."""
+    import metal_kans as mk
+    p = make([(30, 50)], torch.float32, 12)
+    opt = mk.TorchAdamW(p, state_bits=8)
+    opt.step()
+    sd = copy.deepcopy(opt.state_dict())
+    p[0].data = p[0].data.t().contiguous().t()
+    before = p[0].detach().clone()
+    with pytest.raises(ValueError, match="order"):
+        opt.step()
+    assert torch.equal(p[0].detach(), before) and opt.state[p[0]]["step"] == 1
+    q = [torch.nn.Parameter(before.clone(memory_format=torch.preserve_format))]
+    assert q[0].stride() == (1, 30)
+    with pytest.raises(ValueError, match="order"):
+        mk.TorchAdamW(q, state_bits=8).load_state_dict(sd)
+    opt.state.clear()
+    opt.step()
+    sd = copy.deepcopy(opt.state_dict())
+    twin = mk.TorchAdamW(q, state_bits=8)
+    twin.load_state_dict(sd)
+    q[0].data.copy_(p[0].data)
+    q[0].grad = p[0].grad
+    opt.step()
+    twin.step()
+    assert torch.equal(p[0], q[0]) and twin.state[q[0]]["step"] == 2

@@ -257,6 +257,13 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
       const bool there = n < count;
       const float at = there ? lse[n] : 0.0f, rho = there && A.rho ? A.rho[n] : 1.0f;
       const int t = there ? target[n] - A.v0 : -1;
+      if (__builtin_amdgcn_ballot_w64(!there)) {
+        // G is 0 in the rows that fill up the last step; an infinite entry's logit with their zeros would be NaN
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][j][r] = there ? acc[i][j][r] : 0.0f;
+      }
       auto write = [&](const auto& exp_up) {
 #pragma unroll
         for (int i = 0; i < MB; ++i)

@@ -359,3 +359,22 @@ def test_refusals(cuda):
         mk.linear_cross_entropy(h, w, t, reduction="max")
     with pytest.raises(mk.device.KansError):   # more columns than the kernels' places hold
         mk.linear_cross_entropy(torch.zeros(1, 65537, device="cuda"), torch.zeros(2, 65537, device="cuda"), t[:1])
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n", [1, 50, 64, 100])
+def test_gradient_of_infinite_entries(cuda, n, dt):
+    """An entry that is -inf for every row has probability 0 and so no gradient, however many rows fill up a tile."""
+    import metal_kans as mk
+    h, w, t, gen = data(n, 8, 700, dt, 15)
+    h, t = h.abs() + 0.1, t % 5
+    w[5], w[512:600] = float("-inf"), float("-inf")
+    wr = w.clone().requires_grad_(True)
+    grad = torch.randn(n, generator=gen, device="cuda")
+    dw, = torch.autograd.grad(mk.linear_cross_entropy(h, wr, t, reduction="none"), wr, grad)
+    logits = (h.double()[:, None, :] * w.double()[None]).sum(-1)
+    g = (torch.softmax(logits, 1) - torch.nn.functional.one_hot(t, 700)) * grad.double()[:, None]
+    ref, size = g.t() @ h.double(), g.abs().t() @ h.double()
+    assert torch.isfinite(dw).all() and (dw[5] == 0).all() and (dw[512:600] == 0).all()
+    # G's rounding, dW's own, and some hundred roundings of products and exponentials
+    assert ((dw.double() - ref).abs() <= T[dt] * ref.abs() + (2 * T[dt] + 128 * U) * size + LEAST[dt]).all()

@@ -48,6 +48,7 @@ struct XentArgs {
   float2* part;                // XE_STATS: [m tile][Np] largest logit and sum of exp
   float* picked;               // XE_STATS: [N] the target's logit
   long Np, Vp;
+  const int64_t* target;       // XE_GRAD: of the call's rows
   const float* rho;            // XE_GRAD: per compact row, or null (1)
   char* g;                     // XE_GRAD: panels [v / kStep][Np][kStep]
   const float* alpha;          // XE_DW: factor
@@ -69,17 +70,27 @@ __device__ __forceinline__ float exp_of(float x) {
   return h > -126.0f ? __builtin_fmaf(e, l * 0.6931471805599453f, e) : e;
 }
 
-// 2^log_up exp(x - at), for x - at <= 0 or so, as a function of x.  The power of two goes into the exponent, so
-// that results below 2^-126, which exp2 drops, are there.  16-bit G, |at| < 2^8: one fma and exp2; the rounding of `at` and of
-// the exponent is 2^-15 of the result at most, below the 2^-9 and 2^-12 of G.  kExact: what the roundings left as a factor.
+// 2^log_up exp(x - top - rest), for x - top - rest <= 0 or so, as a function of x and a factor `by` of all of them.  The
+// row's largest logit and the logarithm of its sum come apart: their sum would be rounded at the logits' size, and a
+// row's probabilities with it.  The power of two goes into the exponent, so that results below 2^-126, which exp2 drops,
+// are there.  16-bit G, |top| < 2^8: one fma and exp2 a logit, rounded at an exponent below 64: 2^-19 of the result, far below
+// the 2^-9 and 2^-12 of G; what is constant in the exponent is rounded once a row and the rest of it is `by`.
+// kExact: the differences in fp32, and what the roundings of the exponent left as a factor.
 template <bool kExact>
 struct ExpUp {
-  float at, log_up;
-  __device__ __forceinline__ ExpUp(float at_, float log_up_, bool there)
-      : at(there ? (kExact ? at_ : log_up_ - at_ * kLog2e) : (kExact ? __builtin_inff() : -__builtin_inff())), log_up(log_up_) {}
+  float top, rest, log_up, by = 1.0f;
+  __device__ __forceinline__ ExpUp(float top_, float rest_, float log_up_, bool there)
+      : top(there ? top_ : __builtin_inff()), rest(rest_), log_up(log_up_) {
+    if (!kExact) {
+      const double all = (double)log_up_ - (double)top_ * (double)kLog2e - (double)rest_ * ((double)kLog2e + (double)kLog2eRest);
+      const float at = (float)all;
+      if (there) by = __builtin_amdgcn_exp2f((float)(all - (double)at));
+      top = there ? at : -__builtin_inff();
+    }
+  }
   __device__ __forceinline__ float operator()(float x) const {
-    if (!kExact) return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, at));
-    x -= at;
+    if (!kExact) return __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, top));
+    x = (x - top) - rest;
     x = x < -160.0f ? -160.0f : x;  // 0 all the same (-inf would leave a NaN as its rest); a NaN stays
     const float h = __builtin_fmaf(x, kLog2e, log_up), e = __builtin_amdgcn_exp2f(h);
     const float l = __builtin_fmaf(x, kLog2eRest, __builtin_fmaf(x, kLog2e, log_up - h));
@@ -240,8 +251,8 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   } else if constexpr (EPI == XE_GRAD) {
     constexpr float kUp = up_of<TO>(), kLogUp = std::is_same_v<TO, _Float16> ? 14.0f : 32.0f;
     constexpr int K = Step::kStep;
-    const int* target = A.state + kXentHead + A.N;
-    const float* lse = (const float*)(target + A.N);
+    const int* row = A.state + kXentHead;
+    const float *rest_of = (const float*)(row + A.N), *top_of = rest_of + A.N;
     if (m0 + BM > A.V) {
 #pragma unroll
       for (int i = 0; i < MB; ++i)
@@ -255,8 +266,9 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     for (int j = 0; j < NB; ++j) {
       const int n = ncol(j);
       const bool there = n < count;
-      const float at = there ? lse[n] : 0.0f, rho = there && A.rho ? A.rho[n] : 1.0f;
-      const int t = there ? target[n] - A.v0 : -1;
+      const float top = there ? top_of[n] : 0.0f, rest = there ? rest_of[n] : 0.0f, rho = there && A.rho ? A.rho[n] : 1.0f;
+      const int64_t t64 = there ? A.target[row[n]] - A.v0 : -1;
+      const int t = t64 >= 0 && t64 < A.V ? (int)t64 : -1;
       if (__builtin_amdgcn_ballot_w64(!there)) {
         // G is 0 in the rows that fill up the last step; an infinite entry's logit with their zeros would be NaN
 #pragma unroll
@@ -265,6 +277,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
           for (int r = 0; r < 16; ++r) acc[i][j][r] = there ? acc[i][j][r] : 0.0f;
       }
       auto write = [&](const auto& exp_up) {
+        const float times = exp_up.by * rho;
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
@@ -272,11 +285,16 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
             const int m = mrow(i, 4 * q);  // values 0 .. 3 are its rows, 4 .. 7 those 8 further on
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = exp_up(acc[i][j][4 * q + e]) * rho;
+            for (int e = 0; e < 8; ++e) v[e] = exp_up(acc[i][j][4 * q + e]) * times;
             const int own = t - m;
             if (__builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4))) {
+              // p - 1 of the target: what a confident row has left lies far below p's rounding
+              float x = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] -= own == e % 4 + e / 4 * 8 ? kUp * rho : 0.0f;
+              for (int e = 0; e < 8; ++e) x = own == e % 4 + e / 4 * 8 ? acc[i][j][4 * q + e] : x;
+              x = expm1f((x - top) - rest) * (kUp * rho);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = own == e % 4 + e / 4 * 8 ? x : v[e];
             }
             uint4 d[TERMS];
             pack8<T, TERMS>(v, d);
@@ -291,8 +309,8 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
             }
           }
       };
-      if (TERMS == 3 || far(at)) write(ExpUp<true>(at, kLogUp, there));
-      else write(ExpUp<false>(at, kLogUp, there));
+      if (TERMS == 3 || far(top)) write(ExpUp<true>(top, rest, kLogUp, there));
+      else write(ExpUp<false>(top, rest, kLogUp, there));
     }
   } else if constexpr (EPI == XE_DW) {
     const float alpha = *A.alpha;
@@ -589,10 +607,12 @@ __global__ __launch_bounds__(1024) void k_xent_loss(const float2* __restrict__ p
     __syncthreads();
     if (run == 0 && n < count) {
       for (int r = 1; r < 16; ++r) add(join[r][lane]);
-      const bool known = state[kXentHead + N + n] >= 0;
-      const float lse = known ? top + __builtin_logf(sum) : __builtin_nanf("");
-      ((float*)state)[kXentHead + 2 * N + n] = lse;
-      loss[state[kXentHead + n]] = lse - picked[n];
+      if (state[kXentHead + N + n] < 0) top = __builtin_nanf("");
+      // (not the difference to top + log: a logit's rounding is no part of a loss)
+      const float rest = __builtin_logf(sum);
+      ((float*)state)[kXentHead + N + n] = rest;
+      ((float*)state)[kXentHead + 2 * N + n] = top;
+      loss[state[kXentHead + n]] = (top - picked[n]) + rest;
     }
     __syncthreads();
   }
@@ -948,6 +968,7 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     A.steps = p.d_steps;
     A.state = c.state; A.N = c.N; A.V = n; A.v0 = (int)v0; A.D = c.D;
     A.Np = p.Np; A.Vp = p.piece;
+    A.target = c.target;
     A.rho = c.reduction ? nullptr : rho;
     A.g = c.ws + p.g;
     // (every entry of the padded piece is written: tiles of 256 or 128 entries and rows)

@@ -378,3 +378,40 @@ def test_gradient_of_infinite_entries(cuda, n, dt):
     assert torch.isfinite(dw).all() and (dw[5] == 0).all() and (dw[512:600] == 0).all()
     # G's rounding, dW's own, and some hundred roundings of products and exponentials
     assert ((dw.double() - ref).abs() <= T[dt] * ref.abs() + (2 * T[dt] + 128 * U) * size + LEAST[dt]).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shift", [0, -96, 240, 4096])
+@pytest.mark.parametrize("n", [3, 45])
+def test_shifted_logits_and_confident_rows(cuda, n, shift, dt):
+    """Losses and gradients do not depend on what all logits of a row have in common, and rows whose target has nearly all
+    probability keep what is left of it.  All logits here are exact, so what is off is a sum of 300 exponentials (of one
+    rounding each and as many in the sum's tree), its logarithm and the differences of logits: 32 u."""
+    import metal_kans as mk
+    v, rows = 300, torch.arange(n, device="cuda")
+    kinds = 9
+    gap = torch.tensor([0.0, 3.0, 7.0, 10.0, 13.0, 14.0, 15.5, -2.0, 15.0], device="cuda")
+    h, w = torch.zeros(n, 48, device="cuda"), torch.zeros(v, 48, device="cuda")
+    h[:, 0], w[:, 0] = 1, shift
+    h[:, 40], w[:, 40] = 1, 0.25 * (torch.arange(v, device="cuda") % 5 - 2)
+    h[rows, 1 + rows % kinds] = 1
+    own = 20 + 31 * torch.arange(kinds, device="cuda")       # the target of each kind of row
+    w[own, 1 + torch.arange(kinds, device="cuda")] = gap
+    h, w, t = h.to(DT[dt]), w.to(DT[dt]), own[rows % kinds]
+    hr, wr = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = mk.linear_cross_entropy(hr, wr, t, reduction="none")
+    logits = h.double() @ w.double().t()
+    logits -= logits.amax(1, keepdim=True)
+    lse = torch.logsumexp(logits, 1)
+    want = lse - logits.gather(1, t[:, None])[:, 0]
+    assert ((loss.detach().double() - want).abs() <= 32 * U * (1 + want)).all()
+    dh, dw = torch.autograd.grad(loss.sum(), (hr, wr))
+    p = (logits - lse[:, None]).exp()
+    g = p.clone()
+    g[rows, t] = torch.expm1(-want)
+    tg = T[dt] if dt != "f32" else 2 * U
+    m = 6 if dt == "f32" else 1
+    for name, out, G, P, x, k in (("dh", dh, g, p, w.double(), v), ("dw", dw, g.t(), p.t(), h.double(), n)):
+        ref, size = G @ x, G.abs() @ x.abs()
+        bound = T[dt] * ref.abs() + (tg + (m * k / 16 + 20) * U) * size + 32 * U * (P @ x.abs()) + LEAST[dt]
+        assert ((out.double() - ref).abs() <= bound).all(), (name, ((out.double() - ref).abs() / bound).max().item())

@@ -247,7 +247,8 @@ std::optional<std::tuple<std::optional<Tensor>, Tensor>> residual_norm(
     group = *of_gate;
     g = group ? gate->contiguous() : *gate;
   }
-  Norm n{x.contiguous(), contiguous(block), g, contiguous(post), contiguous(pre), dev ? *dev : Tensor(), scale, group, kind, eps, dt};
+  Norm n{x.contiguous(), contiguous(block), g, contiguous(post), contiguous(pre), Tensor(), scale, group, kind, eps, dt};
+  if (dev && block) n.dev = *dev;  // (without a block the scale has no part in the result)
   if (wants_grad({&n.x, &n.block, &n.gate, &n.post, &n.pre, &n.dev})) {
     auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     const auto out = NormFunction::apply(n.x, maybe(n.block), maybe(n.gate), maybe(n.post), maybe(n.pre), maybe(n.dev), scale, group, (int64_t)kind, eps, (int64_t)dt);

@@ -301,3 +301,21 @@ def test_refusals(cuda):
         mk.residual_norm(x.half(), x)
     with pytest.raises(ValueError):
         mk.residual_norm(x.cpu())
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+def test_scale_without_a_block(cuda, kind):
+    """A learned scale has no part in a call without a block: no gradient, and those of x and the weight are there."""
+    import metal_kans as mk
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    x, w, dh = rnd(gen, 7, 50), rnd(gen, 50, shift=1.0), rnd(gen, 7, 50)
+    scale = torch.full((1,), 0.4, device="cuda", requires_grad=True)
+    x.requires_grad_(True), w.requires_grad_(True)
+    y, h = mk.residual_norm(x, scale=scale, pre_weight=w, kind=kind)
+    assert y is x
+    dx, dw, ds = torch.autograd.grad(h, (x, w, scale), dh, allow_unused=True)
+    h1 = mk.residual_norm(x, pre_weight=w, kind=kind)[1]
+    want = torch.autograd.grad(h1, (x, w), dh)
+    assert ds is None and torch.equal(h, h1) and torch.equal(dx, want[0]) and torch.equal(dw, want[1])
+    # alone it makes no graph
+    assert mk.residual_norm(x.detach(), scale=scale, kind=kind)[1].grad_fn is None

@@ -242,10 +242,11 @@ std::optional<std::tuple<std::optional<Tensor>, Tensor>> residual_norm(
   int64_t group = std::max<int64_t>(x.numel() / x.size(-1), 1);
   Tensor g;
   if (gate) {
-    const auto of_gate = gate_group(*gate, x);
+    g = gate->dim() ? *gate : gate->reshape({1});
+    const auto of_gate = gate_group(g, x);
     if (!of_gate) return {};
     group = *of_gate;
-    g = group ? gate->contiguous() : *gate;
+    if (group) g = g.contiguous();
   }
   Norm n{x.contiguous(), contiguous(block), g, contiguous(post), contiguous(pre), Tensor(), scale, group, kind, eps, dt};
   if (dev && block) n.dev = *dev;  // (without a block the scale has no part in the result)

@@ -319,3 +319,28 @@ def test_scale_without_a_block(cuda, kind):
     assert ds is None and torch.equal(h, h1) and torch.equal(dx, want[0]) and torch.equal(dw, want[1])
     # alone it makes no graph
     assert mk.residual_norm(x.detach(), scale=scale, kind=kind)[1].grad_fn is None
+
+
+@pytest.mark.parametrize("types", [("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("d", [1, 48, 777, 9000])
+def test_gate_of_no_dimension(cuda, d, types):
+    import metal_kans as mk
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    rt, dt = (DT[t] for t in types)
+    check(mk, rnd(gen, 4, 9, d, dt=rt), rnd(gen, 4, 9, d, dt=dt), rnd(gen, 1, dt=dt, shift=0.5).reshape(()), 0.4,
+          rnd(gen, d, dt=dt, shift=1.0), rnd(gen, d, dt=dt, shift=1.0), "layer", gen=gen)
+
+
+@pytest.mark.parametrize("shape", [(), (1,), (4, 9, 1)])
+def test_gradient_of_a_repeating_gate_is_rounded_once(cuda, shape):
+    """Each element's share lies below fp16's smallest number, their sum does not."""
+    import metal_kans as mk
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    x, block = rnd(gen, 4, 9, 600), rnd(gen, 4, 9, 600, dt=torch.float16)
+    gate = torch.ones(shape, dtype=torch.float16, device="cuda", requires_grad=True)
+    y, _ = mk.residual_norm(x, block, gate)
+    u, _, _ = norm64(block.double(), "rms", 1e-6)
+    dy = 1e-8 * torch.sign(u).float()
+    got, = torch.autograd.grad(y, gate, dy)
+    want = bcast(dy.double() * u, gate)
+    assert got.shape == gate.shape and ((got.double() - want).abs() <= 2.0 ** -11 * want + 2.0 ** -25).all()

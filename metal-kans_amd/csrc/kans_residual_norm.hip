@@ -19,7 +19,9 @@
 //
 // Sums over rows (weights, a shared gate, the scale): a workgroup takes a run
 // of rows that share their gate row, adds up in fp32 registers and writes one partial row; a
-// second kernel adds the partial rows in a fixed order.  No atomics: the same bits on every run.
+// second kernel adds the partial rows in a fixed order.  Where few rows share a gate row a run is several whole
+// groups of them: it writes each group's gradient itself and one partial row of the rest.  No atomics: the same bits on
+// every run.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -45,7 +47,7 @@ struct NormArgs {
   void *dx, *dblock, *dgate;
   float* part;             // [chunks][parts][D] partial rows: pre_w, post_w, gate
   float* part_scale;       // [chunks]
-  long span, per_chunk, chunks_per_group;  // the runs of rows: NormPlan
+  long span, groups, per_chunk, chunks_per_group, whole;  // the runs of rows: NormPlan
   int parts, at_pre, at_post, at_gate;  // rows of a chunk's partials, -1: not asked for
   int want_scale, gate_f32;  // gate_f32: dgate of a gate row for each row in fp32
 };
@@ -272,9 +274,10 @@ struct RowIn {
   float r_b, r_y, mean_b, mean_y;
 };
 
-// Asks for row `row`; one behind `last` is not there, and its values are zeros, which add nothing to any sum.
+// Asks for row `row`, and with gate_at >= 0 for the gate's elements from there on; a row behind `last` is not there, and its
+// values are zeros, which add nothing to any sum.
 template <typename TX, typename TB, bool kLayer>
-__device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, long row, long last, int at, bool gate_rows) {
+__device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, long row, long last, int at, long gate_at) {
   constexpr bool kx = shifts<TX>(), kb = shifts<TB>();
   const bool there = row <= last;
   const int D = A.D, here = D - at, left = there ? here : 0;
@@ -284,7 +287,7 @@ __device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, l
   if (A.dy) in.dy = load_raw<kx>((const TX*)A.dy + base, here, left, D);
   if (A.dh) in.dh = load_raw<kb>((const TB*)A.dh + base, here, left, D);
   if (A.block) in.b = load_raw<kb>((const TB*)A.block + base, here, left, D);
-  if (gate_rows) in.g = load_raw<kb>((const TB*)A.gate + base, here, left, D);
+  if (gate_at >= 0) in.g = load_raw<kb>((const TB*)A.gate + gate_at, here, left, D);
   const float* s = A.stats + row * (kLayer ? 4 : 2);
   in.r_b = there ? s[0] : 0.0f;
   in.r_y = there ? s[1] : 0.0f;
@@ -295,8 +298,9 @@ __device__ __forceinline__ void load_row(RowIn<TX, TB>& in, const NormArgs& A, l
 // One workgroup takes the rows of a run, rows_of<TPR>() at a time, with the next ones' loads in flight (at
 // 1024 threads the 128 registers that a thread may have do not hold them too).  Two workgroups a CU, with
 // up to 256 registers: held to 128 the kernel spills, and 16384 x 4096 bf16 (805 MB) take 600 us instead of 155 - 190
-// (4.2 - 5.2 TB/s).
-template <typename TX, typename TB, bool kLayer, int TPR>
+// (4.2 - 5.2 TB/s).  whole: the run is several whole gate groups (a kernel of its own: the rows' bookkeeping in all of them
+// spilled at 1024 threads, 8192 x 8192 fp32 both directions 580 -> 628 us).
+template <typename TX, typename TB, bool kLayer, int TPR, bool whole>
 __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnorm_bwd(const NormArgs A) {
   constexpr int ROWS = rows_of<TPR>();
   __shared__ float lds[2][2][16];
@@ -305,14 +309,30 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
   __shared__ float4 kept[kAhead ? 1 : 3 * V / 4 * TPR];
   const int at = threadIdx.x % TPR * V, sub = threadIdx.x / TPR;
   const int D = A.D, left = D - at;
-  const long chunk = blockIdx.x, group = chunk / A.chunks_per_group;
-  const long first = group * A.span + (chunk - group * A.chunks_per_group) * A.per_chunk;
-  const long end = min(min(first + A.per_chunk, (group + 1) * A.span), A.rows);
-  const bool gate_rows = A.gate && A.gate_group == 1;
+  const long chunk = blockIdx.x;
+  const bool gate_rows = !whole && A.gate && A.gate_group == 1;
+  // the rows at a time, one for each `sub`: consecutive ones of the run from row0 on, or row in_group of ROWS consecutive
+  // groups from group0 on
+  long row0 = 0, end, group0;
+  int in_group = 0;
+  if constexpr (whole) {
+    group0 = chunk * A.whole;
+    end = min(group0 + A.whole, A.groups);  // in groups
+  } else {
+    group0 = chunk / A.chunks_per_group;
+    row0 = group0 * A.span + (chunk - group0 * A.chunks_per_group) * A.per_chunk;
+    end = min(min(row0 + A.per_chunk, (group0 + 1) * A.span), A.rows);
+  }
+  const long last = (whole ? end * A.span : end) - 1;
   const float scale = A.scale_dev ? *A.scale_dev : A.scale;
   Raw<TB> pw = load_or_one((const TB*)A.post_w, at, left), nw = load_or_one((const TB*)A.pre_w, at, left);
   RowIn<TX, TB> next{};
-  if (!gate_rows) next.g = load_or_one((const TB*)A.gate, group * D + at, left);
+  if (!gate_rows && !whole) next.g = load_or_one((const TB*)A.gate, group0 * D + at, left);
+  auto ask = [&](long r, long g, int in) {  // for the rows at a time from row r on, or row `in` of the groups from g on
+    const long row = whole ? (g + sub) * A.span + in : r + sub;
+    const long own = gate_rows ? min(row, last) : whole && in == 0 ? min(g + sub, end - 1) : -1;
+    load_row<TX, TB, kLayer>(next, A, row, last, at, own < 0 ? -1L : own * D + at);
+  };
   // sums of this thread's columns over the run's rows: pre_w, post_w, gate.  At 1024 threads a row they lie in LDS, each
   // thread its own, so that the rest fits in 128 registers: 8192 x 8192 bf16, both directions, 382 -> 301 us, fp32 780 -> 573.
   float s[kAhead ? 3 : 1][V], s_scale = 0.0f;
@@ -340,20 +360,23 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
       for (int i = 0; i < V / 4; ++i) *kept_at(k, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
   const float inv_d = 1.0f / (float)D;
-  if (kAhead) load_row<TX, TB, kLayer>(next, A, first + sub, end - 1, at, gate_rows);
-  for (long row0 = first; row0 < end; row0 += ROWS) {
-    const long row = row0 + sub;
-    if (!kAhead) load_row<TX, TB, kLayer>(next, A, row, end - 1, at, gate_rows);
+  if (kAhead) ask(row0, group0, 0);
+  while (whole ? group0 < end : row0 < end) {
+    if (!kAhead) ask(row0, group0, in_group);
     RowIn<TX, TB> in = next;
-    if (kAhead && row0 + ROWS < end) load_row<TX, TB, kLayer>(next, A, row + ROWS, end - 1, at, gate_rows);
+    const int then_in = whole && in_group + 1 < A.span ? in_group + 1 : 0;
+    const long then_group = whole && then_in == 0 ? group0 + ROWS : group0, then_row = row0 + ROWS;
+    if (kAhead && (whole ? then_group < end : then_row < end)) ask(then_row, then_group, then_in);
+    const long group = group0 + sub, row = whole ? group * A.span + in_group : row0 + sub;
     const long base = row * D + at;
-    const int out = row < end ? left : 0;
+    const int out = row <= last ? left : 0;
     constexpr bool kx = shifts<TX>(), kb = shifts<TB>();
     settle<kx>(in.x, out, D);
     settle<kx>(in.dy, out, D);
     settle<kb>(in.dh, out, D);
     settle<kb>(in.b, out, D);
-    if (gate_rows) settle<kb>(in.g, out, D);
+    if (gate_rows || (whole && in_group == 0)) settle<kb>(in.g, out, D);
+    if (whole && in_group == 0) next.g = in.g;  // (two rows at least share it)
     auto bn = [&](int e) { return e < left ? (get(in.b, e) - in.mean_b) * in.r_b : 0.0f; };
     auto yn = [&](int e) {
       const float y = get(in.x, e) + scale * get(in.g, e) * (bn(e) * get(pw, e));
@@ -394,6 +417,23 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
     }
     add_up(1, add);
     add_up(2, dg);
+    if (whole && A.dgate && then_in == 0) {  // the group's last row
+      float v[V];
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[e] = s[2][e];
+          s[2][e] = 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+          __builtin_memcpy(v + 4 * i, kept_at(2, i), 16);
+          *kept_at(2, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+      }
+      store_vec((TB*)A.dgate + group * D + at, out, v);
+    }
     if (A.dx) store_vec((TX*)A.dx + base, out, t);
     if (gate_rows && A.dgate) {
       if (A.gate_f32) store_vec((float*)A.dgate + base, out, dg);
@@ -414,6 +454,9 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
       }
       store_vec((TB*)A.dblock + base, out, db);
     }
+    row0 = then_row;
+    group0 = then_group;
+    in_group = then_in;
   }
   // the run's partial rows; where several rows go at a time, those of the same columns one after the other
   float* part = A.part + chunk * A.parts * D;
@@ -503,14 +546,15 @@ __global__ __launch_bounds__(kWide) void k_resnorm_wide_fwd(const NormArgs A) {
   }
 }
 
-// A chunk's rows one after the other; the partial rows are added up in memory, each column by one thread.
+// A chunk's rows one after the other; the partial rows are added up in memory, each column by one thread (of whole groups the
+// gate's row is that of the group under way).
 template <typename TX, typename TB, bool kLayer>
 __global__ __launch_bounds__(kWide) void k_resnorm_wide_bwd(const NormArgs A) {
   __shared__ float lds[2][2][16];
   const int D = A.D;
-  const long chunk = blockIdx.x, group = chunk / A.chunks_per_group;
-  const long first = group * A.span + (chunk - group * A.chunks_per_group) * A.per_chunk;
-  const long end = min(min(first + A.per_chunk, (group + 1) * A.span), A.rows);
+  const long chunk = blockIdx.x, group = A.whole ? chunk * A.whole : chunk / A.chunks_per_group;
+  const long first = A.whole ? group * A.span : group * A.span + (chunk - group * A.chunks_per_group) * A.per_chunk;
+  const long end = min(A.whole ? (group + A.whole) * A.span : min(first + A.per_chunk, (group + 1) * A.span), A.rows);
   const TB *pw = (const TB*)A.post_w, *nw = (const TB*)A.pre_w;
   const float scale = A.scale_dev ? *A.scale_dev : A.scale, inv_d = 1.0f / (float)D;
   float* part = A.part + chunk * A.parts * D;
@@ -557,6 +601,12 @@ __global__ __launch_bounds__(kWide) void k_resnorm_wide_bwd(const NormArgs A) {
     row_sum2<kWide>(pa, pb, lds, 1);
     pa *= inv_d;
     pb = kLayer ? pb * inv_d : 0.0f;
+    if (A.whole && A.at_gate >= 0 && (row + 1) % A.span == 0)
+      for (int j = threadIdx.x; j < D; j += kWide) {
+        float* sum = part + (long)A.at_gate * D + j;
+        ((TB*)A.dgate)[row / A.span * D + j] = from_f32<TB>(*sum);
+        *sum = 0.0f;
+      }
     if (A.block && A.dblock)
       for (int j = threadIdx.x; j < D; j += kWide) {
         const float p = scale * gt(j) * T(j) * post(j);
@@ -656,7 +706,8 @@ hipError_t launch_bwd(const NormArgs& A, long chunks, hipStream_t st) {
     if constexpr (TPR == 0)
       hipLaunchKernelGGL((k_resnorm_wide_bwd<TX, TB, kLayer>), dim3((unsigned)chunks), dim3(kWide), 0, st, A);
     else
-      hipLaunchKernelGGL((k_resnorm_bwd<TX, TB, kLayer, TPR>), dim3((unsigned)chunks), dim3(threads_of<TPR>()), 0, st, A);
+      hipLaunchKernelGGL((A.whole ? k_resnorm_bwd<TX, TB, kLayer, TPR, true> : k_resnorm_bwd<TX, TB, kLayer, TPR, false>),
+                         dim3((unsigned)chunks), dim3(threads_of<TPR>()), 0, st, A);
   });
   return hipGetLastError();
 }
@@ -671,17 +722,30 @@ hipError_t dispatch(int res_dtype, int dtype, int kind, F f) {
 }
 
 // Runs of rows of the backward: enough workgroups for every CU's four SIMDs, but at least kMinRows rows each where
-// there are that many, so that the partial rows stay a small part of the traffic.
+// there are that many, so that the partial rows stay a small part of the traffic.  Groups of fewer rows than such a run
+// go several to a run, a number that its rows at a time share evenly (16384 x 4096 in groups of 2, bf16: 512 runs,
+// 25 MB of partial rows; a run for each group was 8192 and 403 MB, three times x).
 struct NormPlan {
   long span, groups;                 // rows that share a gate row (all of them where none is shared), and how many such
   long per_chunk, chunks_per_group;  // rows of a run, runs of a span
+  long whole;                        // or whole groups of a run (0: a run lies in one)
   long chunks;
 };
 constexpr long kNormChunks = 512, kMinRows = 8;
-NormPlan plan_norm(long rows, long gate_group) {
-  NormPlan p;
+NormPlan plan_norm(long rows, int D, long gate_group) {
+  NormPlan p{};
   const long span = p.span = gate_group == 1 ? rows : gate_group;  // (a gate row for each row is not summed)
   p.groups = (rows + span - 1) / span;
+  const long run = std::max(kMinRows, (rows + kNormChunks - 1) / kNormChunks);
+  if (p.groups > 1 && span < run) {
+    long at_a_time = 1;
+    by_width(D, [&](auto width) {
+      if constexpr (decltype(width)::value != 0) at_a_time = rows_of<decltype(width)::value>();
+    });
+    p.whole = (run / span + at_a_time - 1) / at_a_time * at_a_time;
+    p.chunks = (p.groups + p.whole - 1) / p.whole;
+    return p;
+  }
   const long want = std::max(1L, kNormChunks / p.groups);
   p.per_chunk = std::min(span, std::max(kMinRows, (span + want - 1) / want));
   p.chunks_per_group = (span + p.per_chunk - 1) / p.per_chunk;
@@ -734,7 +798,7 @@ int kans_residual_norm_forward(int res_dtype, int dtype, int kind, const void* x
 
 long kans_residual_norm_workspace(long rows, int D, long gate_group) {
   if (rows <= 0 || D <= 0) return 0;
-  const NormPlan p = plan_norm(rows, gate_group > 0 ? gate_group : rows);
+  const NormPlan p = plan_norm(rows, D, gate_group > 0 ? gate_group : rows);
   return p.chunks * (3L * D + 1) * (long)sizeof(float);
 }
 
@@ -750,7 +814,7 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
   if ((dgate && !gate) || (dpost_w && !post_w) || (dpre_w && !pre_w) || (!block && (dblock || dscale)))
     return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
   if (dgate_f32 && gate_group != 1) return kans_fail(KANS_ERR_ARG, "dgate_f32 needs a gate row for each row");
-  const NormPlan p = plan_norm(rows, gate ? gate_group : rows);
+  const NormPlan p = plan_norm(rows, D, gate ? gate_group : rows);
   if (!workspace || workspace_bytes < p.chunks * (3L * D + 1) * (long)sizeof(float))
     return kans_fail(KANS_ERR_ARG, "workspace of %ld bytes, %ld needed", workspace ? workspace_bytes : 0,
                      p.chunks * (3L * D + 1) * (long)sizeof(float));
@@ -766,25 +830,28 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
   A.part_scale = (float*)workspace;
   A.part = (float*)workspace + p.chunks;
   A.span = p.span;
+  A.groups = p.groups;
+  A.whole = p.whole;
   A.per_chunk = p.per_chunk;
   A.chunks_per_group = p.chunks_per_group;
   A.at_pre = dpre_w ? A.parts++ : -1;
   A.at_post = dpost_w ? A.parts++ : -1;
-  A.at_gate = dgate && gate_group > 1 ? A.parts++ : -1;
+  const bool kept = p.whole && D <= 1024 * V;  // (the groups' sums stay in the registers of a workgroup)
+  A.at_gate = dgate && gate_group > 1 && !kept ? A.parts++ : -1;
   A.want_scale = dscale != nullptr;
   A.gate_f32 = dgate_f32;
   HIP_TRY(dispatch(res_dtype, dtype, kind, [&](auto tx, auto tb, auto layer) {
     return launch_bwd<decltype(tx), decltype(tb), decltype(layer)::value>(A, p.chunks, st);
   }));
-  if (A.parts == 0 && !dscale) return 0;
+  if (!dpre_w && !dpost_w && !dscale && (A.at_gate < 0 || p.whole)) return 0;
   ReduceArgs R{};
   R.part = A.part; R.part_scale = A.part_scale;
   R.dpre = dpre_w; R.dpost = dpost_w; R.dgate = dgate; R.dscale = dscale;
   R.chunks = p.chunks; R.chunks_per_group = p.chunks_per_group;
-  R.D = D; R.parts = A.parts; R.at_pre = A.at_pre; R.at_post = A.at_post; R.at_gate = A.at_gate;
+  R.D = D; R.parts = A.parts; R.at_pre = A.at_pre; R.at_post = A.at_post; R.at_gate = p.whole ? -1 : A.at_gate;
   R.col_tiles = (D + 63) / 64;
   R.groups = p.groups;
-  const long outs = (A.at_pre >= 0) + (A.at_post >= 0) + (A.at_gate >= 0 ? p.groups : 0);
+  const long outs = (R.at_pre >= 0) + (R.at_post >= 0) + (R.at_gate >= 0 ? p.groups : 0);
   const dim3 grid((unsigned)std::min(outs * R.col_tiles + (dscale ? 1 : 0), 1L << 16));
   auto* reduce = dtype == DT_F16 ? k_resnorm_reduce<_Float16> : dtype == DT_BF16 ? k_resnorm_reduce<__bf16> : k_resnorm_reduce<float>;
   hipLaunchKernelGGL(reduce, grid, dim3(1024), 0, st, R);

@@ -77,3 +77,14 @@ def test_linear_xent_refusals(lib):
     assert lib.kans_linear_xent_workspace(3, 4, 8, 10, 1) == -1
     # no more than a piece of the vocabulary is ever held: below the logits' size
     assert lib.kans_linear_xent_workspace(2, 16384, 4096, 131072, 0) < 16384 * 131072
+
+
+@pytest.mark.parametrize("d", [64, 4096, 10000])
+def test_residual_norm_workspace_of_short_groups(lib, d):
+    """Gate groups of few rows need no more partial sums than runs of rows without a gate (and less than twice x)."""
+    for rows in (24, 1024, 16384, 1 << 20):
+        plain = lib.kans_residual_norm_workspace(rows, d, 0)
+        for group in range(1, 65):
+            if rows % group == 0 or rows > 1000:
+                n = rows // group * group
+                assert lib.kans_residual_norm_workspace(n, d, group) <= 2 * plain + 16 * d, (rows, group)

@@ -344,3 +344,39 @@ def test_gradient_of_a_repeating_gate_is_rounded_once(cuda, shape):
     got, = torch.autograd.grad(y, gate, dy)
     want = bcast(dy.double() * u, gate)
     assert got.shape == gate.shape and ((got.double() - want).abs() <= 2.0 ** -11 * want + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("types", [("f32", "f32"), ("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("groups,group,d", [(1, 5, 200), (3, 2, 100), (700, 2, 72), (2000, 3, 130), (5000, 7, 33), (1030, 2, 1000),
+                                            (515, 13, 600), (600, 2, 4096), (2, 2, 4096), (90, 6, 8192), (1030, 2, 8000), (40, 2, 9000),
+                                            (9, 30, 17000), (1030, 2, 8200)])
+def test_short_groups_of_rows(cuda, groups, group, d, types, kind):
+    """Gate rows of few rows each, several groups to a run, the last of fewer: a row's results are those of the same gate with a
+    row for each row, its gradient their sum (in fp32, and rounded once more), the others' sums in another order."""
+    import metal_kans as mk
+    gen = torch.Generator(device="cuda").manual_seed(group * d)
+    rt, dt = (DT[t] for t in types)
+    x, block, gate = rnd(gen, groups, group, d, dt=rt), rnd(gen, groups, group, d, dt=dt), rnd(gen, groups, 1, d, dt=dt, shift=0.5)
+    scale, post, pre = torch.full((1,), 0.7, device="cuda"), rnd(gen, d, dt=dt, shift=1.0), rnd(gen, d, dt=dt, shift=1.0)
+    dy, dh = rnd(gen, groups, group, d, dt=rt), rnd(gen, groups, group, d, dt=dt)
+    runs = []
+    for g in (gate, gate.expand_as(block).contiguous()):
+        t = [v.clone().requires_grad_(True) for v in (x, block, g, scale, post, pre)]
+        out = mk.residual_norm(*t, kind=kind)
+        runs.append((out, torch.autograd.grad(out, t, (dy, dh))))
+    (out0, (dx0, db0, dg0, *sums0)), (out1, (dx1, db1, dg1, *sums1)) = runs
+    assert all(torch.equal(a, b) for a, b in zip(out0, out1)) and torch.equal(dx0, dx1) and torch.equal(db0, db1)
+    each = dg1.double()
+    want, size = each.sum(1, keepdim=True), each.abs().sum(1, keepdim=True)
+    t, least = STEP[dt]
+    rounded = t * size + group * least if dt != torch.float32 else 0   # of each row's own share
+    assert ((dg0.double() - want).abs() <= t * want.abs() + (group + 1) * U * size + rounded + least).all()
+    _, A = reference(x, block, gate, scale, post, pre, dy, dh, kind, 1e-6)
+    for name, a, b in zip(("scale", "post", "pre"), sums0, sums1):
+        close(name, a, b.double(), A[name].reshape(b.shape) + t / (C * U) * b.double().abs())
+    again = [v.clone().requires_grad_(True) for v in (x, block, gate, post)]
+    y, h = mk.residual_norm(again[0], again[1], again[2], 0.7, again[3], pre, kind)
+    for wants, place in (((2,), dg0), ((3,), sums0[1])):           # some gradients alone
+        got = torch.autograd.grad((y, h), [again[i] for i in wants], (dy, dh), retain_graph=True)[0]
+        assert got.shape == place.shape and torch.isfinite(got).all()

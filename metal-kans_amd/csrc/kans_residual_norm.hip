@@ -6,9 +6,9 @@
 //
 // Backward, from dy and dh (y^ = N(y), r = the reciprocal in N, q = pre_w dh; means over the row):
 //   T = dy + r_y (q - y^ mean(q y^) [- mean(q)])           layer terms in brackets
-//   dx = T,  dpre_w = sum dh y^,  dgate = sum scale T u,  dscale = sum T gate u
+//   dx = T,  dpre_w = sum dh y^,  dgate = sum scale T u
 //   du = scale gate T,  dpost_w = sum du b^,  p = post_w du
-//   dblock = r_b (p - b^ mean(p b^) [- mean(p)])
+//   dblock = r_b (p - b^ mean(p b^) [- mean(p)]),  dscale = sum T gate u = sum p b^ / scale
 //
 // All of it is bound by memory: the forward reads x, block (and a full gate) and
 // writes y and h once; the backward reads x, block, dy, dh and writes dx and dblock.
@@ -46,7 +46,7 @@ struct NormArgs {
   const void *dy, *dh;
   void *dx, *dblock, *dgate;
   float* part;             // [chunks][parts][D] partial rows: pre_w, post_w, gate
-  float* part_scale;       // [chunks]
+  float* part_scale;       // [chunks] doubles at 4-byte addresses
   long span, groups, per_chunk, chunks_per_group, whole;  // the runs of rows: NormPlan
   int parts, at_pre, at_post, at_gate;  // rows of a chunk's partials, -1: not asked for
   int want_scale, gate_f32;  // gate_f32: dgate of a gate row for each row in fp32
@@ -307,6 +307,7 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
   constexpr bool kAhead = TPR <= 512;
   __shared__ float sums[ROWS > 1 ? TPR * V : 1];
   __shared__ float4 kept[kAhead ? 1 : 3 * V / 4 * TPR];
+  __shared__ double sum_scale[ROWS];  // of the rows that each `sub` has done
   const int at = threadIdx.x % TPR * V, sub = threadIdx.x / TPR;
   const int D = A.D, left = D - at;
   const long chunk = blockIdx.x;
@@ -335,7 +336,7 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
   };
   // sums of this thread's columns over the run's rows: pre_w, post_w, gate.  At 1024 threads a row they lie in LDS, each
   // thread its own, so that the rest fits in 128 registers: 8192 x 8192 bf16, both directions, 382 -> 301 us, fp32 780 -> 573.
-  float s[kAhead ? 3 : 1][V], s_scale = 0.0f;
+  float s[kAhead ? 3 : 1][V];
   auto kept_at = [&](int k, int i) { return &kept[(k * (V / 4) + i) * TPR + threadIdx.x]; };
   auto add_up = [&](int k, const float(&v)[V]) {
     if constexpr (kAhead) {
@@ -359,6 +360,7 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
 #pragma unroll
       for (int i = 0; i < V / 4; ++i) *kept_at(k, i) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
+  if (at == 0) sum_scale[sub] = 0.0;
   const float inv_d = 1.0f / (float)D;
   if (kAhead) ask(row0, group0, 0);
   while (whole ? group0 < end : row0 < end) {
@@ -397,7 +399,7 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
     row_sum2<TPR>(sa, sb, lds, 0);
     sa *= inv_d;
     sb = kLayer ? sb * inv_d : 0.0f;
-    float pa = 0.0f, pb = 0.0f, dg[V];
+    float pa = 0.0f, pb = 0.0f, dg[V];  // means of p b^ and p without the scale, so that the first sums up to its gradient too
     repack(in.x);
     repack(in.b);
     repack(in.dh);
@@ -409,9 +411,8 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
       const float q = get(nw, e) * get(in.dh, e), g = get(in.g, e), b = bn(e), u = b * get(pw, e);
       t[e] = get(in.dy, e) + in.r_y * (q - yn(e) * sa - sb);
       dg[e] = scale * t[e] * u;
-      s_scale += e < left ? t[e] * (g * u) : 0.0f;
-      const float du = scale * g * t[e], p = du * get(pw, e);
-      add[e] = du * b;
+      const float du = g * t[e], p = du * get(pw, e);
+      add[e] = scale * du * b;
       pa += p * b;
       pb += e < left ? p : 0.0f;
     }
@@ -440,9 +441,10 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
       else store_vec((TB*)A.dgate + base, out, dg);
     }
     row_sum2<TPR>(pa, pb, lds, 1);
+    if (at == 0 && row <= last) sum_scale[sub] += (double)pa;
     if (A.dblock) {
-      pa *= inv_d;
-      pb = kLayer ? pb * inv_d : 0.0f;
+      pa *= scale * inv_d;
+      pb = kLayer ? pb * (scale * inv_d) : 0.0f;
       float db[V];
       repack(in.b);
       repack(in.g);
@@ -489,10 +491,12 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
   put(A.at_post, 1);
   put(A.at_gate, 2);
   if (A.want_scale) {
-    float none = 0.0f;
     __syncthreads();
-    row_sum2<threads_of<TPR>()>(s_scale, none, lds, 0);
-    if (threadIdx.x == 0) A.part_scale[chunk] = s_scale;
+    if (threadIdx.x == 0) {
+      double all = sum_scale[0];
+      for (int w = 1; w < ROWS; ++w) all += sum_scale[w];
+      __builtin_memcpy(A.part_scale + 2 * chunk, &all, sizeof(all));
+    }
   }
 }
 
@@ -560,7 +564,7 @@ __global__ __launch_bounds__(kWide) void k_resnorm_wide_bwd(const NormArgs A) {
   float* part = A.part + chunk * A.parts * D;
   for (int j = threadIdx.x; j < D; j += kWide)
     for (int k = 0; k < A.parts; ++k) part[(long)k * D + j] = 0.0f;
-  float s_scale = 0.0f;
+  double s_scale = 0.0;
   for (long row = first; row < end; ++row) {
     const TX* x = (const TX*)A.x + row * D;
     const TB* b = A.block ? (const TB*)A.block + row * D : nullptr;
@@ -585,22 +589,22 @@ __global__ __launch_bounds__(kWide) void k_resnorm_wide_bwd(const NormArgs A) {
     auto T = [&](int j) { return (dy ? to_f32(dy[j]) : 0.0f) + r_y * (qv(j) - yn(j) * sa - sb); };
     float pa = 0.0f, pb = 0.0f;
     for (int j = threadIdx.x; j < D; j += kWide) {
-      const float t = T(j), n = bn(j), u = n * post(j), du = scale * gt(j) * t, p = du * post(j);
+      const float t = T(j), n = bn(j), u = n * post(j), du = gt(j) * t, p = du * post(j);
       if (A.dx) ((TX*)A.dx)[row * D + j] = from_f32<TX>(t);
       if (A.dgate && A.gate_group == 1) {
         if (A.gate_f32) ((float*)A.dgate)[row * D + j] = scale * t * u;
         else ((TB*)A.dgate)[row * D + j] = from_f32<TB>(scale * t * u);
       }
       if (A.at_pre >= 0 && dh) part[(long)A.at_pre * D + j] += to_f32(dh[j]) * yn(j);
-      if (A.at_post >= 0) part[(long)A.at_post * D + j] += du * n;
+      if (A.at_post >= 0) part[(long)A.at_post * D + j] += scale * du * n;
       if (A.at_gate >= 0) part[(long)A.at_gate * D + j] += scale * t * u;
-      s_scale += t * (gt(j) * u);
       pa += p * n;
       pb += p;
     }
     row_sum2<kWide>(pa, pb, lds, 1);
-    pa *= inv_d;
-    pb = kLayer ? pb * inv_d : 0.0f;
+    s_scale += (double)pa;
+    pa *= scale * inv_d;
+    pb = kLayer ? pb * (scale * inv_d) : 0.0f;
     if (A.whole && A.at_gate >= 0 && (row + 1) % A.span == 0)
       for (int j = threadIdx.x; j < D; j += kWide) {
         float* sum = part + (long)A.at_gate * D + j;
@@ -613,12 +617,7 @@ __global__ __launch_bounds__(kWide) void k_resnorm_wide_bwd(const NormArgs A) {
         ((TB*)A.dblock)[row * D + j] = from_f32<TB>(r_b * (p - bn(j) * pa - pb));
       }
   }
-  if (A.want_scale) {
-    float none = 0.0f;
-    __syncthreads();
-    row_sum2<kWide>(s_scale, none, lds, 0);
-    if (threadIdx.x == 0) A.part_scale[chunk] = s_scale;
-  }
+  if (A.want_scale && threadIdx.x == 0) __builtin_memcpy(A.part_scale + 2 * chunk, &s_scale, sizeof(s_scale));
 }
 
 // ---- sums of the partial rows -------------------------------------------------------------------------
@@ -631,12 +630,25 @@ struct ReduceArgs {
   int D, parts, at_pre, at_post, at_gate;
 };
 
+// Sum over a workgroup in 64 bits, in its first thread.  The scale's gradient is one number of terms of both signs; all else
+// here is a sum along one row or column.
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.0;
+  if (threadIdx.x == 0)
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) v += lds[w];
+  return v;
+}
+
 // 16384 x 4096: 512 partial rows of 3 x 4096 in 7 us (25 MB, mostly from the last-level cache).
 // A workgroup adds 64 columns of one output row at a time: 16 runs of partial rows, joined in a fixed order.
 // Work by column tile and output row: dpre, dpost, then dgate's groups, and last the scale.
 template <typename TB>
 __global__ __launch_bounds__(1024) void k_resnorm_reduce(const ReduceArgs A) {
-  __shared__ float lds[16][64];
+  __shared__ alignas(8) float lds[16][64];
   const int lane = threadIdx.x & 63, run = threadIdx.x >> 6;
   const int weights = (A.at_pre >= 0) + (A.at_post >= 0);
   const long outs = weights + (A.at_gate >= 0 ? A.groups : 0);
@@ -660,16 +672,14 @@ __global__ __launch_bounds__(1024) void k_resnorm_reduce(const ReduceArgs A) {
     __syncthreads();
   }
   if (A.dscale && blockIdx.x == gridDim.x - 1) {
-    float* flat = &lds[0][0];
-    float s = 0.0f;
-    for (long c = threadIdx.x; c < A.chunks; c += 1024) s += A.part_scale[c];
-    flat[threadIdx.x] = s;
-    __syncthreads();
-    for (int d = 512; d > 0; d >>= 1) {
-      if ((int)threadIdx.x < d) flat[threadIdx.x] += flat[threadIdx.x + d];
-      __syncthreads();
+    double s = 0.0;
+    for (long c = threadIdx.x; c < A.chunks; c += 1024) {
+      double of_chunk;
+      __builtin_memcpy(&of_chunk, A.part_scale + 2 * c, sizeof(of_chunk));
+      s += of_chunk;
     }
-    if (threadIdx.x == 0) *A.dscale = flat[0];
+    s = block_sum(s, (double*)&lds[0][0]);
+    if (threadIdx.x == 0) *A.dscale = (float)s;
   }
 }
 
@@ -799,7 +809,7 @@ int kans_residual_norm_forward(int res_dtype, int dtype, int kind, const void* x
 long kans_residual_norm_workspace(long rows, int D, long gate_group) {
   if (rows <= 0 || D <= 0) return 0;
   const NormPlan p = plan_norm(rows, D, gate_group > 0 ? gate_group : rows);
-  return p.chunks * (3L * D + 1) * (long)sizeof(float);
+  return p.chunks * (3L * D + 2) * (long)sizeof(float);
 }
 
 int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* x, const void* block, const void* gate,
@@ -815,9 +825,9 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
     return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
   if (dgate_f32 && gate_group != 1) return kans_fail(KANS_ERR_ARG, "dgate_f32 needs a gate row for each row");
   const NormPlan p = plan_norm(rows, D, gate ? gate_group : rows);
-  if (!workspace || workspace_bytes < p.chunks * (3L * D + 1) * (long)sizeof(float))
+  if (!workspace || workspace_bytes < p.chunks * (3L * D + 2) * (long)sizeof(float))
     return kans_fail(KANS_ERR_ARG, "workspace of %ld bytes, %ld needed", workspace ? workspace_bytes : 0,
-                     p.chunks * (3L * D + 1) * (long)sizeof(float));
+                     p.chunks * (3L * D + 2) * (long)sizeof(float));
   std::lock_guard<std::mutex> lk(kans_mutex());
   if ((rc = kans_ensure_init())) return rc;
   hipStream_t st = kans_caller_stream(stream);
@@ -828,7 +838,7 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
   A.gate_group = gate ? gate_group : rows;
   A.dy = dy; A.dh = dh; A.dx = dx; A.dblock = dblock; A.dgate = dgate;
   A.part_scale = (float*)workspace;
-  A.part = (float*)workspace + p.chunks;
+  A.part = (float*)workspace + 2 * p.chunks;
   A.span = p.span;
   A.groups = p.groups;
   A.whole = p.whole;

@@ -380,3 +380,18 @@ def test_short_groups_of_rows(cuda, groups, group, d, types, kind):
     for wants, place in (((2,), dg0), ((3,), sums0[1])):           # some gradients alone
         got = torch.autograd.grad((y, h), [again[i] for i in wants], (dy, dh), retain_graph=True)[0]
         assert got.shape == place.shape and torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("d", [100, 1000, 4096, 8192, 17000])
+def test_gradient_of_the_scale_cancels(cuda, d):
+    """Rows in pairs of opposite gradients, far apart: the scale's gradient is 0.  A row's terms are rounded alike in both, so
+    only the sums of rows can leave something: those are held in 64 bits."""
+    import metal_kans as mk
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    half = 1500 if d < 8192 else 300
+    x, block, dy = (rnd(gen, half, d) for _ in range(3))
+    scale = torch.ones(1, device="cuda", requires_grad=True)
+    y, _ = mk.residual_norm(torch.cat([x, x]), torch.cat([block, block]), scale=scale)
+    got, = torch.autograd.grad(y, scale, torch.cat([dy, -dy]))
+    u, _, _ = norm64(block.double(), "rms", 1e-6)
+    assert got.abs().double().item() <= 2.0 ** -44 * 2 * (dy.double() * u).abs().sum().item()

@@ -100,6 +100,12 @@ bool wants_grad(std::initializer_list<const Tensor*> inputs) {
   return false;
 }
 
+// The nodes below differentiate backwards; a tangent would be lost without a word where no input requires grad.
+void no_tangents(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
+}
+
 // Gradients that cannot be differentiated again: an error to whoever tries, where the graph is kept for it.
 variable_list once(variable_list grads, bool graph) {
   variable_list given;
@@ -200,6 +206,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     variable_list d(11);
     const Tensor dy = grads.size() == 2 ? grads[0] : Tensor(), dh = grads.back();
     if (!dy.defined() && !dh.defined()) return d;
+    no_tangents({&dy, &dh}, "residual_norm's backward");
     const Norm n{s[0], s[1], s[2], s[3], s[4], s[5], numbers[0], rest[0], (int)rest[1], numbers[1], (at::ScalarType)rest[2]};
     std::array<bool, 6> need;
     for (size_t i = 0, edge = 0; i < 6; ++i) need[i] = s[i].defined() && ctx->needs_input_grad(edge++);
@@ -250,6 +257,7 @@ std::optional<std::tuple<std::optional<Tensor>, Tensor>> residual_norm(
   }
   Norm n{x.contiguous(), contiguous(block), g, contiguous(post), contiguous(pre), Tensor(), scale, group, kind, eps, dt};
   if (dev && block) n.dev = *dev;  // (without a block the scale has no part in the result)
+  no_tangents({&n.x, &n.block, &n.gate, &n.post, &n.pre, &n.dev}, "residual_norm");
   if (wants_grad({&n.x, &n.block, &n.gate, &n.post, &n.pre, &n.dev})) {
     auto maybe = [](const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; };
     const auto out = NormFunction::apply(n.x, maybe(n.block), maybe(n.gate), maybe(n.post), maybe(n.pre), maybe(n.dev), scale, group, (int64_t)kind, eps, (int64_t)dt);
@@ -321,6 +329,7 @@ struct XentFunction : torch::autograd::Function<XentFunction> {
     at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
     const auto rest = ctx->saved_data["rest"].toIntVector();
+    no_tangents({&grads[0]}, "linear_cross_entropy's backward");
     const Xent x{s[0], s[1], s[2], rest[0], (int)rest[1]};
     const variable_list d = once(x.backward(s[3], grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1)), graph);
     return {d[0], d[1], Tensor(), Tensor(), Tensor()};
@@ -341,6 +350,7 @@ std::optional<Tensor> linear_cross_entropy(const Tensor& hidden, const Tensor& w
                     "hidden and weight have more than 2^31 rows or columns");
   const Xent x{hidden.reshape({-1, hidden.size(-1)}).contiguous(), weight.contiguous(), target.reshape({-1}).contiguous(), ignore,
                reduction};
+  no_tangents({&x.h, &x.w}, "linear_cross_entropy");
   const Tensor loss = wants_grad({&x.h, &x.w}) ? XentFunction::apply(x.h, x.w, x.target, ignore, (int64_t)reduction)[0]
                                                : std::get<0>(x.forward());
   return reduction == 0 ? loss.reshape(target.sizes()) : loss;

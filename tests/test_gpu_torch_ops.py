@@ -121,3 +121,35 @@ def test_saved_tensors_are_guarded(cuda):
         w.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_no_forward_mode_derivative(cuda):
+    """A dual tensor's tangent is never dropped: the calls refuse it, in every input and with or without gradients."""
+    import torch.autograd.forward_ad as fwd
+    import metal_kans as mk
+    for wants in (False, True):
+        with fwd.dual_level():
+            for i in range(6):
+                t, _ = norm_inputs([wants] * 6)
+                t[i] = fwd.make_dual(t[i].detach(), torch.ones_like(t[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    norm_call(t)
+                with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    norm_call(t)
+            for i in range(2):
+                h, w, target = xent_inputs((wants, wants))
+                a = [h, w]
+                a[i] = fwd.make_dual(a[i].detach(), torch.ones_like(a[i]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    mk.linear_cross_entropy(*a, target)
+            t, _ = norm_inputs([wants] * 6)
+            norm_call(t)                     # plain tensors inside the level are as outside
+    t, (dy, dh) = norm_inputs([True] * 6)
+    h, w, target = xent_inputs()
+    y, loss = norm_call(t)[0], mk.linear_cross_entropy(h, w, target)
+    with fwd.dual_level():                   # forward over backward
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(y, t[0], fwd.make_dual(dy, dh))
+        one = torch.ones((), device="cuda")
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(loss, h, fwd.make_dual(one, one))

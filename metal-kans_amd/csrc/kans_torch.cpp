@@ -9,6 +9,9 @@
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
@@ -98,6 +101,13 @@ bool wants_grad(std::initializer_list<const Tensor*> inputs) {
   for (const Tensor* t : inputs)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Results are written through pointers, which a tracer does not see: its graph would hold uninitialized memory.
+void not_traced(const char* what) {
+  const bool traced = torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+                      c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+  TORCH_CHECK(!traced, what, " cannot be traced: its kernels are not operators of torch's dispatcher");
 }
 
 // The nodes below differentiate backwards; a tangent would be lost without a word where no input requires grad.
@@ -236,6 +246,7 @@ std::optional<int64_t> gate_group(const Tensor& gate, const Tensor& x) {
 std::optional<std::tuple<std::optional<Tensor>, Tensor>> residual_norm(
     const Tensor& x, const std::optional<Tensor>& block, const std::optional<Tensor>& gate, const std::optional<Tensor>& dev,
     double scale, const std::optional<Tensor>& post, const std::optional<Tensor>& pre, int kind, double eps) {
+  not_traced("residual_norm");
   if (x.dim() < 1 || x.size(-1) < 1 || kind < 0 || !(eps >= 0.0 && std::isfinite(eps))) return {};
   if (!block && (gate || post)) return {};
   const at::ScalarType dt = (block ? *block : pre ? *pre : x).scalar_type();
@@ -339,6 +350,7 @@ struct XentFunction : torch::autograd::Function<XentFunction> {
 // None where the arguments do not fit together (the caller says why).
 std::optional<Tensor> linear_cross_entropy(const Tensor& hidden, const Tensor& weight, const Tensor& target, int64_t ignore,
                                            int reduction) {
+  not_traced("linear_cross_entropy");
   if (reduction < 0 || hidden.dim() < 1 || weight.dim() != 2 || hidden.size(-1) != weight.size(1) || weight.size(0) == 0 ||
       weight.size(1) == 0 || target.sizes() != hidden.sizes().slice(0, hidden.dim() - 1))
     return {};
@@ -371,6 +383,7 @@ bool same_order(const Tensor& state, const Tensor& p) {
 // states and their values 27; with this loop in Python 23 and 66.
 void adamw_step(const py::dict& state, const py::list& params, const py::buffer& numel, const py::buffer& blocks, const py::dict& flat,
                 int type, int bits, const py::object& start, double lr, double beta1, double beta2, double eps, double decay) {
+  not_traced("TorchAdamW.step");
   const auto n_of = numel.request(), block_of = blocks.request();
   const size_t n = params.size();
   if ((size_t)n_of.size != n || (size_t)block_of.size != n || n_of.itemsize != 8 || block_of.itemsize != 8)

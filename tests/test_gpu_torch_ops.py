@@ -153,3 +153,35 @@ def test_no_forward_mode_derivative(cuda):
         one = torch.ones((), device="cuda")
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(loss, h, fwd.make_dual(one, one))
+
+
+def test_tracers_are_refused(cuda):
+    """A trace would hold the results' memory and not the call that fills it."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch.utils._python_dispatch import TorchDispatchMode
+    import metal_kans as mk
+    t, _ = norm_inputs([False] * 6)
+    h, w, target = xent_inputs((False, False))
+    p = torch.nn.Parameter(torch.ones(5, device="cuda"))
+    opt = mk.TorchAdamW([p], lr=0.5)
+
+    def step(g):
+        p.grad = g
+        opt.step()
+        return g
+    calls = ((lambda *a: norm_call(a)[1], t), (lambda *a: mk.linear_cross_entropy(*a), (h, w, target)),
+             (step, (torch.ones(5, device="cuda"),)))
+    for call, args in calls:
+        for trace in (lambda: torch.jit.trace(call, tuple(args)), lambda: make_fx(call)(*args),
+                      lambda: make_fx(call, pre_dispatch=True)(*args)):
+            with pytest.raises(RuntimeError, match=None if call is step else "trace"):   # (torch may be the first to refuse)
+                trace()
+    assert (p == 1).all() and not opt.state.get(p)
+
+    class Watch(TorchDispatchMode):          # other modes see torch's operators pass and change nothing
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    for call, args in calls[:2]:
+        want = call(*args)
+        with Watch():
+            assert torch.equal(call(*args), want)

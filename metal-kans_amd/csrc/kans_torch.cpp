@@ -369,16 +369,77 @@ std::optional<Tensor> linear_cross_entropy(const Tensor& hidden, const Tensor& w
 }
 
 // ---- TorchAdamW ------------------------------------------------------------------------------------
-// Whether a parameter's elements are paired with those of its states: the same order in memory.
-bool same_order(const Tensor& state, const Tensor& p) {
-  if (state.sizes() != p.sizes()) return false;
-  for (int64_t i = 0; i < p.dim(); ++i)
-    if (p.size(i) != 1 && p.stride(i) != state.stride(i)) return false;
-  return true;
+// An arena's buffers (_Arena.flat), and what a parameter's state holds when it is the arena's own: views of them at the
+// parameter's place, in its order of memory.
+struct Arena {
+  static constexpr int kKinds = 5;
+  Tensor flat[kKinds];  // exp_avg, exp_avg_sq, their scales, master (undefined: none of these)
+
+  explicit Arena(const py::dict& buffers) {
+    for (int k = 0; k < kKinds; ++k)
+      if (PyObject* t = PyDict_GetItemWithError(buffers.ptr(), name(k))) flat[k] = THPVariable_Unpack(t);
+  }
+  static PyObject* name(int k) {
+    static PyObject* const names[kKinds] = {
+        PyUnicode_InternFromString("exp_avg"), PyUnicode_InternFromString("exp_avg_sq"), PyUnicode_InternFromString("exp_avg_scale"),
+        PyUnicode_InternFromString("exp_avg_sq_scale"), PyUnicode_InternFromString("master")};
+    return names[k];
+  }
+
+  bool holds(PyObject* state, const Tensor& p, int64_t block) const {
+    if (!state || !PyDict_Check(state)) return false;
+    for (int k = 0; k < kKinds; ++k) {
+      if (!flat[k].defined()) continue;
+      PyObject* object = PyDict_GetItemWithError(state, name(k));
+      if (!object || !THPVariable_Check(object)) return false;
+      const Tensor& t = THPVariable_Unpack(object);
+      const bool scale = k == 2 || k == 3;
+      if (t.scalar_type() != flat[k].scalar_type() || t.storage().unsafeGetStorageImpl() != flat[k].storage().unsafeGetStorageImpl() ||
+          t.storage_offset() != (scale ? block : block * 256))
+        return false;
+      if (scale) {
+        if (t.dim() != 1 || t.size(0) != (p.numel() + 255) / 256 || !t.is_contiguous()) return false;
+        continue;
+      }
+      if (t.sizes() != p.sizes()) return false;
+      for (int64_t i = 0; i < p.dim(); ++i)
+        if (p.size(i) != 1 && p.stride(i) != t.stride(i)) return false;
+    }
+    return true;
+  }
+};
+
+// The state of parameter i, by start(i) where it is not there, or not the arena's own (a new tensor in its place, or the
+// parameter in another order of memory).  A borrowed reference.
+PyObject* state_of(const py::dict& state, PyObject* object, const Arena& arena, int64_t block, const py::object& start, size_t i) {
+  const Tensor& p = THPVariable_Unpack(object);
+  PyObject* s = PyDict_GetItemWithError(state.ptr(), object);
+  if (!arena.holds(s, p, block)) {
+    if (PyErr_Occurred()) throw py::error_already_set();
+    start(i);
+    s = PyDict_GetItemWithError(state.ptr(), object);
+    if (!arena.holds(s, p, block)) {
+      if (PyErr_Occurred()) throw py::error_already_set();
+      throw py::value_error("a parameter's state is not the optimizer's own");
+    }
+  }
+  return s;
 }
 
-// One step of the parameters of an arena that have gradients.  state: the optimizer's, by parameter; start(i) makes parameter i's,
-// or lays what it has out anew where the parameter's order in memory has changed.
+// Puts every state that is there into the arena.
+void adamw_hold(const py::dict& state, const py::list& params, const py::buffer& blocks, const py::dict& flat, const py::object& start) {
+  const auto block_of = blocks.request();
+  const Arena arena(flat);
+  if (block_of.size != (py::ssize_t)params.size() || block_of.itemsize != 8) throw py::value_error("one block for each parameter");
+  for (size_t i = 0; i < params.size(); ++i) {
+    PyObject* object = PyList_GET_ITEM(params.ptr(), (Py_ssize_t)i);
+    PyObject* s = PyDict_GetItemWithError(state.ptr(), object);
+    if (!s && PyErr_Occurred()) throw py::error_already_set();
+    if (s && PyObject_IsTrue(s) == 1) state_of(state, object, arena, ((const int64_t*)block_of.ptr)[i], start, i);
+  }
+}
+
+// One step of the parameters of an arena that have gradients.  state: the optimizer's, by parameter; start(i) puts parameter i's into the arena.
 // numel, blocks: int64 per parameter; flat: the arena's buffers.  A step of 9 small tensors takes 17 us, of 48 with 8-bit
 // states and their values 27; with this loop in Python 23 and 66.
 void adamw_step(const py::dict& state, const py::list& params, const py::buffer& numel, const py::buffer& blocks, const py::dict& flat,
@@ -388,13 +449,9 @@ void adamw_step(const py::dict& state, const py::list& params, const py::buffer&
   const size_t n = params.size();
   if ((size_t)n_of.size != n || (size_t)block_of.size != n || n_of.itemsize != 8 || block_of.itemsize != 8)
     throw py::value_error("one size and block for each parameter");
-  auto buffer = [&](const char* name) -> Tensor {
-    PyObject* t = PyDict_GetItemString(flat.ptr(), name);
-    return t ? THPVariable_Unpack(t) : Tensor();
-  };
-  const Tensor m = buffer("exp_avg"), v = buffer("exp_avg_sq"), ms = buffer("exp_avg_scale"), vs = buffer("exp_avg_sq_scale"),
-               master = buffer("master");
-  static PyObject *const step_name = PyUnicode_InternFromString("step"), *const avg_name = PyUnicode_InternFromString("exp_avg");
+  const Arena arena(flat);
+  const Tensor &m = arena.flat[0], &v = arena.flat[1], &ms = arena.flat[2], &vs = arena.flat[3], &master = arena.flat[4];
+  static PyObject* const step_name = PyUnicode_InternFromString("step");
   struct One {
     Tensor p, grad;
     PyObject* state;
@@ -421,18 +478,8 @@ void adamw_step(const py::dict& state, const py::list& params, const py::buffer&
       at::NoGradGuard no_grad;
       g = at::empty_like(p).copy_(g);
     }
-    PyObject* s = PyDict_GetItemWithError(state.ptr(), object);
-    if (!s && PyErr_Occurred()) throw py::error_already_set();
-    auto held = [&] {
-      PyObject* avg = s && PyDict_Check(s) ? PyDict_GetItemWithError(s, avg_name) : nullptr;
-      return avg && THPVariable_Check(avg) && same_order(THPVariable_Unpack(avg), p);
-    };
-    if (!held()) {
-      start(i);
-      s = PyDict_GetItemWithError(state.ptr(), object);
-      if (!held()) throw py::value_error("a parameter's state is not in its order of memory");
-    }
-    PyObject* step = s && PyDict_Check(s) ? PyDict_GetItemWithError(s, step_name) : nullptr;
+    PyObject* s = state_of(state, object, arena, ((const int64_t*)block_of.ptr)[i], start, i);
+    PyObject* step = PyDict_GetItemWithError(s, step_name);
     const long count = step ? PyLong_AsLong(step) : -1;
     if (PyErr_Occurred()) throw py::error_already_set();
     if (!step) throw py::value_error("a parameter's state has no step");
@@ -467,5 +514,6 @@ PYBIND11_MODULE(_kans_torch, m) {
   m.def("bind", &bind);
   m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());
   m.def("adamw_step", &adamw_step);
+  m.def("adamw_hold", &adamw_hold);
   m.def("linear_cross_entropy", &linear_cross_entropy, py::call_guard<py::gil_scoped_release>());
 }

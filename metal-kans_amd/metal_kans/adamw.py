@@ -13,6 +13,8 @@ buffers.  Per parameter:
   the values that codes stand for are ``scale * (q / 127) * |q / 127|`` and ``scale * (q / 255) ** 4``;
 * ``master`` (16-bit parameters): the fp32 value that the parameter is the rounding of.
 
+A tensor that a program puts in one's place is copied into the buffer by the next step.
+
 Gradients that are None leave their parameter alone.  Parameters are dense in memory, in any order of their dimensions;
 fp32 states follow a parameter into another order, 8-bit ones refuse it (``state.clear()`` starts anew).  A master follows its parameter only when it is
 made: after other changes to a 16-bit parameter (a loaded model), ``state.clear()`` starts anew.  A step on a
@@ -187,6 +189,7 @@ class TorchAdamW(torch.optim.Optimizer):
         out = []
         for gi in range(len(self.param_groups)):
             for a in self._group_arenas(gi):
+                load().adamw_hold(self.state, a.params, a.blocks_q, a.flat, lambda i, a=a: self._start(a, i))
                 flat = dict(a.flat)
                 if self.state_bits == 8:
                     avg, sq = (torch.empty(a.total * BLOCK, device=a.device) for _ in range(2))

@@ -410,3 +410,40 @@ def test_8_bit_states_belong_to_an_order(cuda):
     opt.step()
     twin.step()
     assert torch.equal(p[0], q[0]) and twin.state[q[0]]["step"] == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_assigned_states_are_taken(cuda, bits):
+    """A state tensor that a program puts in the place of the optimizer's own counts from then on."""
+    import metal_kans as mk
+    a, b = make([(40, 33), (100,)], torch.bfloat16, 14), make([(40, 33), (100,)], torch.bfloat16, 14)
+    one, two = mk.TorchAdamW(a, lr=0.1, state_bits=bits), mk.TorchAdamW(b, lr=0.1, state_bits=bits)
+    one.step()
+    two.step()
+    sd = copy.deepcopy(two.state_dict())
+    for name in list(one.state[a[0]]):
+        if name != "step":
+            new = one.state[a[0]][name].clone()
+            new = new // 2 if not new.is_floating_point() else new * 0.5
+            one.state[a[0]][name] = new
+            sd["state"][0][name] = new.clone()
+    one.state[a[1]]["exp_avg"] = torch.zeros_like(one.state[a[1]]["exp_avg"])
+    sd["state"][1]["exp_avg"] = torch.zeros_like(sd["state"][1]["exp_avg"])
+    two.load_state_dict(sd)
+    for x, y in zip(one.flat_state(), two.flat_state()):
+        for name in ("exp_avg", "exp_avg_sq", "master"):
+            assert torch.equal(x[name], y[name]), name
+    one.state[a[1]]["exp_avg_sq"] = one.state[a[1]]["exp_avg_sq"].clone()
+    for _ in range(2):
+        one.step()
+        two.step()
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
+            for name, s in one.state[p].items():
+                assert torch.equal(s, two.state[q][name]) if isinstance(s, torch.Tensor) else s == two.state[q][name]
+    one.state[a[0]]["exp_avg"] = one.state[a[0]]["exp_avg"][:3].clone()
+    with pytest.raises(ValueError):
+        one.step()
+    del one.state[a[0]]["exp_avg"]
+    with pytest.raises(ValueError):
+        one.step()

@@ -209,7 +209,12 @@ class TorchAdamW(torch.optim.Optimizer):
         return sd
 
     def load_state_dict(self, state_dict) -> None:
-        """As torch's, with the states kept in their own types; refuses states of the other width."""
+        """As torch's, its hooks included, with the states kept in their own types; refuses states of the other width."""
+        state_dict = dict(state_dict)
+        for hook in self._optimizer_load_state_dict_pre_hooks.values():
+            other = hook(self, state_dict)
+            if other is not None:
+                state_dict = other
         bits = state_dict.get("state_bits", self.state_bits)
         if bits != self.state_bits:
             raise ValueError(f"the states are in {bits} bits, the optimizer's in {self.state_bits}")
@@ -235,6 +240,8 @@ class TorchAdamW(torch.optim.Optimizer):
             raise
         for g, sg in zip(self.param_groups, groups):
             g.update({k: v for k, v in sg.items() if k != "params"})
+        for hook in self._optimizer_load_state_dict_post_hooks.values():
+            hook(self)
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits}

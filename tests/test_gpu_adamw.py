@@ -447,3 +447,28 @@ def test_assigned_states_are_taken(cuda, bits):
     del one.state[a[0]]["exp_avg"]
     with pytest.raises(ValueError):
         one.step()
+
+
+def test_hooks_of_a_loaded_state(cuda):
+    """Hooks before a state dict is loaded may replace it, those behind run when it is there; a refused one runs no more."""
+    import metal_kans as mk
+    a, b = make([(20,)], torch.float32, 15), make([(20,)], torch.float32, 15)
+    one, two = mk.TorchAdamW(a, lr=0.1), mk.TorchAdamW(b)
+    one.step()
+    seen = []
+
+    def before(opt, sd):
+        seen.append(("before", len(opt.state)))
+        sd = copy.deepcopy(sd)
+        sd["param_groups"][0]["lr"] = 0.25
+        return sd
+    two.register_load_state_dict_pre_hook(before)
+    two.register_load_state_dict_pre_hook(lambda opt, sd: seen.append(("again", sd["param_groups"][0]["lr"])))
+    two.register_load_state_dict_post_hook(lambda opt: seen.append(("after", opt.state[b[0]]["step"])))
+    sd = one.state_dict()
+    two.load_state_dict(sd)
+    assert seen == [("before", 0), ("again", 0.25), ("after", 1)]
+    assert two.param_groups[0]["lr"] == 0.25 and sd["param_groups"][0]["lr"] == 0.1
+    with pytest.raises(ValueError):
+        two.load_state_dict(mk.TorchAdamW(a, state_bits=8).state_dict())
+    assert seen[3:] == [("before", 1), ("again", 0.25)]

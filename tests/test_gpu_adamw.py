@@ -472,3 +472,34 @@ def test_hooks_of_a_loaded_state(cuda):
     with pytest.raises(ValueError):
         two.load_state_dict(mk.TorchAdamW(a, state_bits=8).state_dict())
     assert seen[3:] == [("before", 1), ("again", 0.25)]
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+def test_8_bit_alignment_and_strides(cuda, dt):
+    """Parameters and gradients at odd addresses and in another order of memory: codes, scales and values as of the same
+    elements in a parameter of its own."""
+    import metal_kans as mk
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    base = torch.randn(20000, generator=gen, device="cuda").to(DT[dt])
+    grads = torch.randn(20000, generator=gen, device="cuda").to(DT[dt])
+    pairs = []
+    for odd in (1, 2, 3):
+        p = torch.nn.Parameter(base[odd:odd + 5003].clone())
+        q = base.clone()[odd:odd + 5003].requires_grad_(True)
+        p.grad, q.grad = grads[:5003].clone(), torch.cat([grads[:odd], grads])[odd:odd + 5003]
+        pairs.append((p, q))
+    q = base[:6000].clone().view(60, 100).t().requires_grad_(True)   # strides (1, 100): the order of `flat`
+    flat = torch.nn.Parameter(base[:6000].clone())
+    q.grad, flat.grad = grads[:6000].view(60, 100).t().contiguous(), grads[:6000].clone()
+    opts = [[mk.TorchAdamW([t], lr=0.1, state_bits=8) for t in pair] for pair in (*pairs, (flat, q))]
+    for _ in range(3):
+        for a, b in opts:
+            a.step()
+            b.step()
+    for (a, b), (x, y) in zip(opts, (*pairs, (flat, q))):
+        order = (lambda v: v.t().reshape(-1)) if y.dim() == 2 else (lambda v: v)
+        assert torch.equal(x, order(y.detach()))
+        for name, s in a.state[x].items():
+            if isinstance(s, torch.Tensor):
+                other = b.state[y][name]
+                assert torch.equal(s, order(other) if other.dim() == 2 else other), name

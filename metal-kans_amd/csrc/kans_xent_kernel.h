@@ -531,22 +531,19 @@ __device__ __forceinline__ void make_scale(const XentBegin& A, float* join) {
     if (threadIdx.x == 0) *A.alpha = count == 0 ? 0.0f : (A.reduction == 1 ? *A.grad / (float)count : *A.grad) / A.up;
     return;
   }
+  // (of the finite gradients: an infinite one or a NaN is its row's own, and the others' G stays in its range)
   float top = 0.0f;
-  bool bad = false;
   for (int n = threadIdx.x; n < count; n += 256) {
     const float g = __builtin_fabsf(A.grad[A.state[kXentHead + n]]);
-    bad |= !(g < __builtin_inff());
-    top = fmaxf(top, g);
+    top = fmaxf(top, g < __builtin_inff() ? g : 0.0f);
   }
-  join[threadIdx.x] = bad ? __builtin_inff() : top;
+  join[threadIdx.x] = top;
   __syncthreads();
   for (int d = 128; d > 0; d >>= 1) {
     if ((int)threadIdx.x < d) join[threadIdx.x] = fmaxf(join[threadIdx.x], join[threadIdx.x + d]);
     __syncthreads();
   }
-  // (an infinite or NaN gradient: as it is, without a common factor)
-  top = join[0];
-  const float by = top > 0.0f && top < __builtin_inff() ? top : 1.0f;
+  const float by = join[0] > 0.0f ? join[0] : 1.0f;
   if (threadIdx.x == 0) *A.alpha = by / A.up;
   for (int n = threadIdx.x; n < count; n += 256) A.rho[n] = A.grad[A.state[kXentHead + n]] / by;
 }

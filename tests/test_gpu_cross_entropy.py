@@ -415,3 +415,20 @@ def test_shifted_logits_and_confident_rows(cuda, n, shift, dt):
         ref, size = G @ x, G.abs() @ x.abs()
         bound = T[dt] * ref.abs() + (tg + (m * k / 16 + 20) * U) * size + 32 * U * (P @ x.abs()) + LEAST[dt]
         assert ((out.double() - ref).abs() <= bound).all(), (name, ((out.double() - ref).abs() / bound).max().item())
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_gradients_that_are_not_numbers(cuda, bad, dt):
+    """A row whose loss has no finite gradient leaves the other rows' gradients as they are."""
+    import metal_kans as mk
+    h, w, t, gen = data(50, 64, 300, dt, 17)
+    grad = 100 * torch.randn(50, generator=gen, device="cuda")
+    rest = torch.arange(50, device="cuda") != 7
+    runs = []
+    for value in (0.0, bad):
+        grad[7] = value
+        hr = h.clone().requires_grad_(True)
+        runs.append(torch.autograd.grad(mk.linear_cross_entropy(hr, w, t, reduction="none"), hr, grad)[0])
+    assert torch.isfinite(runs[0]).all() and torch.equal(runs[0][rest], runs[1][rest])
+    assert not torch.isfinite(runs[1][7]).any()

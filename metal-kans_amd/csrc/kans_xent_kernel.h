@@ -10,9 +10,12 @@
 //
 // G is stored as (p - [v = t]) rho_n up_of<T>() with |rho_n| <= 1 (the row's share of the largest |c_n|; 1 where
 // all rows have the same); the factor common to all rows comes in at the end, in fp32.  So fp16's smallest
-// number stands for p = 2^-38, and p below fp32's normal numbers stays a normal one (the matrix pipe may drop
-// others).  Rounding G to the inputs' type is an error of half a step of that type in each
-// term of a sum whose result is rounded to that type too.
+// number stands for p rho = 2^-38, and p below fp32's normal numbers stays a normal one (the matrix pipe may drop
+// others).  Where an fp16 call's rows differ by more than kXentAlike, dH takes a G without rho_n, which comes in at its end, so
+// that a row's small probabilities do not depend on the other rows; dW adds the rows up, at the scale of the largest.
+// Rounding G to the inputs' type is an error of half a step of that type in each
+// term of a sum whose result is rounded to that type too.  (A gradient of hidden or weight whose sum over G / c_n exceeds 2^96,
+// fp16 2^114, leaves fp32's range on the way.)
 #pragma once
 #include <algorithm>
 #include <cmath>
@@ -28,6 +31,8 @@ constexpr long kXentPiece = 1L << 28;  // elements of G in memory at a time (2^2
 constexpr long kXentHeadPiece = 1L << 28;  // elements of the head that are laid out anew at a time
 constexpr int kPad = 256;              // compact rows and vocabulary of a piece are padded to this
 constexpr float kNoLogit = -__builtin_inff();
+template <typename TO> constexpr bool kOwnG = std::is_same_v<TO, _Float16>;  // types whose rows may need a G of their own
+constexpr float kXentAlike = 64.0f;    // rows whose gradients differ by less share one G: six of fp16's 38 bits below 1
 
 template <typename TO> struct XentTypes { typedef TO T; static constexpr int TERMS = 1; };
 template <> struct XentTypes<float> { typedef __bf16 T; static constexpr int TERMS = 3; };
@@ -51,7 +56,8 @@ struct XentArgs {
   const int64_t* target;       // XE_GRAD: of the call's rows
   const float* rho;            // XE_GRAD: per compact row, or null (1)
   char* g;                     // XE_GRAD: panels [v / kStep][Np][kStep]
-  const float* alpha;          // XE_DW: factor
+  char* g_own;                 // the same without rho, for dH (fp16; null: one G); made and read where alpha[1] is not 0
+  const float* alpha;          // factor of all of G; whether the rows' own factors come in behind dH
   void* out;                   // XE_DW: dW of the piece [V][D]
   int D;
   float* acc;                  // XE_DH: [split][rows of its tiles][Dq] fp32; XE_DW_SPLIT: [split][Vp][Dq]
@@ -181,7 +187,10 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     steps = min(each, steps - first);
   }
   floatx16 acc[MB][NB];
-  Tile::run(A.A, A.B, m0, n0, kOverD ? A.D : A.V, kOverRows ? A.V : count, first, steps, a_st0, a_st1, a_st2, b_st0, b_st1, acc);
+  GemmOperand operand_b = A.B;
+  if constexpr (EPI == XE_DH && kOwnG<TO>)
+    if (A.g_own && A.alpha[1] != 0.0f) operand_b.p = A.g_own;
+  Tile::run(A.A, operand_b, m0, n0, kOverD ? A.D : A.V, kOverRows ? A.V : count, first, steps, a_st0, a_st1, a_st2, b_st0, b_st1, acc);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / WAVES_N, wn = wave % WAVES_N, col = lane & 31, half = lane >> 5;
@@ -276,41 +285,54 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[i][j][r] = there ? acc[i][j][r] : 0.0f;
       }
-      auto write = [&](const auto& exp_up) {
-        const float times = exp_up.by * rho;
+      auto write = [&](const auto& exp_up, auto both) {  // both: G with and without rho
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int q = 0; q < 4; q += 2) {
             const int m = mrow(i, 4 * q);  // values 0 .. 3 are its rows, 4 .. 7 those 8 further on
-            float v[8];
+            float e_up[8], of_target = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = exp_up(acc[i][j][4 * q + e]) * times;
+            for (int e = 0; e < 8; ++e) e_up[e] = exp_up(acc[i][j][4 * q + e]);
             const int own = t - m;
-            if (__builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4))) {
+            const bool targets = __builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4)) != 0;
+            if (targets) {
               // p - 1 of the target: what a confident row has left lies far below p's rounding
-              float x = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) x = own == e % 4 + e / 4 * 8 ? acc[i][j][4 * q + e] : x;
-              x = expm1f((x - top) - rest) * (kUp * rho);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = own == e % 4 + e / 4 * 8 ? x : v[e];
+              for (int e = 0; e < 8; ++e) of_target = own == e % 4 + e / 4 * 8 ? acc[i][j][4 * q + e] : of_target;
+              of_target = expm1f((of_target - top) - rest);
             }
-            uint4 d[TERMS];
-            pack8<T, TERMS>(v, d);
             // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
             const int m8 = m - 4 * half + 8 * half;
-            char* o = A.g + ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
+            const long o = ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
+            auto put = [&](char* g, float factor) {
+              const float times = exp_up.by * factor;
+              float v[8];
 #pragma unroll
-            for (int c = 0; c < TERMS; ++c) {
-              const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
-              const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
-              *(uint4*)(o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
-            }
+              for (int e = 0; e < 8; ++e) v[e] = e_up[e] * times;
+              if (targets) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = own == e % 4 + e / 4 * 8 ? of_target * (kUp * factor) : v[e];
+              }
+              uint4 d[TERMS];
+              pack8<T, TERMS>(v, d);
+#pragma unroll
+              for (int c = 0; c < TERMS; ++c) {
+                const auto x = __builtin_amdgcn_permlane32_swap(d[c].x, d[c].z, false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(d[c].y, d[c].w, false, false);
+                *(uint4*)(g + o + c * K * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+              }
+            };
+            if constexpr (decltype(both)::value) put(A.g_own, 1.0f);
+            put(A.g, rho);
           }
       };
-      if (TERMS == 3 || far(top)) write(ExpUp<true>(top, rest, kLogUp, there));
-      else write(ExpUp<false>(top, rest, kLogUp, there));
+      auto with = [&](auto both) {
+        if (TERMS == 3 || far(top)) write(ExpUp<true>(top, rest, kLogUp, there), both);
+        else write(ExpUp<false>(top, rest, kLogUp, there), both);
+      };
+      if (kOwnG<TO> && A.g_own && A.alpha[1] != 0.0f) with(std::bool_constant<kOwnG<TO>>{});
+      else with(std::false_type{});
     }
   } else if constexpr (EPI == XE_DW) {
     const float alpha = *A.alpha;
@@ -528,29 +550,40 @@ __device__ __forceinline__ void lay_out(const XentBegin& A, const XentLayout& L,
 __device__ __forceinline__ void make_scale(const XentBegin& A, float* join) {
   const int count = A.state[0];
   if (A.reduction != 0) {
-    if (threadIdx.x == 0) *A.alpha = count == 0 ? 0.0f : (A.reduction == 1 ? *A.grad / (float)count : *A.grad) / A.up;
+    if (threadIdx.x == 0) {
+      A.alpha[0] = count == 0 ? 0.0f : (A.reduction == 1 ? *A.grad / (float)count : *A.grad) / A.up;
+      A.alpha[1] = 0.0f;
+    }
     return;
   }
   // (of the finite gradients: an infinite one or a NaN is its row's own, and the others' G stays in its range)
-  float top = 0.0f;
+  float top = 0.0f, least = __builtin_inff();
   for (int n = threadIdx.x; n < count; n += 256) {
     const float g = __builtin_fabsf(A.grad[A.state[kXentHead + n]]);
     top = fmaxf(top, g < __builtin_inff() ? g : 0.0f);
+    least = g > 0.0f ? fminf(least, g) : least;
   }
   join[threadIdx.x] = top;
+  join[256 + threadIdx.x] = least;
   __syncthreads();
   for (int d = 128; d > 0; d >>= 1) {
-    if ((int)threadIdx.x < d) join[threadIdx.x] = fmaxf(join[threadIdx.x], join[threadIdx.x + d]);
+    if ((int)threadIdx.x < d) {
+      join[threadIdx.x] = fmaxf(join[threadIdx.x], join[threadIdx.x + d]);
+      join[256 + threadIdx.x] = fminf(join[256 + threadIdx.x], join[256 + threadIdx.x + d]);
+    }
     __syncthreads();
   }
   const float by = join[0] > 0.0f ? join[0] : 1.0f;
-  if (threadIdx.x == 0) *A.alpha = by / A.up;
+  if (threadIdx.x == 0) {
+    A.alpha[0] = by / A.up;
+    A.alpha[1] = join[256] * kXentAlike < by ? 1.0f : 0.0f;
+  }
   for (int n = threadIdx.x; n < count; n += 256) A.rho[n] = A.grad[A.state[kXentHead + n]] / by;
 }
 
 template <typename TO>
 __global__ __launch_bounds__(256) void k_xent_begin(const XentBegin A) {
-  __shared__ float join[256];
+  __shared__ float join[512];
   int block = blockIdx.x;
   if (A.number_rows && block-- == 0) return keep_numbers(A, (int*)join);
   if (A.make_scale && block-- == 0) return make_scale(A, join);
@@ -649,14 +682,16 @@ __device__ __forceinline__ void finish_row(const float* acc, int splits, long st
 template <typename TO>
 __global__ __launch_bounds__(256) void k_xent_dh(const float* __restrict__ acc, int bn, int n_tiles, int splits, int most, long Dq, int D,
                                                  const int* __restrict__ state, const int64_t* __restrict__ target,
-                                                 int64_t ignore, const float* __restrict__ alpha, TO* __restrict__ dH) {
+                                                 int64_t ignore, const float* __restrict__ alpha, const float* __restrict__ own,
+                                                 TO* __restrict__ dH) {
   const int row = blockIdx.x;
   if (target[row] == ignore)
     for (int d = threadIdx.x; d < D; d += 256) dH[(long)row * D + d] = (TO)0.0f;
   const int count = state[0];
   if (row >= count) return;
   const XentShare share = share_of(count, bn, n_tiles, splits, most);
-  finish_row(acc + row * Dq, share.splits, (long)share.n_tiles * bn * Dq, D, *alpha, dH + (long)state[kXentHead + row] * D);
+  const float factor = own && alpha[1] != 0.0f ? alpha[0] * own[row] : alpha[0];  // (own: the rows' factors, if G lacks them)
+  finish_row(acc + row * Dq, share.splits, (long)share.n_tiles * bn * Dq, D, factor, dH + (long)state[kXentHead + row] * D);
 }
 
 template <typename TO>
@@ -740,11 +775,12 @@ struct XentPlan {
   SplitTile dh, dw;        // dw in splits only where the vocabulary is one piece
   int dh_most;             // splits of dh where rows are ignored (share_of)
   // offsets into the workspace
-  size_t h, w, part, picked, rows, g, acc, acc_w, alpha, rho, bytes;
+  bool own;                // a second G of the rows' own scale
+  size_t h, w, part, picked, rows, g, g_own, acc, acc_w, alpha, rho, bytes;
 };
 
 template <typename TO>
-XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
+XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward, bool own) {
   XentPlan<TO> p{};
   typedef XentPlan<TO> P;
   p.Np = up_to(N, kPad);
@@ -755,7 +791,9 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
   // reading them (24 x 800 x 77870, 249 MB: 69 us, with panels 191)
   p.pack_w = (P::TERMS == 3 && (backward || N > Tiles<TO>::narrow_n)) || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
   const long all = up_to(V, kPad);
-  p.piece = std::max<long>(kPad, std::min({all, kXentPiece / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
+  p.own = own && kOwnG<TO> && backward;
+  const long elements = p.own ? kXentPiece / 2 : kXentPiece;
+  p.piece = std::max<long>(kPad, std::min({all, elements / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
   // (in one piece where nothing of it is laid out; a grid holds fewer than 2^32 threads, 2^-7 of the logits)
   if (!backward && !p.pack_w) p.piece = std::max<long>(kPad, std::min(all, (1L << 37) / p.Np / kPad * kPad));
   p.pieces = (V + p.piece - 1) / p.piece;
@@ -779,9 +817,10 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward) {
     p.dh_most = std::max<int>(p.dh.splits, (int)(std::min<long>(V, p.piece) / P::K / 8));
     p.dw = split_tile<TO>(D, std::min<long>(V, p.piece), p.Np / P::K, p.pieces > 1 ? 1 : 32);
     p.g = take((size_t)p.piece / P::K * p.Np * P::ROW);
+    p.g_own = p.own ? take((size_t)p.piece / P::K * p.Np * P::ROW) : 0;
     p.acc = take((size_t)p.dh.splits * p.Np * p.Dq * 4);
     p.acc_w = p.dw.splits > 1 ? take((size_t)p.dw.splits * p.piece * p.Dq * 4) : 0;
-    p.alpha = take(4);
+    p.alpha = take(8);
     p.rho = take((size_t)N * 4);
   }
   p.bytes = at;
@@ -887,15 +926,17 @@ hipError_t launch_begin(const XentBegin& A, hipStream_t st) {
 
 template <typename TO>
 size_t xent_workspace(int N, int D, int V, bool backward) {
-  // (W's address decides whether it is packed: the larger plan)
-  const size_t a = plan_xent<TO>(N, D, V, nullptr, backward).bytes;
-  return std::max(a, plan_xent<TO>(N, D, V, (const void*)1, backward).bytes);
+  // (W's address decides whether it is packed, the reduction whether there may be two of G: the largest plan)
+  size_t most = 0;
+  for (const bool own : {false, true})
+    for (const void* W : {(const void*)nullptr, (const void*)1}) most = std::max(most, plan_xent<TO>(N, D, V, W, backward, own).bytes);
+  return most;
 }
 
 template <typename TO>
 hipError_t xent_forward(const XentCall& c, hipStream_t st) {
   typedef XentPlan<TO> P;
-  const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, false);
+  const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, false, false);
   float* rows = c.reduction ? (float*)(c.ws + p.rows) : c.loss;
   float* picked = (float*)(c.ws + p.picked);
   const int bm = tile_rows<TO>(p.stats_tile);
@@ -946,7 +987,7 @@ hipError_t xent_forward(const XentCall& c, hipStream_t st) {
 template <typename TO>
 hipError_t xent_backward(const XentCall& c, hipStream_t st) {
   typedef XentPlan<TO> P;
-  const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, true);
+  const P p = plan_xent<TO>(c.N, c.D, c.V, c.W, true, c.reduction == 0 && c.dH);
   float *alpha = (float*)(c.ws + p.alpha), *rho = (float*)(c.ws + p.rho);
   for (long v0 = 0; v0 < c.V; v0 += p.piece) {
     const int n = (int)std::min<long>(p.piece, c.V - v0);
@@ -968,9 +1009,10 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     A.target = c.target;
     A.rho = c.reduction ? nullptr : rho;
     A.g = c.ws + p.g;
+    A.g_own = p.own ? c.ws + p.g_own : nullptr;
+    A.alpha = alpha;
     // (every entry of the padded piece is written: tiles of 256 or 128 entries and rows)
     XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile_for<TO>(n, c.N, p.d_steps), 1, st)));
-    A.alpha = alpha;
     if (c.dW) {
       XentArgs B = A;
       B.A = panel_columns<TO>(c.ws + p.h, p.Np, p.d_steps);
@@ -1000,7 +1042,7 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
   if (c.dH) {
     const int dh_columns = tile_columns<TO>(p.dh.tile);
     hipLaunchKernelGGL((k_xent_dh<TO>), dim3(c.N), dim3(256), 0, st, (const float*)(c.ws + p.acc), dh_columns, (c.N + dh_columns - 1) / dh_columns,
-                       p.dh.splits, p.dh_most, p.Dq, c.D, c.state, c.target, c.ignore, alpha, (TO*)c.dH);
+                       p.dh.splits, p.dh_most, p.Dq, c.D, c.state, c.target, c.ignore, alpha, p.own ? rho : nullptr, (TO*)c.dH);
     XENT_TRY(hipGetLastError());
   }
   return hipSuccess;

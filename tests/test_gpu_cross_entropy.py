@@ -432,3 +432,35 @@ def test_gradients_that_are_not_numbers(cuda, bad, dt):
         runs.append(torch.autograd.grad(mk.linear_cross_entropy(hr, w, t, reduction="none"), hr, grad)[0])
     assert torch.isfinite(runs[0]).all() and torch.equal(runs[0][rest], runs[1][rest])
     assert not torch.isfinite(runs[1][7]).any()
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,d,v", [(40, 64, 60000), (300, 72, 20011), (40, 1024, 900)])
+@pytest.mark.parametrize("least", [2.0 ** -7, 2.0 ** -12, 2.0 ** 9])
+def test_gradients_of_very_different_rows(cuda, least, n, d, v, dt):
+    """One row's gradient is 2^12, the others' down to 2^-24 of that: they keep their own small probabilities in dH.  (dW adds
+    all rows up: relative to the largest.)"""
+    import metal_kans as mk
+    h, w, t, gen = data(n, d, v, dt, 16)
+    h[::2] = 0                                       # probabilities of 1 / v
+    w[:, 0] = 1
+    w[t, 0] = 0
+    grad = torch.full((n,), least, device="cuda")
+    grad[1::4] *= -1.5
+    grad[3], grad[n // 2 | 1] = 2.0 ** 12, 0.0
+    hr, wr = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dh, dw = torch.autograd.grad(mk.linear_cross_entropy(hr, wr, t, reduction="none"), (hr, wr), grad)
+    alone = [torch.autograd.grad(mk.linear_cross_entropy(hr, wr, t, reduction="none"), x, grad)[0] for x in (hr, wr)]
+    assert torch.equal(alone[0], dh) and torch.equal(alone[1], dw)
+    g = torch.softmax(h.double() @ w.double().t(), 1) - torch.nn.functional.one_hot(t, v)
+    g *= grad.double()[:, None]
+    tg, m = (2 * U, 6) if dt == "f32" else (T[dt], 1)
+    for name, out, G, x, k in (("dh", dh, g, w.double(), v), ("dw", dw, g.t(), h.double(), n)):
+        ref, size = G @ x, G.abs() @ x.abs()
+        # G and the result rounded; logits of sums of d products, exponentials, sums of k products (as for the other sizes)
+        bound = T[dt] * ref.abs() + (tg + (m * k / 16 + m * d / 2 + 500) * U) * size + LEAST[dt]
+        if name == "dw" and dt == "f16":             # G below 2^-25 of 2^-14 of the largest gradient has no number
+            bound = bound + 2.0 ** -39 * 2.0 ** 12 * x.abs().sum(0)
+        assert torch.isfinite(out).all() and ((out.double() - ref).abs() <= bound).all(), (
+            name, ((out.double() - ref).abs() / bound).max().item())
+    assert (dh[n // 2 | 1] == 0).all()

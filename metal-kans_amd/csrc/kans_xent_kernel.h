@@ -39,7 +39,8 @@ template <> struct XentTypes<float> { typedef __bf16 T; static constexpr int TER
 
 template <typename T> __host__ __device__ constexpr float up_of() { return std::is_same_v<T, _Float16> ? 0x1p14f : 0x1p32f; }
 
-enum XentEpilogue { XE_STATS, XE_GRAD, XE_DW, XE_DW_SPLIT, XE_DH };
+// (XE_GRAD_OWN: XE_GRAD of a call that may need two of G, a kernel of its own so that the others' stays as short as it is)
+enum XentEpilogue { XE_STATS, XE_GRAD, XE_GRAD_OWN, XE_DW, XE_DW_SPLIT, XE_DH };
 
 struct XentArgs {
   GemmOperand A, B;
@@ -153,7 +154,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
   // a third stage of A where the tile has a CU's LDS for itself and it still fits (160 KB)
   constexpr int A_STAGES = (TERMS == 1 && BM == 256 && BN == 256) || A_RAW ? 3 : 2;
   // dW = G^T H and dH = G W run along the rows of their operands: H and G, or W
-  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES, EPI != XE_STATS && EPI != XE_GRAD,
+  using Tile = GemmTile<T, TERMS, BM, BN, WAVES_M, WAVES_N, A_STAGES, (EPI > XE_GRAD_OWN),
                         EPI == XE_DW || EPI == XE_DW_SPLIT, A_ONCE, A_RAW>;
   using Step = StepOf<TERMS>;
   constexpr int MB = Tile::MB, NB = Tile::NB;
@@ -173,7 +174,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
     split = blockIdx.y;
   } else if constexpr (!kOverRows) {
     // (G of the rows that fill up the last step of k is written too: zeros)
-    n_tiles = min(n_tiles, ((EPI == XE_GRAD ? (count + 63) / 64 * 64 : count) + BN - 1) / BN);
+    n_tiles = min(n_tiles, ((EPI != XE_STATS ? (count + 63) / 64 * 64 : count) + BN - 1) / BN);
   }
   if (id >= A.m_tiles * n_tiles) return;
   int mt, nt;
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
       }
       A.part[(long)mt * A.Np + n0 + c] = s;
     }
-  } else if constexpr (EPI == XE_GRAD) {
+  } else if constexpr (EPI == XE_GRAD || EPI == XE_GRAD_OWN) {
     constexpr float kUp = up_of<TO>(), kLogUp = std::is_same_v<TO, _Float16> ? 14.0f : 32.0f;
     constexpr int K = Step::kStep;
     const int* row = A.state + kXentHead;
@@ -285,23 +286,28 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[i][j][r] = there ? acc[i][j][r] : 0.0f;
       }
+      // p - 1 of the target: what a confident row has left lies far below p's rounding
+      float of_target = 0.0f;
+      const int at = t - (m0 + wm * MB * 32);  // among this wave's entries
+      if (__builtin_amdgcn_ballot_w64((unsigned)at < (unsigned)(MB * 32))) {
+#pragma unroll
+        for (int i = 0; i < MB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            of_target = at == i * 32 + 8 * (r / 4) + 4 * half + r % 4 ? acc[i][j][r] : of_target;
+        of_target = expm1f((of_target - top) - rest);
+      }
       auto write = [&](const auto& exp_up, auto both) {  // both: G with and without rho
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
           for (int q = 0; q < 4; q += 2) {
             const int m = mrow(i, 4 * q);  // values 0 .. 3 are its rows, 4 .. 7 those 8 further on
-            float e_up[8], of_target = 0.0f;
+            float e_up[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) e_up[e] = exp_up(acc[i][j][4 * q + e]);
             const int own = t - m;
             const bool targets = __builtin_amdgcn_ballot_w64((unsigned)own < 12u && !(own & 4)) != 0;
-            if (targets) {
-              // p - 1 of the target: what a confident row has left lies far below p's rounding
-#pragma unroll
-              for (int e = 0; e < 8; ++e) of_target = own == e % 4 + e / 4 * 8 ? acc[i][j][4 * q + e] : of_target;
-              of_target = expm1f((of_target - top) - rest);
-            }
             // the two halves of the wave hold rows 0 .. 3 and 4 .. 7 of each 8: the lower takes the first 8, the upper the others
             const int m8 = m - 4 * half + 8 * half;
             const long o = ((long)(m8 / K) * A.Np + n) * Step::row_bytes + m8 % K * 2;
@@ -331,7 +337,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
         if (TERMS == 3 || far(top)) write(ExpUp<true>(top, rest, kLogUp, there), both);
         else write(ExpUp<false>(top, rest, kLogUp, there), both);
       };
-      if (kOwnG<TO> && A.g_own && A.alpha[1] != 0.0f) with(std::bool_constant<kOwnG<TO>>{});
+      if (EPI == XE_GRAD_OWN && A.alpha[1] != 0.0f) with(std::bool_constant<EPI == XE_GRAD_OWN>{});
       else with(std::false_type{});
     }
   } else if constexpr (EPI == XE_DW) {
@@ -792,8 +798,7 @@ XentPlan<TO> plan_xent(int N, int D, int V, const void* W, bool backward, bool o
   p.pack_w = (P::TERMS == 3 && (backward || N > Tiles<TO>::narrow_n)) || D % P::K != 0 || ((uintptr_t)W & 15) != 0;
   const long all = up_to(V, kPad);
   p.own = own && kOwnG<TO> && backward;
-  const long elements = p.own ? kXentPiece / 2 : kXentPiece;
-  p.piece = std::max<long>(kPad, std::min({all, elements / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
+  p.piece = std::max<long>(kPad, std::min({all, kXentPiece / p.Np / kPad * kPad, kXentHeadPiece / p.Dk / kPad * kPad}));
   // (in one piece where nothing of it is laid out; a grid holds fewer than 2^32 threads, 2^-7 of the logits)
   if (!backward && !p.pack_w) p.piece = std::max<long>(kPad, std::min(all, (1L << 37) / p.Np / kPad * kPad));
   p.pieces = (V + p.piece - 1) / p.piece;
@@ -847,7 +852,7 @@ hipError_t launch_gemm(XentArgs A, long m, long n, int tile, int splits, hipStre
   typedef integral_constant<int, 128> c128;
   typedef integral_constant<int, 256> c256;
   constexpr std::false_type no{};
-  if constexpr (EPI == XE_STATS || EPI == XE_GRAD)
+  if constexpr (EPI <= XE_GRAD_OWN)
     if (tile == TILE_NARROW) {
       // One tile of rows reads the head's entries once.  The forward does so nontemporal where the caches (256 MB) will not hold
       // the most of the head until its next pass: 16 x 4096 x 131072 bf16 (1.1 GB) 193.8 -> 175.1 us, a step of 20 rows (820 MB)
@@ -1012,7 +1017,10 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     A.g_own = p.own ? c.ws + p.g_own : nullptr;
     A.alpha = alpha;
     // (every entry of the padded piece is written: tiles of 256 or 128 entries and rows)
-    XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile_for<TO>(n, c.N, p.d_steps), 1, st)));
+    constexpr int kMaybeOwn = kOwnG<TO> ? XE_GRAD_OWN : XE_GRAD;
+    const int tile = tile_for<TO>(n, c.N, p.d_steps);
+    if (p.own) XENT_TRY((launch_gemm<TO, kMaybeOwn>(A, up_to(n, kPad), up_to(c.N, 64), tile, 1, st)));
+    else XENT_TRY((launch_gemm<TO, XE_GRAD>(A, up_to(n, kPad), up_to(c.N, 64), tile, 1, st)));
     if (c.dW) {
       XentArgs B = A;
       B.A = panel_columns<TO>(c.ws + p.h, p.Np, p.d_steps);

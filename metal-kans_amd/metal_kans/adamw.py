@@ -127,6 +127,13 @@ def _dense(p: torch.Tensor) -> bool:
     return True
 
 
+def _refuse_variants(group: dict) -> None:
+    """Options of torch's AdamW, as in the state it saves, that make another step than this one."""
+    for name in ("amsgrad", "maximize"):
+        if group.get(name):
+            raise ValueError(f"TorchAdamW has no {name!r}")
+
+
 class TorchAdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) on device tensors.
 
@@ -153,6 +160,7 @@ class TorchAdamW(torch.optim.Optimizer):
                 raise ValueError("lr, eps and weight_decay must be >= 0")
             if not (0 <= b1 < 1 and 0 <= b2 < 1):
                 raise ValueError(f"betas must be in [0, 1), got {g['betas']}")
+            _refuse_variants(g)
             for p in g["params"]:
                 if p.dtype not in _DT:
                     raise TypeError(f"unsupported parameter dtype {p.dtype}")
@@ -221,6 +229,8 @@ class TorchAdamW(torch.optim.Optimizer):
         groups = state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("the parameter groups differ in number or size")
+        for g in groups:
+            _refuse_variants(g)
         state, arenas = dict(self.state), self._arenas
         loaded = {}
         for g, sg in zip(self.param_groups, groups):

@@ -90,3 +90,17 @@ def test_adamw_states_follow_the_order_of_memory(mk):
     b.params[0].data = torch.zeros(5, 3).t()
     with pytest.raises(ValueError, match="order"):
         b.start(0, codes)
+
+
+def test_adamw_refuses_other_steps(mk):
+    """Options of torch's AdamW in a group or a saved state that would be dropped without a word."""
+    p, q = torch.nn.Parameter(torch.zeros(3)), torch.nn.Parameter(torch.zeros(3))
+    for option in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError, match=option):
+            mk.TorchAdamW([dict(params=[p], **{option: True})])
+        other = torch.optim.AdamW([q], lr=0.5, **{option: True})
+        opt = mk.TorchAdamW([p])
+        with pytest.raises(ValueError, match=option):
+            opt.load_state_dict(other.state_dict())
+        assert opt.param_groups[0]["lr"] == 1e-3
+    mk.TorchAdamW([dict(params=[p], amsgrad=False, maximize=False)])

@@ -431,7 +431,7 @@ int kans_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* 
 int kans_residual_norm_forward(int res_dtype, int dtype, int kind, const void* x, const void* block, const void* gate,
                                long gate_group, const void* post_w, const void* pre_w, const float* scale_dev, double scale,
                                double eps, void* y, void* h, float* stats, long rows, int D, void* stream);
-/* bytes of device memory that the backward works in (gate_group 0: no gate) */
+/* bytes of device memory that the backward works in, whatever gradients are asked for (gate_group 0: no gate) */
 long kans_residual_norm_workspace(long rows, int D, long gate_group);
 /* Gradients from dy (res_dtype) and dh (dtype), either of which may be null (zero): dx in res_dtype, dscale one
  * fp32, the others in `dtype` (dgate summed over the rows that share a gate row, or with dgate_f32 = 1, for
@@ -449,13 +449,16 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
  * Rows whose target is ignore_index take part in nothing, whatever H holds there; another target outside
  * [0, V) makes its row's loss NaN.  `state` (int32, 4 + 3 N) is filled for the backward.  The workspace
  * (device memory, 16-byte aligned) has kans_linear_xent_workspace bytes, which is negative for refused sizes: N up to
- * 2^21, D to 2^16, V to 2^24. */
+ * 2^21, D to 2^16, V to 2^24.  Losses do not depend on what all logits of a row have in common, beyond the
+ * logits' own rounding. */
 long kans_linear_xent_workspace(int dtype, int N, int D, int V, int backward);
 int kans_linear_xent_forward(int dtype, const void* H, const void* W, const int64_t* target, int N, int D, int V,
                              int64_t ignore_index, int reduction, float* loss, int* state, void* workspace,
                              long workspace_bytes, void* stream);
 /* dH [N][D] and dW [V][D] of `dtype` (null: not computed) from grad, d(result): fp32, [N] for reduction 0, else
- * one; zeros in dH's ignored rows. */
+ * one; zeros in dH's ignored rows.  target is the forward's.  p - [v = target] is rounded to `dtype` before the products (fp32:
+ * to 24 bits).  A row with an infinite or NaN grad leaves the other rows' dH as they are.  Sums over p - [v = target] of more
+ * than 2^96 (fp16 2^114) become infinite. */
 int kans_linear_xent_backward(int dtype, const void* H, const void* W, const int64_t* target, int N, int D, int V,
                               int64_t ignore_index, int reduction, const int* state, const float* grad, void* dH, void* dW,
                               void* workspace, long workspace_bytes, void* stream);

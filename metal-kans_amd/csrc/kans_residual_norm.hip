@@ -335,7 +335,7 @@ __global__ __launch_bounds__(threads_of<TPR>(), TPR > 512 ? 4 : 2) void k_resnor
     load_row<TX, TB, kLayer>(next, A, row, last, at, own < 0 ? -1L : own * D + at);
   };
   // sums of this thread's columns over the run's rows: pre_w, post_w, gate.  At 1024 threads a row they lie in LDS, each
-  // thread its own, so that the rest fits in 128 registers: 8192 x 8192 bf16, both directions, 382 -> 301 us, fp32 780 -> 573.
+  // thread its own, so that the rest fits in 128 registers: 8192 x 8192 bf16, both directions, 382 -> 310 us, fp32 780 -> 585.
   float s[kAhead ? 3 : 1][V];
   auto kept_at = [&](int k, int i) { return &kept[(k * (V / 4) + i) * TPR + threadIdx.x]; };
   auto add_up = [&](int k, const float(&v)[V]) {

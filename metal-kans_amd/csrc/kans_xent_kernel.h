@@ -141,12 +141,12 @@ __device__ __forceinline__ int xcd_tile(int id, int tiles) {
 }
 
 // The products.  8192 x 4096 x 65536 bf16, 256 x 256 tiles (two pieces in the backward):
-//   XE_STATS 3.2 ms (1.37 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 2 x 1.68, XE_DW 2 x 1.69,
-//   XE_DH 2 x 1.62 ms (1.30 - 1.36).
-// The matrix pipe is busy 78 - 84 % of the cycles at the 1.55 GHz that its power leaves; LDS reads meet no
-// bank conflict.  4096 (3686 count) x 1024 x 32768 fp32, 256 x 128: 1.11, 1.18, 1.09 and 1.13 ms (1.25 - 1.36 PFLOP/s of bf16
+//   XE_STATS 3.15 ms (1.40 PFLOP/s; a library's product of the same size 3.10), XE_GRAD 2 x 1.68, XE_DW 2 x 1.62,
+//   XE_DH 2 x 1.58 ms (1.31 - 1.39).
+// The matrix pipe is busy 77 - 84 % of the cycles at the 1.6 GHz that its power leaves; LDS reads meet no
+// bank conflict.  4096 (3686 count) x 1024 x 32768 fp32, 256 x 128: 1.11, 1.19, 1.08 and 1.11 ms (1.25 - 1.37 PFLOP/s of bf16
 // products).  Short sums leave the tiles' beginnings and ends (7 us of 27 at 13 steps of 64): 3001 (2251 count) x 777 x 50021 fp16
-// 0.19, 0.21, 0.24 and 0.20 ms (0.73 - 0.92).
+// 0.19, 0.22, 0.24 and 0.20 ms (0.73 - 0.92).
 template <typename TO, int EPI, int BM, int BN, int WAVES_M, int WAVES_N, bool A_ONCE = false, bool A_RAW = false>
 __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentArgs A) {
   typedef typename XentTypes<TO>::T T;

@@ -37,7 +37,12 @@ constexpr float kXentAlike = 64.0f;    // rows whose gradients differ by less sh
 template <typename TO> struct XentTypes { typedef TO T; static constexpr int TERMS = 1; };
 template <> struct XentTypes<float> { typedef __bf16 T; static constexpr int TERMS = 3; };
 
+template <typename T> constexpr int kLogUpOf = std::is_same_v<T, _Float16> ? 14 : 32;
 template <typename T> __host__ __device__ constexpr float up_of() { return std::is_same_v<T, _Float16> ? 0x1p14f : 0x1p32f; }
+// A product's sum times the factor common to all rows, without the power of two of G: by itself, since a small factor times
+// 1 / up_of would be no normal number any more where the result still is one.
+template <typename T>
+__device__ __forceinline__ float unscaled(float sum, float alpha) { return __builtin_amdgcn_ldexpf(sum * alpha, -kLogUpOf<T>); }
 
 // (XE_GRAD_OWN: XE_GRAD of a call that may need two of G, a kernel of its own so that the others' stays as short as it is)
 enum XentEpilogue { XE_STATS, XE_GRAD, XE_GRAD_OWN, XE_DW, XE_DW_SPLIT, XE_DH };
@@ -259,7 +264,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
       A.part[(long)mt * A.Np + n0 + c] = s;
     }
   } else if constexpr (EPI == XE_GRAD || EPI == XE_GRAD_OWN) {
-    constexpr float kUp = up_of<TO>(), kLogUp = std::is_same_v<TO, _Float16> ? 14.0f : 32.0f;
+    constexpr float kUp = up_of<TO>(), kLogUp = (float)kLogUpOf<TO>;
     constexpr int K = Step::kStep;
     const int* row = A.state + kXentHead;
     const float *rest_of = (const float*)(row + A.N), *top_of = rest_of + A.N;
@@ -356,7 +361,7 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
           for (int q = 0; q < 4; q += 2) {
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = acc[i][j][4 * q + e] * alpha;
+            for (int e = 0; e < 8; ++e) x[e] = unscaled<TO>(acc[i][j][4 * q + e], alpha);
             uint4 d[1];
             pack8<TO, 1>(x, d);
             const auto lo = __builtin_amdgcn_permlane32_swap(d[0].x, d[0].z, false, false);
@@ -379,8 +384,9 @@ __global__ __launch_bounds__(WAVES_M* WAVES_N * 64) void k_xent_gemm(const XentA
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int d = mrow(i, 4 * q);
-            const float x[4] = {acc[i][j][4 * q] * alpha, acc[i][j][4 * q + 1] * alpha, acc[i][j][4 * q + 2] * alpha,
-                                acc[i][j][4 * q + 3] * alpha};
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = unscaled<TO>(acc[i][j][4 * q + e], alpha);
             if (d + 4 <= A.D) {
               __builtin_memcpy(o + d, x, sizeof(x));
             } else {
@@ -470,7 +476,6 @@ struct XentBegin {
   float *picked, *loss;        // cleared with the numbering: what the products may not write
   const float* grad;
   int reduction;
-  float up;
   float *alpha, *rho;
 };
 
@@ -552,12 +557,12 @@ __device__ __forceinline__ void lay_out(const XentBegin& A, const XentLayout& L,
   }
 }
 
-// The factor common to all rows of G (up: the scale that G is stored with) and each row's share of it.
+// The factor common to all rows of G and each row's share of it.
 __device__ __forceinline__ void make_scale(const XentBegin& A, float* join) {
   const int count = A.state[0];
   if (A.reduction != 0) {
     if (threadIdx.x == 0) {
-      A.alpha[0] = count == 0 ? 0.0f : (A.reduction == 1 ? *A.grad / (float)count : *A.grad) / A.up;
+      A.alpha[0] = count == 0 ? 0.0f : A.reduction == 1 ? *A.grad / (float)count : *A.grad;
       A.alpha[1] = 0.0f;
     }
     return;
@@ -581,7 +586,7 @@ __device__ __forceinline__ void make_scale(const XentBegin& A, float* join) {
   }
   const float by = join[0] > 0.0f ? join[0] : 1.0f;
   if (threadIdx.x == 0) {
-    A.alpha[0] = by / A.up;
+    A.alpha[0] = by;
     A.alpha[1] = join[256] * kXentAlike < by ? 1.0f : 0.0f;
   }
   for (int n = threadIdx.x; n < count; n += 256) A.rho[n] = A.grad[A.state[kXentHead + n]] / by;
@@ -670,7 +675,7 @@ __device__ __forceinline__ void finish_row(const float* acc, int splits, long st
       const float4 x = *(const float4*)(acc + k * stride + d);
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
-    const float v[4] = {s.x * alpha, s.y * alpha, s.z * alpha, s.w * alpha};
+    const float v[4] = {unscaled<TO>(s.x, alpha), unscaled<TO>(s.y, alpha), unscaled<TO>(s.z, alpha), unscaled<TO>(s.w, alpha)};
     TO e[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) e[i] = from_f32<TO>(v[i]);
@@ -1002,7 +1007,7 @@ hipError_t xent_backward(const XentCall& c, hipStream_t st) {
     if (v0 == 0) {
       F.m[1] = hidden_layout<TO>(p, c);
       F.make_scale = 1;
-      F.state = c.state; F.grad = c.grad; F.reduction = c.reduction; F.up = up_of<TO>(); F.alpha = alpha; F.rho = rho;
+      F.state = c.state; F.grad = c.grad; F.reduction = c.reduction; F.alpha = alpha; F.rho = rho;
     }
     XENT_TRY(launch_begin<TO>(F, st));
     XentArgs A{};

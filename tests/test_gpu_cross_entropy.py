@@ -464,3 +464,23 @@ def test_gradients_of_very_different_rows(cuda, least, n, d, v, dt):
         assert torch.isfinite(out).all() and ((out.double() - ref).abs() <= bound).all(), (
             name, ((out.double() - ref).abs() / bound).max().item())
     assert (dh[n // 2 | 1] == 0).all()
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("power", [-112, -20, 60])
+def test_size_of_the_gradient(cuda, power, reduction, dt):
+    """Gradients scale with that of the loss, bit for bit, as far as they are normal numbers: here 2^-112 to 2^60 times those
+    of 1, both directions of products included."""
+    import metal_kans as mk
+    h, w, t, gen = data(70, 96, 500, dt, 18)
+    runs = []
+    for p in (0, power):
+        hr, wr = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+        loss = mk.linear_cross_entropy(hr, wr, t, reduction=reduction)
+        grad = torch.full_like(loss, 1.2345 * 2.0 ** p)
+        runs.append(torch.autograd.grad(loss, (hr, wr), grad))
+    for one, other in zip(*runs):
+        want = one.double() * 2.0 ** power
+        normal = want.abs() >= 2.0 ** -126
+        assert normal.any() and torch.equal(other.double()[normal], want[normal])

@@ -448,7 +448,8 @@ int kans_residual_norm_backward(int res_dtype, int dtype, int kind, const void* 
  *   are none), 2: their sum.
  * Rows whose target is ignore_index take part in nothing, whatever H holds there; another target outside
  * [0, V) makes its row's loss NaN.  `state` (int32, 4 + 3 N) is filled for the backward.  The workspace
- * (device memory, 16-byte aligned) has kans_linear_xent_workspace bytes, which is negative for refused sizes: N up to
+ * (device memory, 16-byte aligned) has kans_linear_xent_workspace bytes (backward 0: of the forward, 1: of the backward, 2: of
+ * one for reduction 1 or 2, which may need less), which is negative for refused sizes: N up to
  * 2^21, D to 2^16, V to 2^24.  Losses do not depend on what all logits of a row have in common, beyond the
  * logits' own rounding. */
 long kans_linear_xent_workspace(int dtype, int N, int D, int V, int backward);

@@ -292,7 +292,7 @@ struct Xent {
   int n() const { return (int)h.size(0); }
   int d() const { return (int)h.size(1); }
   int v() const { return (int)w.size(0); }
-  Tensor workspace(bool backward) const {
+  Tensor workspace(int backward) const {
     const long size = lib.xent_workspace(type(), n(), d(), v(), backward);
     check(size, "kans_linear_xent_workspace");
     return bytes(h, size);
@@ -306,7 +306,7 @@ struct Xent {
       if (reduction != 0) loss.fill_(reduction == 1 ? std::numeric_limits<double>::quiet_NaN() : 0.0);
       return {loss, state};
     }
-    const Tensor ws = workspace(false);
+    const Tensor ws = workspace(0);
     check(lib.xent_forward(type(), data(h), data(w), (const int64_t*)data(target), n(), d(), v(), ignore, reduction,
                            (float*)data(loss), (int*)data(state), data(ws), ws.numel(), stream_of(h)),
           "kans_linear_xent_forward");
@@ -319,7 +319,7 @@ struct Xent {
       if (dw.defined()) dw.zero_();
       return {dh, dw};
     }
-    const Tensor ws = workspace(true), g = grad.contiguous();
+    const Tensor ws = workspace(reduction == 0 ? 1 : 2), g = grad.contiguous();
     check(lib.xent_backward(type(), data(h), data(w), (const int64_t*)data(target), n(), d(), v(), ignore, reduction,
                             (const int*)data(state), (const float*)data(g), data(dh), data(dw), data(ws), ws.numel(), stream_of(h)),
           "kans_linear_xent_backward");

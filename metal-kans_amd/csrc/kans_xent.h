@@ -31,8 +31,8 @@ struct XentCall {
   char* ws;
 };
 
-// Bytes of workspace, and the calls, of one element type (launches are enqueued on st).
-template <typename TO> size_t xent_workspace(int N, int D, int V, bool backward);
+// Bytes of workspace (rows: of a call without reduction too), and the calls, of one element type (launches are enqueued on st).
+template <typename TO> size_t xent_workspace(int N, int D, int V, bool backward, bool rows);
 template <typename TO> hipError_t xent_forward(const XentCall& c, hipStream_t st);
 template <typename TO> hipError_t xent_backward(const XentCall& c, hipStream_t st);
 

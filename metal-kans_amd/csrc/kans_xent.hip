@@ -19,10 +19,10 @@ int check_xent(int dtype, const void* H, const void* W, const void* target, int 
   return 0;
 }
 
-size_t workspace(int dtype, int N, int D, int V, bool backward) {
-  return dtype == DT_F16 ? xent_workspace<_Float16>(N, D, V, backward)
-         : dtype == DT_BF16 ? xent_workspace<__bf16>(N, D, V, backward)
-                            : xent_workspace<float>(N, D, V, backward);
+size_t workspace(int dtype, int N, int D, int V, bool backward, bool rows) {
+  return dtype == DT_F16 ? xent_workspace<_Float16>(N, D, V, backward, rows)
+         : dtype == DT_BF16 ? xent_workspace<__bf16>(N, D, V, backward, rows)
+                            : xent_workspace<float>(N, D, V, backward, rows);
 }
 
 }  // namespace
@@ -32,7 +32,7 @@ extern "C" {
 long kans_linear_xent_workspace(int dtype, int N, int D, int V, int backward) {
   const int rc = check_xent(dtype, (void*)8, (void*)8, (void*)8, N, D, V, 0, (void*)8);
   if (rc || N == 0) return rc;
-  return (long)workspace(dtype, N, D, V, backward != 0);
+  return (long)workspace(dtype, N, D, V, backward != 0, backward != 2);
 }
 
 int kans_linear_xent_forward(int dtype, const void* H, const void* W, const int64_t* target, int N, int D, int V,
@@ -42,7 +42,7 @@ int kans_linear_xent_forward(int dtype, const void* H, const void* W, const int6
   if (rc) return rc;
   if (N == 0) return 0;
   if (!loss) return kans_fail(KANS_ERR_ARG, "null loss");
-  const size_t need = workspace(dtype, N, D, V, false);
+  const size_t need = workspace(dtype, N, D, V, false, false);
   if (!workspace_p || ((uintptr_t)workspace_p & 15) || workspace_bytes < (long)need)
     return kans_fail(KANS_ERR_ARG, "workspace of %ld bytes (16-byte aligned), %zu needed", workspace_p ? workspace_bytes : 0, need);
   std::lock_guard<std::mutex> lk(kans_mutex());
@@ -62,7 +62,7 @@ int kans_linear_xent_backward(int dtype, const void* H, const void* W, const int
   if (rc) return rc;
   if (N == 0 || (!dH && !dW)) return 0;
   if (!grad) return kans_fail(KANS_ERR_ARG, "null gradient");
-  const size_t need = workspace(dtype, N, D, V, true);
+  const size_t need = workspace(dtype, N, D, V, true, reduction == 0);
   if (!workspace_p || ((uintptr_t)workspace_p & 15) || workspace_bytes < (long)need)
     return kans_fail(KANS_ERR_ARG, "workspace of %ld bytes (16-byte aligned), %zu needed", workspace_p ? workspace_bytes : 0, need);
   std::lock_guard<std::mutex> lk(kans_mutex());

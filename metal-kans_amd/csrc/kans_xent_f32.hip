@@ -2,7 +2,7 @@
 #include "kans_xent_kernel.h"
 
 namespace kans {
-template size_t xent_workspace<float>(int, int, int, bool);
+template size_t xent_workspace<float>(int, int, int, bool, bool);
 template hipError_t xent_forward<float>(const XentCall&, hipStream_t);
 template hipError_t xent_backward<float>(const XentCall&, hipStream_t);
 }  // namespace kans

@@ -935,10 +935,10 @@ hipError_t launch_begin(const XentBegin& A, hipStream_t st) {
 }  // namespace
 
 template <typename TO>
-size_t xent_workspace(int N, int D, int V, bool backward) {
+size_t xent_workspace(int N, int D, int V, bool backward, bool rows) {
   // (W's address decides whether it is packed, the reduction whether there may be two of G: the largest plan)
   size_t most = 0;
-  for (const bool own : {false, true})
+  for (const bool own : {false, rows})
     for (const void* W : {(const void*)nullptr, (const void*)1}) most = std::max(most, plan_xent<TO>(N, D, V, W, backward, own).bytes);
   return most;
 }

@@ -88,3 +88,15 @@ def test_residual_norm_workspace_of_short_groups(lib, d):
             if rows % group == 0 or rows > 1000:
                 n = rows // group * group
                 assert lib.kans_residual_norm_workspace(n, d, group) <= 2 * plain + 16 * d, (rows, group)
+
+
+def test_linear_xent_workspace_of_a_reduced_loss(lib):
+    """Only a loss of each row may need a second G (fp16): the others' backward takes no more than it did."""
+    def bwd(red, size):
+        return lib.kans_linear_xent_backward(1, 64, 64, 64, 3001, 777, 50021, -100, red, 64, 64, 64, None, 64, size, None)
+    forward, rows, reduced = (lib.kans_linear_xent_workspace(1, 3001, 777, 50021, b) for b in (0, 1, 2))
+    g = 3072 * 50176 * 2
+    assert forward < reduced and g < reduced < 2 * g and rows >= reduced + g
+    for dt in (0, 2):
+        assert lib.kans_linear_xent_workspace(dt, 3001, 777, 50021, 1) == lib.kans_linear_xent_workspace(dt, 3001, 777, 50021, 2)
+    assert bwd(0, reduced) == -1 and bwd(1, reduced - 1) == -1 and bwd(2, reduced - 1) == -1

@@ -439,22 +439,68 @@ void adamw_hold(const py::dict& state, const py::list& params, const py::buffer&
   }
 }
 
+// seen: int64 [2 n], each parameter's address and version behind its last step (version < 0: none).  Both are looked at before and
+// noted behind the whole step, since views of one buffer share a version.
+constexpr int64_t kStepped = -2;
+int64_t version_of(const Tensor& p) { return p.is_inference() ? -1 : p._version(); }
+
+py::buffer_info seen_of(const py::list& params, const py::buffer& seen) {
+  py::buffer_info info = seen.request(/*writable=*/true);
+  if (info.size != 2 * (py::ssize_t)params.size() || info.itemsize != 8) throw py::value_error("one address and version for each parameter");
+  return info;
+}
+
+// Where a parameter with a gradient has changed since its last step: follow(i) brings its master in line.
+void adamw_follow(const py::dict& state, const py::list& params, const py::buffer& blocks, const py::dict& flat, const py::object& start,
+                  const py::buffer& seen, const py::object& follow) {
+  const auto info = seen_of(params, seen), block_of = blocks.request();
+  if (block_of.size != (py::ssize_t)params.size() || block_of.itemsize != 8) throw py::value_error("one block for each parameter");
+  const Arena arena(flat);
+  for (size_t i = 0; i < params.size(); ++i) {
+    const int64_t* const was = (const int64_t*)info.ptr + 2 * i;
+    PyObject* object = PyList_GET_ITEM(params.ptr(), (Py_ssize_t)i);
+    const Tensor& p = THPVariable_Unpack(object);
+    if (was[1] < 0 || (was[0] == (int64_t)(intptr_t)p.data_ptr() && was[1] == version_of(p)) || !p.grad().defined()) continue;
+    PyObject* s = PyDict_GetItemWithError(state.ptr(), object);
+    if (!s && PyErr_Occurred()) throw py::error_already_set();
+    if (!s || PyObject_IsTrue(s) != 1) continue;
+    state_of(state, object, arena, ((const int64_t*)block_of.ptr)[i], start, i);
+    follow(i);
+  }
+}
+
+void adamw_seen(const py::list& params, const py::buffer& seen) {
+  const auto info = seen_of(params, seen);
+  for (size_t i = 0; i < params.size(); ++i) {
+    int64_t* const at = (int64_t*)info.ptr + 2 * i;
+    if (at[1] != kStepped) continue;
+    const Tensor& p = THPVariable_Unpack(PyList_GET_ITEM(params.ptr(), (Py_ssize_t)i));
+    at[0] = (int64_t)(intptr_t)p.data_ptr();
+    at[1] = version_of(p);
+  }
+}
+
 // One step of the parameters of an arena that have gradients.  state: the optimizer's, by parameter; start(i) puts parameter i's into the arena.
+// seen: marks those that a step has written for adamw_seen.
 // numel, blocks: int64 per parameter; flat: the arena's buffers.  A step of 9 small tensors takes 17 us, of 48 with 8-bit
 // states and their values 27; with this loop in Python 23 and 66.
 void adamw_step(const py::dict& state, const py::list& params, const py::buffer& numel, const py::buffer& blocks, const py::dict& flat,
-                int type, int bits, const py::object& start, double lr, double beta1, double beta2, double eps, double decay) {
+                int type, int bits, const py::object& start, double lr, double beta1, double beta2, double eps, double decay,
+                const std::optional<py::buffer>& seen) {
   not_traced("TorchAdamW.step");
   const auto n_of = numel.request(), block_of = blocks.request();
   const size_t n = params.size();
   if ((size_t)n_of.size != n || (size_t)block_of.size != n || n_of.itemsize != 8 || block_of.itemsize != 8)
     throw py::value_error("one size and block for each parameter");
+  std::optional<py::buffer_info> marks;
+  if (seen) marks = seen_of(params, *seen);
   const Arena arena(flat);
   const Tensor &m = arena.flat[0], &v = arena.flat[1], &ms = arena.flat[2], &vs = arena.flat[3], &master = arena.flat[4];
   static PyObject* const step_name = PyUnicode_InternFromString("step");
   struct One {
     Tensor p, grad;
     PyObject* state;
+    int64_t* seen;
   };
   std::vector<One> ones;
   std::vector<void*> at;
@@ -483,7 +529,7 @@ void adamw_step(const py::dict& state, const py::list& params, const py::buffer&
     const long count = step ? PyLong_AsLong(step) : -1;
     if (PyErr_Occurred()) throw py::error_already_set();
     if (!step) throw py::value_error("a parameter's state has no step");
-    ones.push_back({p, g, s});
+    ones.push_back({p, g, s, marks ? (int64_t*)marks->ptr + 2 * i : nullptr});
     at.push_back(p.data_ptr());
     grads.push_back(g.data_ptr());
     sizes.push_back(p.numel());
@@ -498,6 +544,7 @@ void adamw_step(const py::dict& state, const py::list& params, const py::buffer&
     const py::int_ step(steps[i]);
     if (PyDict_SetItem(ones[i].state, step_name, step.ptr()) < 0) throw py::error_already_set();
     ones[i].p.unsafeGetTensorImpl()->bump_version();
+    if (ones[i].seen) ones[i].seen[1] = kStepped;
   }
 }
 
@@ -513,7 +560,11 @@ PYBIND11_MODULE(_kans_torch, m) {
   });
   m.def("bind", &bind);
   m.def("residual_norm", &residual_norm, py::call_guard<py::gil_scoped_release>());
-  m.def("adamw_step", &adamw_step);
+  m.def("adamw_step", &adamw_step, py::arg("state"), py::arg("params"), py::arg("numel"), py::arg("blocks"), py::arg("flat"),
+        py::arg("type"), py::arg("bits"), py::arg("start"), py::arg("lr"), py::arg("beta1"), py::arg("beta2"), py::arg("eps"),
+        py::arg("decay"), py::arg("seen") = py::none());
   m.def("adamw_hold", &adamw_hold);
+  m.def("adamw_follow", &adamw_follow);
+  m.def("adamw_seen", &adamw_seen);
   m.def("linear_cross_entropy", &linear_cross_entropy, py::call_guard<py::gil_scoped_release>());
 }

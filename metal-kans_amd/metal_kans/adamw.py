@@ -16,8 +16,9 @@ buffers.  Per parameter:
 A tensor that a program puts in one's place is copied into the buffer by the next step.
 
 Gradients that are None leave their parameter alone.  Parameters are dense in memory, in any order of their dimensions;
-fp32 states follow a parameter into another order, 8-bit ones refuse it (``state.clear()`` starts anew).  A master follows its parameter only when it is
-made: after other changes to a 16-bit parameter (a loaded model), ``state.clear()`` starts anew.  A step on a
+fp32 states follow a parameter into another order, 8-bit ones refuse it (``state.clear()`` starts anew).  A 16-bit
+parameter that was changed between steps (a loaded model; by its version or address, which an edit through ``.data`` moves
+neither) gives its master its value where it is not the master's rounding any more.  A step on a
 capturing stream is refused (its bias corrections belong to that one step).
 """
 from __future__ import annotations
@@ -62,6 +63,7 @@ class _Arena:
         if self.dtype != f32:
             self.flat["master"] = zeros(total * BLOCK, f32)
         self.numel_q, self.blocks_q = array("q", self.numel), array("q", self.blocks)
+        self.seen = array("q", [-1] * (2 * len(params)))  # address and version behind the last step
 
     def views(self, i: int) -> Dict[str, torch.Tensor]:
         b, n, shape = self.blocks[i], self.numel[i], self.params[i].shape
@@ -104,6 +106,13 @@ class _Arena:
             else:
                 v.zero_()
         return {"step": int(state.get("step", 0)), **views}
+
+    def follow(self, i: int) -> None:
+        """Parameter i's master where the parameter is not its rounding any more: its value."""
+        p, master = self.params[i].detach(), self.views(i)["master"]
+        if p.dtype != self.dtype or p.device != self.device:
+            return  # (the step refuses it)
+        torch.where(master.to(p.dtype) == p, master, p.float(), out=master)
 
 
 _NOT_DENSE = "parameters must be dense (no gaps or overlaps in memory)"
@@ -267,11 +276,16 @@ class TorchAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for gi, group in enumerate(self.param_groups):
-            lr, (b1, b2), eps, decay = group["lr"], group["betas"], group["eps"], group["weight_decay"]
-            for a in self._group_arenas(gi):
-                load().adamw_step(self.state, a.params, a.numel_q, a.blocks_q, a.flat, _DT[a.dtype], a.bits,
-                                  lambda i, a=a: self._start(a, i), lr, b1, b2, eps, decay)
+        arenas = [(group, a) for gi, group in enumerate(self.param_groups) for a in self._group_arenas(gi)]
+        masters = [a for _, a in arenas if "master" in a.flat]
+        for a in masters:
+            load().adamw_follow(self.state, a.params, a.blocks_q, a.flat, lambda i, a=a: self._start(a, i), a.seen, a.follow)
+        for group, a in arenas:
+            b1, b2 = group["betas"]
+            load().adamw_step(self.state, a.params, a.numel_q, a.blocks_q, a.flat, _DT[a.dtype], a.bits,
+                              lambda i, a=a: self._start(a, i), group["lr"], b1, b2, group["eps"], group["weight_decay"], a.seen)
+        for a in masters:
+            load().adamw_seen(a.params, a.seen)
         return loss
 
     def _start(self, a: _Arena, i: int) -> None:

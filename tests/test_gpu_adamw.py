@@ -503,3 +503,65 @@ def test_8_bit_alignment_and_strides(cuda, dt):
             if isinstance(s, torch.Tensor):
                 other = b.state[y][name]
                 assert torch.equal(s, order(other) if other.dim() == 2 else other), name
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+def test_master_follows_a_changed_parameter(cuda, bits, dt):
+    """A 16-bit parameter that a program writes between steps (a loaded model, a clamp, other memory) counts where it is not
+    its master's rounding any more; elsewhere the master keeps its bits."""
+    import metal_kans as mk
+    p = make([(30, 70)], DT[dt], 16)
+    opt = mk.TorchAdamW(p, lr=0.01, weight_decay=0.0, state_bits=bits)
+    opt.step()
+
+    def change_rows():
+        with torch.no_grad():
+            p[0][:10] = 3.0
+
+    def new_memory():
+        new = p[0].detach().clone()
+        new[:10] = -2.0
+        p[0].data = new
+
+    def load():
+        module = torch.nn.Module()
+        module.p = p[0]
+        module.load_state_dict({"p": torch.full((30, 70), 0.5)})
+
+    def nothing_new():
+        with torch.no_grad():
+            p[0].copy_(p[0].clone())
+    for change, value, rows in ((change_rows, 3.0, 10), (new_memory, -2.0, 10), (nothing_new, None, 0), (load, 0.5, 30)):
+        before = opt.state[p[0]]["master"].clone()
+        change()
+        p[0].grad.zero_()                 # a step of the moments alone: lr an element, or twice that with 8-bit codes
+        opt.step()
+        master = opt.state[p[0]]["master"]
+        assert torch.equal(p[0].detach(), master.to(DT[dt]))
+        if rows:
+            assert (master[:rows] - value).abs().max() <= 0.05
+        assert (master[rows:] - before[rows:]).abs().max() <= 0.05 if rows < 30 else True
+        if rows < 30:                     # (the bits below the parameter's own are still there)
+            assert not torch.equal(master[rows:], master[rows:].to(DT[dt]).float())
+
+
+def test_views_of_one_buffer_are_not_taken_for_changed(cuda):
+    """Parameters that share a buffer share its version: a step of one is no change of another."""
+    import metal_kans as mk
+    flat = torch.randn(3000, device="cuda").to(torch.bfloat16)
+    params = [flat[i:i + 1000].view(10, 100) for i in (0, 1000, 2000)]
+    for p in params:
+        p.grad = torch.randn_like(p)
+    opt = mk.TorchAdamW([dict(params=params[:2]), dict(params=params[2:], lr=0.1)])
+    called = []
+    opt.step()
+    for arenas in opt._arenas.values():
+        for a in arenas:
+            a.follow = lambda i, a=a: called.append(i)
+    for _ in range(3):
+        opt.step()
+    assert not called
+    flat[1500] = 2.0
+    opt.step()
+    assert 1 in called

@@ -403,6 +403,24 @@ int kans_prefill_set_block_pairs(int on);
  * The training step around the layers (no reference counterpart in this form): device pointers,
  * work enqueued on `stream`.
  * ======================================================================= */
+/* Rows of a table for the tokens of a batch: out[n] = scale * W[tokens[n]] (W [V][D], out [N][D] of `dtype`, rows contiguous,
+ * any alignment).  Tokens equal to ignore_index give rows of zeros, others outside [0, V) rows of NaN.  N up to 2^23, D to
+ * 2^16, V to 2^24. */
+int kans_embedding_forward(int dtype, const int64_t* tokens, const void* W, long N, int D, int V, int64_t ignore_index, double scale,
+                           void* out, void* stream);
+/* bytes of device memory (16-byte aligned) that the backward works in; negative for refused sizes */
+long kans_embedding_workspace(int dtype, long N, int D, int V);
+/* dW[v] = scale * the sum of dout[n] over the n with tokens[n] = v, for every v in [0, V), summed in fp32 in a fixed order;
+ * rows of dout whose token is ignore_index or outside [0, V) take no part. */
+int kans_embedding_backward(int dtype, const int64_t* tokens, const void* dout, long N, int D, int V, int64_t ignore_index,
+                            double scale, void* dW, void* workspace, long workspace_bytes, void* stream);
+
+/* Dropout of n elements: y[i] = 0 where r[i] < p 2^32, else x[i] / (1 - p), with r[i] word i % 4 of Philox4x32-10 under the key
+ * `seed` at the counter whose low 64 bits are i / 4 and high 64 bits `offset`.  The key is *seed_dev (device memory) where that is
+ * not null; seed_used (device memory, may be null) receives the key, for the same call on y's gradient. */
+int kans_dropout(int dtype, const void* x, void* y, long n, double p, int64_t seed, const int64_t* seed_dev, int64_t* seed_used,
+                 int64_t offset, void* stream);
+
 /* One AdamW step over n_tensors tensors of element type `dtype`:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),  all in fp32.

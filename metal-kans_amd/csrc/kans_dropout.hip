@@ -1,0 +1,119 @@
+// Dropout from a counter-based generator (gfx950): the mask is computed where it is needed and never stored.
+//
+//   r[i] = word i % 4 of Philox4x32-10 with key `seed` at the counter (i / 4, offset)
+//   y[i] = r[i] < p 2^32 ? 0 : x[i] / (1 - p)
+//
+// The generator (Salmon et al., "Parallel random numbers: as easy as 1, 2, 3", 2011) is a function of the element's
+// index, the call's offset and the seed, so the backward is the same call on the output's gradient and the mask does not
+// depend on how the elements are dealt to threads.
+//
+// Reading x and writing y once is the least traffic.  Beside it stand ten rounds of two 32 x 32 -> 64 bit products
+// for every four elements.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "kans_api_internal.h"
+
+namespace kans {
+namespace {
+
+struct DropArgs {
+  const void* x;
+  void* y;
+  long n;
+  unsigned threshold;  // dropped below it
+  int all;             // p = 1: nothing is kept
+  float scale;
+  unsigned long long seed, offset;
+  const int64_t* seed_dev;
+  int64_t* seed_used;
+};
+
+// Four random words of 32 bits.
+__device__ __forceinline__ void philox(unsigned long long block, unsigned long long offset, unsigned long long key, unsigned (&r)[4]) {
+  unsigned c0 = (unsigned)block, c1 = (unsigned)(block >> 32), c2 = (unsigned)offset, c3 = (unsigned)(offset >> 32);
+  unsigned k0 = (unsigned)key, k1 = (unsigned)(key >> 32);
+#pragma unroll
+  for (int i = 0; i < 10; ++i) {
+    const unsigned long long a = (unsigned long long)c0 * 0xD2511F53u, b = (unsigned long long)c2 * 0xCD9E8D57u;
+    c0 = (unsigned)(b >> 32) ^ c1 ^ k0;
+    c2 = (unsigned)(a >> 32) ^ c3 ^ k1;
+    c1 = (unsigned)b;
+    c3 = (unsigned)a;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  r[0] = c0; r[1] = c1; r[2] = c2; r[3] = c3;
+}
+
+template <typename T> using Wide = unsigned __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+
+// A thread takes 16 bytes.
+template <typename T>
+__global__ __launch_bounds__(256) void k_dropout(const DropArgs A) {
+  constexpr int V = 16 / sizeof(T);
+  const unsigned long long seed = A.seed_dev ? (unsigned long long)*A.seed_dev : A.seed;
+  const long at = ((long)blockIdx.x * 256 + threadIdx.x) * V;
+  if (A.seed_used && at == 0) *A.seed_used = (int64_t)seed;
+  if (at >= A.n) return;
+  const T* x = (const T*)A.x + at;
+  T* y = (T*)A.y + at;
+  const bool whole = at + V <= A.n;
+  T v[V];
+  if (whole) __builtin_memcpy(v, x, sizeof(v));
+  else
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = at + e < A.n ? x[e] : from_f32<T>(0.0f);
+#pragma unroll
+  for (int g = 0; g < V / 4; ++g) {
+    unsigned r[4];
+    philox((unsigned long long)at / 4 + g, A.offset, seed, r);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool keep = r[e] >= A.threshold && !A.all;
+      v[4 * g + e] = keep ? from_f32<T>(to_f32(v[4 * g + e]) * A.scale) : from_f32<T>(0.0f);
+    }
+  }
+  if (whole) {
+    __builtin_nontemporal_store(__builtin_bit_cast(Wide<T>, v), (Wide<T>*)y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (at + e < A.n) y[e] = v[e];
+  }
+}
+
+}  // namespace
+}  // namespace kans
+
+using namespace kans;
+
+extern "C" int kans_dropout(int dtype, const void* x, void* y, long n, double p, int64_t seed, const int64_t* seed_dev,
+                            int64_t* seed_used, int64_t offset, void* stream) {
+  if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return kans_fail(KANS_ERR_ARG, "dtype %d", dtype);
+  if (n < 0) return kans_fail(KANS_ERR_ARG, "bad dims n=%ld", n);
+  if (!(p >= 0.0 && p <= 1.0)) return kans_fail(KANS_ERR_ARG, "p must be in [0, 1]");
+  if (n && (!x || !y)) return kans_fail(KANS_ERR_ARG, "null argument");
+  if (n >= 1L << 34) return kans_fail(KANS_ERR_UNSUPPORTED, "n=%ld, fewer than 2^34 elements", n);  // (2^32 threads of 4)
+  std::lock_guard<std::mutex> lk(kans_mutex());
+  int rc = kans_ensure_init();
+  if (rc) return rc;
+  const double below = std::nearbyint(p * 4294967296.0);
+  DropArgs A{};
+  A.x = x; A.y = y; A.n = n;
+  A.all = below >= 4294967296.0;
+  A.threshold = A.all ? 0u : (unsigned)below;
+  A.scale = A.all ? 0.0f : (float)(1.0 / (1.0 - p));
+  A.seed = (unsigned long long)seed; A.offset = (unsigned long long)offset;
+  A.seed_dev = seed_dev; A.seed_used = seed_used;
+  const long per = 256L * (dtype == DT_F32 ? 4 : 8);
+  const dim3 grid((unsigned)std::max(1L, (n + per - 1) / per));
+  hipStream_t st = kans_caller_stream(stream);
+  if (dtype == DT_F32) hipLaunchKernelGGL(k_dropout<float>, grid, dim3(256), 0, st, A);
+  else if (dtype == DT_F16) hipLaunchKernelGGL(k_dropout<_Float16>, grid, dim3(256), 0, st, A);
+  else hipLaunchKernelGGL(k_dropout<__bf16>, grid, dim3(256), 0, st, A);
+  HIP_TRY(hipGetLastError());
+  return 0;
+}

@@ -1,5 +1,5 @@
-// residual_norm and linear_cross_entropy on torch tensors as autograd nodes around the library's entry points, and the
-// optimizer's way through its parameters (host code, a Python module of its own).
+// residual_norm, linear_cross_entropy, embedding, dropout, causal_conv and selective_scan on torch tensors as autograd nodes around
+// the library's entry points, and the optimizer's way through its parameters (host code, a Python module of its own).
 //
 // Small calls wait for the host, not for the GPU: torch runs a backward in a thread of its own, and each turn through the
 // interpreter there starts with cold caches.  A forward and backward of 2047 x 1000 fp32 (36 us of kernels) took 165 us
@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -44,6 +45,10 @@ struct Library {
   decltype(&kans_linear_xent_forward) xent_forward;
   decltype(&kans_linear_xent_backward) xent_backward;
   decltype(&kans_adamw_step) adamw_step;
+  decltype(&kans_embedding_forward) embedding_forward;
+  decltype(&kans_embedding_workspace) embedding_workspace;
+  decltype(&kans_embedding_backward) embedding_backward;
+  decltype(&kans_dropout) dropout;
 } lib;
 PyObject* kans_error;  // the package's exception for a negative code
 
@@ -68,6 +73,10 @@ void bind(const py::dict& functions, py::object error) {
   get("kans_linear_xent_forward", lib.xent_forward);
   get("kans_linear_xent_backward", lib.xent_backward);
   get("kans_adamw_step", lib.adamw_step);
+  get("kans_embedding_forward", lib.embedding_forward);
+  get("kans_embedding_workspace", lib.embedding_workspace);
+  get("kans_embedding_backward", lib.embedding_backward);
+  get("kans_dropout", lib.dropout);
   kans_error = error.release().ptr();
 }
 
@@ -116,13 +125,30 @@ void no_tangents(std::initializer_list<const Tensor*> inputs, const char* what) 
     TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative");
 }
 
+// A backward under capture hands its gradients to the streams of the nodes before it.  Where one of these is the default
+// stream -- an eager graph of the same leaf still lives and with it the node that collects the leaf's gradient -- the
+// capture is torn and the process ends at its end: refused here, while there is a call to name.
+void capturable(std::initializer_list<const Tensor*> inputs, const char* what) {
+  for (const Tensor* t : inputs) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    const auto current = c10::hip::getCurrentHIPStream(t->get_device());
+    if (!current.stream()) return;  // (the default stream is never under capture)
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    const auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() != 0, what,
+                " under a graph capture: an autograd graph from outside of it, on the default stream, still holds an input; delete it first");
+  }
+}
+
 // Gradients that cannot be differentiated again: an error to whoever tries, where the graph is kept for it.
 variable_list once(variable_list grads, bool graph) {
   variable_list given;
   for (auto& g : grads)
     if (graph && g.defined()) given.push_back(g.detach().requires_grad_(true));
   if (given.empty()) return grads;
-  const auto node = std::make_shared<torch::autograd::DelayedError>("residual_norm and linear_cross_entropy have no second derivative",
+  const auto node = std::make_shared<torch::autograd::DelayedError>("metal_kans' torch operators have no second derivative",
                                                                    (int64_t)given.size());
   variable_list out = (*node)(std::move(given));
   size_t at = 0;
@@ -368,6 +394,110 @@ std::optional<Tensor> linear_cross_entropy(const Tensor& hidden, const Tensor& w
   return reduction == 0 ? loss.reshape(target.sizes()) : loss;
 }
 
+// ---- embedding -------------------------------------------------------------------------------------
+struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
+  static Tensor call(const Tensor& tokens, const Tensor& w, double scale, int64_t ignore) {
+    auto shape = tokens.sizes().vec();
+    shape.push_back(w.size(1));
+    Tensor out = at::empty(shape, w.options());
+    if (tokens.numel() == 0) return out;
+    check(lib.embedding_forward(type_of(w.scalar_type()), (const int64_t*)data(tokens), data(w), tokens.numel(), (int)w.size(1),
+                                (int)w.size(0), ignore, scale, data(out), stream_of(w)),
+          "kans_embedding_forward");
+    return out;
+  }
+
+  static variable_list forward(AutogradContext* ctx, Tensor tokens, Tensor w, double scale, int64_t ignore) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["rest"] = std::vector<int64_t>{ignore, w.size(0), w.size(1)};
+    return {call(tokens, w, scale, ignore)};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    if (!grads[0].defined()) return variable_list(4);
+    no_tangents({&grads[0]}, "embedding's backward");
+    const auto s = ctx->get_saved_variables();
+    const auto rest = ctx->saved_data["rest"].toIntVector();
+    const Tensor dout = grads[0].contiguous(), &tokens = s[0];
+    const at::OptionalDeviceGuard device(dout.device());
+    Tensor dw = at::empty({rest[1], rest[2]}, dout.options());
+    const int type = type_of(dout.scalar_type()), D = (int)rest[2], V = (int)rest[1];
+    const long size = lib.embedding_workspace(type, tokens.numel(), D, V);
+    check(size, "kans_embedding_workspace");
+    const Tensor ws = bytes(dout, size);
+    check(lib.embedding_backward(type, (const int64_t*)data(tokens), data(dout), tokens.numel(), D, V, rest[0],
+                                 ctx->saved_data["scale"].toDouble(), data(dw), data(ws), size, stream_of(dout)),
+          "kans_embedding_backward");
+    return {Tensor(), once({dw}, graph)[0], Tensor(), Tensor()};
+  }
+};
+
+// None where the arguments do not fit together (the caller says why).
+std::optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t ignore) {
+  not_traced("embedding");
+  if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0 || type_of(weight.scalar_type()) < 0 || !std::isfinite(scale) ||
+      tokens.scalar_type() != at::kLong || !weight.is_cuda() || tokens.device() != weight.device())
+    return {};
+  TORCH_CHECK_VALUE(weight.size(0) <= INT_MAX && weight.size(1) <= INT_MAX, "weight has more than 2^31 rows or columns");
+  const Tensor t = tokens.contiguous(), w = weight.contiguous();
+  no_tangents({&w}, "embedding");
+  const at::OptionalDeviceGuard device(w.device());
+  if (!wants_grad({&w})) return EmbeddingFunction::call(t, w, scale, ignore);
+  capturable({&w}, "embedding");
+  return EmbeddingFunction::apply(t, w, scale, ignore)[0];
+}
+
+// ---- dropout ---------------------------------------------------------------------------------------
+struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
+  // The key is `dev`'s where that is given; used (where wanted) keeps it for the backward, since dev may hold another one by then.
+  static Tensor call(const Tensor& x, double p, int64_t seed, const Tensor& dev, const Tensor& used, int64_t offset) {
+    Tensor y = at::empty_like(x);
+    if (x.numel() == 0) return y;
+    check(lib.dropout(type_of(x.scalar_type()), data(x), data(y), x.numel(), p, seed, (const int64_t*)data(dev), (int64_t*)data(used),
+                      offset, stream_of(x)),
+          "kans_dropout");
+    return y;
+  }
+
+  static variable_list forward(AutogradContext* ctx, Tensor x, double p, int64_t seed, std::optional<Tensor> dev, int64_t offset) {
+    const Tensor used = dev ? at::empty({1}, dev->options()) : Tensor();
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({used});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["rest"] = std::vector<int64_t>{seed, offset};
+    return {call(x, p, seed, dev ? *dev : Tensor(), used, offset)};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    if (!grads[0].defined()) return variable_list(5);
+    no_tangents({&grads[0]}, "dropout's backward");
+    const auto rest = ctx->saved_data["rest"].toIntVector();
+    const Tensor dy = grads[0].contiguous();
+    const at::OptionalDeviceGuard device(dy.device());
+    const Tensor dx = call(dy, ctx->saved_data["p"].toDouble(), rest[0], ctx->get_saved_variables()[0], Tensor(), rest[1]);
+    return {once({dx}, graph)[0], Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// None where the arguments do not fit together (the caller says why).
+std::optional<Tensor> dropout(const Tensor& x, double p, int64_t seed, const std::optional<Tensor>& dev, int64_t offset) {
+  not_traced("dropout");
+  if (type_of(x.scalar_type()) < 0 || !x.is_cuda() || !(p >= 0.0 && p <= 1.0)) return {};
+  if (dev && (dev->numel() != 1 || dev->scalar_type() != at::kLong || dev->device() != x.device())) return {};
+  const Tensor in = x.contiguous();
+  no_tangents({&in}, "dropout");
+  const at::OptionalDeviceGuard device(in.device());
+  if (!wants_grad({&in})) return DropoutFunction::call(in, p, seed, dev ? *dev : Tensor(), Tensor(), offset);
+  capturable({&in}, "dropout");
+  return DropoutFunction::apply(in, p, seed, dev, offset)[0];
+}
+
 // ---- TorchAdamW ------------------------------------------------------------------------------------
 // An arena's buffers (_Arena.flat), and what a parameter's state holds when it is the arena's own: views of them at the
 // parameter's place, in its order of memory.
@@ -567,4 +697,6 @@ PYBIND11_MODULE(_kans_torch, m) {
   m.def("adamw_follow", &adamw_follow);
   m.def("adamw_seen", &adamw_seen);
   m.def("linear_cross_entropy", &linear_cross_entropy, py::call_guard<py::gil_scoped_release>());
+  m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
+  m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
 }

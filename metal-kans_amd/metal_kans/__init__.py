@@ -21,7 +21,7 @@ __version__ = "0.6.0+mi355x"
 # What works on torch tensors and the module it is in: imported on first use so that `import metal_kans` does
 # not import torch; None without torch, as in the reference (metal_kans/__init__.py:34-38).
 _TORCH = {"TorchMetalKANLinear": "torch_module", "TorchMetalKAN": "torch_module", "TorchAdamW": "adamw",
-          "residual_norm": "residual", "linear_cross_entropy": "cross_entropy"}
+          "residual_norm": "residual", "linear_cross_entropy": "cross_entropy", "embedding": "embeddings", "dropout": "dropouts"}
 
 
 def __getattr__(name):
@@ -40,5 +40,5 @@ __all__ = [
     "set_async", "sync", "get_metal_bridge", "is_metal_available", "is_gpu_available",
     "ChebyKAN", "FastKAN", "BSplineKAN", "KAN", "MetalKAN", "GatedKAN",
     "QuantizedWeight", "TernaryQuantizedWeight", "quantize", "to_int8", "to_int4", "to_ternary",
-    "TorchMetalKANLinear", "TorchMetalKAN", "TorchAdamW", "residual_norm", "linear_cross_entropy",
+    "TorchMetalKANLinear", "TorchMetalKAN", "TorchAdamW", "residual_norm", "linear_cross_entropy", "embedding", "dropout",
 ]

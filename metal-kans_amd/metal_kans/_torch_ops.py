@@ -9,7 +9,8 @@ from . import device
 
 _FUNCTIONS = ("kans_last_error", "kans_stream_keep", "kans_residual_norm_forward", "kans_residual_norm_workspace",
               "kans_residual_norm_backward", "kans_linear_xent_workspace", "kans_linear_xent_forward",
-              "kans_linear_xent_backward", "kans_adamw_step")
+              "kans_linear_xent_backward", "kans_adamw_step", "kans_embedding_forward", "kans_embedding_workspace",
+              "kans_embedding_backward", "kans_dropout")
 _module = None
 
 

@@ -145,6 +145,10 @@ SIGNATURES = {
     "kans_linear_xent_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int]),
     "kans_linear_xent_forward": (c_int, [c_int, P, P, P, c_int, c_int, c_int, c_longlong, c_int, P, P, P, c_long, P]),
     "kans_linear_xent_backward": (c_int, [c_int, P, P, P, c_int, c_int, c_int, c_longlong, c_int, P, P, P, P, P, c_long, P]),
+    "kans_embedding_forward": (c_int, [c_int, P, P, c_long, c_int, c_int, c_longlong, c_double, P, P]),
+    "kans_embedding_workspace": (c_long, [c_int, c_long, c_int, c_int]),
+    "kans_embedding_backward": (c_int, [c_int, P, P, c_long, c_int, c_int, c_longlong, c_double, P, P, c_long, P]),
+    "kans_dropout": (c_int, [c_int, P, P, c_long, c_double, c_longlong, P, P, c_longlong, P]),
     "kans_mfma_ceiling": (c_int, [c_int, P, P, c_int, P]),
     "kans_stream_ceiling": (c_int, [P, c_size_t, P]),
 }

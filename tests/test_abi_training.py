@@ -100,3 +100,28 @@ def test_linear_xent_workspace_of_a_reduced_loss(lib):
     for dt in (0, 2):
         assert lib.kans_linear_xent_workspace(dt, 3001, 777, 50021, 1) == lib.kans_linear_xent_workspace(dt, 3001, 777, 50021, 2)
     assert bwd(0, reduced) == -1 and bwd(1, reduced - 1) == -1 and bwd(2, reduced - 1) == -1
+def test_embedding_refusals(lib):
+    def fwd(dt=0, tokens=64, w=64, n=4, d=8, v=5, scale=1.0, out=64):
+        return lib.kans_embedding_forward(dt, tokens, w, n, d, v, -100, scale, out, None)
+
+    def bwd(tokens=64, dout=64, n=4, dw=64, ws=64, size=1 << 20):
+        return lib.kans_embedding_backward(0, tokens, dout, n, 8, 5, -100, 1.0, dw, ws, size, None)
+    for bad in (dict(dt=3), dict(tokens=None), dict(w=None), dict(out=None), dict(n=-1), dict(d=0), dict(v=0),
+                dict(scale=float("inf"))):
+        assert fwd(**bad) == -1, bad
+    for bad in (dict(n=(1 << 23) + 1), dict(d=(1 << 16) + 1), dict(v=(1 << 24) + 1)):
+        assert fwd(**bad) == -5, bad
+    assert fwd(n=0, tokens=None) == 0
+    for bad in (dict(tokens=None), dict(dout=None), dict(dw=None), dict(ws=None), dict(ws=72), dict(size=16), dict(n=-1)):
+        assert bwd(**bad) == -1, bad
+    assert lib.kans_embedding_workspace(0, -1, 8, 5) == -1
+    assert lib.kans_embedding_workspace(0, 4, 8, 1 << 25) == -5
+    assert lib.kans_embedding_workspace(0, 4, 8, 5) >= 4 * (2 * 4 + 5 + 1)
+
+
+def test_dropout_refusals(lib):
+    def go(dt=0, x=64, y=64, n=4, p=0.5):
+        return lib.kans_dropout(dt, x, y, n, p, 1, None, None, 0, None)
+    for bad in (dict(dt=3), dict(x=None), dict(y=None), dict(n=-1), dict(p=-0.1), dict(p=1.1), dict(p=float("nan"))):
+        assert go(**bad) == -1, bad
+    assert go(n=1 << 34) == -5

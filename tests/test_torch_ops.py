@@ -104,3 +104,22 @@ def test_adamw_refuses_other_steps(mk):
             opt.load_state_dict(other.state_dict())
         assert opt.param_groups[0]["lr"] == 1e-3
     mk.TorchAdamW([dict(params=[p], amsgrad=False, maximize=False)])
+
+
+def test_embedding_refuses(mk):
+    t, w = torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4)
+    for bad, error in (((t, w), ValueError), ((t, w[0]), ValueError), ((t, w[:0]), ValueError), ((t, w[:, :0]), ValueError),
+                       ((t, w, float("nan")), ValueError), ((t, w.double()), TypeError), ((t.int(), w), TypeError),
+                       ((None, w), TypeError), ((t, w, "1"), TypeError)):
+        with pytest.raises(error):
+            mk.embedding(*bad)
+
+
+def test_dropout_refuses(mk):
+    x = torch.zeros(3, 4)
+    for bad, error in (((x, 0.1, 1), ValueError), ((x, -0.1, 1), ValueError), ((x, 1.5, 1), ValueError),
+                       ((x, float("nan"), 1), ValueError), ((x, 0.1, 1 << 64), ValueError), ((x, 0.1, 1, -(1 << 63) - 1), ValueError),
+                       ((x.double(), 0.1, 1), TypeError), ((x, 0.1, torch.zeros(2, dtype=torch.int64)), TypeError),
+                       ((x, 0.1, torch.zeros(1)), TypeError), ((x, 0.1, 1.5), TypeError), ((None, 0.1, 1), TypeError)):
+        with pytest.raises(error):
+            mk.dropout(*bad)

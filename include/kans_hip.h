@@ -421,6 +421,47 @@ int kans_embedding_backward(int dtype, const int64_t* tokens, const void* dout, 
 int kans_dropout(int dtype, const void* x, void* y, long n, double p, int64_t seed, const int64_t* seed_dev, int64_t* seed_used,
                  int64_t offset, void* stream);
 
+/* Short causal convolution along the sequence, channel by channel, over B sequences of L steps and D channels of `dtype`:
+ *   u[t] = bias + sum_j w[d][j] x[t - W + 1 + j],  y[t] = silu ? u[t] sigmoid(u[t]) : u[t],
+ * w [D][W], W from 1 to 8; bias [D] or null.  Channels lie side by side; x_batch and x_row are elements between sequences and
+ * between steps of x, y is contiguous.  Inputs before the first step are `state` [B][W - 1][D] (null: zeros), which becomes the last
+ * W - 1 inputs of each sequence.  lengths [B] (device memory; null: L each): steps from a sequence's length on give zeros
+ * and are not looked at. */
+int kans_causal_conv_forward(int dtype, const void* x, long x_batch, long x_row, const void* w, const void* bias, void* state,
+                             const int64_t* lengths, int silu, void* y, int B, int L, int D, int W, void* stream);
+/* bytes of device memory (16-byte aligned) that the backward works in; negative for refused sizes */
+long kans_causal_conv_workspace(int dtype, int B, int L, int D, int W);
+/* Gradients of a forward without a state, from dy (contiguous): dx [B][L][D], dw [D][W], dbias [D] of `dtype`; null ones are not
+ * computed.  Sums over steps are fp32, in a fixed order. */
+int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row, const void* w, const void* bias,
+                              const int64_t* lengths, int silu, const void* dy, void* dx, void* dw, void* dbias, int B, int L, int D,
+                              int W, void* workspace, long workspace_bytes, void* stream);
+
+/* Selective state space scan over B sequences of L steps, D channels and N states (N up to 64):
+ *   s[t] = softplus(dt[t] + dt_bias) (softplus 0: dt[t] + dt_bias),
+ *   h[t] = exp(s[t] A) h[t-1] + s[t] x[t] Bm[t],  out[t] = (Cm[t] . h[t] + skip x[t]) (z[t] sigmoid(z[t])),
+ * all in fp32.  x, dt, z and out [B][L][D], Bm and Cm [B][L][N] are of `dtype`, channels (states) side by side, *_batch and *_row
+ * elements between sequences and between steps, out contiguous; A [D][N] (16-byte aligned), skip [D], dt_bias [D] and state
+ * [B][D][N] (16-byte aligned) are fp32.  skip, z and dt_bias may be null.  state (null: zeros) is the state before the first step
+ * and becomes the one behind the last.  lengths as above: steps from a sequence's length on give zeros and leave the state.
+ * saved (null: not wanted) is filled for the backward, kans_selective_scan_saved bytes.  The workspaces (16-byte aligned
+ * device memory, kans_selective_scan_workspace bytes, which may be 0) are negative for refused sizes. */
+long kans_selective_scan_saved(int B, int L, int D, int N);
+long kans_selective_scan_workspace(int B, int L, int D, int N, int backward);
+int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_row, const void* dt, long dt_batch, long dt_row,
+                                const float* A, const void* Bm, long b_batch, long b_row, const void* Cm, long c_batch, long c_row,
+                                const float* skip, const void* z, long z_batch, long z_row, const float* dt_bias, int softplus,
+                                float* state, const int64_t* lengths, void* out, float* saved, int B, int L, int D, int N,
+                                void* workspace, long workspace_bytes, void* stream);
+/* Gradients of a forward without a state, from dout (contiguous): dx, ddt and, where there is a z, dz [B][L][D] of `dtype`; dB and
+ * dC [B][L][N] of `dtype`, dA [D][N], dskip and ddt_bias [D] in fp32, null ones not computed.  Sums are fp32, in a fixed order. */
+int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_row, const void* dt, long dt_batch, long dt_row,
+                                 const float* A, const void* Bm, long b_batch, long b_row, const void* Cm, long c_batch, long c_row,
+                                 const float* skip, const void* z, long z_batch, long z_row, const float* dt_bias, int softplus,
+                                 const int64_t* lengths, const float* saved, const void* dout, void* dx, void* ddt, float* dA, void* dB,
+                                 void* dC, float* dskip, void* dz, float* ddt_bias, int B, int L, int D, int N, void* workspace,
+                                 long workspace_bytes, void* stream);
+
 /* One AdamW step over n_tensors tensors of element type `dtype`:
  *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *   p = p (1 - lr wd) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps),  all in fp32.

@@ -1,0 +1,342 @@
+// Short causal convolution along the sequence, channel by channel, with its activation (gfx950).
+//
+//   u[t] = bias + sum_j w[j] x[t - W + 1 + j],   y[t] = u[t] sigmoid(u[t])  (or u[t])
+//   du[t] = dy[t] y'(u[t]),   dx[t] = sum_j w[j] du[t + W - 1 - j],   dw[j] = sum_t du[t] x[t - W + 1 + j],   dbias = sum_t du[t]
+//
+// Inputs before the first step are the state (zeros without one); steps behind a sequence's length count as zeros.
+//
+// Bound by memory: the forward reads x and writes y, the backward reads x and dy and writes dx (u is computed again).
+// Channels lie side by side, so a thread takes a few neighbouring ones and walks a tile of steps with the last W - 1
+// inputs in registers; a tile reads W - 1 steps of its neighbour again.  Sums over steps and sequences: a tile writes
+// one partial row for each tap and the bias, and a second kernel adds the rows in a fixed order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kans_api_internal.h"
+
+namespace kans {
+namespace {
+
+constexpr int kMaxTaps = 8;
+
+struct ConvArgs {
+  const void *x, *w, *bias, *dy;
+  void *y, *state, *dx;
+  const int64_t* lengths;
+  float* part;                 // [tiles of all sequences][W + 1][D]
+  long x_batch, x_row;         // elements between sequences and between steps of x
+  int B, L, D, tile, tiles;    // tile: steps of a thread, tiles: of a sequence
+  int vecs;                    // threads beside each other along the channels
+  int silu;
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load(float (&o)[V], const T* p) {
+  T v[V];
+  __builtin_memcpy(v, p, sizeof(v));
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = to_f32(v[e]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&o)[V], int skip) {
+  T v[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = from_f32<T>(o[e]);
+  if (skip == 0) {
+    __builtin_memcpy(p, v, sizeof(v));
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (e >= skip) p[e] = v[e];
+}
+
+__device__ __forceinline__ float sigmoid(float u) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(u * -1.44269504f)); }
+
+// The place of a thread: channels [c, c + V) of which the first `skip` are its neighbour's (the last access of a row ends
+// with it), steps [t0, t1) of sequence b, of which `len` count.
+struct Place {
+  int b, tile, c, skip, t0, t1, len;
+};
+template <int V>
+__device__ __forceinline__ bool place(const ConvArgs& A, Place& p) {
+  const long id = (long)blockIdx.x * 256 + threadIdx.x, row = id / A.vecs;
+  if (row >= (long)A.B * A.tiles) return false;
+  p.b = (int)(row / A.tiles);
+  p.tile = (int)(row - (long)p.b * A.tiles);
+  const int c = (int)(id - row * A.vecs) * V;
+  p.c = min(c, A.D - V);
+  p.skip = c - p.c;
+  p.t0 = p.tile * A.tile;
+  p.t1 = min(p.t0 + A.tile, A.L);
+  p.len = A.lengths ? (int)min(max(A.lengths[p.b], (int64_t)0), (int64_t)A.L) : A.L;
+  return true;
+}
+
+template <typename T, int W, int V>
+__global__ __launch_bounds__(256) void k_conv_fwd(const ConvArgs A) {
+  Place p;
+  if (!place<V>(A, p)) return;
+  const T* x = (const T*)A.x + p.b * A.x_batch + p.c;
+  T* y = (T*)A.y + (long)p.b * A.L * A.D + p.c;
+  T* state = A.state ? (T*)A.state + (long)p.b * (W - 1) * A.D + p.c : nullptr;
+  float w[W][V], bias[V] = {}, before[W][V];  // before: the last W inputs, the newest last
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][e] = to_f32(((const T*)A.w)[(long)(p.c + e) * W + j]);
+  if (A.bias) load(bias, (const T*)A.bias + p.c);
+  auto input = [&](float (&o)[V], int t) {  // the input of step t >= -(W - 1)
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = 0.0f;
+    if (t >= 0 && t < p.len) load(o, x + (long)t * A.x_row);
+    else if (t < 0 && state) load(o, state + (long)(t + W - 1) * A.D);
+  };
+#pragma unroll
+  for (int j = 1; j < W; ++j) input(before[j], p.t0 - W + j);
+  // The new state: the last W - 1 inputs of the sequence.  The first tile writes it, which alone reads the old one; the
+  // thread's own channels, so that no other reads what it has written.
+  float last[W][V];
+  if (state && p.tile == 0)
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) input(last[j], p.len - (W - 1) + j);
+  for (int t = p.t0; t < p.t1; ++t) {
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) before[j][e] = before[j + 1][e];
+    input(before[W - 1], t);
+    float o[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float u = bias[e];
+#pragma unroll
+      for (int j = 0; j < W; ++j) u += w[j][e] * before[j][e];
+      o[e] = t >= p.len ? 0.0f : A.silu ? u * sigmoid(u) : u;
+    }
+    store(y + (long)t * A.D, o, p.skip);
+  }
+  if (state && p.tile == 0)
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j) store(state + (long)j * A.D, last[j], p.skip);
+}
+
+template <typename T, int W, int V>
+__global__ __launch_bounds__(256) void k_conv_bwd(const ConvArgs A) {
+  Place p;
+  if (!place<V>(A, p)) return;
+  const T* x = (const T*)A.x + p.b * A.x_batch + p.c;
+  const T* dy = (const T*)A.dy + (long)p.b * A.L * A.D + p.c;
+  T* dx = A.dx ? (T*)A.dx + (long)p.b * A.L * A.D + p.c : nullptr;
+  float w[W][V], bias[V] = {}, before[W][V] = {}, du[W][V] = {}, dw[W][V] = {}, dbias[V] = {};
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+#pragma unroll
+    for (int j = 0; j < W; ++j) w[j][e] = to_f32(((const T*)A.w)[(long)(p.c + e) * W + j]);
+  if (A.bias) load(bias, (const T*)A.bias + p.c);
+  auto input = [&](float (&o)[V], int t) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = 0.0f;
+    if (t >= 0 && t < p.len) load(o, x + (long)t * A.x_row);
+  };
+#pragma unroll
+  for (int j = 1; j < W; ++j) input(before[j], p.t0 - W + j);
+  // dx[t] needs du up to t + W - 1: the walk goes W - 1 steps beyond the tile, whose du the next tile adds up
+  for (int t = p.t0; t < p.t1 + W - 1; ++t) {
+#pragma unroll
+    for (int j = 0; j < W - 1; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        before[j][e] = before[j + 1][e];
+        du[j][e] = du[j + 1][e];
+      }
+    input(before[W - 1], t);
+    float d[V] = {};
+    if (t < p.len) load(d, dy + (long)t * A.D);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float u = bias[e], g = 1.0f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) u += w[j][e] * before[j][e];
+      if (A.silu) {
+        const float s = sigmoid(u);
+        g = s * (1.0f + u * (1.0f - s));
+      }
+      du[W - 1][e] = t < p.len ? d[e] * g : 0.0f;
+      if (t < p.t1) {
+        dbias[e] += du[W - 1][e];
+#pragma unroll
+        for (int j = 0; j < W; ++j) dw[j][e] += du[W - 1][e] * before[j][e];
+      }
+    }
+    if (dx && t - (W - 1) >= p.t0) {  // du[j] is that of step t - (W - 1) + j
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        o[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[e] += w[W - 1 - j][e] * du[j][e];
+        if (t - (W - 1) >= p.len) o[e] = 0.0f;
+      }
+      store(dx + (long)(t - (W - 1)) * A.D, o, p.skip);
+    }
+  }
+  if (!A.part) return;
+  float* part = A.part + ((long)p.b * A.tiles + p.tile) * (W + 1) * A.D + p.c;
+#pragma unroll
+  for (int j = 0; j < W; ++j) store(part + (long)j * A.D, dw[j], p.skip);
+  store(part + (long)W * A.D, dbias, p.skip);
+}
+
+// Partial rows [rows][taps][D] to dw [D][W] and dbias [D], 64 channels a workgroup: 16 runs of rows, joined in order.
+template <typename T>
+__global__ __launch_bounds__(1024) void k_conv_reduce(const float* part, long rows, int D, int W, T* dw, T* dbias) {
+  __shared__ float lds[16][64];
+  const int lane = threadIdx.x & 63, run = threadIdx.x >> 6, c = blockIdx.x * 64 + lane, tap = blockIdx.y;
+  float s = 0.0f;
+  if (c < D)
+#pragma unroll 8
+    for (long r = run; r < rows; r += 16) s += part[(r * (W + 1) + tap) * D + c];
+  lds[run][lane] = s;
+  __syncthreads();
+  if (run != 0 || c >= D) return;
+#pragma unroll
+  for (int r = 1; r < 16; ++r) s += lds[r][lane];
+  if (tap < W) {
+    if (dw) dw[(long)c * W + tap] = from_f32<T>(s);
+  } else if (dbias) {
+    dbias[c] = from_f32<T>(s);
+  }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------
+struct ConvPlan {
+  int tile, tiles, v, vecs;
+  long threads;
+};
+// v: channels of a thread, of 16 bytes an access (backward, whose windows are as many again: of 8 in 16 bits).
+ConvPlan plan_conv(int esize, int B, int L, int D, bool backward) {
+  ConvPlan p{};
+  p.v = esize == 4 || backward ? 4 : 8;
+  if (D < p.v) p.v = 1;
+  p.vecs = (D + p.v - 1) / p.v;
+  p.tile = 64;
+  while (p.tile > 8 && (long)B * ((L + p.tile - 1) / p.tile) * p.vecs < 256L * 256) p.tile /= 2;
+  p.tiles = (L + p.tile - 1) / p.tile;
+  p.threads = (long)B * p.tiles * p.vecs;
+  return p;
+}
+
+int check_conv(int dtype, int B, int L, int D, int W) {
+  if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return kans_fail(KANS_ERR_ARG, "dtype %d", dtype);
+  if (B < 0 || L < 0 || D <= 0) return kans_fail(KANS_ERR_ARG, "bad dims B=%d L=%d D=%d", B, L, D);
+  if (W < 1 || W > kMaxTaps) return kans_fail(KANS_ERR_UNSUPPORTED, "%d taps, 1 to %d", W, kMaxTaps);
+  // (a grid holds fewer than 2^32 threads along x)
+  if (L > (1 << 30) || plan_conv(4, B, L, D, true).threads >= 1L << 31)
+    return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
+  return 0;
+}
+
+template <typename F>
+hipError_t by_conv(int dtype, int W, int v, F f) {
+  hipError_t rc = hipErrorInvalidValue;
+  auto taps = [&](auto t, auto vec) {
+    auto go = [&](auto w) { rc = f(t, w, vec); };
+    switch (W) {
+      case 1: go(std::integral_constant<int, 1>{}); break;
+      case 2: go(std::integral_constant<int, 2>{}); break;
+      case 3: go(std::integral_constant<int, 3>{}); break;
+      case 4: go(std::integral_constant<int, 4>{}); break;
+      case 5: go(std::integral_constant<int, 5>{}); break;
+      case 6: go(std::integral_constant<int, 6>{}); break;
+      case 7: go(std::integral_constant<int, 7>{}); break;
+      case 8: go(std::integral_constant<int, 8>{}); break;
+    }
+  };
+  auto widths = [&](auto t) {
+    if (v == 1) taps(t, std::integral_constant<int, 1>{});
+    else if (v == 4) taps(t, std::integral_constant<int, 4>{});
+    else if constexpr (sizeof(t) == 2) taps(t, std::integral_constant<int, 8>{});
+  };
+  if (dtype == DT_F32) widths(0.0f);
+  else if (dtype == DT_F16) widths((_Float16)0.0f);
+  else widths((__bf16)0.0f);
+  return rc;
+}
+
+}  // namespace
+}  // namespace kans
+
+using namespace kans;
+
+extern "C" {
+
+int kans_causal_conv_forward(int dtype, const void* x, long x_batch, long x_row, const void* w, const void* bias, void* state,
+                             const int64_t* lengths, int silu, void* y, int B, int L, int D, int W, void* stream) {
+  int rc = check_conv(dtype, B, L, D, W);
+  if (rc || B == 0 || L == 0) return rc;
+  if (!x || !w || !y) return kans_fail(KANS_ERR_ARG, "null argument");
+  std::lock_guard<std::mutex> lk(kans_mutex());
+  if ((rc = kans_ensure_init())) return rc;
+  const ConvPlan p = plan_conv(dtype == DT_F32 ? 4 : 2, B, L, D, false);
+  ConvArgs A{};
+  A.x = x; A.w = w; A.bias = bias; A.y = y; A.state = W > 1 ? state : nullptr; A.lengths = lengths; A.silu = silu;
+  A.x_batch = x_batch; A.x_row = x_row; A.B = B; A.L = L; A.D = D; A.tile = p.tile; A.tiles = p.tiles; A.vecs = p.vecs;
+  HIP_TRY(by_conv(dtype, W, p.v, [&](auto t, auto taps, auto vec) {
+    hipLaunchKernelGGL((k_conv_fwd<decltype(t), decltype(taps)::value, decltype(vec)::value>), dim3((unsigned)((p.threads + 255) / 256)),
+                       dim3(256), 0, kans_caller_stream(stream), A);
+    return hipGetLastError();
+  }));
+  return 0;
+}
+
+long kans_causal_conv_workspace(int dtype, int B, int L, int D, int W) {
+  const int rc = check_conv(dtype, B, L, D, W);
+  if (rc) return rc;
+  const ConvPlan p = plan_conv(dtype == DT_F32 ? 4 : 2, B, L, D, true);
+  return (long)B * p.tiles * (W + 1) * D * (long)sizeof(float);
+}
+
+int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row, const void* w, const void* bias,
+                              const int64_t* lengths, int silu, const void* dy, void* dx, void* dw, void* dbias, int B, int L, int D,
+                              int W, void* workspace, long workspace_bytes, void* stream) {
+  int rc = check_conv(dtype, B, L, D, W);
+  if (rc) return rc;
+  const bool any = B > 0 && L > 0;
+  if (any && (!x || !w || !dy)) return kans_fail(KANS_ERR_ARG, "null argument");
+  if (dbias && !bias) return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
+  const ConvPlan p = plan_conv(dtype == DT_F32 ? 4 : 2, B, L, D, true);
+  const long rows = (long)B * p.tiles, need = rows * (W + 1) * D * (long)sizeof(float);
+  const bool sums = dw || dbias;
+  if (sums && need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
+    return kans_fail(KANS_ERR_ARG, "workspace of %ld bytes, %ld at a multiple of 16 needed", workspace ? workspace_bytes : 0, need);
+  std::lock_guard<std::mutex> lk(kans_mutex());
+  if ((rc = kans_ensure_init())) return rc;
+  hipStream_t st = kans_caller_stream(stream);
+  if (any) {
+    ConvArgs A{};
+    A.x = x; A.w = w; A.bias = bias; A.dy = dy; A.dx = dx; A.lengths = lengths; A.silu = silu;
+    A.part = sums ? (float*)workspace : nullptr;
+    A.x_batch = x_batch; A.x_row = x_row; A.B = B; A.L = L; A.D = D; A.tile = p.tile; A.tiles = p.tiles; A.vecs = p.vecs;
+    HIP_TRY(by_conv(dtype, W, p.v, [&](auto t, auto taps, auto vec) {
+      if constexpr (decltype(vec)::value <= 4)
+        hipLaunchKernelGGL((k_conv_bwd<decltype(t), decltype(taps)::value, decltype(vec)::value>), dim3((unsigned)((p.threads + 255) / 256)),
+                           dim3(256), 0, st, A);
+      return hipGetLastError();
+    }));
+  }
+  if (!sums) return 0;
+  const dim3 grid((D + 63) / 64, W + 1);
+  auto reduce = [&](auto t) {
+    typedef decltype(t) T;
+    hipLaunchKernelGGL(k_conv_reduce<T>, grid, dim3(1024), 0, st, (const float*)workspace, any ? rows : 0, D, W, (T*)dw, (T*)dbias);
+  };
+  if (dtype == DT_F32) reduce(0.0f);
+  else if (dtype == DT_F16) reduce((_Float16)0.0f);
+  else reduce((__bf16)0.0f);
+  HIP_TRY(hipGetLastError());
+  return 0;
+}
+
+}  // extern "C"

@@ -1,0 +1,211 @@
+// Selective state space scan: entry points, and what joins a sequence's chunks (gfx950).  The kernels are in kans_scan_kernel.h.
+//
+//   s[t] = softplus(dt[t] + bias),  h[t] = exp(s[t] A) h[t-1] + s[t] x[t] B[t],  y[t] = C[t] . h[t] + skip x[t],  out = y z sigmoid(z)
+//
+// for each channel, with a state h of N numbers; B and C are shared by a sequence's channels.  Backward, with dy = dout z sigmoid(z):
+//   g[t] = C[t] dy[t] + exp(s[t+1] A) g[t+1]                       (the gradient of h[t])
+//   dC[t] = sum dy h[t],  dB[t] = sum g[t] s x                     (over the channels)
+//   k[t] = g[t] exp(s[t] A) h[t-1]
+//   dx = s (g . B) + skip dy,  ds = x (g . B) + k . A,  dA = sum k s,  dskip = sum dy x,  ddt = ds softplus'(dt + bias)
+//
+// All of it in fp32; h does not leave the registers but for every 16th step (8th or 4th for many states), where the forward of a
+// training step keeps it: the backward runs through the 16 steps again and then back.
+//
+// The exponential of every state bounds it (16 cycles of a SIMD for 64 of them, the other products and sums 16 more),
+// not memory.  So four lanes share a channel: a quarter of the sequence's channels is a wave, with the sums over the
+// states two permutes and sums a step, and B and C from LDS for 64 channels at once.  A batch of B sequences and D
+// channels has B D / 16 waves.  Where those are too few for the card the sequence is cut in chunks: a first pass runs each from a
+// state of zeros for its last state (the decay over a chunk is exp(A sum s)), k_scan_join adds these up to the state
+// before each chunk, and the scan runs the chunks beside each other.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kans_scan.h"
+
+namespace kans {
+namespace {
+
+// Per chunk in order (backward: from the last), edge becomes what comes into it: H, then H exp(A sum s) + edge.
+__global__ __launch_bounds__(256) void k_scan_join(const ScanArgs A, bool backward) {
+  const long at = (long)blockIdx.x * 256 + threadIdx.x, states = (long)A.D * A.N;
+  if (at >= A.B * states) return;
+  const long b = at / states, in = at - b * states, d = in / A.N;
+  const float a2 = A.A[in] * 1.44269504088896340736f;
+  float h = !backward && A.state ? A.state[at] : 0.0f;
+  for (int i = 0; i < A.chunks; ++i) {
+    const long place = b * A.chunks + (backward ? A.chunks - 1 - i : i);
+    const float e = A.edge[place * states + in], s = A.sums[place * A.D + d];
+    A.edge[place * states + in] = h;
+    h = __builtin_amdgcn_exp2f(a2 * s) * h + e;
+  }
+}
+
+// Sums of the parameters' partial rows, [rows][D][N + 2].
+__global__ __launch_bounds__(256) void k_scan_params(const float* part, long rows, int D, int N, float* dA, float* dskip, float* dbias) {
+  const long at = (long)blockIdx.x * 256 + threadIdx.x, all = (long)D * (N + 2);
+  if (at >= all) return;
+  float s = 0.0f;
+#pragma unroll 4
+  for (long r = 0; r < rows; ++r) s += part[r * all + at];
+  const long d = at / (N + 2);
+  const int n = (int)(at - d * (N + 2));
+  if (n < N) {
+    if (dA) dA[d * N + n] = s;
+  } else if (n == N) {
+    if (dskip) dskip[d] = s;
+  } else if (dbias) {
+    dbias[d] = s;
+  }
+}
+
+hipError_t launch(int dtype, ScanPass pass, const ScanArgs& A, hipStream_t st) {
+  return dtype == DT_F32 ? scan_launch_f32(pass, A, st) : dtype == DT_F16 ? scan_launch_f16(pass, A, st) : scan_launch_bf16(pass, A, st);
+}
+
+constexpr int kMaxStates = 64, kMinChunk = 64;
+constexpr long kEnoughWaves = 1024, kWantedWaves = 2048;
+
+struct ScanPlan {
+  int blocks, chunk, chunks, interval, padded;
+  long edges;                        // floats of the chunks' edges and sums
+  long part_bc, part_par, saved;     // floats
+};
+ScanPlan plan_scan(int B, int L, int D, int N) {
+  ScanPlan p{};
+  const int regs = scan_regs(N);
+  p.interval = scan_interval(regs);
+  p.padded = 4 * regs;
+  p.blocks = (D + kScanChannels - 1) / kScanChannels;
+  const long waves = 4L * p.blocks * std::max(B, 1);
+  p.chunk = std::max(L, 1);
+  if (waves < kEnoughWaves && L >= 2 * kMinChunk) {
+    const long want = std::min((kWantedWaves + waves - 1) / waves, (long)L / kMinChunk);
+    p.chunk = (int)(((L + want - 1) / want + 15) & ~15L);
+  }
+  p.chunks = std::max(1, (L + p.chunk - 1) / p.chunk);
+  p.edges = p.chunks > 1 ? (long)B * p.chunks * D * (N + 1) : 0;
+  p.edges = (p.edges + 3) & ~3L;
+  p.part_bc = (long)p.blocks * B * L * 2 * p.padded;
+  p.part_par = (long)B * p.chunks * D * (N + 2);
+  p.saved = (long)B * ((L + p.interval - 1) / p.interval) * D * N;
+  return p;
+}
+
+int check_scan(int dtype, int B, int L, int D, int N) {
+  if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return kans_fail(KANS_ERR_ARG, "dtype %d", dtype);
+  if (B < 0 || L < 0 || D <= 0 || N <= 0) return kans_fail(KANS_ERR_ARG, "bad dims B=%d L=%d D=%d N=%d", B, L, D, N);
+  if (N > kMaxStates) return kans_fail(KANS_ERR_UNSUPPORTED, "%d states, up to %d", N, kMaxStates);
+  // (a grid holds fewer than 2^32 threads along x, a channel four)
+  const long blocks = ((long)D + kScanChannels - 1) / kScanChannels;
+  if (L > (1 << 30) || (long)B * blocks >= 1L << 22 || (long)B * L * 2 * kMaxStates >= 1L << 38)
+    return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
+  return 0;
+}
+
+int check_workspace(const void* workspace, long bytes, long need) {
+  if (need && (!workspace || (uintptr_t)workspace % 16 || bytes < need))
+    return kans_fail(KANS_ERR_ARG, "workspace of %ld bytes, %ld at a multiple of 16 needed", workspace ? bytes : 0, need);
+  return 0;
+}
+
+}  // namespace
+}  // namespace kans
+
+using namespace kans;
+
+extern "C" {
+
+long kans_selective_scan_saved(int B, int L, int D, int N) {
+  const int rc = check_scan(DT_F32, B, L, D, N);
+  return rc ? rc : plan_scan(B, L, D, N).saved * (long)sizeof(float);
+}
+
+long kans_selective_scan_workspace(int B, int L, int D, int N, int backward) {
+  const int rc = check_scan(DT_F32, B, L, D, N);
+  if (rc) return rc;
+  const ScanPlan p = plan_scan(B, L, D, N);
+  return (p.edges + (backward ? p.part_bc + p.part_par : 0)) * (long)sizeof(float);
+}
+
+int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_row, const void* dt, long dt_batch, long dt_row,
+                                const float* A, const void* Bm, long b_batch, long b_row, const void* Cm, long c_batch, long c_row,
+                                const float* skip, const void* z, long z_batch, long z_row, const float* dt_bias, int softplus,
+                                float* state, const int64_t* lengths, void* out, float* saved, int B, int L, int D, int N,
+                                void* workspace, long workspace_bytes, void* stream) {
+  int rc = check_scan(dtype, B, L, D, N);
+  if (rc || B == 0 || L == 0) return rc;
+  if (!x || !dt || !A || !Bm || !Cm || !out) return kans_fail(KANS_ERR_ARG, "null argument");
+  if ((uintptr_t)state % 16 || (uintptr_t)A % 16) return kans_fail(KANS_ERR_ARG, "A and the state start at multiples of 16 bytes");
+  const ScanPlan p = plan_scan(B, L, D, N);
+  if ((rc = check_workspace(workspace, workspace_bytes, p.edges * (long)sizeof(float)))) return rc;
+  std::lock_guard<std::mutex> lk(kans_mutex());
+  if ((rc = kans_ensure_init())) return rc;
+  hipStream_t st = kans_caller_stream(stream);
+  ScanArgs S{};
+  S.x = x; S.dt = dt; S.Bm = Bm; S.Cm = Cm; S.z = z; S.A = A; S.skip = skip; S.bias = dt_bias;
+  S.x_batch = x_batch; S.x_row = x_row; S.dt_batch = dt_batch; S.dt_row = dt_row; S.b_batch = b_batch; S.b_row = b_row;
+  S.c_batch = c_batch; S.c_row = c_row; S.z_batch = z_batch; S.z_row = z_row;
+  S.state = state; S.lengths = lengths; S.out = out; S.saved = saved;
+  S.B = B; S.L = L; S.D = D; S.N = N; S.softplus = softplus; S.chunk = p.chunk; S.chunks = p.chunks;
+  if (L == 1 && state && !saved) {
+    HIP_TRY(launch(dtype, ScanPass::kStep, S, st));
+    return 0;
+  }
+  if (p.chunks > 1) {
+    S.edge = (float*)workspace;
+    S.sums = S.edge + (long)B * p.chunks * D * N;
+    HIP_TRY(launch(dtype, ScanPass::kEdges, S, st));
+    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, false);
+    HIP_TRY(hipGetLastError());
+  }
+  HIP_TRY(launch(dtype, ScanPass::kForward, S, st));
+  return 0;
+}
+
+int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_row, const void* dt, long dt_batch, long dt_row,
+                                 const float* A, const void* Bm, long b_batch, long b_row, const void* Cm, long c_batch, long c_row,
+                                 const float* skip, const void* z, long z_batch, long z_row, const float* dt_bias, int softplus,
+                                 const int64_t* lengths, const float* saved, const void* dout, void* dx, void* ddt, float* dA, void* dB,
+                                 void* dC, float* dskip, void* dz, float* ddt_bias, int B, int L, int D, int N, void* workspace,
+                                 long workspace_bytes, void* stream) {
+  int rc = check_scan(dtype, B, L, D, N);
+  if (rc) return rc;
+  const bool any = B > 0 && L > 0;
+  if (any && (!x || !dt || !A || !Bm || !Cm || !saved || !dout || !dx || !ddt || (z && !dz))) return kans_fail(KANS_ERR_ARG, "null argument");
+  if ((dskip && !skip) || (dz && !z) || (ddt_bias && !dt_bias)) return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
+  const ScanPlan p = plan_scan(B, L, D, N);
+  if ((rc = check_workspace(workspace, workspace_bytes, (p.edges + p.part_bc + p.part_par) * (long)sizeof(float)))) return rc;
+  std::lock_guard<std::mutex> lk(kans_mutex());
+  if ((rc = kans_ensure_init())) return rc;
+  hipStream_t st = kans_caller_stream(stream);
+  ScanArgs S{};
+  S.x = x; S.dt = dt; S.Bm = Bm; S.Cm = Cm; S.z = z; S.A = A; S.skip = skip; S.bias = dt_bias; S.dout = dout;
+  S.x_batch = x_batch; S.x_row = x_row; S.dt_batch = dt_batch; S.dt_row = dt_row; S.b_batch = b_batch; S.b_row = b_row;
+  S.c_batch = c_batch; S.c_row = c_row; S.z_batch = z_batch; S.z_row = z_row;
+  S.lengths = lengths; S.saved = (float*)saved; S.dx = dx; S.ddt = ddt; S.dz = dz;
+  S.B = B; S.L = L; S.D = D; S.N = N; S.softplus = softplus; S.chunk = p.chunk; S.chunks = p.chunks;
+  S.edge = (float*)workspace;
+  S.sums = S.edge + (long)B * p.chunks * D * N;
+  S.part_bc = (float*)workspace + p.edges;
+  S.part_par = S.part_bc + p.part_bc;
+  if (any) {
+    if (p.chunks > 1) {
+      HIP_TRY(launch(dtype, ScanPass::kBackwardEdges, S, st));
+      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, true);
+      HIP_TRY(hipGetLastError());
+    }
+    HIP_TRY(launch(dtype, ScanPass::kBackward, S, st));
+    if (dB || dC)
+      HIP_TRY(dtype == DT_F32 ? scan_reduce_f32(S, p.padded, dB, dC, st) : dtype == DT_F16 ? scan_reduce_f16(S, p.padded, dB, dC, st)
+                                                                                           : scan_reduce_bf16(S, p.padded, dB, dC, st));
+  }
+  if (dA || dskip || ddt_bias) {
+    hipLaunchKernelGGL(k_scan_params, dim3((unsigned)(((long)D * (N + 2) + 255) / 256)), dim3(256), 0, st, S.part_par,
+                       any ? (long)B * p.chunks : 0L, D, N, dA, dskip, ddt_bias);
+    HIP_TRY(hipGetLastError());
+  }
+  return 0;
+}
+
+}  // extern "C"

@@ -49,6 +49,13 @@ struct Library {
   decltype(&kans_embedding_workspace) embedding_workspace;
   decltype(&kans_embedding_backward) embedding_backward;
   decltype(&kans_dropout) dropout;
+  decltype(&kans_causal_conv_forward) conv_forward;
+  decltype(&kans_causal_conv_workspace) conv_workspace;
+  decltype(&kans_causal_conv_backward) conv_backward;
+  decltype(&kans_selective_scan_saved) scan_saved;
+  decltype(&kans_selective_scan_workspace) scan_workspace;
+  decltype(&kans_selective_scan_forward) scan_forward;
+  decltype(&kans_selective_scan_backward) scan_backward;
 } lib;
 PyObject* kans_error;  // the package's exception for a negative code
 
@@ -77,6 +84,13 @@ void bind(const py::dict& functions, py::object error) {
   get("kans_embedding_workspace", lib.embedding_workspace);
   get("kans_embedding_backward", lib.embedding_backward);
   get("kans_dropout", lib.dropout);
+  get("kans_causal_conv_forward", lib.conv_forward);
+  get("kans_causal_conv_workspace", lib.conv_workspace);
+  get("kans_causal_conv_backward", lib.conv_backward);
+  get("kans_selective_scan_saved", lib.scan_saved);
+  get("kans_selective_scan_workspace", lib.scan_workspace);
+  get("kans_selective_scan_forward", lib.scan_forward);
+  get("kans_selective_scan_backward", lib.scan_backward);
   kans_error = error.release().ptr();
 }
 
@@ -498,6 +512,222 @@ std::optional<Tensor> dropout(const Tensor& x, double p, int64_t seed, const std
   return DropoutFunction::apply(in, p, seed, dev, offset)[0];
 }
 
+// ---- causal_conv -----------------------------------------------------------------------------------
+// A [B, L, C] tensor whose channels lie side by side, as it is where it can be read so.
+Tensor with_channels(const Tensor& t) { return t.size(2) == 1 || t.stride(2) == 1 ? t : t.contiguous(); }
+std::optional<Tensor> maybe(const Tensor& t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+Tensor given(const std::optional<Tensor>& t) { return t ? *t : Tensor(); }
+
+// lengths and a state beside a [B, L, C] tensor
+bool fits_lengths(const std::optional<Tensor>& lengths, const Tensor& x) {
+  return !lengths || (lengths->dim() == 1 && lengths->size(0) == x.size(0) && lengths->scalar_type() == at::kLong &&
+                      lengths->device() == x.device());
+}
+bool sizes_fit_int(const Tensor& x) { return x.size(0) <= INT_MAX && x.size(1) <= INT_MAX && x.size(2) <= INT_MAX; }
+
+struct Conv {
+  Tensor x, w, bias, lengths;  // (undefined: not given)
+  bool silu;
+
+  int B() const { return (int)x.size(0); }
+  int L() const { return (int)x.size(1); }
+  int D() const { return (int)x.size(2); }
+  int W() const { return (int)w.size(1); }
+  int type() const { return type_of(x.scalar_type()); }
+
+  Tensor forward(const Tensor& state) const {
+    Tensor y = at::empty(x.sizes(), x.options());
+    check(lib.conv_forward(type(), data(x), x.stride(0), x.stride(1), data(w), data(bias), data(state), (const int64_t*)data(lengths),
+                           silu, data(y), B(), L(), D(), W(), stream_of(x)),
+          "kans_causal_conv_forward");
+    return y;
+  }
+
+  variable_list backward(const Tensor& dy, const std::array<bool, 3>& need) const {
+    Tensor dx = need[0] ? at::empty(x.sizes(), x.options()) : Tensor(), dw = need[1] ? at::empty_like(w) : Tensor(),
+           dbias = need[2] ? at::empty_like(bias) : Tensor();
+    const long size = lib.conv_workspace(type(), B(), L(), D(), W());
+    check(size, "kans_causal_conv_workspace");
+    const Tensor ws = need[1] || need[2] ? bytes(x, size) : Tensor();
+    check(lib.conv_backward(type(), data(x), x.stride(0), x.stride(1), data(w), data(bias), (const int64_t*)data(lengths), silu, data(dy),
+                            data(dx), data(dw), data(dbias), B(), L(), D(), W(), data(ws), size, stream_of(x)),
+          "kans_causal_conv_backward");
+    return {dx, dw, dbias};
+  }
+};
+
+struct ConvFunction : torch::autograd::Function<ConvFunction> {
+  typedef std::optional<Tensor> Maybe;
+  static variable_list forward(AutogradContext* ctx, Tensor x, Tensor w, Maybe bias, Maybe lengths, bool silu) {
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, w, given(bias), given(lengths)});
+    ctx->saved_data["silu"] = silu;
+    return {Conv{x, w, given(bias), given(lengths), silu}.forward(Tensor())};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    variable_list d(5);
+    if (!grads[0].defined()) return d;
+    no_tangents({&grads[0]}, "causal_conv's backward");
+    const auto s = ctx->get_saved_variables();
+    const at::OptionalDeviceGuard device(s[0].device());
+    const Conv c{s[0], s[1], s[2], s[3], ctx->saved_data["silu"].toBool()};
+    std::array<bool, 3> need;
+    for (size_t i = 0, edge = 0; i < 3; ++i) need[i] = s[i].defined() && ctx->needs_input_grad(edge++);
+    const variable_list three = once(c.backward(grads[0].contiguous(), need), graph);
+    std::copy(three.begin(), three.end(), d.begin());
+    return d;
+  }
+};
+
+// None where the arguments do not fit together (the caller says why).
+std::optional<Tensor> causal_conv(const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, int silu,
+                                  const std::optional<Tensor>& state, const std::optional<Tensor>& lengths) {
+  not_traced("causal_conv");
+  const at::ScalarType dt = x.scalar_type();
+  auto fits = [&](const Tensor& t) { return t.scalar_type() == dt && t.device() == x.device(); };
+  if (silu < 0 || x.dim() != 3 || type_of(dt) < 0 || !x.is_cuda() || x.size(2) == 0 || w.dim() != 2 || w.size(0) != x.size(2) ||
+      w.size(1) < 1 || w.size(1) > 8 || !fits(w) || !fits_lengths(lengths, x))
+    return {};
+  if (bias && (!fits(*bias) || bias->dim() != 1 || bias->size(0) != x.size(2))) return {};
+  if (state && (!fits(*state) || !state->is_contiguous() || state->dim() != 3 || state->size(0) != x.size(0) ||
+                state->size(1) != w.size(1) - 1 || state->size(2) != x.size(2)))
+    return {};
+  TORCH_CHECK_VALUE(sizes_fit_int(x), "x has a size of more than 2^31");
+  const Conv c{with_channels(x), w.contiguous(), contiguous(bias), contiguous(lengths), silu != 0};
+  no_tangents({&c.x, &c.w, &c.bias}, "causal_conv");
+  const at::OptionalDeviceGuard device(x.device());
+  if (wants_grad({&c.x, &c.w, &c.bias})) {
+    TORCH_CHECK(!state, "causal_conv with a state has no gradients: call it under torch.no_grad()");
+    capturable({&c.x, &c.w, &c.bias}, "causal_conv");
+    return ConvFunction::apply(c.x, c.w, maybe(c.bias), maybe(c.lengths), c.silu)[0];
+  }
+  TORCH_CHECK(!state || !(at::GradMode::is_enabled() && state->requires_grad()),
+              "causal_conv with a state has no gradients: call it under torch.no_grad()");
+  const Tensor y = c.forward(given(state));
+  if (state && !state->is_inference()) state->unsafeGetTensorImpl()->bump_version();
+  return y;
+}
+
+// ---- selective_scan --------------------------------------------------------------------------------
+struct Scan {
+  Tensor x, dt, A, B, C, skip, z, bias, lengths;  // (undefined: not given)
+  bool softplus;
+
+  int b() const { return (int)x.size(0); }
+  int l() const { return (int)x.size(1); }
+  int d() const { return (int)x.size(2); }
+  int n() const { return (int)A.size(1); }
+  int type() const { return type_of(x.scalar_type()); }
+  static long stride(const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; }
+  Tensor workspace(int backward) const {
+    const long size = lib.scan_workspace(b(), l(), d(), n(), backward);
+    check(size, "kans_selective_scan_workspace");
+    return bytes(x, size);
+  }
+
+  std::tuple<Tensor, Tensor> forward(const Tensor& state, bool save) const {
+    Tensor out = at::empty(x.sizes(), x.options()), saved;
+    if (save) {
+      const long size = lib.scan_saved(b(), l(), d(), n());
+      check(size, "kans_selective_scan_saved");
+      saved = at::empty({size / 4}, x.options().dtype(at::kFloat));
+    }
+    const Tensor ws = workspace(0);
+    check(lib.scan_forward(type(), data(x), x.stride(0), x.stride(1), data(dt), dt.stride(0), dt.stride(1), (const float*)data(A), data(B),
+                           B.stride(0), B.stride(1), data(C), C.stride(0), C.stride(1), (const float*)data(skip), data(z), stride(z, 0),
+                           stride(z, 1), (const float*)data(bias), softplus, (float*)data(state), (const int64_t*)data(lengths), data(out),
+                           (float*)data(saved), b(), l(), d(), n(), data(ws), ws.numel(), stream_of(x)),
+          "kans_selective_scan_forward");
+    return {out, saved};
+  }
+
+  // Gradients of the eight inputs, undefined where need is false.
+  variable_list backward(const Tensor& saved, const Tensor& dout, const std::array<bool, 8>& need) const {
+    auto like = [&](const Tensor& t, bool on) { return on ? at::empty(t.sizes(), t.options()) : Tensor(); };
+    // (the kernel writes dx, ddt and dz in any case)
+    Tensor dx = like(x, true), ddt = like(dt, true), dA = like(A, need[2]), dB = like(B, need[3]), dC = like(C, need[4]),
+           dskip = like(skip, need[5]), dz = like(z, z.defined()), dbias = like(bias, need[7]);
+    const Tensor ws = workspace(1);
+    check(lib.scan_backward(type(), data(x), x.stride(0), x.stride(1), data(dt), dt.stride(0), dt.stride(1), (const float*)data(A), data(B),
+                            B.stride(0), B.stride(1), data(C), C.stride(0), C.stride(1), (const float*)data(skip), data(z), stride(z, 0),
+                            stride(z, 1), (const float*)data(bias), softplus, (const int64_t*)data(lengths), (const float*)data(saved),
+                            data(dout), data(dx), data(ddt), (float*)data(dA), data(dB), data(dC), (float*)data(dskip), data(dz),
+                            (float*)data(dbias), b(), l(), d(), n(), data(ws), ws.numel(), stream_of(x)),
+          "kans_selective_scan_backward");
+    return {need[0] ? dx : Tensor(), need[1] ? ddt : Tensor(), dA, dB, dC, dskip, need[6] ? dz : Tensor(), dbias};
+  }
+};
+
+struct ScanFunction : torch::autograd::Function<ScanFunction> {
+  typedef std::optional<Tensor> Maybe;
+  static variable_list forward(AutogradContext* ctx, Tensor x, Tensor dt, Tensor A, Tensor B, Tensor C, Maybe skip, Maybe z, Maybe bias,
+                               Maybe lengths, bool softplus) {
+    const Scan s{x, dt, A, B, C, given(skip), given(z), given(bias), given(lengths), softplus};
+    auto [out, saved] = s.forward(Tensor(), true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, dt, A, B, C, s.skip, s.z, s.bias, s.lengths, saved});
+    ctx->saved_data["softplus"] = softplus;
+    return {out};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const bool graph = at::GradMode::is_enabled();
+    at::NoGradGuard no_grad;
+    variable_list d(10);
+    if (!grads[0].defined()) return d;
+    no_tangents({&grads[0]}, "selective_scan's backward");
+    const auto s = ctx->get_saved_variables();
+    const at::OptionalDeviceGuard device(s[0].device());
+    const Scan scan{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], ctx->saved_data["softplus"].toBool()};
+    std::array<bool, 8> need;
+    for (size_t i = 0, edge = 0; i < 8; ++i) need[i] = s[i].defined() && ctx->needs_input_grad(edge++);
+    const variable_list eight = once(scan.backward(s[9], grads[0].contiguous(), need), graph);
+    std::copy(eight.begin(), eight.end(), d.begin());
+    return d;
+  }
+};
+
+// None where the arguments do not fit together (the caller says why).
+std::optional<Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C,
+                                     const std::optional<Tensor>& skip, const std::optional<Tensor>& z, const std::optional<Tensor>& bias,
+                                     bool softplus, const std::optional<Tensor>& state, const std::optional<Tensor>& lengths) {
+  not_traced("selective_scan");
+  auto of_type = [&](const Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.device() == x.device(); };
+  auto channel = [&](const std::optional<Tensor>& t) {
+    return !t || (of_type(*t, at::kFloat) && t->dim() == 1 && t->size(0) == x.size(2));
+  };
+  if (x.dim() != 3 || type_of(x.scalar_type()) < 0 || !x.is_cuda() || x.size(2) == 0) return {};
+  if (!of_type(A, at::kFloat) || A.dim() != 2 || A.size(0) != x.size(2) || A.size(1) < 1 || A.size(1) > 64) return {};
+  auto wide = [&](const Tensor& t, int64_t channels) {
+    return of_type(t, x.scalar_type()) && t.dim() == 3 && t.size(0) == x.size(0) && t.size(1) == x.size(1) && t.size(2) == channels;
+  };
+  if (!wide(dt, x.size(2)) || (z && !wide(*z, x.size(2))) || !wide(B, A.size(1)) || !wide(C, A.size(1)) || !channel(skip) ||
+      !channel(bias) || !fits_lengths(lengths, x))
+    return {};
+  if (state && (!of_type(*state, at::kFloat) || !state->is_contiguous() || state->dim() != 3 || state->size(0) != x.size(0) ||
+                state->size(1) != x.size(2) || state->size(2) != A.size(1) || (uintptr_t)state->data_ptr() % 16))
+    return {};
+  TORCH_CHECK_VALUE(sizes_fit_int(x), "x has a size of more than 2^31");
+  Scan s{with_channels(x), with_channels(dt), A.contiguous(), with_channels(B), with_channels(C), contiguous(skip),
+         z ? with_channels(*z) : Tensor(), contiguous(bias), contiguous(lengths), softplus};
+  if ((uintptr_t)s.A.data_ptr() % 16) s.A = s.A.clone();
+  no_tangents({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias}, "selective_scan");
+  const at::OptionalDeviceGuard device(x.device());
+  if (wants_grad({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias})) {
+    TORCH_CHECK(!state, "selective_scan with a state has no gradients: call it under torch.no_grad()");
+    capturable({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias}, "selective_scan");
+    return ScanFunction::apply(s.x, s.dt, s.A, s.B, s.C, maybe(s.skip), maybe(s.z), maybe(s.bias), maybe(s.lengths), softplus)[0];
+  }
+  TORCH_CHECK(!state || !(at::GradMode::is_enabled() && state->requires_grad()),
+              "selective_scan with a state has no gradients: call it under torch.no_grad()");
+  const Tensor out = std::get<0>(s.forward(given(state), false));
+  if (state && !state->is_inference()) state->unsafeGetTensorImpl()->bump_version();
+  return out;
+}
+
 // ---- TorchAdamW ------------------------------------------------------------------------------------
 // An arena's buffers (_Arena.flat), and what a parameter's state holds when it is the arena's own: views of them at the
 // parameter's place, in its order of memory.
@@ -699,4 +929,6 @@ PYBIND11_MODULE(_kans_torch, m) {
   m.def("linear_cross_entropy", &linear_cross_entropy, py::call_guard<py::gil_scoped_release>());
   m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
   m.def("dropout", &dropout, py::call_guard<py::gil_scoped_release>());
+  m.def("causal_conv", &causal_conv, py::call_guard<py::gil_scoped_release>());
+  m.def("selective_scan", &selective_scan, py::call_guard<py::gil_scoped_release>());
 }

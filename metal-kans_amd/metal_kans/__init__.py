@@ -3,8 +3,9 @@
 Drop-in for the hot-path surface of Shuril/metal-kans (metal_kans/__init__.py:6-40):
 Chebyshev / Gaussian-RBF / cubic B-spline layers, the multi-layer container, the
 GatedKAN block, INT8 / INT4 / ternary weight quantization, the Chebyshev layer
-backward and the torch modules.  Around them, on torch tensors, the rest of a training
-step: ``residual_norm``, ``linear_cross_entropy`` and ``TorchAdamW``.  The reference's NumPy
+backward and the torch modules.  Around them, on torch tensors, the rest of a token model and
+its training step: ``embedding``, ``dropout``, ``residual_norm``, ``causal_conv``, ``selective_scan``,
+``linear_cross_entropy`` and ``TorchAdamW``.  The reference's NumPy
 optimizers, pruning, symbolic export and the other KAN families are outside this build's scope.
 """
 from .device import get_metal_bridge, is_gpu_available, is_metal_available, set_async, sync
@@ -21,7 +22,8 @@ __version__ = "0.6.0+mi355x"
 # What works on torch tensors and the module it is in: imported on first use so that `import metal_kans` does
 # not import torch; None without torch, as in the reference (metal_kans/__init__.py:34-38).
 _TORCH = {"TorchMetalKANLinear": "torch_module", "TorchMetalKAN": "torch_module", "TorchAdamW": "adamw",
-          "residual_norm": "residual", "linear_cross_entropy": "cross_entropy", "embedding": "embeddings", "dropout": "dropouts"}
+          "residual_norm": "residual", "linear_cross_entropy": "cross_entropy", "embedding": "embeddings", "dropout": "dropouts",
+          "causal_conv": "sequence", "selective_scan": "sequence"}
 
 
 def __getattr__(name):
@@ -41,4 +43,5 @@ __all__ = [
     "ChebyKAN", "FastKAN", "BSplineKAN", "KAN", "MetalKAN", "GatedKAN",
     "QuantizedWeight", "TernaryQuantizedWeight", "quantize", "to_int8", "to_int4", "to_ternary",
     "TorchMetalKANLinear", "TorchMetalKAN", "TorchAdamW", "residual_norm", "linear_cross_entropy", "embedding", "dropout",
+    "causal_conv", "selective_scan",
 ]

@@ -10,7 +10,9 @@ from . import device
 _FUNCTIONS = ("kans_last_error", "kans_stream_keep", "kans_residual_norm_forward", "kans_residual_norm_workspace",
               "kans_residual_norm_backward", "kans_linear_xent_workspace", "kans_linear_xent_forward",
               "kans_linear_xent_backward", "kans_adamw_step", "kans_embedding_forward", "kans_embedding_workspace",
-              "kans_embedding_backward", "kans_dropout")
+              "kans_embedding_backward", "kans_dropout", "kans_causal_conv_forward", "kans_causal_conv_workspace",
+              "kans_causal_conv_backward", "kans_selective_scan_saved", "kans_selective_scan_workspace",
+              "kans_selective_scan_forward", "kans_selective_scan_backward")
 _module = None
 
 

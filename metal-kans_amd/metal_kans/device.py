@@ -149,6 +149,17 @@ SIGNATURES = {
     "kans_embedding_workspace": (c_long, [c_int, c_long, c_int, c_int]),
     "kans_embedding_backward": (c_int, [c_int, P, P, c_long, c_int, c_int, c_longlong, c_double, P, P, c_long, P]),
     "kans_dropout": (c_int, [c_int, P, P, c_long, c_double, c_longlong, P, P, c_longlong, P]),
+    "kans_causal_conv_forward": (c_int, [c_int, P, c_long, c_long, P, P, P, P, c_int, P, c_int, c_int, c_int, c_int, P]),
+    "kans_causal_conv_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int]),
+    "kans_causal_conv_backward": (c_int, [c_int, P, c_long, c_long, P, P, P, c_int, P, P, P, P, c_int, c_int, c_int, c_int, P, c_long,
+                                          P]),
+    "kans_selective_scan_saved": (c_long, [c_int, c_int, c_int, c_int]),
+    "kans_selective_scan_workspace": (c_long, [c_int, c_int, c_int, c_int, c_int]),
+    "kans_selective_scan_forward": (c_int, [c_int, P, c_long, c_long, P, c_long, c_long, P, P, c_long, c_long, P, c_long, c_long, P, P,
+                                            c_long, c_long, P, c_int, P, P, P, P, c_int, c_int, c_int, c_int, P, c_long, P]),
+    "kans_selective_scan_backward": (c_int, [c_int, P, c_long, c_long, P, c_long, c_long, P, P, c_long, c_long, P, c_long, c_long, P, P,
+                                             c_long, c_long, P, c_int, P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, P,
+                                             c_long, P]),
     "kans_mfma_ceiling": (c_int, [c_int, P, P, c_int, P]),
     "kans_stream_ceiling": (c_int, [P, c_size_t, P]),
 }

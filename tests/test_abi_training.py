@@ -125,3 +125,43 @@ def test_dropout_refusals(lib):
     for bad in (dict(dt=3), dict(x=None), dict(y=None), dict(n=-1), dict(p=-0.1), dict(p=1.1), dict(p=float("nan"))):
         assert go(**bad) == -1, bad
     assert go(n=1 << 34) == -5
+
+
+def test_causal_conv_refusals(lib):
+    def fwd(dt=0, x=64, w=64, y=64, b=2, n=5, d=4, taps=3):
+        return lib.kans_causal_conv_forward(dt, x, 20, 4, w, None, None, None, 1, y, b, n, d, taps, None)
+
+    def bwd(x=64, dy=64, bias=None, dbias=None, ws=64, size=1 << 20):
+        return lib.kans_causal_conv_backward(0, x, 20, 4, 64, bias, None, 1, dy, 64, 64, dbias, 2, 5, 4, 3, ws, size, None)
+    for bad in (dict(dt=3), dict(x=None), dict(w=None), dict(y=None), dict(b=-1), dict(n=-1), dict(d=0)):
+        assert fwd(**bad) == -1, bad
+    for bad in (dict(taps=0), dict(taps=9), dict(b=1 << 15, n=1 << 25), dict(n=(1 << 30) + 1)):
+        assert fwd(**bad) == -5, bad
+    assert fwd(b=0, x=None) == 0 and fwd(n=0, x=None) == 0
+    for bad in (dict(x=None), dict(dy=None), dict(dbias=64), dict(ws=None), dict(ws=72), dict(size=16)):
+        assert bwd(**bad) == -1, bad
+    assert lib.kans_causal_conv_workspace(0, 2, 5, 4, 9) == -5
+    assert lib.kans_causal_conv_workspace(0, 2, 5, 4, 3) >= 2 * 4 * 4 * 4
+
+
+def test_selective_scan_refusals(lib):
+    def fwd(dt=0, x=64, A=64, bm=64, out=64, state=None, b=2, n=5, d=4, states=16, ws=64, size=1 << 24):
+        return lib.kans_selective_scan_forward(dt, x, 20, 4, 64, 20, 4, A, bm, 80, 16, 64, 80, 16, None, None, 0, 0, None, 1, state, None,
+                                               out, None, b, n, d, states, ws, size, None)
+
+    def bwd(saved=64, z=None, dz=None, skip=None, dskip=None, dbias=None, ws=64, size=1 << 24, dx=64):
+        return lib.kans_selective_scan_backward(0, 64, 20, 4, 64, 20, 4, 64, 64, 80, 16, 64, 80, 16, skip, z, 20, 4, None, 1, None, saved,
+                                                64, dx, 64, 64, 64, 64, dskip, dz, dbias, 2, 5, 4, 16, ws, size, None)
+    for bad in (dict(dt=3), dict(x=None), dict(A=None), dict(A=68), dict(bm=None), dict(out=None), dict(state=68), dict(b=-1), dict(n=-1),
+                dict(d=0), dict(states=0), dict(n=300, ws=None), dict(n=300, ws=72), dict(n=300, size=16)):
+        assert fwd(**bad) == -1, bad
+    for bad in (dict(states=65), dict(b=1 << 22), dict(n=(1 << 30) + 1), dict(b=1 << 21, n=1 << 20)):
+        assert fwd(**bad) == -5, bad
+    assert fwd(b=0, x=None) == 0 and fwd(n=0, x=None) == 0
+    for bad in (dict(saved=None), dict(z=64), dict(dz=64), dict(dskip=64), dict(dbias=64), dict(ws=None), dict(ws=72), dict(size=16),
+                dict(dx=None)):
+        assert bwd(**bad) == -1, bad
+    assert lib.kans_selective_scan_workspace(2, 5, 4, 65, 0) == -5 and lib.kans_selective_scan_saved(2, 5, 4, 65) == -5
+    assert lib.kans_selective_scan_workspace(2, 5, 4, 16, 0) == 0
+    assert lib.kans_selective_scan_workspace(1, 700, 4, 16, 0) > 0
+    assert lib.kans_selective_scan_saved(2, 17, 4, 16) == 2 * 2 * 4 * 16 * 4

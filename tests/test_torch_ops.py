@@ -123,3 +123,34 @@ def test_dropout_refuses(mk):
                        ((x, 0.1, torch.zeros(1)), TypeError), ((x, 0.1, 1.5), TypeError), ((None, 0.1, 1), TypeError)):
         with pytest.raises(error):
             mk.dropout(*bad)
+
+
+def test_causal_conv_refuses(mk):
+    x, w, b = torch.zeros(2, 5, 4), torch.zeros(4, 3), torch.zeros(4)
+    n = torch.zeros(2, dtype=torch.int64)
+    for bad, error in (((x, w), ValueError), ((x[0], w), ValueError), ((x[..., :0], w[:0]), ValueError), ((x, w[:3]), ValueError),
+                       ((x, torch.zeros(4, 9)), ValueError), ((x, w[:, :0]), ValueError), ((x, w, b[:3]), ValueError),
+                       ((x, w, b, "relu"), ValueError), ((x, w, b, None, torch.zeros(2, 3, 4)), ValueError),
+                       ((x, w, b, None, torch.zeros(2, 4, 2).transpose(1, 2)), ValueError),
+                       ((x, w, b, None, torch.zeros(2, 2, 4).half()), TypeError), ((x, w, b, None, None, n[:1]), ValueError),
+                       ((x, w, b, None, None, n.int()), TypeError), ((x.double(), w.double()), TypeError), ((x, w.half()), TypeError),
+                       ((x, w, b.half()), TypeError), ((None, w), TypeError)):
+        with pytest.raises(error):
+            mk.causal_conv(*bad)
+
+
+def test_selective_scan_refuses(mk):
+    x, A, B = torch.zeros(2, 5, 4), torch.zeros(4, 16), torch.zeros(2, 5, 16)
+    n, state = torch.zeros(2, dtype=torch.int64), torch.zeros(2, 4, 16)
+    ok = dict(x=x, dt=x, A=A, B=B, C=B)
+    for bad, error in ((dict(), ValueError), (dict(x=x[0]), ValueError), (dict(A=A[:3]), ValueError), (dict(A=A[:, :0]), ValueError),
+                       (dict(A=torch.zeros(4, 65), B=torch.zeros(2, 5, 65), C=torch.zeros(2, 5, 65)), ValueError),
+                       (dict(dt=x[:, :4]), ValueError), (dict(z=x[:1]), ValueError), (dict(B=B[..., :15]), ValueError),
+                       (dict(C=B.half()), TypeError), (dict(dt=x.half()), TypeError), (dict(z=x.half()), TypeError),
+                       (dict(A=A.half()), TypeError), (dict(D=torch.zeros(3)), ValueError), (dict(D=torch.zeros(4).half()), TypeError),
+                       (dict(dt_bias=torch.zeros(4, 1)), ValueError), (dict(state=state[:1]), ValueError),
+                       (dict(state=state.half()), TypeError), (dict(state=torch.zeros(2, 16, 4).transpose(1, 2)), ValueError),
+                       (dict(lengths=n[:1]), ValueError), (dict(lengths=n.int()), TypeError),
+                       (dict(x=x.double(), dt=x.double(), B=B.double(), C=B.double()), TypeError), (dict(x=None), TypeError)):
+        with pytest.raises(error):
+            mk.selective_scan(**{**ok, **bad})

@@ -13,13 +13,13 @@ struct ScanArgs {
   float* state;               // [B][D][N], read and written; or null
   const int64_t* lengths;
   void* out;
-  float* saved;               // [B][ceil(L / interval)][D][N]: the states before every `interval` steps
+  float* saved;               // [B][ceil(L / interval)][D][padded N]: the states before every `interval` steps
   // Elements between sequences and between steps of the inputs, whose channels and states lie side by side.
   long x_batch, x_row, dt_batch, dt_row, b_batch, b_row, c_batch, c_row, z_batch, z_row;
   int B, L, D, N;
   int softplus;
-  // Where a sequence is cut in chunks (chunks > 1): of `chunk` steps each, their first states [B][chunks][D][N] (or, backward,
-  // the gradients behind their last), and the sums of the step sizes [B][chunks][D].
+  // Where a sequence is cut in chunks (chunks > 1): of `chunk` steps each, their first states [B][chunks][D][padded N] (or,
+  // backward, the gradients behind their last), and the sums of the step sizes [B][chunks][D].
   int chunk, chunks;
   float *edge, *sums;
   // backward
@@ -36,7 +36,7 @@ inline int scan_regs(int N) {
     if (N <= 4 * r) return r;
   return 0;
 }
-constexpr int scan_interval(int regs) { return regs <= 4 ? 16 : regs <= 8 ? 8 : 4; }
+constexpr int scan_interval(int regs) { return regs <= 4 ? 16 : regs <= 6 ? 8 : 4; }
 
 enum class ScanPass { kForward, kEdges, kBackward, kBackwardEdges, kStep };
 hipError_t scan_launch_f32(ScanPass pass, const ScanArgs& A, hipStream_t st);

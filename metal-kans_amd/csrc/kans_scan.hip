@@ -20,6 +20,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <initializer_list>
 
 #include "kans_scan.h"
 
@@ -27,16 +28,18 @@ namespace kans {
 namespace {
 
 // Per chunk in order (backward: from the last), edge becomes what comes into it: H, then H exp(A sum s) + edge.
-__global__ __launch_bounds__(256) void k_scan_join(const ScanArgs A, bool backward) {
+__global__ __launch_bounds__(256) void k_scan_join(const ScanArgs A, int padded, bool backward) {
   const long at = (long)blockIdx.x * 256 + threadIdx.x, states = (long)A.D * A.N;
   if (at >= A.B * states) return;
-  const long b = at / states, in = at - b * states, d = in / A.N;
+  const long b = at / states, in = at - b * states, d = in / A.N, to = d * padded + (in - d * A.N);
   const float a2 = A.A[in] * 1.44269504088896340736f;
   float h = !backward && A.state ? A.state[at] : 0.0f;
+#pragma unroll 4
   for (int i = 0; i < A.chunks; ++i) {
     const long place = b * A.chunks + (backward ? A.chunks - 1 - i : i);
-    const float e = A.edge[place * states + in], s = A.sums[place * A.D + d];
-    A.edge[place * states + in] = h;
+    float* edge = A.edge + place * A.D * padded + to;
+    const float e = *edge, s = A.sums[place * A.D + d];
+    *edge = h;
     h = __builtin_amdgcn_exp2f(a2 * s) * h + e;
   }
 }
@@ -84,11 +87,11 @@ ScanPlan plan_scan(int B, int L, int D, int N) {
     p.chunk = (int)(((L + want - 1) / want + 15) & ~15L);
   }
   p.chunks = std::max(1, (L + p.chunk - 1) / p.chunk);
-  p.edges = p.chunks > 1 ? (long)B * p.chunks * D * (N + 1) : 0;
+  p.edges = p.chunks > 1 ? (long)B * p.chunks * D * (p.padded + 1) : 0;
   p.edges = (p.edges + 3) & ~3L;
   p.part_bc = (long)p.blocks * B * L * 2 * p.padded;
   p.part_par = (long)B * p.chunks * D * (N + 2);
-  p.saved = (long)B * ((L + p.interval - 1) / p.interval) * D * N;
+  p.saved = (long)B * ((L + p.interval - 1) / p.interval) * D * p.padded;
   return p;
 }
 
@@ -100,6 +103,13 @@ int check_scan(int dtype, int B, int L, int D, int N) {
   const long blocks = ((long)D + kScanChannels - 1) / kScanChannels;
   if (L > (1 << 30) || (long)B * blocks >= 1L << 22 || (long)B * L * 2 * kMaxStates >= 1L << 38)
     return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
+  return 0;
+}
+
+// The kernels reach 16 steps of a tensor by 32-bit offsets.
+int check_rows(std::initializer_list<long> rows) {
+  for (long r : rows)
+    if (r < 0 || r >= 1L << 25) return kans_fail(KANS_ERR_UNSUPPORTED, "%ld elements between steps, fewer than 2^25", r);
   return 0;
 }
 
@@ -137,6 +147,7 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
   if (rc || B == 0 || L == 0) return rc;
   if (!x || !dt || !A || !Bm || !Cm || !out) return kans_fail(KANS_ERR_ARG, "null argument");
   if ((uintptr_t)state % 16 || (uintptr_t)A % 16) return kans_fail(KANS_ERR_ARG, "A and the state start at multiples of 16 bytes");
+  if ((rc = check_rows({x_row, dt_row, b_row, c_row, z ? z_row : 0, D}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, p.edges * (long)sizeof(float)))) return rc;
   std::lock_guard<std::mutex> lk(kans_mutex());
@@ -154,9 +165,9 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
   }
   if (p.chunks > 1) {
     S.edge = (float*)workspace;
-    S.sums = S.edge + (long)B * p.chunks * D * N;
+    S.sums = S.edge + (long)B * p.chunks * D * p.padded;
     HIP_TRY(launch(dtype, ScanPass::kEdges, S, st));
-    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, false);
+    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, p.padded, false);
     HIP_TRY(hipGetLastError());
   }
   HIP_TRY(launch(dtype, ScanPass::kForward, S, st));
@@ -174,6 +185,7 @@ int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_
   const bool any = B > 0 && L > 0;
   if (any && (!x || !dt || !A || !Bm || !Cm || !saved || !dout || !dx || !ddt || (z && !dz))) return kans_fail(KANS_ERR_ARG, "null argument");
   if ((dskip && !skip) || (dz && !z) || (ddt_bias && !dt_bias)) return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
+  if (any && (rc = check_rows({x_row, dt_row, b_row, c_row, z ? z_row : 0, D}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, (p.edges + p.part_bc + p.part_par) * (long)sizeof(float)))) return rc;
   std::lock_guard<std::mutex> lk(kans_mutex());
@@ -186,13 +198,13 @@ int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_
   S.lengths = lengths; S.saved = (float*)saved; S.dx = dx; S.ddt = ddt; S.dz = dz;
   S.B = B; S.L = L; S.D = D; S.N = N; S.softplus = softplus; S.chunk = p.chunk; S.chunks = p.chunks;
   S.edge = (float*)workspace;
-  S.sums = S.edge + (long)B * p.chunks * D * N;
+  S.sums = S.edge + (long)B * p.chunks * D * p.padded;
   S.part_bc = (float*)workspace + p.edges;
   S.part_par = S.part_bc + p.part_bc;
   if (any) {
     if (p.chunks > 1) {
       HIP_TRY(launch(dtype, ScanPass::kBackwardEdges, S, st));
-      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, true);
+      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, p.padded, true);
       HIP_TRY(hipGetLastError());
     }
     HIP_TRY(launch(dtype, ScanPass::kBackward, S, st));

@@ -84,21 +84,90 @@ template <int kRegs> struct Shape {
   static constexpr int kPad = 4 * kRegs;                 // states, rounded up
   static constexpr int kTile = 16;                       // steps of a forward tile
   static constexpr int kInterval = scan_interval(kRegs); // steps of a backward tile
+  // steps whose B and C are read from LDS together, forward and (with fewer registers to spare) backward
+  static constexpr int kAhead = kRegs <= 4 ? 4 : kRegs <= 8 ? 2 : 1, kAheadBack = kRegs <= 2 ? 4 : 1;
 };
+
+// ---- memory -------------------------------------------------------------------------------------------
+// Buffers with an end: what lies behind it reads as zero and is not written, so that the last steps, the last channels and
+// absent tensors need no branch (a branch ends what the compiler can move: the loads of the next steps).
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr unsigned kNowhere = 0xffffffffu;  // an offset behind every end
+__device__ __forceinline__ Buffer buffer(const void* p, long bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+}
+template <typename T>
+__device__ __forceinline__ T fetch(Buffer b, unsigned offset) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(b, (int)offset, 0, 0));
+  else return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(b, (int)offset, 0, 0));
+}
+template <typename T>
+__device__ __forceinline__ void put(Buffer b, unsigned offset, T v) {
+  if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, v), b, (int)offset, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, v), b, (int)offset, 0, 0);
+}
+// A lane's states in the padded layouts of saved and edge.
+template <int kRegs>
+__device__ __forceinline__ void fetch_states(float (&h)[kRegs], Buffer b, unsigned offset) {
+  typedef unsigned Two __attribute__((ext_vector_type(2)));
+  typedef unsigned Four __attribute__((ext_vector_type(4)));
+  if constexpr (kRegs == 1) {
+    h[0] = fetch<float>(b, offset);
+  } else if constexpr (kRegs % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < kRegs; i += 4) {
+      const Four v = __builtin_amdgcn_raw_buffer_load_b128(b, (int)(offset + 4 * i), 0, 0);
+      __builtin_memcpy(h + i, &v, 16);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRegs; i += 2) {
+      const Two v = __builtin_amdgcn_raw_buffer_load_b64(b, (int)(offset + 4 * i), 0, 0);
+      __builtin_memcpy(h + i, &v, 8);
+    }
+  }
+}
+template <int kRegs>
+__device__ __forceinline__ void put_states(const float (&h)[kRegs], Buffer b, unsigned offset) {
+  typedef unsigned Two __attribute__((ext_vector_type(2)));
+  typedef unsigned Four __attribute__((ext_vector_type(4)));
+  if constexpr (kRegs == 1) {
+    put(b, offset, h[0]);
+  } else if constexpr (kRegs % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < kRegs; i += 4) {
+      Four v;
+      __builtin_memcpy(&v, h + i, 16);
+      __builtin_amdgcn_raw_buffer_store_b128(v, b, (int)(offset + 4 * i), 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kRegs; i += 2) {
+      Two v;
+      __builtin_memcpy(&v, h + i, 8);
+      __builtin_amdgcn_raw_buffer_store_b64(v, b, (int)(offset + 4 * i), 0, 0);
+    }
+  }
+}
 
 // Where a lane stands.
 struct Lane {
-  int b, chunk, c, q, len, t0, t1;  // c: its channel (maybe behind the last), steps [t0, t1) of the chunk, len of the sequence
-  bool on;                          // the channel exists
-  long row;                         // the channel, or the last one
+  int b, chunk, block, c0, c, q, len, t0, t1;  // c: its channel (maybe behind the last), c0: the workgroup's first; steps [t0, t1)
+                                               // of the chunk, len of the sequence
+  bool on;                                     // the channel exists
+  int row;                                     // the channel, or the last one
+  int in;                                      // the channel in the workgroup
 };
 __device__ __forceinline__ Lane lane_of(const ScanArgs& A) {
   Lane l;
   const int blocks = (A.D + kScanChannels - 1) / kScanChannels;
-  const int id = blockIdx.x / blocks, block = blockIdx.x - id * blocks;
+  const int id = blockIdx.x / blocks;
+  l.block = blockIdx.x - id * blocks;
   l.b = id / A.chunks;
   l.chunk = id - l.b * A.chunks;
-  l.c = block * kScanChannels + (int)threadIdx.x / 4;
+  l.in = threadIdx.x / 4;
+  l.c0 = l.block * kScanChannels;
+  l.c = l.c0 + l.in;
   l.q = threadIdx.x & 3;
   l.on = l.c < A.D;
   l.row = min(l.c, A.D - 1);
@@ -108,288 +177,344 @@ __device__ __forceinline__ Lane lane_of(const ScanArgs& A) {
   return l;
 }
 
+// A [B][L][channels] tensor, seen from a workgroup: lane q's values of the steps first + 4 m + q.
+template <typename T>
+struct Steps {
+  const T* base;  // of the sequence and the workgroup's first channel
+  long row;
+  unsigned at;    // the lane's place in four steps
+  int L, width;   // width: channels from the first one on
+  __device__ __forceinline__ Steps(const void* p, long batch, long row, const Lane& l, int L, int D, bool writes)
+      : base((const T*)p + l.b * batch + l.c0), row(row),
+        at(writes && !l.on ? kNowhere : ((unsigned)l.q * (unsigned)row + (unsigned)l.in) * (unsigned)sizeof(T)), L(L), width(D - l.c0) {}
+  __device__ __forceinline__ Buffer four(int first) const {
+    const long steps = min(L - first, 4);
+    return buffer(base + first * row, steps > 0 && base ? ((steps - 1) * row + width) * (long)sizeof(T) : 0);
+  }
+  template <int kCount>
+  __device__ __forceinline__ void read(T (&v)[kCount], int first) const {
+#pragma unroll
+    for (int m = 0; m < kCount; ++m) v[m] = fetch<T>(four(first + 4 * m), at);
+  }
+  __device__ __forceinline__ void write(int first, float v) const { put(four(first), at, from_f32<T>(v)); }
+};
+
+// The states of the workgroup's channels at a place of the padded layouts.
+template <int kRegs>
+__device__ __forceinline__ Buffer states_at(const float* base, long place, const Lane& l, int D, bool there) {
+  constexpr int kPad = 4 * kRegs;
+  return buffer(base + (place * D + l.c0) * kPad, there && base ? (long)min(D - l.c0, kScanChannels) * kPad * 4 : 0);
+}
+
 // B and C of kSteps steps, on their way from memory to LDS.  Steps and states that are not there are zeros.
 template <typename T, int kRegs, int kSteps>
 struct Rows {
-  static constexpr int kPad = 4 * kRegs, kEach = kSteps * 2 * kPad, kPer = (kEach + kThreads - 1) / kThreads;
-  T v[kPer];
-  __device__ __forceinline__ void read(const ScanArgs& A, int b, int first, int len) {
+  static constexpr int kPad = 4 * kRegs, kEach = kSteps * kPad, kPer = (kEach + kThreads - 1) / kThreads;
+  T v[2][kPer];
+  unsigned at[2][kPer];
+  __device__ __forceinline__ Rows(const ScanArgs& A) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = i * kThreads + threadIdx.x, step = at / (2 * kPad), n = at % kPad, t = first + step;
-      const bool is_c = at / kPad & 1, there = at < kEach && t < len && n < A.N;
-      const T* from = is_c ? (const T*)A.Cm + b * A.c_batch + (long)t * A.c_row : (const T*)A.Bm + b * A.b_batch + (long)t * A.b_row;
-      v[i] = there ? from[n] : from_f32<T>(0.0f);
+      const int e = i * kThreads + threadIdx.x, step = e / kPad, n = e % kPad;
+      const bool there = e < kEach && n < A.N;
+      at[0][i] = there ? ((unsigned)step * (unsigned)A.b_row + n) * (unsigned)sizeof(T) : kNowhere;
+      at[1][i] = there ? ((unsigned)step * (unsigned)A.c_row + n) * (unsigned)sizeof(T) : kNowhere;
     }
   }
+  __device__ __forceinline__ void read(const ScanArgs& A, int b, int first, int len) {
+    const long steps = min(len - first, kSteps);
+    const Buffer from_b = buffer((const T*)A.Bm + b * A.b_batch + first * A.b_row, steps > 0 ? ((steps - 1) * A.b_row + A.N) * (long)sizeof(T) : 0);
+    const Buffer from_c = buffer((const T*)A.Cm + b * A.c_batch + first * A.c_row, steps > 0 ? ((steps - 1) * A.c_row + A.N) * (long)sizeof(T) : 0);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      v[0][i] = fetch<T>(from_b, at[0][i]);
+      v[1][i] = fetch<T>(from_c, at[1][i]);
+    }
+  }
+  // [step][B, then C][state]
   __device__ __forceinline__ void write(float* lds) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = i * kThreads + threadIdx.x;
-      if (kEach % kThreads == 0 || at < kEach) lds[at] = to_f32(v[i]);
+      const int e = i * kThreads + threadIdx.x;
+      if (kEach % kThreads == 0 || e < kEach) {
+        float* to = lds + e / kPad * 2 * kPad + e % kPad;
+        to[0] = to_f32(v[0][i]);
+        to[kPad] = to_f32(v[1][i]);
+      }
     }
   }
 };
 
-template <int kRegs>
-__device__ __forceinline__ void read_states(float (&o)[kRegs], const float* lds) {
+// B and C of kAhead steps, read while the steps before are computed.
+template <int kRegs, int kAhead, bool kB, bool kC>
+struct Ahead {
+  static constexpr int kPad = 4 * kRegs;
+  float B[kAhead][kRegs], C[kAhead][kRegs];
+  __device__ __forceinline__ void read(const float* lds, int first) {
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i) o[i] = lds[i];
-}
+    for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+      for (int i = 0; i < kRegs; ++i) {
+        if (kB) B[k][i] = lds[(first + k) * 2 * kPad + i];
+        if (kC) C[k][i] = lds[(first + k) * 2 * kPad + kPad + i];
+      }
+  }
+};
 
-// A lane's states in memory (those from N on are not there).
+// A lane's A log2(e).
 template <int kRegs>
-__device__ __forceinline__ void load_states(float (&h)[kRegs], const float* p, int q, int N, bool on) {
+__device__ __forceinline__ void load_decays(float (&a2)[kRegs], const ScanArgs& A, const Lane& l) {
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int n = q * kRegs + i;
-    h[i] = on && n < N ? p[n] : 0.0f;
-  }
-}
-template <int kRegs>
-__device__ __forceinline__ void store_states(const float (&h)[kRegs], float* p, int q, int N, bool on) {
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    const int n = q * kRegs + i;
-    if (on && n < N) p[n] = h[i];
+    const int n = l.q * kRegs + i;
+    a2[i] = n < A.N ? A.A[(long)l.row * A.N + n] * kLog2e : 0.0f;
   }
 }
 
-// A lane's values of an input at the steps first + 4 m + q.
-template <typename T, int kCount>
-__device__ __forceinline__ void read_steps(T (&v)[kCount], const T* p, long row, int first, int q, int L) {
-#pragma unroll
-  for (int m = 0; m < kCount; ++m) v[m] = p[(long)min(first + 4 * m + q, L - 1) * row];
+// Keeps a value from being computed in a branch of its own.
+__device__ __forceinline__ float here(float v) {
+  asm volatile("" : "+v"(v));
+  return v;
 }
 
 // ---- forward ------------------------------------------------------------------------------------------
 // kEdges: of each chunk alone, from a state of zeros, its last state and the sum of its step sizes.
-template <typename T, int kRegs, bool kEdges>
+template <typename T, int kRegs, bool kEdges, bool kGated>
 __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   constexpr int kPad = Shape<kRegs>::kPad, kTile = Shape<kRegs>::kTile, kInterval = Shape<kRegs>::kInterval, kM = kTile / 4;
+  constexpr int kAhead = Shape<kRegs>::kAhead;
   __shared__ float bc[2][kTile * 2 * kPad];
   const Lane l = lane_of(A);
-  const T* x = (const T*)A.x + l.b * A.x_batch + l.row;
-  const T* dt = (const T*)A.dt + l.b * A.dt_batch + l.row;
-  const T* z = A.z ? (const T*)A.z + l.b * A.z_batch + l.row : nullptr;
+  const Steps<T> x(A.x, A.x_batch, A.x_row, l, A.L, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, A.L, A.D, false);
+  const Steps<T> z(A.z, A.z_batch, A.z_row, l, A.L, A.D, false), out(A.out, (long)A.L * A.D, A.D, l, A.L, A.D, true);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
+  const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], h[kRegs];
-  load_states<kRegs>(a2, A.A + l.row * A.N, l.q, A.N, true);
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i) a2[i] *= kLog2e;
+  load_decays<kRegs>(a2, A, l);
   const long place = (long)l.b * A.chunks + l.chunk;
-  if (kEdges) {
+  float* state = A.state ? A.state + ((long)l.b * A.D + l.row) * A.N : nullptr;
 #pragma unroll
-    for (int i = 0; i < kRegs; ++i) h[i] = 0.0f;
-  } else if (A.chunks > 1) {
-    load_states<kRegs>(h, A.edge + (place * A.D + l.row) * A.N, l.q, A.N, true);
-  } else {
-    load_states<kRegs>(h, A.state + ((long)l.b * A.D + l.row) * A.N, l.q, A.N, A.state != nullptr);
-  }
+  for (int i = 0; i < kRegs; ++i) h[i] = 0.0f;
+  if (!kEdges && A.chunks > 1) fetch_states<kRegs>(h, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
+  else if (!kEdges && state)
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (l.q * kRegs + i < A.N) h[i] = state[l.q * kRegs + i];
   float total = 0.0f;
-  const int intervals = (A.L + kInterval - 1) / kInterval;
+  const long intervals = (A.L + kInterval - 1) / kInterval;
 
   T xv[kM], dv[kM], zv[kM];
-  Rows<T, kRegs, kTile> rows;
-  read_steps(xv, x, A.x_row, l.t0, l.q, A.L);
-  read_steps(dv, dt, A.dt_row, l.t0, l.q, A.L);
-  if (!kEdges && z) read_steps(zv, z, A.z_row, l.t0, l.q, A.L);
+  Rows<T, kRegs, kTile> rows(A);
+  x.read(xv, l.t0);
+  dt.read(dv, l.t0);
+  if (kGated) z.read(zv, l.t0);
   rows.read(A, l.b, l.t0, l.len);
   rows.write(bc[0]);
   __syncthreads();
   for (int t = l.t0, turn = 0; t < l.t1; t += kTile, turn ^= 1) {
-    float s[kM], u[kM], xs[kM], zs[kM];
+    float s[kM], u[kM], xs[kM], gate[kM];
+    const int left = l.len - t - l.q;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      const bool counts = t + 4 * m + l.q < l.len;
-      const float v = to_f32(dv[m]) + bias;
-      s[m] = counts ? (A.softplus ? softplus(v) : v) : 0.0f;
+      const bool counts = 4 * m < left;
+      const float v = to_f32(dv[m]) + bias, soft = here(softplus(v));
+      s[m] = counts ? (A.softplus ? soft : v) : 0.0f;
       xs[m] = counts ? to_f32(xv[m]) : 0.0f;
       u[m] = s[m] * xs[m];
+      gate[m] = 1.0f;
       if (kEdges) total += s[m];
-      else if (z) zs[m] = to_f32(zv[m]);
+      else if (kGated) gate[m] = to_f32(zv[m]) * sigmoid(to_f32(zv[m]));
     }
-    const bool more = t + kTile < l.t1;
-    if (more) {
-      read_steps(xv, x, A.x_row, t + kTile, l.q, A.L);
-      read_steps(dv, dt, A.dt_row, t + kTile, l.q, A.L);
-      if (!kEdges && z) read_steps(zv, z, A.z_row, t + kTile, l.q, A.L);
-      rows.read(A, l.b, t + kTile, l.len);
-    }
-    const float* mine = bc[turn] + l.q * kRegs;
-    static_for<0, kM>([&](auto m_) {
-      constexpr int m = decltype(m_)::value;
-      float y[4];
-      static_for<0, 4>([&](auto k_) {
-        constexpr int k = decltype(k_)::value, j = 4 * m + k;
-        if (!kEdges && j % kInterval == 0 && A.saved && t + j < A.L)
-          store_states<kRegs>(h, A.saved + (((long)l.b * intervals + (t + j) / kInterval) * A.D + l.row) * A.N, l.q, A.N, l.on);
-        float Bv[kRegs], Cv[kRegs];
-        read_states<kRegs>(Bv, mine + j * 2 * kPad);
-        if (!kEdges) read_states<kRegs>(Cv, mine + j * 2 * kPad + kPad);
+    // (behind the chunk's last tile the reads are another chunk's, or nothing)
+    x.read(xv, t + kTile);
+    dt.read(dv, t + kTile);
+    if (kGated) z.read(zv, t + kTile);
+    rows.read(A, l.b, t + kTile, l.len);
+    const float* lds = bc[turn] + l.q * kRegs;
+    Ahead<kRegs, kAhead, true, !kEdges> ahead;
+    ahead.read(lds, 0);
+    float y[4];
+    static_for<0, kTile / kAhead>([&](auto g_) {
+      constexpr int g = decltype(g_)::value;
+      const Ahead<kRegs, kAhead, true, !kEdges> now = ahead;
+      if constexpr (g + 1 < kTile / kAhead) ahead.read(lds, (g + 1) * kAhead);
+      static_for<0, kAhead>([&](auto k_) {
+        constexpr int j = g * kAhead + decltype(k_)::value, m = j / 4, k = j % 4;
+        if constexpr (!kEdges && j % kInterval == 0)
+          put_states<kRegs>(h, states_at<kRegs>(A.saved, l.b * intervals + (t + j) / kInterval, l, A.D, t + j < A.L), mine);
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
-          h[i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]) * h[i] + of_lane<k>(u[m]) * Bv[i];
-          if (!kEdges) sum += h[i] * Cv[i];
+          h[i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]) * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i];
+          if (!kEdges) sum += h[i] * now.C[j - g * kAhead][i];
         }
         y[k] = sum;
+        if constexpr (!kEdges && k == 3) {
+          const float o = (quad_sums(y) + skip * xs[m]) * gate[m];  // (outside the condition: all lanes of the quad take part)
+          out.write(t + 4 * m, 4 * m < left ? o : 0.0f);
+        }
       });
-      if (!kEdges) {
-        const int at = t + 4 * m + l.q;
-        float o = quad_sums(y) + skip * xs[m];
-        if (z) o *= zs[m] * sigmoid(zs[m]);
-        if (l.on && at < A.L) ((T*)A.out)[((long)l.b * A.L + at) * A.D + l.c] = from_f32<T>(at < l.len ? o : 0.0f);
-      }
     });
-    if (more) rows.write(bc[turn ^ 1]);
+    rows.write(bc[turn ^ 1]);
     __syncthreads();
   }
   if (kEdges) {
-    store_states<kRegs>(h, A.edge + (place * A.D + l.row) * A.N, l.q, A.N, l.on);
+    put_states<kRegs>(h, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
     total = quad_sum(total);
     if (l.on && l.q == 0) A.sums[place * A.D + l.c] = total;
-  } else if (A.state && l.chunk == A.chunks - 1) {
-    store_states<kRegs>(h, A.state + ((long)l.b * A.D + l.row) * A.N, l.q, A.N, l.on);
+  } else if (state && l.on && l.chunk == A.chunks - 1) {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i)
+      if (l.q * kRegs + i < A.N) state[l.q * kRegs + i] = h[i];
   }
 }
 
 // ---- backward -----------------------------------------------------------------------------------------
 // kEdges: of each chunk alone, without a gradient from behind it, the gradient of its first state, and the sum of its step sizes.
-template <typename T, int kRegs, bool kEdges>
-__global__ __launch_bounds__(kThreads) void k_scan_bwd(const ScanArgs A) {
+// (At most 256 registers: two waves a SIMD, where one leaves a third of its cycles unused; 64 states need more.)
+template <typename T, int kRegs, bool kEdges, bool kGated>
+__global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const ScanArgs A) {
   constexpr int kPad = Shape<kRegs>::kPad, kTile = Shape<kRegs>::kInterval, kM = kTile / 4, kGroups = kTile * 2 * kRegs / 16;
+  constexpr int kAhead = Shape<kRegs>::kAheadBack;
   __shared__ float bc[2][kTile * 2 * kPad];
   __shared__ float red[kEdges ? 1 : 2][4][kEdges ? 1 : kGroups * 64];
   const Lane l = lane_of(A);
-  const T* x = (const T*)A.x + l.b * A.x_batch + l.row;
-  const T* dt = (const T*)A.dt + l.b * A.dt_batch + l.row;
-  const T* z = A.z ? (const T*)A.z + l.b * A.z_batch + l.row : nullptr;
-  const T* dout = (const T*)A.dout + (long)l.b * A.L * A.D + l.row;
+  const Steps<T> x(A.x, A.x_batch, A.x_row, l, A.L, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, A.L, A.D, false);
+  const Steps<T> z(A.z, A.z_batch, A.z_row, l, A.L, A.D, false), dout(A.dout, (long)A.L * A.D, A.D, l, A.L, A.D, false);
+  const Steps<T> dx(A.dx, (long)A.L * A.D, A.D, l, A.L, A.D, true), ddt(A.ddt, (long)A.L * A.D, A.D, l, A.L, A.D, true),
+      dz(A.dz, (long)A.L * A.D, A.D, l, A.L, A.D, true);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
+  const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], carry[kRegs], dA[kRegs] = {}, dskip = 0.0f, dbias = 0.0f, total = 0.0f;
-  load_states<kRegs>(a2, A.A + l.row * A.N, l.q, A.N, true);
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i) a2[i] *= kLog2e;
+  load_decays<kRegs>(a2, A, l);
   const long place = (long)l.b * A.chunks + l.chunk;
-  load_states<kRegs>(carry, A.edge + (place * A.D + l.row) * A.N, l.q, A.N, !kEdges && A.chunks > 1 && l.on);
-  const int intervals = (A.L + kTile - 1) / kTile;
-  const float* saved = A.saved + ((long)l.b * intervals * A.D + l.row) * A.N;
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i) carry[i] = 0.0f;
+  if (!kEdges && A.chunks > 1) fetch_states<kRegs>(carry, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
+  const long intervals = (A.L + kTile - 1) / kTile;
 
   const int tiles = (l.t1 - l.t0 + kTile - 1) / kTile;
   T xv[kM], dv[kM], zv[kM], gv[kM];
   float first[kRegs];
-  Rows<T, kRegs, kTile> rows;
-  auto read = [&](int t) {
-    read_steps(xv, x, A.x_row, t, l.q, A.L);
-    read_steps(dv, dt, A.dt_row, t, l.q, A.L);
-    read_steps(gv, dout, A.D, t, l.q, A.L);
-    if (z) read_steps(zv, z, A.z_row, t, l.q, A.L);
+  Rows<T, kRegs, kTile> rows(A);
+  auto read = [&](int tile) {
+    const int t = l.t0 + max(tile, 0) * kTile;
+    x.read(xv, t);
+    dt.read(dv, t);
+    dout.read(gv, t);
+    if (kGated) z.read(zv, t);
     rows.read(A, l.b, t, l.len);
-    if (!kEdges) load_states<kRegs>(first, saved + (long)(t / kTile) * A.D * A.N, l.q, A.N, true);
+    if (!kEdges) fetch_states<kRegs>(first, states_at<kRegs>(A.saved, l.b * intervals + t / kTile, l, A.D, true), mine);
   };
-  read(l.t0 + (tiles - 1) * kTile);
+  read(tiles - 1);
   rows.write(bc[0]);
   __syncthreads();
   for (int tile = tiles - 1, turn = 0; tile >= 0; --tile, turn ^= 1) {
     const int t = l.t0 + tile * kTile;
-    float s[kM], u[kM], xs[kM], dy[kM], vs[kM], zs[kM], ds[kM], h[kRegs];
+    // dzs: dout times silu's slope, slope: the step size's
+    float s[kM], u[kM], xs[kM], dy[kM], dzs[kM], slope[kM], h[kRegs];
+    const int left = l.on ? l.len - t - l.q : 0;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
-      const bool counts = l.on && t + 4 * m + l.q < l.len;
-      vs[m] = to_f32(dv[m]) + bias;
-      s[m] = counts ? (A.softplus ? softplus(vs[m]) : vs[m]) : 0.0f;
+      const bool counts = 4 * m < left;
+      const float v = to_f32(dv[m]) + bias, soft = here(softplus(v)), sig = here(sigmoid(v));
+      s[m] = counts ? (A.softplus ? soft : v) : 0.0f;
+      slope[m] = counts ? (A.softplus ? sig : 1.0f) : 0.0f;
       xs[m] = counts ? to_f32(xv[m]) : 0.0f;
       u[m] = s[m] * xs[m];
-      ds[m] = counts ? to_f32(gv[m]) : 0.0f;  // (dout)
-      zs[m] = z && counts ? to_f32(zv[m]) : 0.0f;
-      dy[m] = z ? ds[m] * (zs[m] * sigmoid(zs[m])) : ds[m];
+      dy[m] = counts ? to_f32(gv[m]) : 0.0f;
+      dzs[m] = 0.0f;
+      if (kGated) {
+        const float zf = counts ? to_f32(zv[m]) : 0.0f, sg = sigmoid(zf);
+        dzs[m] = dy[m] * (sg * (1.0f + zf * (1.0f - sg)));
+        dy[m] *= zf * sg;
+      }
       if (kEdges) total += s[m];
     }
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) h[i] = first[i];
-    if (tile > 0) read(t - kTile);
-    const float* mine = bc[turn] + l.q * kRegs;
+    read(tile - 1);
+    const float* lds = bc[turn] + l.q * kRegs;
     // the states of the tile again: before each step, and what the step leaves of them
-    float before[kEdges ? 1 : kTile][kRegs], left[kTile][kRegs], ys[kM];
-    static_for<0, kM>([&](auto m_) {
-      constexpr int m = decltype(m_)::value;
+    float before[kEdges ? 1 : kTile][kRegs], stay[kTile][kRegs];
+    {
+      Ahead<kRegs, kAhead, !kEdges, !kEdges && kGated> ahead;
+      ahead.read(lds, 0);
       float y[4];
-      static_for<0, 4>([&](auto k_) {
-        constexpr int k = decltype(k_)::value, j = 4 * m + k;
-        float Bv[kRegs], Cv[kRegs], sum = 0.0f;
-        if (!kEdges) read_states<kRegs>(Bv, mine + j * 2 * kPad);
-        if (!kEdges && z) read_states<kRegs>(Cv, mine + j * 2 * kPad + kPad);
+      static_for<0, kTile / kAhead>([&](auto g_) {
+        constexpr int g = decltype(g_)::value;
+        const Ahead<kRegs, kAhead, !kEdges, !kEdges && kGated> now = ahead;
+        if constexpr (g + 1 < kTile / kAhead) ahead.read(lds, (g + 1) * kAhead);
+        static_for<0, kAhead>([&](auto k_) {
+          constexpr int j = g * kAhead + decltype(k_)::value, m = j / 4, k = j % 4;
+          float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < kRegs; ++i) {
-          left[j][i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]);
-          if (kEdges) continue;
-          before[kEdges ? 0 : j][i] = h[i];
-          h[i] = left[j][i] * h[i] + of_lane<k>(u[m]) * Bv[i];
-          if (z) sum += h[i] * Cv[i];
-        }
-        y[k] = sum;
-      });
-      ys[m] = !kEdges && z ? quad_sums(y) + skip * xs[m] : 0.0f;
-    });
-    float vals[16], dA_tile[kRegs] = {};
-    static_for<0, kM>([&](auto m_) {
-      constexpr int m = kM - 1 - decltype(m_)::value;
-      float yB[4], yA[4];
-      static_for<0, 4>([&](auto k_) {
-        constexpr int k = 3 - decltype(k_)::value, j = 4 * m + k;
-        float Bv[kRegs], Cv[kRegs], g[kRegs], sB = 0.0f, sA = 0.0f;
-        if (!kEdges) read_states<kRegs>(Bv, mine + j * 2 * kPad);
-        read_states<kRegs>(Cv, mine + j * 2 * kPad + kPad);
-#pragma unroll
-        for (int i = 0; i < kRegs; ++i) {
-          g[i] = Cv[i] * of_lane<k>(dy[m]) + carry[i];
-          carry[i] = g[i] * left[j][i];
-          if (kEdges) continue;
-          sB += g[i] * Bv[i];
-          const float w = carry[i] * before[kEdges ? 0 : j][i];
-          sA += w * a2[i];
-          dA_tile[i] += w * of_lane<k>(s[m]);
-        }
-        if (kEdges) return;
-        yB[k] = sB;
-        yA[k] = sA;
-        static_for<0, 2 * kRegs>([&](auto i_) {
-          constexpr int i = decltype(i_)::value, value = (kTile - 1 - j) * 2 * kRegs + i;
-          vals[value % 16] = i < kRegs ? g[i % kRegs] * of_lane<k>(u[m]) : h[i % kRegs] * of_lane<k>(dy[m]);
-          if (value % 16 == 15) red[turn][threadIdx.x >> 6][value / 16 * 64 + (threadIdx.x & 63)] = wave_sums(vals);
+          for (int i = 0; i < kRegs; ++i) {
+            stay[j][i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]);
+            if constexpr (!kEdges) {
+              before[j][i] = h[i];
+              h[i] = stay[j][i] * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i];
+              if (kGated) sum += h[i] * now.C[j - g * kAhead][i];
+            }
+          }
+          y[k] = sum;
+          if constexpr (!kEdges && kGated && k == 3) {
+            const float o = dzs[m] * (quad_sums(y) + skip * xs[m]);
+            dz.write(t + 4 * m, 4 * m < left ? o : 0.0f);
+          }
         });
-#pragma unroll
-        for (int i = 0; i < kRegs; ++i) h[i] = before[kEdges ? 0 : j][i];
       });
-      if (!kEdges) {
-        const float gB = quad_sums(yB), gA = quad_sums(yA) * kLn2;
-        const int at = t + 4 * m + l.q;
-        const bool counts = l.on && at < l.len;
-        const float dstep = xs[m] * gB + gA;
-        const float ddt = counts ? (A.softplus ? dstep * sigmoid(vs[m]) : dstep) : 0.0f;
-        const float dxv = counts ? s[m] * gB + skip * dy[m] : 0.0f;
-        dskip += dy[m] * xs[m];
-        dbias += ddt;
-        if (l.on && at < A.L) {
-          const long to = ((long)l.b * A.L + at) * A.D + l.c;
-          ((T*)A.dx)[to] = from_f32<T>(dxv);
-          ((T*)A.ddt)[to] = from_f32<T>(ddt);
-          if (z) {
-            const float sg = sigmoid(zs[m]);
-            ((T*)A.dz)[to] = from_f32<T>(counts ? ds[m] * ys[m] * (sg * (1.0f + zs[m] * (1.0f - sg))) : 0.0f);
+    }
+    float vals[16], dA_tile[kRegs] = {}, yB[4], yA[4];
+    Ahead<kRegs, kAhead, !kEdges, true> ahead;
+    ahead.read(lds, kTile - kAhead);
+    static_for<0, kTile / kAhead>([&](auto g_) {
+      constexpr int g = kTile / kAhead - 1 - decltype(g_)::value;
+      const Ahead<kRegs, kAhead, !kEdges, true> now = ahead;
+      if constexpr (g > 0) ahead.read(lds, (g - 1) * kAhead);
+      static_for<0, kAhead>([&](auto k_) {
+        constexpr int j = g * kAhead + kAhead - 1 - decltype(k_)::value, m = j / 4, k = j % 4;
+        float gr[kRegs], sB = 0.0f, sA = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kRegs; ++i) {
+          gr[i] = now.C[j - g * kAhead][i] * of_lane<k>(dy[m]) + carry[i];
+          carry[i] = gr[i] * stay[j][i];
+          if constexpr (!kEdges) {
+            sB += gr[i] * now.B[j - g * kAhead][i];
+            const float w = carry[i] * before[j][i];
+            sA += w * a2[i];
+            dA_tile[i] += w * of_lane<k>(s[m]);
           }
         }
-      }
+        if constexpr (!kEdges) {
+          yB[k] = sB;
+          yA[k] = sA;
+          static_for<0, 2 * kRegs>([&](auto i_) {
+            constexpr int i = decltype(i_)::value, value = (kTile - 1 - j) * 2 * kRegs + i;
+            vals[value % 16] = i < kRegs ? gr[i % kRegs] * of_lane<k>(u[m]) : h[i % kRegs] * of_lane<k>(dy[m]);
+            if (value % 16 == 15) red[turn][threadIdx.x >> 6][value / 16 * 64 + (threadIdx.x & 63)] = wave_sums(vals);
+          });
+#pragma unroll
+          for (int i = 0; i < kRegs; ++i) h[i] = before[j][i];
+          if constexpr (k == 0) {
+            const float gB = quad_sums(yB), gA = quad_sums(yA) * kLn2;
+            const bool counts = 4 * m < left;
+            const float ddtv = counts ? (xs[m] * gB + gA) * slope[m] : 0.0f;
+            dskip += dy[m] * xs[m];
+            dbias += ddtv;
+            dx.write(t + 4 * m, counts ? s[m] * gB + skip * dy[m] : 0.0f);
+            ddt.write(t + 4 * m, ddtv);
+          }
+        }
+      });
     });
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) dA[i] += dA_tile[i];
-    if (tile > 0) rows.write(bc[turn ^ 1]);
+    rows.write(bc[turn ^ 1]);
     __syncthreads();
     if (!kEdges) {
       // the sums over this workgroup's channels: [step][B or C][state]
-      const int block = (int)(blockIdx.x % ((A.D + kScanChannels - 1) / kScanChannels));
-      float* part = A.part_bc + (((long)block * A.B + l.b) * A.L + t) * 2 * kPad;
+      float* part = A.part_bc + (((long)l.block * A.B + l.b) * A.L + t) * 2 * kPad;
       const int there = min(kTile, A.L - t) * 2 * kPad;
 #pragma unroll
       for (int i = 0; i < (kTile * 2 * kPad + kThreads - 1) / kThreads; ++i) {
@@ -402,16 +527,19 @@ __global__ __launch_bounds__(kThreads) void k_scan_bwd(const ScanArgs A) {
     }
   }
   if (kEdges) {
-    store_states<kRegs>(carry, A.edge + (place * A.D + l.row) * A.N, l.q, A.N, l.on);
+    put_states<kRegs>(carry, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
     total = quad_sum(total);
     if (l.on && l.q == 0) A.sums[place * A.D + l.c] = total;
     return;
   }
   float* par = A.part_par + (place * A.D + l.row) * (A.N + 2);
-  store_states<kRegs>(dA, par, l.q, A.N, l.on);
   dskip = quad_sum(dskip);
   dbias = quad_sum(dbias);
-  if (l.on && l.q == 0) {
+  if (!l.on) return;
+#pragma unroll
+  for (int i = 0; i < kRegs; ++i)
+    if (l.q * kRegs + i < A.N) par[l.q * kRegs + i] = dA[i];
+  if (l.q == 0) {
     par[A.N] = dskip;
     par[A.N + 1] = dbias;
   }
@@ -480,14 +608,18 @@ __global__ __launch_bounds__(256) void k_scan_reduce(const float* part, int bloc
 template <typename T, int kRegs>
 hipError_t launch(ScanPass pass, const ScanArgs& A, hipStream_t st) {
   const dim3 grid((unsigned)((long)A.B * A.chunks * ((A.D + kScanChannels - 1) / kScanChannels)));
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, st, A);
+    return hipGetLastError();
+  };
   switch (pass) {
-    case ScanPass::kForward: hipLaunchKernelGGL((k_scan_fwd<T, kRegs, false>), grid, dim3(kThreads), 0, st, A); break;
-    case ScanPass::kEdges: hipLaunchKernelGGL((k_scan_fwd<T, kRegs, true>), grid, dim3(kThreads), 0, st, A); break;
-    case ScanPass::kBackward: hipLaunchKernelGGL((k_scan_bwd<T, kRegs, false>), grid, dim3(kThreads), 0, st, A); break;
-    case ScanPass::kBackwardEdges: hipLaunchKernelGGL((k_scan_bwd<T, kRegs, true>), grid, dim3(kThreads), 0, st, A); break;
+    case ScanPass::kForward: return A.z ? go(k_scan_fwd<T, kRegs, false, true>) : go(k_scan_fwd<T, kRegs, false, false>);
+    case ScanPass::kEdges: return go(k_scan_fwd<T, kRegs, true, false>);
+    case ScanPass::kBackward: return A.z ? go(k_scan_bwd<T, kRegs, false, true>) : go(k_scan_bwd<T, kRegs, false, false>);
+    case ScanPass::kBackwardEdges: return A.z ? go(k_scan_bwd<T, kRegs, true, true>) : go(k_scan_bwd<T, kRegs, true, false>);
     case ScanPass::kStep: break;
   }
-  return hipGetLastError();
+  return hipErrorInvalidValue;
 }
 
 template <typename T>

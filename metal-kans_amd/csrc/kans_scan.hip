@@ -106,10 +106,10 @@ int check_scan(int dtype, int B, int L, int D, int N) {
   return 0;
 }
 
-// The kernels reach 16 steps of a tensor by 32-bit offsets.
+// The kernels reach 16 steps of a tensor by offsets below 2^30.
 int check_rows(std::initializer_list<long> rows) {
   for (long r : rows)
-    if (r < 0 || r >= 1L << 25) return kans_fail(KANS_ERR_UNSUPPORTED, "%ld elements between steps, fewer than 2^25", r);
+    if (r < 0 || r >= 1L << 23) return kans_fail(KANS_ERR_UNSUPPORTED, "%ld elements between steps, fewer than 2^23", r);
   return 0;
 }
 

@@ -92,9 +92,9 @@ template <int kRegs> struct Shape {
 // Buffers with an end: what lies behind it reads as zero and is not written, so that the last steps, the last channels and
 // absent tensors need no branch (a branch ends what the compiler can move: the loads of the next steps).
 typedef __amdgpu_buffer_rsrc_t Buffer;
-constexpr unsigned kNowhere = 0xffffffffu;  // an offset behind every end
-__device__ __forceinline__ Buffer buffer(const void* p, long bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
+constexpr unsigned kNowhere = 0x80000000u;  // an offset behind every end (none reaches 2^30), also with 16 steps added
+__device__ __forceinline__ Buffer buffer(const void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
 }
 template <typename T>
 __device__ __forceinline__ T fetch(Buffer b, unsigned offset) {
@@ -177,58 +177,72 @@ __device__ __forceinline__ Lane lane_of(const ScanArgs& A) {
   return l;
 }
 
-// A [B][L][channels] tensor, seen from a workgroup: lane q's values of the steps first + 4 m + q.
-template <typename T>
+// A [B][L][channels] tensor, seen from a workgroup: lane q's values of the steps t + 4 m + q of a tile of kTile steps.  The
+// tile's buffer is made of a pointer that moves with it and the steps left, by the same few scalar instructions for all.
+template <typename T, int kTile>
 struct Steps {
-  const T* base;  // of the sequence and the workgroup's first channel
-  long row;
-  unsigned at;    // the lane's place in four steps
-  int L, width;   // width: channels from the first one on
-  __device__ __forceinline__ Steps(const void* p, long batch, long row, const Lane& l, int L, int D, bool writes)
-      : base((const T*)p + l.b * batch + l.c0), row(row),
-        at(writes && !l.on ? kNowhere : ((unsigned)l.q * (unsigned)row + (unsigned)l.in) * (unsigned)sizeof(T)), L(L), width(D - l.c0) {}
-  __device__ __forceinline__ Buffer four(int first) const {
-    const long steps = min(L - first, 4);
-    return buffer(base + first * row, steps > 0 && base ? ((steps - 1) * row + width) * (long)sizeof(T) : 0);
+  const char* tile;     // the sequence's and workgroup's first channel in the tile's first step
+  int row, width;       // bytes of a step, and of the channels from the first one on (0: no tensor)
+  unsigned at;          // the lane's place in four steps
+  __device__ __forceinline__ Steps(const void* p, long batch, long row_, const Lane& l, int t, int D, bool writes)
+      : tile((const char*)p + (l.b * batch + l.c0 + t * row_) * (long)sizeof(T)), row((int)row_ * (int)sizeof(T)),
+        width(p ? (D - l.c0) * (int)sizeof(T) : 0),
+        at(writes && !l.on ? kNowhere : (unsigned)l.q * (unsigned)row + (unsigned)(l.in * (int)sizeof(T))) {}
+  __device__ __forceinline__ void move(int tiles) { tile += (long)tiles * kTile * row; }
+  __device__ __forceinline__ Buffer steps(int left) const {  // left: of the tensor from the tile's first step on
+    const int there = min(left, kTile);
+    return buffer(tile, ((there - 1) * row + width) & (there > 0 && width > 0 ? -1 : 0));
   }
+  __device__ __forceinline__ unsigned four(int m) const { return at + (unsigned)(4 * m * row); }
   template <int kCount>
-  __device__ __forceinline__ void read(T (&v)[kCount], int first) const {
+  __device__ __forceinline__ void read(T (&v)[kCount], int left) const {
+    const Buffer from = steps(left);
 #pragma unroll
-    for (int m = 0; m < kCount; ++m) v[m] = fetch<T>(four(first + 4 * m), at);
+    for (int m = 0; m < kCount; ++m) v[m] = fetch<T>(from, four(m));
   }
-  __device__ __forceinline__ void write(int first, float v) const { put(four(first), at, from_f32<T>(v)); }
+  __device__ __forceinline__ void write(Buffer to, int m, float v) const { put(to, four(m), from_f32<T>(v)); }
 };
 
 // The states of the workgroup's channels at a place of the padded layouts.
 template <int kRegs>
 __device__ __forceinline__ Buffer states_at(const float* base, long place, const Lane& l, int D, bool there) {
   constexpr int kPad = 4 * kRegs;
-  return buffer(base + (place * D + l.c0) * kPad, there && base ? (long)min(D - l.c0, kScanChannels) * kPad * 4 : 0);
+  return buffer(base + (place * D + l.c0) * kPad, (min(D - l.c0, kScanChannels) * kPad * 4) & (there ? -1 : 0));
 }
 
 // B and C of kSteps steps, on their way from memory to LDS.  Steps and states that are not there are zeros.
 template <typename T, int kRegs, int kSteps>
 struct Rows {
   static constexpr int kPad = 4 * kRegs, kEach = kSteps * kPad, kPer = (kEach + kThreads - 1) / kThreads;
+  const char* tile[2];
+  int row[2], width;
   T v[2][kPer];
   unsigned at[2][kPer];
-  __device__ __forceinline__ Rows(const ScanArgs& A) {
+  __device__ __forceinline__ Rows(const ScanArgs& A, int b, int t) {
+    tile[0] = (const char*)A.Bm + (b * A.b_batch + t * A.b_row) * (long)sizeof(T);
+    tile[1] = (const char*)A.Cm + (b * A.c_batch + t * A.c_row) * (long)sizeof(T);
+    row[0] = (int)A.b_row * (int)sizeof(T);
+    row[1] = (int)A.c_row * (int)sizeof(T);
+    width = A.N * (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int e = i * kThreads + threadIdx.x, step = e / kPad, n = e % kPad;
-      const bool there = e < kEach && n < A.N;
-      at[0][i] = there ? ((unsigned)step * (unsigned)A.b_row + n) * (unsigned)sizeof(T) : kNowhere;
-      at[1][i] = there ? ((unsigned)step * (unsigned)A.c_row + n) * (unsigned)sizeof(T) : kNowhere;
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        at[w][i] = e < kEach && n < A.N ? (unsigned)step * (unsigned)row[w] + (unsigned)(n * (int)sizeof(T)) : kNowhere;
     }
   }
-  __device__ __forceinline__ void read(const ScanArgs& A, int b, int first, int len) {
-    const long steps = min(len - first, kSteps);
-    const Buffer from_b = buffer((const T*)A.Bm + b * A.b_batch + first * A.b_row, steps > 0 ? ((steps - 1) * A.b_row + A.N) * (long)sizeof(T) : 0);
-    const Buffer from_c = buffer((const T*)A.Cm + b * A.c_batch + first * A.c_row, steps > 0 ? ((steps - 1) * A.c_row + A.N) * (long)sizeof(T) : 0);
+  __device__ __forceinline__ void move(int tiles) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      v[0][i] = fetch<T>(from_b, at[0][i]);
-      v[1][i] = fetch<T>(from_c, at[1][i]);
+    for (int w = 0; w < 2; ++w) tile[w] += (long)tiles * kSteps * row[w];
+  }
+  __device__ __forceinline__ void read(int left) {  // left: steps of the sequence from the tile's first on
+    const int there = min(left, kSteps);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const Buffer from = buffer(tile[w], ((there - 1) * row[w] + width) & (there > 0 ? -1 : 0));
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) v[w][i] = fetch<T>(from, at[w][i]);
     }
   }
   // [step][B, then C][state]
@@ -285,8 +299,8 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   constexpr int kAhead = Shape<kRegs>::kAhead;
   __shared__ float bc[2][kTile * 2 * kPad];
   const Lane l = lane_of(A);
-  const Steps<T> x(A.x, A.x_batch, A.x_row, l, A.L, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, A.L, A.D, false);
-  const Steps<T> z(A.z, A.z_batch, A.z_row, l, A.L, A.D, false), out(A.out, (long)A.L * A.D, A.D, l, A.L, A.D, true);
+  Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, l.t0, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, l.t0, A.D, false);
+  Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, l.t0, A.D, false), out(A.out, (long)A.L * A.D, A.D, l, l.t0, A.D, true);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], h[kRegs];
@@ -301,14 +315,22 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     for (int i = 0; i < kRegs; ++i)
       if (l.q * kRegs + i < A.N) h[i] = state[l.q * kRegs + i];
   float total = 0.0f;
-  const long intervals = (A.L + kInterval - 1) / kInterval;
+  const float* saved = A.saved + ((l.b * (long)((A.L + kInterval - 1) / kInterval) + l.t0 / kInterval) * A.D + l.c0) * kPad;
+  const int saved_bytes = A.saved ? min(A.D - l.c0, kScanChannels) * kPad * 4 : 0;
 
   T xv[kM], dv[kM], zv[kM];
-  Rows<T, kRegs, kTile> rows(A);
-  x.read(xv, l.t0);
-  dt.read(dv, l.t0);
-  if (kGated) z.read(zv, l.t0);
-  rows.read(A, l.b, l.t0, l.len);
+  Rows<T, kRegs, kTile> rows(A, l.b, l.t0);
+  auto read = [&](int t) {
+    x.read(xv, A.L - t);
+    dt.read(dv, A.L - t);
+    if (kGated) z.read(zv, A.L - t);
+    rows.read(l.len - t);
+    x.move(1);
+    dt.move(1);
+    if (kGated) z.move(1);
+    rows.move(1);
+  };
+  read(l.t0);
   rows.write(bc[0]);
   __syncthreads();
   for (int t = l.t0, turn = 0; t < l.t1; t += kTile, turn ^= 1) {
@@ -326,10 +348,8 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
       else if (kGated) gate[m] = to_f32(zv[m]) * sigmoid(to_f32(zv[m]));
     }
     // (behind the chunk's last tile the reads are another chunk's, or nothing)
-    x.read(xv, t + kTile);
-    dt.read(dv, t + kTile);
-    if (kGated) z.read(zv, t + kTile);
-    rows.read(A, l.b, t + kTile, l.len);
+    read(t + kTile);
+    const Buffer to = out.steps(A.L - t);
     const float* lds = bc[turn] + l.q * kRegs;
     Ahead<kRegs, kAhead, true, !kEdges> ahead;
     ahead.read(lds, 0);
@@ -340,8 +360,10 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
       if constexpr (g + 1 < kTile / kAhead) ahead.read(lds, (g + 1) * kAhead);
       static_for<0, kAhead>([&](auto k_) {
         constexpr int j = g * kAhead + decltype(k_)::value, m = j / 4, k = j % 4;
-        if constexpr (!kEdges && j % kInterval == 0)
-          put_states<kRegs>(h, states_at<kRegs>(A.saved, l.b * intervals + (t + j) / kInterval, l, A.D, t + j < A.L), mine);
+        if constexpr (!kEdges && j % kInterval == 0) {
+          put_states<kRegs>(h, buffer(saved, saved_bytes & (t + j < A.L ? -1 : 0)), mine);
+          saved += (long)A.D * kPad;
+        }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
@@ -351,10 +373,11 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
         y[k] = sum;
         if constexpr (!kEdges && k == 3) {
           const float o = (quad_sums(y) + skip * xs[m]) * gate[m];  // (outside the condition: all lanes of the quad take part)
-          out.write(t + 4 * m, 4 * m < left ? o : 0.0f);
+          out.write(to, m, 4 * m < left ? o : 0.0f);
         }
       });
     });
+    out.move(1);
     rows.write(bc[turn ^ 1]);
     __syncthreads();
   }
@@ -379,10 +402,11 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   __shared__ float bc[2][kTile * 2 * kPad];
   __shared__ float red[kEdges ? 1 : 2][4][kEdges ? 1 : kGroups * 64];
   const Lane l = lane_of(A);
-  const Steps<T> x(A.x, A.x_batch, A.x_row, l, A.L, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, A.L, A.D, false);
-  const Steps<T> z(A.z, A.z_batch, A.z_row, l, A.L, A.D, false), dout(A.dout, (long)A.L * A.D, A.D, l, A.L, A.D, false);
-  const Steps<T> dx(A.dx, (long)A.L * A.D, A.D, l, A.L, A.D, true), ddt(A.ddt, (long)A.L * A.D, A.D, l, A.L, A.D, true),
-      dz(A.dz, (long)A.L * A.D, A.D, l, A.L, A.D, true);
+  const int tiles = (l.t1 - l.t0 + kTile - 1) / kTile, last = l.t0 + (tiles - 1) * kTile;
+  const long full = (long)A.L * A.D;
+  Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, last, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, last, A.D, false);
+  Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, last, A.D, false), dout(A.dout, full, A.D, l, last, A.D, false);
+  Steps<T, kTile> dx(A.dx, full, A.D, l, last, A.D, true), ddt(A.ddt, full, A.D, l, last, A.D, true), dz(A.dz, full, A.D, l, last, A.D, true);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], carry[kRegs], dA[kRegs] = {}, dskip = 0.0f, dbias = 0.0f, total = 0.0f;
@@ -391,22 +415,27 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) carry[i] = 0.0f;
   if (!kEdges && A.chunks > 1) fetch_states<kRegs>(carry, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
-  const long intervals = (A.L + kTile - 1) / kTile;
+  const float* saved = A.saved + ((l.b * (long)((A.L + kTile - 1) / kTile) + last / kTile) * A.D + l.c0) * kPad;
+  const int saved_bytes = min(A.D - l.c0, kScanChannels) * kPad * 4;
 
-  const int tiles = (l.t1 - l.t0 + kTile - 1) / kTile;
   T xv[kM], dv[kM], zv[kM], gv[kM];
   float first[kRegs];
-  Rows<T, kRegs, kTile> rows(A);
-  auto read = [&](int tile) {
-    const int t = l.t0 + max(tile, 0) * kTile;
-    x.read(xv, t);
-    dt.read(dv, t);
-    dout.read(gv, t);
-    if (kGated) z.read(zv, t);
-    rows.read(A, l.b, t, l.len);
-    if (!kEdges) fetch_states<kRegs>(first, states_at<kRegs>(A.saved, l.b * intervals + t / kTile, l, A.D, true), mine);
+  Rows<T, kRegs, kTile> rows(A, l.b, last);
+  auto read = [&](int t, bool there) {  // (before the chunk's first tile nothing is)
+    x.read(xv, there ? A.L - t : 0);
+    dt.read(dv, there ? A.L - t : 0);
+    dout.read(gv, there ? A.L - t : 0);
+    if (kGated) z.read(zv, there ? A.L - t : 0);
+    rows.read(there ? l.len - t : 0);
+    if (!kEdges) fetch_states<kRegs>(first, buffer(saved, saved_bytes & (there ? -1 : 0)), mine);
+    x.move(-1);
+    dt.move(-1);
+    dout.move(-1);
+    if (kGated) z.move(-1);
+    rows.move(-1);
+    saved -= (long)A.D * kPad;
   };
-  read(tiles - 1);
+  read(last, true);
   rows.write(bc[0]);
   __syncthreads();
   for (int tile = tiles - 1, turn = 0; tile >= 0; --tile, turn ^= 1) {
@@ -433,7 +462,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     }
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) h[i] = first[i];
-    read(tile - 1);
+    const Buffer to_dx = dx.steps(A.L - t), to_ddt = ddt.steps(A.L - t), to_dz = dz.steps(kGated ? A.L - t : 0);
     const float* lds = bc[turn] + l.q * kRegs;
     // the states of the tile again: before each step, and what the step leaves of them
     float before[kEdges ? 1 : kTile][kRegs], stay[kTile][kRegs];
@@ -460,7 +489,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           y[k] = sum;
           if constexpr (!kEdges && kGated && k == 3) {
             const float o = dzs[m] * (quad_sums(y) + skip * xs[m]);
-            dz.write(t + 4 * m, 4 * m < left ? o : 0.0f);
+            dz.write(to_dz, m, 4 * m < left ? o : 0.0f);
           }
         });
       });
@@ -474,6 +503,8 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
       if constexpr (g > 0) ahead.read(lds, (g - 1) * kAhead);
       static_for<0, kAhead>([&](auto k_) {
         constexpr int j = g * kAhead + kAhead - 1 - decltype(k_)::value, m = j / 4, k = j % 4;
+        // the tile before, once the first of its successor's states are done with (their registers hold it)
+        if constexpr (j == kTile * 3 / 4 - 1) read(t - kTile, tile > 0);
         float gr[kRegs], sB = 0.0f, sA = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
@@ -502,14 +533,17 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
             const float ddtv = counts ? (xs[m] * gB + gA) * slope[m] : 0.0f;
             dskip += dy[m] * xs[m];
             dbias += ddtv;
-            dx.write(t + 4 * m, counts ? s[m] * gB + skip * dy[m] : 0.0f);
-            ddt.write(t + 4 * m, ddtv);
+            dx.write(to_dx, m, counts ? s[m] * gB + skip * dy[m] : 0.0f);
+            ddt.write(to_ddt, m, ddtv);
           }
         }
       });
     });
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) dA[i] += dA_tile[i];
+    dx.move(-1);
+    ddt.move(-1);
+    if (kGated) dz.move(-1);
     rows.write(bc[turn ^ 1]);
     __syncthreads();
     if (!kEdges) {

@@ -31,28 +31,39 @@ struct ConvArgs {
   int silu;
 };
 
+// V neighbouring channels as they lie in memory, at any address (the device takes wide accesses anywhere).
+template <typename T, int V> struct Vec { T v[V]; };
 template <typename T, int V>
-__device__ __forceinline__ void load(float (&o)[V], const T* p) {
-  T v[V];
-  __builtin_memcpy(v, p, sizeof(v));
-#pragma unroll
-  for (int e = 0; e < V; ++e) o[e] = to_f32(v[e]);
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p) {
+  Vec<T, V> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store(T* p, const float (&o)[V], int skip) {
-  T v[V];
+__device__ __forceinline__ void load(float (&o)[V], const T* p) {
+  const Vec<T, V> v = load_vec<T, V>(p);
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = from_f32<T>(o[e]);
-  if (skip == 0) {
-    __builtin_memcpy(p, v, sizeof(v));
-    return;
+  for (int e = 0; e < V; ++e) o[e] = to_f32(v.v[e]);
+}
+// Without the first `skip` channels.  Results leave nontemporal: lines that are written whole need not be read or kept.
+template <typename T, int V>
+__device__ __forceinline__ void store(T* p, const float (&o)[V], int skip) {
+  typedef unsigned Wide __attribute__((ext_vector_type(V * sizeof(T) >= 4 ? V * sizeof(T) / 4 : 1), aligned(sizeof(T))));
+  Vec<T, V> v;
+#pragma unroll
+  for (int e = 0; e < V; ++e) v.v[e] = from_f32<T>(o[e]);
+  if constexpr (V > 1) {
+    if (skip == 0) {
+      __builtin_nontemporal_store(__builtin_bit_cast(Wide, v), (Wide*)p);
+      return;
+    }
   }
 #pragma unroll
   for (int e = 0; e < V; ++e)
-    if (e >= skip) p[e] = v[e];
+    if (e >= skip) p[e] = v.v[e];
 }
 
-__device__ __forceinline__ float sigmoid(float u) { return 1.0f / (1.0f + __builtin_amdgcn_exp2f(u * -1.44269504f)); }
+__device__ __forceinline__ float sigmoid(float u) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(u * -1.44269504f)); }
 
 // The place of a thread: channels [c, c + V) of which the first `skip` are its neighbour's (the last access of a row ends
 // with it), steps [t0, t1) of sequence b, of which `len` count.
@@ -74,14 +85,24 @@ __device__ __forceinline__ bool place(const ConvArgs& A, Place& p) {
   return true;
 }
 
+// The inputs of kSteps steps from t >= 0 on; steps behind the last are the last one's (their results are not kept).
+template <typename T, int V, int kSteps>
+__device__ __forceinline__ void read(Vec<T, V> (&v)[kSteps], const T* p, long row, int t, int L) {
+#pragma unroll
+  for (int g = 0; g < kSteps; ++g) v[g] = load_vec<T, V>(p + min(t + g, L - 1) * row);
+}
+
 template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv_fwd(const ConvArgs A) {
+  constexpr int G = 8;  // steps whose inputs are under way together
   Place p;
   if (!place<V>(A, p)) return;
   const T* x = (const T*)A.x + p.b * A.x_batch + p.c;
-  T* y = (T*)A.y + (long)p.b * A.L * A.D + p.c;
+  T* y = (T*)A.y + ((long)p.b * A.L + p.t0) * A.D + p.c;
   T* state = A.state ? (T*)A.state + (long)p.b * (W - 1) * A.D + p.c : nullptr;
-  float w[W][V], bias[V] = {}, before[W][V];  // before: the last W inputs, the newest last
+  Vec<T, V> next[G];
+  read(next, x, A.x_row, p.t0, A.L);
+  float w[W][V], bias[V] = {}, in[W - 1 + G][V];  // in: the W - 1 inputs before a group of steps, and theirs
 #pragma unroll
   for (int e = 0; e < V; ++e)
 #pragma unroll
@@ -94,28 +115,36 @@ __global__ __launch_bounds__(256) void k_conv_fwd(const ConvArgs A) {
     else if (t < 0 && state) load(o, state + (long)(t + W - 1) * A.D);
   };
 #pragma unroll
-  for (int j = 1; j < W; ++j) input(before[j], p.t0 - W + j);
+  for (int j = 0; j < W - 1; ++j) input(in[j], p.t0 - (W - 1) + j);
   // The new state: the last W - 1 inputs of the sequence.  The first tile writes it, which alone reads the old one; the
   // thread's own channels, so that no other reads what it has written.
   float last[W][V];
   if (state && p.tile == 0)
 #pragma unroll
     for (int j = 0; j < W - 1; ++j) input(last[j], p.len - (W - 1) + j);
-  for (int t = p.t0; t < p.t1; ++t) {
+  for (int t = p.t0; t < p.t1; t += G) {
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int e = 0; e < V; ++e) in[W - 1 + g][e] = t + g < p.len ? to_f32(next[g].v[e]) : 0.0f;
+    read(next, x, A.x_row, t + G, A.L);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float u = bias[e];
+#pragma unroll
+        for (int j = 0; j < W; ++j) u += w[j][e] * in[g + j][e];
+        o[e] = t + g >= p.len ? 0.0f : A.silu ? u * sigmoid(u) : u;
+      }
+      if (t + g < p.t1) store(y, o, p.skip);
+      y += A.D;
+    }
 #pragma unroll
     for (int j = 0; j < W - 1; ++j)
 #pragma unroll
-      for (int e = 0; e < V; ++e) before[j][e] = before[j + 1][e];
-    input(before[W - 1], t);
-    float o[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float u = bias[e];
-#pragma unroll
-      for (int j = 0; j < W; ++j) u += w[j][e] * before[j][e];
-      o[e] = t >= p.len ? 0.0f : A.silu ? u * sigmoid(u) : u;
-    }
-    store(y + (long)t * A.D, o, p.skip);
+      for (int e = 0; e < V; ++e) in[j][e] = in[G + j][e];
   }
   if (state && p.tile == 0)
 #pragma unroll
@@ -124,63 +153,76 @@ __global__ __launch_bounds__(256) void k_conv_fwd(const ConvArgs A) {
 
 template <typename T, int W, int V>
 __global__ __launch_bounds__(256) void k_conv_bwd(const ConvArgs A) {
+  constexpr int G = 4;
   Place p;
   if (!place<V>(A, p)) return;
   const T* x = (const T*)A.x + p.b * A.x_batch + p.c;
   const T* dy = (const T*)A.dy + (long)p.b * A.L * A.D + p.c;
   T* dx = A.dx ? (T*)A.dx + (long)p.b * A.L * A.D + p.c : nullptr;
-  float w[W][V], bias[V] = {}, before[W][V] = {}, du[W][V] = {}, dw[W][V] = {}, dbias[V] = {};
+  Vec<T, V> next_x[G], next_dy[G];
+  read(next_x, x, A.x_row, p.t0, A.L);
+  read(next_dy, dy, A.D, p.t0, A.L);
+  // in, du: those of a group of steps behind those of the W - 1 steps before it
+  float w[W][V], bias[V] = {}, in[W - 1 + G][V] = {}, du[W - 1 + G][V] = {}, dw[W][V] = {}, dbias[V] = {};
 #pragma unroll
   for (int e = 0; e < V; ++e)
 #pragma unroll
     for (int j = 0; j < W; ++j) w[j][e] = to_f32(((const T*)A.w)[(long)(p.c + e) * W + j]);
   if (A.bias) load(bias, (const T*)A.bias + p.c);
-  auto input = [&](float (&o)[V], int t) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) o[e] = 0.0f;
-    if (t >= 0 && t < p.len) load(o, x + (long)t * A.x_row);
-  };
-#pragma unroll
-  for (int j = 1; j < W; ++j) input(before[j], p.t0 - W + j);
+  for (int j = 0; j < W - 1; ++j) {
+    const int t = p.t0 - (W - 1) + j;
+    if (t >= 0 && t < p.len) load(in[j], x + (long)t * A.x_row);
+  }
   // dx[t] needs du up to t + W - 1: the walk goes W - 1 steps beyond the tile, whose du the next tile adds up
-  for (int t = p.t0; t < p.t1 + W - 1; ++t) {
+  for (int t = p.t0; t < p.t1 + W - 1; t += G) {
+    float d[G][V];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        in[W - 1 + g][e] = t + g < p.len ? to_f32(next_x[g].v[e]) : 0.0f;
+        d[g][e] = t + g < p.len ? to_f32(next_dy[g].v[e]) : 0.0f;
+      }
+    read(next_x, x, A.x_row, t + G, A.L);
+    read(next_dy, dy, A.D, t + G, A.L);
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        float u = bias[e], slope = 1.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) u += w[j][e] * in[g + j][e];
+        if (A.silu) {
+          const float s = sigmoid(u);
+          slope = s * (1.0f + u * (1.0f - s));
+        }
+        const float v = t + g < p.len ? d[g][e] * slope : 0.0f, mine = t + g < p.t1 ? v : 0.0f;
+        du[W - 1 + g][e] = v;
+        dbias[e] += mine;
+#pragma unroll
+        for (int j = 0; j < W; ++j) dw[j][e] += mine * in[g + j][e];
+      }
+      const int to = t + g - (W - 1);  // du[g + j] is that of step to + j
+      if (dx && to >= p.t0 && to < p.t1) {
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          o[e] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < W; ++j) o[e] += w[W - 1 - j][e] * du[g + j][e];
+          if (to >= p.len) o[e] = 0.0f;
+        }
+        store(dx + (long)to * A.D, o, p.skip);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < W - 1; ++j)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        before[j][e] = before[j + 1][e];
-        du[j][e] = du[j + 1][e];
+        in[j][e] = in[G + j][e];
+        du[j][e] = du[G + j][e];
       }
-    input(before[W - 1], t);
-    float d[V] = {};
-    if (t < p.len) load(d, dy + (long)t * A.D);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float u = bias[e], g = 1.0f;
-#pragma unroll
-      for (int j = 0; j < W; ++j) u += w[j][e] * before[j][e];
-      if (A.silu) {
-        const float s = sigmoid(u);
-        g = s * (1.0f + u * (1.0f - s));
-      }
-      du[W - 1][e] = t < p.len ? d[e] * g : 0.0f;
-      if (t < p.t1) {
-        dbias[e] += du[W - 1][e];
-#pragma unroll
-        for (int j = 0; j < W; ++j) dw[j][e] += du[W - 1][e] * before[j][e];
-      }
-    }
-    if (dx && t - (W - 1) >= p.t0) {  // du[j] is that of step t - (W - 1) + j
-      float o[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        o[e] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < W; ++j) o[e] += w[W - 1 - j][e] * du[j][e];
-        if (t - (W - 1) >= p.len) o[e] = 0.0f;
-      }
-      store(dx + (long)(t - (W - 1)) * A.D, o, p.skip);
-    }
   }
   if (!A.part) return;
   float* part = A.part + ((long)p.b * A.tiles + p.tile) * (W + 1) * A.D + p.c;
@@ -215,11 +257,10 @@ struct ConvPlan {
   int tile, tiles, v, vecs;
   long threads;
 };
-// v: channels of a thread, of 16 bytes an access (backward, whose windows are as many again: of 8 in 16 bits).
-ConvPlan plan_conv(int esize, int B, int L, int D, bool backward) {
+// v: channels of a thread.
+ConvPlan plan_conv(int B, int L, int D) {
   ConvPlan p{};
-  p.v = esize == 4 || backward ? 4 : 8;
-  if (D < p.v) p.v = 1;
+  p.v = D < 4 ? 1 : 4;
   p.vecs = (D + p.v - 1) / p.v;
   p.tile = 64;
   while (p.tile > 8 && (long)B * ((L + p.tile - 1) / p.tile) * p.vecs < 256L * 256) p.tile /= 2;
@@ -233,7 +274,7 @@ int check_conv(int dtype, int B, int L, int D, int W) {
   if (B < 0 || L < 0 || D <= 0) return kans_fail(KANS_ERR_ARG, "bad dims B=%d L=%d D=%d", B, L, D);
   if (W < 1 || W > kMaxTaps) return kans_fail(KANS_ERR_UNSUPPORTED, "%d taps, 1 to %d", W, kMaxTaps);
   // (a grid holds fewer than 2^32 threads along x)
-  if (L > (1 << 30) || plan_conv(4, B, L, D, true).threads >= 1L << 31)
+  if (L > (1 << 30) || plan_conv(B, L, D).threads >= 1L << 31)
     return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
   return 0;
 }
@@ -256,8 +297,7 @@ hipError_t by_conv(int dtype, int W, int v, F f) {
   };
   auto widths = [&](auto t) {
     if (v == 1) taps(t, std::integral_constant<int, 1>{});
-    else if (v == 4) taps(t, std::integral_constant<int, 4>{});
-    else if constexpr (sizeof(t) == 2) taps(t, std::integral_constant<int, 8>{});
+    else taps(t, std::integral_constant<int, 4>{});
   };
   if (dtype == DT_F32) widths(0.0f);
   else if (dtype == DT_F16) widths((_Float16)0.0f);
@@ -279,7 +319,7 @@ int kans_causal_conv_forward(int dtype, const void* x, long x_batch, long x_row,
   if (!x || !w || !y) return kans_fail(KANS_ERR_ARG, "null argument");
   std::lock_guard<std::mutex> lk(kans_mutex());
   if ((rc = kans_ensure_init())) return rc;
-  const ConvPlan p = plan_conv(dtype == DT_F32 ? 4 : 2, B, L, D, false);
+  const ConvPlan p = plan_conv(B, L, D);
   ConvArgs A{};
   A.x = x; A.w = w; A.bias = bias; A.y = y; A.state = W > 1 ? state : nullptr; A.lengths = lengths; A.silu = silu;
   A.x_batch = x_batch; A.x_row = x_row; A.B = B; A.L = L; A.D = D; A.tile = p.tile; A.tiles = p.tiles; A.vecs = p.vecs;
@@ -294,7 +334,7 @@ int kans_causal_conv_forward(int dtype, const void* x, long x_batch, long x_row,
 long kans_causal_conv_workspace(int dtype, int B, int L, int D, int W) {
   const int rc = check_conv(dtype, B, L, D, W);
   if (rc) return rc;
-  const ConvPlan p = plan_conv(dtype == DT_F32 ? 4 : 2, B, L, D, true);
+  const ConvPlan p = plan_conv(B, L, D);
   return (long)B * p.tiles * (W + 1) * D * (long)sizeof(float);
 }
 
@@ -306,7 +346,7 @@ int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row
   const bool any = B > 0 && L > 0;
   if (any && (!x || !w || !dy)) return kans_fail(KANS_ERR_ARG, "null argument");
   if (dbias && !bias) return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
-  const ConvPlan p = plan_conv(dtype == DT_F32 ? 4 : 2, B, L, D, true);
+  const ConvPlan p = plan_conv(B, L, D);
   const long rows = (long)B * p.tiles, need = rows * (W + 1) * D * (long)sizeof(float);
   const bool sums = dw || dbias;
   if (sums && need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
@@ -320,8 +360,7 @@ int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row
     A.part = sums ? (float*)workspace : nullptr;
     A.x_batch = x_batch; A.x_row = x_row; A.B = B; A.L = L; A.D = D; A.tile = p.tile; A.tiles = p.tiles; A.vecs = p.vecs;
     HIP_TRY(by_conv(dtype, W, p.v, [&](auto t, auto taps, auto vec) {
-      if constexpr (decltype(vec)::value <= 4)
-        hipLaunchKernelGGL((k_conv_bwd<decltype(t), decltype(taps)::value, decltype(vec)::value>), dim3((unsigned)((p.threads + 255) / 256)),
+      hipLaunchKernelGGL((k_conv_bwd<decltype(t), decltype(taps)::value, decltype(vec)::value>), dim3((unsigned)((p.threads + 255) / 256)),
                            dim3(256), 0, st, A);
       return hipGetLastError();
     }));

@@ -28,19 +28,29 @@ namespace kans {
 namespace {
 
 // Per chunk in order (backward: from the last), edge becomes what comes into it: H, then H exp(A sum s) + edge.
-__global__ __launch_bounds__(256) void k_scan_join(const ScanArgs A, int padded, bool backward) {
-  const long at = (long)blockIdx.x * 256 + threadIdx.x, states = (long)A.D * A.N;
+__global__ __launch_bounds__(64) void k_scan_join(const ScanArgs A, int padded, bool backward) {
+  const long at = (long)blockIdx.x * 64 + threadIdx.x, states = (long)A.D * A.N;
   if (at >= A.B * states) return;
   const long b = at / states, in = at - b * states, d = in / A.N, to = d * padded + (in - d * A.N);
   const float a2 = A.A[in] * 1.44269504088896340736f;
   float h = !backward && A.state ? A.state[at] : 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < A.chunks; ++i) {
-    const long place = b * A.chunks + (backward ? A.chunks - 1 - i : i);
-    float* edge = A.edge + place * A.D * padded + to;
-    const float e = *edge, s = A.sums[place * A.D + d];
-    *edge = h;
-    h = __builtin_amdgcn_exp2f(a2 * s) * h + e;
+  constexpr int kAhead = 16;  // chunks whose values are under way together
+  for (int first = 0; first < A.chunks; first += kAhead) {
+    float e[kAhead], s[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int in_order = min(first + i, A.chunks - 1);
+      const long place = b * A.chunks + (backward ? A.chunks - 1 - in_order : in_order);
+      e[i] = A.edge[place * A.D * padded + to];
+      s[i] = A.sums[place * A.D + d];
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (first + i >= A.chunks) break;
+      const long place = b * A.chunks + (backward ? A.chunks - 1 - first - i : first + i);
+      A.edge[place * A.D * padded + to] = h;
+      h = __builtin_amdgcn_exp2f(a2 * s[i]) * h + e[i];
+    }
   }
 }
 
@@ -67,8 +77,14 @@ hipError_t launch(int dtype, ScanPass pass, const ScanArgs& A, hipStream_t st) {
 }
 
 constexpr int kMaxStates = 64, kMinChunk = 64;
-constexpr long kEnoughWaves = 1024, kWantedWaves = 2048;
+constexpr long kEnoughWaves = 1024, kWantedWaves = 4096;
 
+// Chunks of a sequence where its waves do not give every SIMD one: four for each, eight if the chunks keep 128 steps.  us, bf16,
+// 16 states, forward and both directions, one chunk | two | four | eight waves a SIMD:
+//   1 x 8192 x 1024   869  3276 |  94 290 |  88 275 |  96 294
+//   2 x 8192 x 4096   978  3484 |         | 502 1735 | 471 1661
+//   3 x 777 x 1300    140   455 |  71 213 |  63 185 |  62 183  (24 states)
+//   16 x 1000 x 1500  158   660 |         | 201  720 | 186  686  (1536 waves: whole)
 struct ScanPlan {
   int blocks, chunk, chunks, interval, padded;
   long edges;                        // floats of the chunks' edges and sums
@@ -83,7 +99,8 @@ ScanPlan plan_scan(int B, int L, int D, int N) {
   const long waves = 4L * p.blocks * std::max(B, 1);
   p.chunk = std::max(L, 1);
   if (waves < kEnoughWaves && L >= 2 * kMinChunk) {
-    const long want = std::min((kWantedWaves + waves - 1) / waves, (long)L / kMinChunk);
+    const long four = (kWantedWaves + waves - 1) / waves;
+    const long want = std::min(std::max(four, std::min(2 * four, (long)L / (2 * kMinChunk))), (long)L / kMinChunk);
     p.chunk = (int)(((L + want - 1) / want + 15) & ~15L);
   }
   p.chunks = std::max(1, (L + p.chunk - 1) / p.chunk);
@@ -167,7 +184,7 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
     S.edge = (float*)workspace;
     S.sums = S.edge + (long)B * p.chunks * D * p.padded;
     HIP_TRY(launch(dtype, ScanPass::kEdges, S, st));
-    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, p.padded, false);
+    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 63) / 64)), dim3(64), 0, st, S, p.padded, false);
     HIP_TRY(hipGetLastError());
   }
   HIP_TRY(launch(dtype, ScanPass::kForward, S, st));
@@ -204,7 +221,7 @@ int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_
   if (any) {
     if (p.chunks > 1) {
       HIP_TRY(launch(dtype, ScanPass::kBackwardEdges, S, st));
-      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 255) / 256)), dim3(256), 0, st, S, p.padded, true);
+      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 63) / 64)), dim3(64), 0, st, S, p.padded, true);
       HIP_TRY(hipGetLastError());
     }
     HIP_TRY(launch(dtype, ScanPass::kBackward, S, st));

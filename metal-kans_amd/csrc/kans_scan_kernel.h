@@ -27,14 +27,26 @@ __device__ __forceinline__ float quad_sum(float v) {
   v += dpp<0xb1>(v);
   return v + dpp<0x4e>(v);
 }
-// Lane q of the quad gets the quad's sum of v[q].
-__device__ __forceinline__ float quad_sums(const float (&v)[4]) {
-  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
-  const float v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
-  const float a = (odd ? v1 : v0) + dpp<0xb1>(odd ? v0 : v1);
-  const float b = (odd ? v3 : v2) + dpp<0xb1>(odd ? v2 : v3);
-  return (high ? b : a) + dpp<0x4e>(high ? a : b);
-}
+typedef float Acc __attribute__((ext_vector_type(4)));
+
+// Lane q of the quad gets the quad's sum of v[q].  A 4 x 4 x 1 product for each quad by itself: times a column that is 1 in lane
+// k, step k's values of the four lanes go to lane k.
+struct QuadSums {
+  float one[4];
+  __device__ __forceinline__ QuadSums() {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      one[k] = (threadIdx.x & 3) == k ? 1.0f : 0.0f;
+      asm volatile("" : "+v"(one[k]));  // (a register each, not computed again at every use)
+    }
+  }
+  template <int K>
+  __device__ __forceinline__ static void add(Acc& acc, const QuadSums& s, float v, bool first) {
+    acc = __builtin_amdgcn_mfma_f32_4x4x1f32(v, s.one[K], first ? Acc{0.0f, 0.0f, 0.0f, 0.0f} : acc, 0, 0, 0);
+  }
+  __device__ __forceinline__ static float sum(const Acc& acc) { return (acc.x + acc.y) + (acc.z + acc.w); }
+};
+
 // Lane l gets the sum of v[l / 4] over the 16 lanes with its place in the quad.
 typedef unsigned Pair __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float sum_of(Pair v) {
@@ -291,6 +303,15 @@ __device__ __forceinline__ float here(float v) {
   return v;
 }
 
+// Where a grid has no more than two workgroups a CU, the two waves of a SIMD come first by turns.  The older one always came first,
+// was done early and left the other alone, which cannot use all cycles: forward of bf16 8 x 2048 x 4096 386 -> 359 us.
+// (Larger grids fill the places themselves: 3 % slower with turns.)  Workgroups go over the card's 256 CUs in order.
+__device__ __forceinline__ void take_turns(int tile) {
+  if (gridDim.x > 512) return;
+  if ((tile ^ (int)(blockIdx.x >> 8)) & 1) __builtin_amdgcn_s_setprio(1);
+  else __builtin_amdgcn_s_setprio(0);
+}
+
 // ---- forward ------------------------------------------------------------------------------------------
 // kEdges: of each chunk alone, from a state of zeros, its last state and the sum of its step sizes.
 template <typename T, int kRegs, bool kEdges, bool kGated>
@@ -315,6 +336,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     for (int i = 0; i < kRegs; ++i)
       if (l.q * kRegs + i < A.N) h[i] = state[l.q * kRegs + i];
   float total = 0.0f;
+  const QuadSums quad;
   const float* saved = A.saved + ((l.b * (long)((A.L + kInterval - 1) / kInterval) + l.t0 / kInterval) * A.D + l.c0) * kPad;
   const int saved_bytes = A.saved ? min(A.D - l.c0, kScanChannels) * kPad * 4 : 0;
 
@@ -334,6 +356,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   rows.write(bc[0]);
   __syncthreads();
   for (int t = l.t0, turn = 0; t < l.t1; t += kTile, turn ^= 1) {
+    take_turns(t / kTile);
     float s[kM], u[kM], xs[kM], gate[kM];
     const int left = l.len - t - l.q;
 #pragma unroll
@@ -353,7 +376,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     const float* lds = bc[turn] + l.q * kRegs;
     Ahead<kRegs, kAhead, true, !kEdges> ahead;
     ahead.read(lds, 0);
-    float y[4];
+    Acc y;
     static_for<0, kTile / kAhead>([&](auto g_) {
       constexpr int g = decltype(g_)::value;
       const Ahead<kRegs, kAhead, true, !kEdges> now = ahead;
@@ -370,9 +393,9 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
           h[i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]) * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i];
           if (!kEdges) sum += h[i] * now.C[j - g * kAhead][i];
         }
-        y[k] = sum;
+        if (!kEdges) QuadSums::template add<k>(y, quad, sum, k == 0);
         if constexpr (!kEdges && k == 3) {
-          const float o = (quad_sums(y) + skip * xs[m]) * gate[m];  // (outside the condition: all lanes of the quad take part)
+          const float o = (QuadSums::sum(y) + skip * xs[m]) * gate[m];  // (outside the condition: all lanes of the quad take part)
           out.write(to, m, 4 * m < left ? o : 0.0f);
         }
       });
@@ -415,6 +438,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) carry[i] = 0.0f;
   if (!kEdges && A.chunks > 1) fetch_states<kRegs>(carry, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
+  const QuadSums quad;
   const float* saved = A.saved + ((l.b * (long)((A.L + kTile - 1) / kTile) + last / kTile) * A.D + l.c0) * kPad;
   const int saved_bytes = min(A.D - l.c0, kScanChannels) * kPad * 4;
 
@@ -440,6 +464,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   __syncthreads();
   for (int tile = tiles - 1, turn = 0; tile >= 0; --tile, turn ^= 1) {
     const int t = l.t0 + tile * kTile;
+    take_turns(tile);
     // dzs: dout times silu's slope, slope: the step size's
     float s[kM], u[kM], xs[kM], dy[kM], dzs[kM], slope[kM], h[kRegs];
     const int left = l.on ? l.len - t - l.q : 0;
@@ -469,7 +494,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     {
       Ahead<kRegs, kAhead, !kEdges, !kEdges && kGated> ahead;
       ahead.read(lds, 0);
-      float y[4];
+      Acc y;
       static_for<0, kTile / kAhead>([&](auto g_) {
         constexpr int g = decltype(g_)::value;
         const Ahead<kRegs, kAhead, !kEdges, !kEdges && kGated> now = ahead;
@@ -486,15 +511,17 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
               if (kGated) sum += h[i] * now.C[j - g * kAhead][i];
             }
           }
-          y[k] = sum;
+          if (!kEdges && kGated) QuadSums::template add<k>(y, quad, sum, k == 0);
+          if constexpr (!kEdges && k == 3) __builtin_amdgcn_sched_barrier(0);  // (nothing moves over four steps: no registers for it)
           if constexpr (!kEdges && kGated && k == 3) {
-            const float o = dzs[m] * (quad_sums(y) + skip * xs[m]);
+            const float o = dzs[m] * (QuadSums::sum(y) + skip * xs[m]);
             dz.write(to_dz, m, 4 * m < left ? o : 0.0f);
           }
         });
       });
     }
-    float vals[16], dA_tile[kRegs] = {}, yB[4], yA[4];
+    float vals[16], dA_tile[kRegs] = {};
+    Acc of_b, of_a;
     Ahead<kRegs, kAhead, !kEdges, true> ahead;
     ahead.read(lds, kTile - kAhead);
     static_for<0, kTile / kAhead>([&](auto g_) {
@@ -518,8 +545,8 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           }
         }
         if constexpr (!kEdges) {
-          yB[k] = sB;
-          yA[k] = sA;
+          QuadSums::template add<k>(of_b, quad, sB, k == 3);
+          QuadSums::template add<k>(of_a, quad, sA, k == 3);
           static_for<0, 2 * kRegs>([&](auto i_) {
             constexpr int i = decltype(i_)::value, value = (kTile - 1 - j) * 2 * kRegs + i;
             vals[value % 16] = i < kRegs ? gr[i % kRegs] * of_lane<k>(u[m]) : h[i % kRegs] * of_lane<k>(dy[m]);
@@ -527,8 +554,9 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           });
 #pragma unroll
           for (int i = 0; i < kRegs; ++i) h[i] = before[j][i];
+          if constexpr (k == 0) __builtin_amdgcn_sched_barrier(0);
           if constexpr (k == 0) {
-            const float gB = quad_sums(yB), gA = quad_sums(yA) * kLn2;
+            const float gB = QuadSums::sum(of_b), gA = QuadSums::sum(of_a) * kLn2;
             const bool counts = 4 * m < left;
             const float ddtv = counts ? (xs[m] * gB + gA) * slope[m] : 0.0f;
             dskip += dy[m] * xs[m];

@@ -47,28 +47,53 @@ struct QuadSums {
   __device__ __forceinline__ static float sum(const Acc& acc) { return (acc.x + acc.y) + (acc.z + acc.w); }
 };
 
-// Lane l gets the sum of v[l / 4] over the 16 lanes with its place in the quad.
+// The backward's lanes hold their states in mirrored order in every other quad: lane q of an odd one those of 3 - q, so that a lane's
+// partner in a mirrored row, or half of a row, holds the same states.
+__device__ __forceinline__ int states_of(int lane) { return lane & 4 ? 3 - (lane & 3) : lane & 3; }
+
+// The sums of 16 values over the 16 lanes with the same states: lane l gets that of value 8 b3 + 4 b2 + 2 b4 + b5, b its bits.  Half of the lanes that are added
+// take one value of a pair, half the other: sums with the mirrored row (and half row) are written to some banks of four lanes
+// only, two instructions a pair; the rows meet by swaps.  33 cycles of four for 16 values, by swaps and selections alone 47.
 typedef unsigned Pair __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float sum_of(Pair v) {
   const unsigned a = v.x, b = v.y;  // (a bit cast of v.y itself takes v.x)
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
 __device__ __forceinline__ float wave_sums(float (&v)[16]) {
+  // (a lane permute reads what is at least two instructions old, and five behind a change of the lanes that are on)
+  asm("s_nop 4\n"
+      "v_add_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %1, %1, %1 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %2, %2, %2 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %3, %3, %3 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %4, %4, %4 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %5, %5, %5 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %6, %6, %6 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %7, %7, %7 row_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %0, %8, %8 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %1, %9, %9 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %2, %10, %10 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %3, %11, %11 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %4, %12, %12 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %5, %13, %13 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %6, %14, %14 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %7, %15, %15 row_mirror row_mask:0xf bank_mask:0xc\n"
+      "v_add_f32_dpp %0, %0, %0 row_half_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %1, %1, %1 row_half_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %2, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %3, %3, %3 row_half_mirror row_mask:0xf bank_mask:0xf\n"
+      "v_add_f32_dpp %0, %4, %4 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+      "v_add_f32_dpp %1, %5, %5 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+      "v_add_f32_dpp %2, %6, %6 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+      "v_add_f32_dpp %3, %7, %7 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+      "s_nop 1"
+      : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7])
+      : "v"(v[8]), "v"(v[9]), "v"(v[10]), "v"(v[11]), "v"(v[12]), "v"(v[13]), "v"(v[14]), "v"(v[15]));
   auto bits = [](float f) { return __builtin_bit_cast(unsigned, f); };
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    v[i] = sum_of(__builtin_bit_cast(Pair, __builtin_amdgcn_permlane32_swap(bits(v[i]), bits(v[i + 8]), false, false)));
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    v[i] = sum_of(__builtin_bit_cast(Pair, __builtin_amdgcn_permlane16_swap(bits(v[i]), bits(v[i + 4]), false, false)));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[i] += dpp<0x128>(v[i]);  // 8 lanes on in the row
-    v[i] += dpp<0x124>(v[i]);  // 4 lanes on
-  }
-  const bool b2 = threadIdx.x & 4, b3 = threadIdx.x & 8;
-  const float v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3], low = b2 ? v1 : v0, high = b2 ? v3 : v2;
-  return b3 ? high : low;
+  for (int i = 0; i < 2; ++i)
+    v[i] = sum_of(__builtin_bit_cast(Pair, __builtin_amdgcn_permlane16_swap(bits(v[i]), bits(v[i + 2]), false, false)));
+  return sum_of(__builtin_bit_cast(Pair, __builtin_amdgcn_permlane32_swap(bits(v[0]), bits(v[1]), false, false)));
 }
 
 __device__ __forceinline__ float exp_neg(float v) { return __builtin_amdgcn_exp2f(v * -kLog2e); }
@@ -289,10 +314,10 @@ struct Ahead {
 
 // A lane's A log2(e).
 template <int kRegs>
-__device__ __forceinline__ void load_decays(float (&a2)[kRegs], const ScanArgs& A, const Lane& l) {
+__device__ __forceinline__ void load_decays(float (&a2)[kRegs], const ScanArgs& A, const Lane& l, int group) {
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
-    const int n = l.q * kRegs + i;
+    const int n = group * kRegs + i;
     a2[i] = n < A.N ? A.A[(long)l.row * A.N + n] * kLog2e : 0.0f;
   }
 }
@@ -325,7 +350,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], h[kRegs];
-  load_decays<kRegs>(a2, A, l);
+  load_decays<kRegs>(a2, A, l, l.q);
   const long place = (long)l.b * A.chunks + l.chunk;
   float* state = A.state ? A.state + ((long)l.b * A.D + l.row) * A.N : nullptr;
 #pragma unroll
@@ -431,9 +456,10 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, last, A.D, false), dout(A.dout, full, A.D, l, last, A.D, false);
   Steps<T, kTile> dx(A.dx, full, A.D, l, last, A.D, true), ddt(A.ddt, full, A.D, l, last, A.D, true), dz(A.dz, full, A.D, l, last, A.D, true);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
-  const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
+  const int group = states_of(threadIdx.x);  // of the lane's states
+  const unsigned mine = (unsigned)(l.in * kPad + group * kRegs) * 4;
   float a2[kRegs], carry[kRegs], dA[kRegs] = {}, dskip = 0.0f, dbias = 0.0f, total = 0.0f;
-  load_decays<kRegs>(a2, A, l);
+  load_decays<kRegs>(a2, A, l, group);
   const long place = (long)l.b * A.chunks + l.chunk;
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) carry[i] = 0.0f;
@@ -488,7 +514,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) h[i] = first[i];
     const Buffer to_dx = dx.steps(A.L - t), to_ddt = ddt.steps(A.L - t), to_dz = dz.steps(kGated ? A.L - t : 0);
-    const float* lds = bc[turn] + l.q * kRegs;
+    const float* lds = bc[turn] + group * kRegs;
     // the states of the tile again: before each step, and what the step leaves of them
     float before[kEdges ? 1 : kTile][kRegs], stay[kTile][kRegs];
     {
@@ -583,7 +609,9 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
         const int at = i * kThreads + (int)threadIdx.x;
         if (at >= there) break;
         const int j = at / (2 * kPad), which = at / kPad & 1, n = at % kPad;
-        const int value = (kTile - 1 - j) * 2 * kRegs + which * kRegs + n % kRegs, from = value / 16 * 64 + value % 16 * 4 + n / kRegs;
+        const int value = (kTile - 1 - j) * 2 * kRegs + which * kRegs + n % kRegs, v = value % 16, odd = v >> 2 & 1;
+        // (where wave_sums leaves it)
+        const int lane = (v & 8) + (v & 4) + (v & 2) * 8 + (v & 1) * 32 + (odd ? 3 - n / kRegs : n / kRegs), from = value / 16 * 64 + lane;
         part[at] = (red[turn][0][from] + red[turn][1][from]) + (red[turn][2][from] + red[turn][3][from]);
       }
     }
@@ -600,7 +628,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   if (!l.on) return;
 #pragma unroll
   for (int i = 0; i < kRegs; ++i)
-    if (l.q * kRegs + i < A.N) par[l.q * kRegs + i] = dA[i];
+    if (group * kRegs + i < A.N) par[group * kRegs + i] = dA[i];
   if (l.q == 0) {
     par[A.N] = dskip;
     par[A.N + 1] = dbias;

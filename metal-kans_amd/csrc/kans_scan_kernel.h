@@ -53,7 +53,8 @@ __device__ __forceinline__ int states_of(int lane) { return lane & 4 ? 3 - (lane
 
 // The sums of 16 values over the 16 lanes with the same states: lane l gets that of value 8 b3 + 4 b2 + 2 b4 + b5, b its bits.  Half of the lanes that are added
 // take one value of a pair, half the other: sums with the mirrored row (and half row) are written to some banks of four lanes
-// only, two instructions a pair; the rows meet by swaps.  33 cycles of four for 16 values, by swaps and selections alone 47.
+// only, two instructions a pair; the rows meet by swaps.  33 issue slots for 16 values, 47 by swaps and selections alone (a swap
+// takes two).  On the matrix pipe, 16 products of 16 x 16 x 4 in a chain, the backward took twice as long.
 typedef unsigned Pair __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float sum_of(Pair v) {
   const unsigned a = v.x, b = v.y;  // (a bit cast of v.y itself takes v.x)

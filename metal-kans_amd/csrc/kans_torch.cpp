@@ -537,7 +537,7 @@ struct Conv {
 
   Tensor forward(const Tensor& state) const {
     Tensor y = at::empty(x.sizes(), x.options());
-    check(lib.conv_forward(type(), data(x), x.stride(0), x.stride(1), data(w), data(bias), data(state), (const int64_t*)data(lengths),
+    check(lib.conv_forward(type(), data(x), stride(x, 0), stride(x, 1), data(w), data(bias), data(state), (const int64_t*)data(lengths),
                            silu, data(y), B(), L(), D(), W(), stream_of(x)),
           "kans_causal_conv_forward");
     return y;
@@ -549,7 +549,7 @@ struct Conv {
     const long size = lib.conv_workspace(type(), B(), L(), D(), W());
     check(size, "kans_causal_conv_workspace");
     const Tensor ws = need[1] || need[2] ? bytes(x, size) : Tensor();
-    check(lib.conv_backward(type(), data(x), x.stride(0), x.stride(1), data(w), data(bias), (const int64_t*)data(lengths), silu, data(dy),
+    check(lib.conv_backward(type(), data(x), stride(x, 0), stride(x, 1), data(w), data(bias), (const int64_t*)data(lengths), silu, data(dy),
                             data(dx), data(dw), data(dbias), B(), L(), D(), W(), data(ws), size, stream_of(x)),
           "kans_causal_conv_backward");
     return {dx, dw, dbias};
@@ -612,6 +612,11 @@ std::optional<Tensor> causal_conv(const Tensor& x, const Tensor& w, const std::o
 }
 
 // ---- selective_scan --------------------------------------------------------------------------------
+// (the scan's kernels take fewer than 2^23 elements between steps)
+Tensor with_steps(const Tensor& t) {
+  return (t.size(2) == 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) < 1 << 23) ? t : t.contiguous();
+}
+
 struct Scan {
   Tensor x, dt, A, B, C, skip, z, bias, lengths;  // (undefined: not given)
   bool softplus;
@@ -621,7 +626,8 @@ struct Scan {
   int d() const { return (int)x.size(2); }
   int n() const { return (int)A.size(1); }
   int type() const { return type_of(x.scalar_type()); }
-  static long stride(const Tensor& t, int i) { return t.defined() ? t.stride(i) : 0; }
+  // (of a single step or sequence there is none: it may be anything)
+  static long stride(const Tensor& t, int i) { return t.defined() && t.size(i) > 1 ? t.stride(i) : 0; }
   Tensor workspace(int backward) const {
     const long size = lib.scan_workspace(b(), l(), d(), n(), backward);
     check(size, "kans_selective_scan_workspace");
@@ -636,8 +642,8 @@ struct Scan {
       saved = at::empty({size / 4}, x.options().dtype(at::kFloat));
     }
     const Tensor ws = workspace(0);
-    check(lib.scan_forward(type(), data(x), x.stride(0), x.stride(1), data(dt), dt.stride(0), dt.stride(1), (const float*)data(A), data(B),
-                           B.stride(0), B.stride(1), data(C), C.stride(0), C.stride(1), (const float*)data(skip), data(z), stride(z, 0),
+    check(lib.scan_forward(type(), data(x), stride(x, 0), stride(x, 1), data(dt), stride(dt, 0), stride(dt, 1), (const float*)data(A), data(B),
+                           stride(B, 0), stride(B, 1), data(C), stride(C, 0), stride(C, 1), (const float*)data(skip), data(z), stride(z, 0),
                            stride(z, 1), (const float*)data(bias), softplus, (float*)data(state), (const int64_t*)data(lengths), data(out),
                            (float*)data(saved), b(), l(), d(), n(), data(ws), ws.numel(), stream_of(x)),
           "kans_selective_scan_forward");
@@ -651,8 +657,8 @@ struct Scan {
     Tensor dx = like(x, true), ddt = like(dt, true), dA = like(A, need[2]), dB = like(B, need[3]), dC = like(C, need[4]),
            dskip = like(skip, need[5]), dz = like(z, z.defined()), dbias = like(bias, need[7]);
     const Tensor ws = workspace(1);
-    check(lib.scan_backward(type(), data(x), x.stride(0), x.stride(1), data(dt), dt.stride(0), dt.stride(1), (const float*)data(A), data(B),
-                            B.stride(0), B.stride(1), data(C), C.stride(0), C.stride(1), (const float*)data(skip), data(z), stride(z, 0),
+    check(lib.scan_backward(type(), data(x), stride(x, 0), stride(x, 1), data(dt), stride(dt, 0), stride(dt, 1), (const float*)data(A), data(B),
+                            stride(B, 0), stride(B, 1), data(C), stride(C, 0), stride(C, 1), (const float*)data(skip), data(z), stride(z, 0),
                             stride(z, 1), (const float*)data(bias), softplus, (const int64_t*)data(lengths), (const float*)data(saved),
                             data(dout), data(dx), data(ddt), (float*)data(dA), data(dB), data(dC), (float*)data(dskip), data(dz),
                             (float*)data(dbias), b(), l(), d(), n(), data(ws), ws.numel(), stream_of(x)),
@@ -711,8 +717,8 @@ std::optional<Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Te
                 state->size(1) != x.size(2) || state->size(2) != A.size(1) || (uintptr_t)state->data_ptr() % 16))
     return {};
   TORCH_CHECK_VALUE(sizes_fit_int(x), "x has a size of more than 2^31");
-  Scan s{with_channels(x), with_channels(dt), A.contiguous(), with_channels(B), with_channels(C), contiguous(skip),
-         z ? with_channels(*z) : Tensor(), contiguous(bias), contiguous(lengths), softplus};
+  Scan s{with_steps(x), with_steps(dt), A.contiguous(), with_steps(B), with_steps(C), contiguous(skip),
+         z ? with_steps(*z) : Tensor(), contiguous(bias), contiguous(lengths), softplus};
   if ((uintptr_t)s.A.data_ptr() % 16) s.A = s.A.clone();
   no_tangents({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias}, "selective_scan");
   const at::OptionalDeviceGuard device(x.device());

@@ -221,6 +221,22 @@ def test_extreme_steps(cuda):
     check(s)
 
 
+def test_growing_states_in_chunks(cuda):
+    """A chunk may multiply a state by more than fp32 holds where there is none yet, or a small one: 700 steps of one,
+    growing by up to 2^115 in a chunk (of 48 steps and more), inputs at the end and output gradients at the beginning only."""
+    s = inputs(1, 700, 40, 16, torch.float32, without=("dt_bias", "z"))
+    s["dt"] = torch.full_like(s["dt"], 1.0)
+    s["A"] = s["A"].abs().clamp(max=1.6)
+    s["x"][:, :690] = 0.0
+    s["dout"][:, 10:] = 0.0
+    check(s, softplus=False)
+    s["A"][::2] = -1.0
+    s["x"].fill_(1e-20)
+    s["state"].fill_(1e-35)
+    s["lengths"] = torch.tensor([650], device="cuda")
+    check(s, softplus=False)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_masked_places_are_not_looked_at(cuda, dt):
     s = inputs(3, 150, 19, 16, dt, lengths=[0, 20, 150])
@@ -295,6 +311,27 @@ def test_orders_of_memory(cuda):
                 one = {k: v[:, 7:8] if k in ("x", "dt", "B", "C", "z") else v for k, v in m.items()}
                 same = {k: v[:, 7:8].contiguous() if k in ("x", "dt", "B", "C", "z") else v for k, v in s.items()}
                 assert torch.equal(call(one, state=state), call(same, state=other)) and torch.equal(state, other)
+
+
+def test_far_steps(cuda):
+    """Steps 2^23 elements and more apart, batches that repeat, and single steps whose strides mean nothing."""
+    s = inputs(1, 3, 24, 16, torch.float16)
+    want = train(s)
+    far = {}
+    for k in ("x", "dt", "B", "C", "z"):
+        space = torch.zeros(3 << 23, device="cuda", dtype=torch.float16)
+        far[k] = space.as_strided((1, 3, s[k].shape[2]), (1, 1 << 23, 1))
+        far[k].copy_(s[k])
+    got = train({**s, **far})
+    assert all(torch.equal(got[k], want[k]) for k in want)
+    two = {k: v.expand(2, *v.shape[1:]) if k in ("x", "dt", "B", "C", "z") else v for k, v in s.items()}
+    with torch.no_grad():
+        assert torch.equal(call(two), want["out"].expand(2, 3, 24))
+        one = {k: v[:, 1:2].as_strided((1, 1, v.shape[2]), (0, 1 << 40, 1), v[:, 1:2].storage_offset())
+               if k in ("x", "dt", "B", "C", "z") else v for k, v in s.items()}
+        same = {k: v[:, 1:2].contiguous() if k in ("x", "dt", "B", "C", "z") else v for k, v in s.items()}
+        assert torch.equal(call(one), call(same))
+        assert torch.equal(call(one, state=s["state"].clone()), call(same, state=s["state"].clone()))
 
 
 def test_nothing(cuda):

@@ -103,8 +103,10 @@ __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf
 // log(1 + exp(v)) = max(v, 0) + log(1 + e), e = exp(-|v|) in [0, 1].  log(1 + e) / e by a polynomial of degree 9 (least largest
 // relative error, 5e-9 before its coefficients are rounded): the usual small step sizes keep all their digits, which a
 // logarithm of the rounded 1 + e would not.
-__device__ __forceinline__ float softplus(float v) {
-  const float e = exp_neg(fabsf(v));
+// slope: sigmoid(v), from the same exponential.
+__device__ __forceinline__ float softplus(float v, float& slope) {
+  const float e = exp_neg(fabsf(v)), r = __builtin_amdgcn_rcpf(1.0f + e);
+  slope = v < 0.0f ? e * r : r;
   float p = -0.0032440251670777798f;
   p = p * e + 0.01985146477818489f;
   p = p * e - 0.056959547102451324f;
@@ -116,6 +118,10 @@ __device__ __forceinline__ float softplus(float v) {
   p = p * e - 0.4999990165233612f;
   p = p * e + 1.0f;
   return (v < 0.0f ? 0.0f : v) + p * e;  // (NaN stays NaN)
+}
+__device__ __forceinline__ float softplus(float v) {
+  float slope;
+  return softplus(v, slope);
 }
 
 template <int kRegs> struct Shape {
@@ -215,17 +221,17 @@ __device__ __forceinline__ Lane lane_of(const ScanArgs& A) {
   return l;
 }
 
-// A [B][L][channels] tensor, seen from a workgroup: lane q's values of the steps t + 4 m + q of a tile of kTile steps.  The
-// tile's buffer is made of a pointer that moves with it and the steps left, by the same few scalar instructions for all.
+// A [B][L][channels] tensor, seen from a workgroup: lane q's values of the steps t + 4 m + q of a tile of kTile steps, zeros
+// behind the sequence's length and the last channel (so x and dout, whatever memory holds there).  The tile's buffer is made of a pointer that moves with it and the steps left, by the same few scalar instructions for all.
 template <typename T, int kTile>
 struct Steps {
   const char* tile;     // the sequence's and workgroup's first channel in the tile's first step
   int row, width;       // bytes of a step, and of the channels from the first one on (0: no tensor)
   unsigned at;          // the lane's place in four steps
-  __device__ __forceinline__ Steps(const void* p, long batch, long row_, const Lane& l, int t, int D, bool writes)
+  __device__ __forceinline__ Steps(const void* p, long batch, long row_, const Lane& l, int t, int D)
       : tile((const char*)p + (l.b * batch + l.c0 + t * row_) * (long)sizeof(T)), row((int)row_ * (int)sizeof(T)),
         width(p ? (D - l.c0) * (int)sizeof(T) : 0),
-        at(writes && !l.on ? kNowhere : (unsigned)l.q * (unsigned)row + (unsigned)(l.in * (int)sizeof(T))) {}
+        at(!l.on ? kNowhere : (unsigned)l.q * (unsigned)row + (unsigned)(l.in * (int)sizeof(T))) {}
   __device__ __forceinline__ void move(int tiles) { tile += (long)tiles * kTile * row; }
   __device__ __forceinline__ Buffer steps(int left) const {  // left: of the tensor from the tile's first step on
     const int there = min(left, kTile);
@@ -346,8 +352,8 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   constexpr int kAhead = Shape<kRegs>::kAhead;
   __shared__ float bc[2][kTile * 2 * kPad];
   const Lane l = lane_of(A);
-  Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, l.t0, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, l.t0, A.D, false);
-  Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, l.t0, A.D, false), out(A.out, (long)A.L * A.D, A.D, l, l.t0, A.D, true);
+  Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, l.t0, A.D), dt(A.dt, A.dt_batch, A.dt_row, l, l.t0, A.D);
+  Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, l.t0, A.D), out(A.out, (long)A.L * A.D, A.D, l, l.t0, A.D);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], h[kRegs];
@@ -369,9 +375,9 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   T xv[kM], dv[kM], zv[kM];
   Rows<T, kRegs, kTile> rows(A, l.b, l.t0);
   auto read = [&](int t) {
-    x.read(xv, A.L - t);
-    dt.read(dv, A.L - t);
-    if (kGated) z.read(zv, A.L - t);
+    x.read(xv, l.len - t);
+    dt.read(dv, l.len - t);
+    if (kGated) z.read(zv, l.len - t);
     rows.read(l.len - t);
     x.move(1);
     dt.move(1);
@@ -389,8 +395,8 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     for (int m = 0; m < kM; ++m) {
       const bool counts = 4 * m < left;
       const float v = to_f32(dv[m]) + bias, soft = here(softplus(v));
-      s[m] = counts ? (A.softplus ? soft : v) : 0.0f;
-      xs[m] = counts ? to_f32(xv[m]) : 0.0f;
+      s[m] = counts ? (A.softplus ? soft : v) : 0.0f;  // (no step: the state stays)
+      xs[m] = to_f32(xv[m]);
       u[m] = s[m] * xs[m];
       gate[m] = 1.0f;
       if (kEdges) total += s[m];
@@ -453,9 +459,9 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   const Lane l = lane_of(A);
   const int tiles = (l.t1 - l.t0 + kTile - 1) / kTile, last = l.t0 + (tiles - 1) * kTile;
   const long full = (long)A.L * A.D;
-  Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, last, A.D, false), dt(A.dt, A.dt_batch, A.dt_row, l, last, A.D, false);
-  Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, last, A.D, false), dout(A.dout, full, A.D, l, last, A.D, false);
-  Steps<T, kTile> dx(A.dx, full, A.D, l, last, A.D, true), ddt(A.ddt, full, A.D, l, last, A.D, true), dz(A.dz, full, A.D, l, last, A.D, true);
+  Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, last, A.D), dt(A.dt, A.dt_batch, A.dt_row, l, last, A.D);
+  Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, last, A.D), dout(A.dout, full, A.D, l, last, A.D);
+  Steps<T, kTile> dx(A.dx, full, A.D, l, last, A.D), ddt(A.ddt, full, A.D, l, last, A.D), dz(A.dz, full, A.D, l, last, A.D);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const int group = states_of(threadIdx.x);  // of the lane's states
   const unsigned mine = (unsigned)(l.in * kPad + group * kRegs) * 4;
@@ -473,11 +479,12 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   float first[kRegs];
   Rows<T, kRegs, kTile> rows(A, l.b, last);
   auto read = [&](int t, bool there) {  // (before the chunk's first tile nothing is)
-    x.read(xv, there ? A.L - t : 0);
-    dt.read(dv, there ? A.L - t : 0);
-    dout.read(gv, there ? A.L - t : 0);
-    if (kGated) z.read(zv, there ? A.L - t : 0);
-    rows.read(there ? l.len - t : 0);
+    const int left = there ? l.len - t : 0;
+    x.read(xv, left);
+    dt.read(dv, left);
+    dout.read(gv, left);
+    if (kGated) z.read(zv, left);
+    rows.read(left);
     if (!kEdges) fetch_states<kRegs>(first, buffer(saved, saved_bytes & (there ? -1 : 0)), mine);
     x.move(-1);
     dt.move(-1);
@@ -494,19 +501,21 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     take_turns(tile);
     // dzs: dout times silu's slope, slope: the step size's
     float s[kM], u[kM], xs[kM], dy[kM], dzs[kM], slope[kM], h[kRegs];
-    const int left = l.on ? l.len - t - l.q : 0;
+    const int left = l.len - t - l.q;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
       const bool counts = 4 * m < left;
-      const float v = to_f32(dv[m]) + bias, soft = here(softplus(v)), sig = here(sigmoid(v));
+      const float v = to_f32(dv[m]) + bias;
+      float sig;
+      const float soft = here(softplus(v, sig));
       s[m] = counts ? (A.softplus ? soft : v) : 0.0f;
-      slope[m] = counts ? (A.softplus ? sig : 1.0f) : 0.0f;
-      xs[m] = counts ? to_f32(xv[m]) : 0.0f;
+      slope[m] = A.softplus ? here(sig) : 1.0f;  // (of the length's end on it meets zeros)
+      xs[m] = to_f32(xv[m]);
       u[m] = s[m] * xs[m];
-      dy[m] = counts ? to_f32(gv[m]) : 0.0f;
+      dy[m] = to_f32(gv[m]);
       dzs[m] = 0.0f;
       if (kGated) {
-        const float zf = counts ? to_f32(zv[m]) : 0.0f, sg = sigmoid(zf);
+        const float zf = to_f32(zv[m]), sg = sigmoid(zf);
         dzs[m] = dy[m] * (sg * (1.0f + zf * (1.0f - sg)));
         dy[m] *= zf * sg;
       }

@@ -32,11 +32,13 @@ namespace {
 
 // Per chunk in order (backward: from the last), edge becomes what comes into it: H, then H exp(A sum s) + edge.
 __global__ __launch_bounds__(64) void k_scan_join(const ScanArgs A, int padded, bool backward) {
-  const long at = (long)blockIdx.x * 64 + threadIdx.x, states = (long)A.D * A.N;
+  const long at = (long)blockIdx.x * 64 + threadIdx.x, states = (long)A.D * padded;
   if (at >= A.B * states) return;
-  const long b = at / states, in = at - b * states, d = in / A.N, to = d * padded + (in - d * A.N);
-  const float a2 = A.A[in] * 1.44269504088896340736f;
-  float h = !backward && A.state ? A.state[at] : 0.0f;
+  const long b = at / states, to = at - b * states, d = to / padded;
+  const int n = (int)(to - d * padded);
+  if (n >= A.N) return;  // (zeros throughout)
+  const float a2 = A.A[d * A.N + n] * 1.44269504088896340736f;
+  float h = !backward && A.state ? A.state[(b * A.D + d) * A.N + n] : 0.0f;
   constexpr int kAhead = 16;  // chunks whose values are under way together
   for (int first = 0; first < A.chunks; first += kAhead) {
     float e[kAhead], s[kAhead];
@@ -170,7 +172,6 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
   int rc = check_scan(dtype, B, L, D, N);
   if (rc || B == 0 || L == 0) return rc;
   if (!x || !dt || !A || !Bm || !Cm || !out) return kans_fail(KANS_ERR_ARG, "null argument");
-  if ((uintptr_t)state % 16 || (uintptr_t)A % 16) return kans_fail(KANS_ERR_ARG, "A and the state start at multiples of 16 bytes");
   if ((rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0, D}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, p.edges * (long)sizeof(float)))) return rc;
@@ -191,7 +192,7 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
     S.edge = (float*)workspace;
     S.sums = S.edge + (long)B * p.chunks * D * p.padded;
     HIP_TRY(launch(dtype, ScanPass::kEdges, S, st));
-    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 63) / 64)), dim3(64), 0, st, S, p.padded, false);
+    hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * p.padded + 63) / 64)), dim3(64), 0, st, S, p.padded, false);
     HIP_TRY(hipGetLastError());
   }
   HIP_TRY(launch(dtype, ScanPass::kForward, S, st));
@@ -228,7 +229,7 @@ int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_
   if (any) {
     if (p.chunks > 1) {
       HIP_TRY(launch(dtype, ScanPass::kBackwardEdges, S, st));
-      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * N + 63) / 64)), dim3(64), 0, st, S, p.padded, true);
+      hipLaunchKernelGGL(k_scan_join, dim3((unsigned)(((long)B * D * p.padded + 63) / 64)), dim3(64), 0, st, S, p.padded, true);
       HIP_TRY(hipGetLastError());
     }
     HIP_TRY(launch(dtype, ScanPass::kBackward, S, st));

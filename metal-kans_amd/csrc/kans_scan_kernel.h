@@ -27,25 +27,16 @@ __device__ __forceinline__ float quad_sum(float v) {
   v += dpp<0xb1>(v);
   return v + dpp<0x4e>(v);
 }
-typedef float Acc __attribute__((ext_vector_type(4)));
-
-// Lane q of the quad gets the quad's sum of v[q].  A 4 x 4 x 1 product for each quad by itself: times a column that is 1 in lane
-// k, step k's values of the four lanes go to lane k.
-struct QuadSums {
-  float one[4];
-  __device__ __forceinline__ QuadSums() {
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      one[k] = (threadIdx.x & 3) == k ? 1.0f : 0.0f;
-      asm volatile("" : "+v"(one[k]));  // (a register each, not computed again at every use)
-    }
-  }
-  template <int K>
-  __device__ __forceinline__ static void add(Acc& acc, const QuadSums& s, float v, bool first) {
-    acc = __builtin_amdgcn_mfma_f32_4x4x1f32(v, s.one[K], first ? Acc{0.0f, 0.0f, 0.0f, 0.0f} : acc, 0, 0, 0);
-  }
-  __device__ __forceinline__ static float sum(const Acc& acc) { return (acc.x + acc.y) + (acc.z + acc.w); }
-};
+// Lane q of the quad gets the quad's sum of v[q].  (By selections: 4 x 4 x 1 products with unit columns on the matrix pipe take 3 vector
+// instructions instead of 9, but their waits made the kernels 5 - 7 % slower, and 0 times infinity would carry one step's
+// infinity to the three beside it.)
+__device__ __forceinline__ float quad_sums(const float (&v)[4]) {
+  const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+  const float v0 = v[0], v1 = v[1], v2 = v[2], v3 = v[3];
+  const float a = (odd ? v1 : v0) + dpp<0xb1>(odd ? v0 : v1);
+  const float b = (odd ? v3 : v2) + dpp<0xb1>(odd ? v2 : v3);
+  return (high ? b : a) + dpp<0x4e>(high ? a : b);
+}
 
 // The backward's lanes hold their states in mirrored order in every other quad: lane q of an odd one those of 3 - q, so that a lane's
 // partner in a mirrored row, or half of a row, holds the same states.
@@ -319,6 +310,17 @@ struct Ahead {
   }
 };
 
+// The states that are there (kFull: all).  Others stay zeros: what multiplies them is zero too, but may meet infinity.
+template <int kRegs, bool kFull>
+struct There {
+  bool is[kRegs];
+  __device__ __forceinline__ There(const ScanArgs& A, int group) {
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) is[i] = kFull || group * kRegs + i < A.N;
+  }
+  __device__ __forceinline__ float operator()(int i, float v) const { return kFull || is[i] ? v : 0.0f; }
+};
+
 // A lane's A log2(e).
 template <int kRegs>
 __device__ __forceinline__ void load_decays(float (&a2)[kRegs], const ScanArgs& A, const Lane& l, int group) {
@@ -346,7 +348,7 @@ __device__ __forceinline__ void take_turns(int tile) {
 
 // ---- forward ------------------------------------------------------------------------------------------
 // kEdges: of each chunk alone, from a state of zeros, its last state and the sum of its step sizes.
-template <typename T, int kRegs, bool kEdges, bool kGated>
+template <typename T, int kRegs, bool kFull, bool kEdges, bool kGated>
 __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   constexpr int kPad = Shape<kRegs>::kPad, kTile = Shape<kRegs>::kTile, kInterval = Shape<kRegs>::kInterval, kM = kTile / 4;
   constexpr int kAhead = Shape<kRegs>::kAhead;
@@ -357,6 +359,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
   float a2[kRegs], h[kRegs];
+  const There<kRegs, kFull> there(A, l.q);
   load_decays<kRegs>(a2, A, l, l.q);
   const long place = (long)l.b * A.chunks + l.chunk;
   float* state = A.state ? A.state + ((long)l.b * A.D + l.row) * A.N : nullptr;
@@ -368,7 +371,6 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     for (int i = 0; i < kRegs; ++i)
       if (l.q * kRegs + i < A.N) h[i] = state[l.q * kRegs + i];
   float total = 0.0f;
-  const QuadSums quad;
   const float* saved = A.saved + ((l.b * (long)((A.L + kInterval - 1) / kInterval) + l.t0 / kInterval) * A.D + l.c0) * kPad;
   const int saved_bytes = A.saved ? min(A.D - l.c0, kScanChannels) * kPad * 4 : 0;
 
@@ -408,7 +410,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     const float* lds = bc[turn] + l.q * kRegs;
     Ahead<kRegs, kAhead, true, !kEdges> ahead;
     ahead.read(lds, 0);
-    Acc y;
+    float y[4];
     static_for<0, kTile / kAhead>([&](auto g_) {
       constexpr int g = decltype(g_)::value;
       const Ahead<kRegs, kAhead, true, !kEdges> now = ahead;
@@ -422,12 +424,12 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
-          h[i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]) * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i];
+          h[i] = there(i, __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]) * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i]);
           if (!kEdges) sum += h[i] * now.C[j - g * kAhead][i];
         }
-        if (!kEdges) QuadSums::template add<k>(y, quad, sum, k == 0);
+        y[k] = sum;
         if constexpr (!kEdges && k == 3) {
-          const float o = (QuadSums::sum(y) + skip * xs[m]) * gate[m];  // (outside the condition: all lanes of the quad take part)
+          const float o = (quad_sums(y) + skip * xs[m]) * gate[m];  // (outside the condition: all lanes of the quad take part)
           out.write(to, m, 4 * m < left ? o : 0.0f);
         }
       });
@@ -450,7 +452,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
 // ---- backward -----------------------------------------------------------------------------------------
 // kEdges: of each chunk alone, without a gradient from behind it, the gradient of its first state, and the sum of its step sizes.
 // (At most 256 registers: two waves a SIMD, where one leaves a third of its cycles unused; 64 states need more.)
-template <typename T, int kRegs, bool kEdges, bool kGated>
+template <typename T, int kRegs, bool kFull, bool kEdges, bool kGated>
 __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const ScanArgs A) {
   constexpr int kPad = Shape<kRegs>::kPad, kTile = Shape<kRegs>::kInterval, kM = kTile / 4, kGroups = kTile * 2 * kRegs / 16;
   constexpr int kAhead = Shape<kRegs>::kAheadBack;
@@ -466,12 +468,12 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   const int group = states_of(threadIdx.x);  // of the lane's states
   const unsigned mine = (unsigned)(l.in * kPad + group * kRegs) * 4;
   float a2[kRegs], carry[kRegs], dA[kRegs] = {}, dskip = 0.0f, dbias = 0.0f, total = 0.0f;
+  const There<kRegs, kFull> is_there(A, group);
   load_decays<kRegs>(a2, A, l, group);
   const long place = (long)l.b * A.chunks + l.chunk;
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) carry[i] = 0.0f;
   if (!kEdges && A.chunks > 1) fetch_states<kRegs>(carry, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
-  const QuadSums quad;
   const float* saved = A.saved + ((l.b * (long)((A.L + kTile - 1) / kTile) + last / kTile) * A.D + l.c0) * kPad;
   const int saved_bytes = min(A.D - l.c0, kScanChannels) * kPad * 4;
 
@@ -530,7 +532,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     {
       Ahead<kRegs, kAhead, !kEdges, !kEdges && kGated> ahead;
       ahead.read(lds, 0);
-      Acc y;
+      float y[4];
       static_for<0, kTile / kAhead>([&](auto g_) {
         constexpr int g = decltype(g_)::value;
         const Ahead<kRegs, kAhead, !kEdges, !kEdges && kGated> now = ahead;
@@ -543,21 +545,20 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
             stay[j][i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]);
             if constexpr (!kEdges) {
               before[j][i] = h[i];
-              h[i] = stay[j][i] * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i];
+              h[i] = is_there(i, stay[j][i] * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i]);
               if (kGated) sum += h[i] * now.C[j - g * kAhead][i];
             }
           }
-          if (!kEdges && kGated) QuadSums::template add<k>(y, quad, sum, k == 0);
+          y[k] = sum;
           if constexpr (!kEdges && k == 3) __builtin_amdgcn_sched_barrier(0);  // (nothing moves over four steps: no registers for it)
           if constexpr (!kEdges && kGated && k == 3) {
-            const float o = dzs[m] * (QuadSums::sum(y) + skip * xs[m]);
+            const float o = dzs[m] * (quad_sums(y) + skip * xs[m]);
             dz.write(to_dz, m, 4 * m < left ? o : 0.0f);
           }
         });
       });
     }
-    float vals[16], dA_tile[kRegs] = {};
-    Acc of_b, of_a;
+    float vals[16], dA_tile[kRegs] = {}, of_b[4], of_a[4];
     Ahead<kRegs, kAhead, !kEdges, true> ahead;
     ahead.read(lds, kTile - kAhead);
     static_for<0, kTile / kAhead>([&](auto g_) {
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
         float gr[kRegs], sB = 0.0f, sA = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
-          gr[i] = now.C[j - g * kAhead][i] * of_lane<k>(dy[m]) + carry[i];
+          gr[i] = is_there(i, now.C[j - g * kAhead][i] * of_lane<k>(dy[m]) + carry[i]);
           carry[i] = gr[i] * stay[j][i];
           if constexpr (!kEdges) {
             sB += gr[i] * now.B[j - g * kAhead][i];
@@ -581,8 +582,8 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           }
         }
         if constexpr (!kEdges) {
-          QuadSums::template add<k>(of_b, quad, sB, k == 3);
-          QuadSums::template add<k>(of_a, quad, sA, k == 3);
+          of_b[k] = sB;
+          of_a[k] = sA;
           static_for<0, 2 * kRegs>([&](auto i_) {
             constexpr int i = decltype(i_)::value, value = (kTile - 1 - j) * 2 * kRegs + i;
             vals[value % 16] = i < kRegs ? gr[i % kRegs] * of_lane<k>(u[m]) : h[i % kRegs] * of_lane<k>(dy[m]);
@@ -592,7 +593,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           for (int i = 0; i < kRegs; ++i) h[i] = before[j][i];
           if constexpr (k == 0) __builtin_amdgcn_sched_barrier(0);
           if constexpr (k == 0) {
-            const float gB = QuadSums::sum(of_b), gA = QuadSums::sum(of_a) * kLn2;
+            const float gB = quad_sums(of_b), gA = quad_sums(of_a) * kLn2;
             const bool counts = 4 * m < left;
             const float ddtv = counts ? (xs[m] * gB + gA) * slope[m] : 0.0f;
             dskip += dy[m] * xs[m];
@@ -622,7 +623,8 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
         const int value = (kTile - 1 - j) * 2 * kRegs + which * kRegs + n % kRegs, v = value % 16, odd = v >> 2 & 1;
         // (where wave_sums leaves it)
         const int lane = (v & 8) + (v & 4) + (v & 2) * 8 + (v & 1) * 32 + (odd ? 3 - n / kRegs : n / kRegs), from = value / 16 * 64 + lane;
-        part[at] = (red[turn][0][from] + red[turn][1][from]) + (red[turn][2][from] + red[turn][3][from]);
+        const float sum = (red[turn][0][from] + red[turn][1][from]) + (red[turn][2][from] + red[turn][3][from]);
+        part[at] = t + j < l.len ? sum : 0.0f;  // (an infinite state times no gradient is not zero)
       }
     }
   }
@@ -661,10 +663,9 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
   float* h = A.state + row * A.N;
   const float* a = A.A + (long)c * A.N;
   float y = 0.0f;
-  if (A.N % 4 == 0) {  // (the state and A start at multiples of 16 bytes)
+  if (A.N % 4 == 0 && (((uintptr_t)A.state | (uintptr_t)A.A) & 15) == 0) {
     for (int n = 4 * q; n < A.N; n += 16) {
-      float4 hv = *(const float4*)(h + n);
-      const float4 av = *(const float4*)(a + n);
+      const float4 hv = *(const float4*)(h + n), av = *(const float4*)(a + n);
       float hs[4] = {hv.x, hv.y, hv.z, hv.w}, as[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -673,12 +674,13 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
       }
       if (counts && at < all) *(float4*)(h + n) = make_float4(hs[0], hs[1], hs[2], hs[3]);
     }
-  } else {
-    for (int n = q; n < A.N; n += 4) {
-      const float v = __builtin_amdgcn_exp2f(s * (a[n] * kLog2e)) * h[n] + u * to_f32(Bm[n]);
-      y += v * to_f32(Cm[n]);
-      if (counts && at < all) h[n] = v;
-    }
+  } else {  // (in the same order)
+    for (int first = 4 * q; first < A.N; first += 16)
+      for (int n = first; n < min(first + 4, A.N); ++n) {
+        const float v = __builtin_amdgcn_exp2f(s * (a[n] * kLog2e)) * h[n] + u * to_f32(Bm[n]);
+        y += v * to_f32(Cm[n]);
+        if (counts && at < all) h[n] = v;
+      }
   }
   y = quad_sum(y);
   if (q != 0 || at >= all) return;
@@ -705,7 +707,7 @@ __global__ __launch_bounds__(256) void k_scan_reduce(const float* part, int bloc
   if (to) to[at / (2 * padded) * N + n] = from_f32<T>(s);
 }
 
-template <typename T, int kRegs>
+template <typename T, int kRegs, bool kFull>
 hipError_t launch(ScanPass pass, const ScanArgs& A, hipStream_t st) {
   const dim3 grid((unsigned)((long)A.B * A.chunks * ((A.D + kScanChannels - 1) / kScanChannels)));
   auto go = [&](auto kernel) {
@@ -713,10 +715,10 @@ hipError_t launch(ScanPass pass, const ScanArgs& A, hipStream_t st) {
     return hipGetLastError();
   };
   switch (pass) {
-    case ScanPass::kForward: return A.z ? go(k_scan_fwd<T, kRegs, false, true>) : go(k_scan_fwd<T, kRegs, false, false>);
-    case ScanPass::kEdges: return go(k_scan_fwd<T, kRegs, true, false>);
-    case ScanPass::kBackward: return A.z ? go(k_scan_bwd<T, kRegs, false, true>) : go(k_scan_bwd<T, kRegs, false, false>);
-    case ScanPass::kBackwardEdges: return A.z ? go(k_scan_bwd<T, kRegs, true, true>) : go(k_scan_bwd<T, kRegs, true, false>);
+    case ScanPass::kForward: return A.z ? go(k_scan_fwd<T, kRegs, kFull, false, true>) : go(k_scan_fwd<T, kRegs, kFull, false, false>);
+    case ScanPass::kEdges: return go(k_scan_fwd<T, kRegs, kFull, true, false>);
+    case ScanPass::kBackward: return A.z ? go(k_scan_bwd<T, kRegs, kFull, false, true>) : go(k_scan_bwd<T, kRegs, kFull, false, false>);
+    case ScanPass::kBackwardEdges: return A.z ? go(k_scan_bwd<T, kRegs, kFull, true, true>) : go(k_scan_bwd<T, kRegs, kFull, true, false>);
     case ScanPass::kStep: break;
   }
   return hipErrorInvalidValue;
@@ -729,12 +731,12 @@ hipError_t launch_scan(ScanPass pass, const ScanArgs& A, hipStream_t st) {
     return hipGetLastError();
   }
   switch (scan_regs(A.N)) {
-    case 1: return launch<T, 1>(pass, A, st);
-    case 2: return launch<T, 2>(pass, A, st);
-    case 4: return launch<T, 4>(pass, A, st);
-    case 6: return launch<T, 6>(pass, A, st);
-    case 8: return launch<T, 8>(pass, A, st);
-    case 16: return launch<T, 16>(pass, A, st);
+    case 1: return A.N == 4 * 1 ? launch<T, 1, true>(pass, A, st) : launch<T, 1, false>(pass, A, st);
+    case 2: return A.N == 4 * 2 ? launch<T, 2, true>(pass, A, st) : launch<T, 2, false>(pass, A, st);
+    case 4: return A.N == 4 * 4 ? launch<T, 4, true>(pass, A, st) : launch<T, 4, false>(pass, A, st);
+    case 6: return A.N == 4 * 6 ? launch<T, 6, true>(pass, A, st) : launch<T, 6, false>(pass, A, st);
+    case 8: return A.N == 4 * 8 ? launch<T, 8, true>(pass, A, st) : launch<T, 8, false>(pass, A, st);
+    case 16: return A.N == 4 * 16 ? launch<T, 16, true>(pass, A, st) : launch<T, 16, false>(pass, A, st);
   }
   return hipErrorInvalidValue;
 }

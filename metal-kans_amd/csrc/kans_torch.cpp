@@ -714,12 +714,11 @@ std::optional<Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Te
       !channel(bias) || !fits_lengths(lengths, x))
     return {};
   if (state && (!of_type(*state, at::kFloat) || !state->is_contiguous() || state->dim() != 3 || state->size(0) != x.size(0) ||
-                state->size(1) != x.size(2) || state->size(2) != A.size(1) || (uintptr_t)state->data_ptr() % 16))
+                state->size(1) != x.size(2) || state->size(2) != A.size(1)))
     return {};
   TORCH_CHECK_VALUE(sizes_fit_int(x), "x has a size of more than 2^31");
-  Scan s{with_steps(x), with_steps(dt), A.contiguous(), with_steps(B), with_steps(C), contiguous(skip),
+  const Scan s{with_steps(x), with_steps(dt), A.contiguous(), with_steps(B), with_steps(C), contiguous(skip),
          z ? with_steps(*z) : Tensor(), contiguous(bias), contiguous(lengths), softplus};
-  if ((uintptr_t)s.A.data_ptr() % 16) s.A = s.A.clone();
   no_tangents({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias}, "selective_scan");
   const at::OptionalDeviceGuard device(x.device());
   if (wants_grad({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias})) {

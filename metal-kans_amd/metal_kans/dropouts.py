@@ -36,7 +36,8 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], offset: i
         p: in [0, 1]; an element is dropped where its random number of 32 bits is below p 2^32
         seed: 64 bits that choose the random numbers: an int, or an int64 tensor of one element on x's device,
             which is read when the kernel runs (a captured graph drops others on every replay if the program
-            changes it in between; the backward uses the value that its forward had)
+            changes it in between; the backward uses the value that its forward had, but a checkpoint, which runs the
+            forward again in the backward, reads the seed again)
         offset: 64 bits more, for calls that share a seed (layers, steps)
 
     The random number of element i (counted in row-major order) is word i % 4 of Philox4x32-10 with key ``seed``

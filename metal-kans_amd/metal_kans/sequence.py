@@ -17,7 +17,7 @@ _DT = (torch.float32, torch.float16, torch.bfloat16)
 _ACTIVATIONS = {None: 0, "silu": 1}
 
 
-def _refuse_common(what, x, state, shape, dtype, lengths):
+def _refuse_common(x, state, shape, dtype, lengths):
     if x.dim() != 3 or x.shape[-1] == 0:
         raise ValueError(f"x {tuple(x.shape)} must be [B, L, D]")
     if x.dtype not in _DT:
@@ -27,8 +27,6 @@ def _refuse_common(what, x, state, shape, dtype, lengths):
             raise TypeError(f"state is {state.dtype}, expected {dtype}")
         if tuple(state.shape) != shape or not state.is_contiguous():
             raise ValueError(f"state {tuple(state.shape)} must be {shape} and contiguous")
-        if state.device == x.device and state.data_ptr() % 16 and what == "selective_scan":
-            raise ValueError("state must start at a multiple of 16 bytes")
     if lengths is not None:
         if lengths.dtype != torch.int64:
             raise TypeError(f"lengths are {lengths.dtype}, expected torch.int64")
@@ -44,7 +42,7 @@ def _refuse_conv(x, weight, bias, activation, state, lengths):
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [B, L, D] and [D, W], W from 1 to 8")
     if bias is not None and tuple(bias.shape) != (x.shape[-1],):
         raise ValueError(f"bias {tuple(bias.shape)} must be ({x.shape[-1]},)")
-    _refuse_common("causal_conv", x, state, (x.shape[0], weight.shape[1] - 1, x.shape[-1]), x.dtype, lengths)
+    _refuse_common(x, state, (x.shape[0], weight.shape[1] - 1, x.shape[-1]), x.dtype, lengths)
     for name, t in (("weight", weight), ("bias", bias)):
         if t is not None and t.dtype != x.dtype:
             raise TypeError(f"{name} is {t.dtype}, expected {x.dtype}")
@@ -77,7 +75,7 @@ def _refuse_scan(x, dt, A, B, C, D, z, dt_bias, state, lengths):
     """What is wrong with the arguments of a call."""
     if x.dim() != 3 or A.dim() != 2 or A.shape[0] != x.shape[-1] or not 1 <= A.shape[1] <= 64:
         raise ValueError(f"x {tuple(x.shape)} and A {tuple(A.shape)} must be [B, L, D] and [D, N], N from 1 to 64")
-    _refuse_common("selective_scan", x, state, (x.shape[0], x.shape[-1], A.shape[1]), torch.float32, lengths)
+    _refuse_common(x, state, (x.shape[0], x.shape[-1], A.shape[1]), torch.float32, lengths)
     for name, t, last in (("dt", dt, x.shape[-1]), ("B", B, A.shape[1]), ("C", C, A.shape[1]), ("z", z, x.shape[-1])):
         if t is None:
             continue

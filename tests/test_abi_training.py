@@ -152,7 +152,7 @@ def test_selective_scan_refusals(lib):
     def bwd(saved=64, z=None, dz=None, skip=None, dskip=None, dbias=None, ws=64, size=1 << 24, dx=64):
         return lib.kans_selective_scan_backward(0, 64, 20, 4, 64, 20, 4, 64, 64, 80, 16, 64, 80, 16, skip, z, 20, 4, None, 1, None, saved,
                                                 64, dx, 64, 64, 64, 64, dskip, dz, dbias, 2, 5, 4, 16, ws, size, None)
-    for bad in (dict(dt=3), dict(x=None), dict(A=None), dict(A=68), dict(bm=None), dict(out=None), dict(state=68), dict(b=-1), dict(n=-1),
+    for bad in (dict(dt=3), dict(x=None), dict(A=None), dict(bm=None), dict(out=None), dict(b=-1), dict(n=-1),
                 dict(d=0), dict(states=0), dict(n=300, ws=None), dict(n=300, ws=72), dict(n=300, size=16)):
         assert fwd(**bad) == -1, bad
     for bad in (dict(states=65), dict(b=1 << 22), dict(n=(1 << 30) + 1), dict(b=1 << 21, n=1 << 20)):

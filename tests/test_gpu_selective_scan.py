@@ -256,6 +256,64 @@ def test_masked_places_are_not_looked_at(cuda, dt):
         assert state.isfinite().all() and torch.equal(state[0], s["state"][0])
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("n", [16, 30])
+def test_infinities_stay_where_they_belong(cuda, n, bad):
+    """An infinite or NaN input reaches its own channel (B's and C's: all) from its step on, a gradient its channel up to its
+    step, and what sums over them; everything else keeps its bits."""
+    s = inputs(2, 150, 20, n, torch.float32, lengths=[150, 90])
+    want = train(s)
+    for name in ("x", "dt", "z"):
+        hurt = {**s, name: s[name].clone()}
+        hurt[name][1, 41, 7] = bad
+        got = train(hurt)
+        assert not got["out"][1, 41, 7].isfinite()
+        for a, b in ((got["out"][0], want["out"][0]), (got["out"][1, :41], want["out"][1, :41]), (got["out"][1, :, :7], want["out"][1, :, :7]),
+                     (got["out"][1, :, 8:], want["out"][1, :, 8:])):
+            assert torch.equal(a, b), name
+        others = torch.arange(20, device="cuda") != 7
+        for k in ("dx", "ddt", "dz"):
+            assert torch.equal(got[k][..., others], want[k][..., others]) and torch.equal(got[k][0], want[k][0]), (name, k)
+            assert not got[k][1, 90:].any(), (name, k)
+        for k in ("dA", "dD", "ddt_bias"):
+            assert torch.equal(got[k][others], want[k][others]), (name, k)
+        for k in ("dB", "dC"):
+            assert torch.equal(got[k][0], want[k][0]) and not got[k][1, 90:].any(), (name, k)
+    for name, at in (("B", 5), ("C", 2)):
+        hurt = {**s, name: s[name].clone()}
+        hurt[name][1, 41, at] = bad
+        got = train(hurt)
+        assert torch.equal(got["out"][0], want["out"][0]) and torch.equal(got["out"][1, :41], want["out"][1, :41])
+        assert not got["out"][1, 90:].any() and not got["dC"][1, 90:].any() and not got["dB"][1, 90:].any()
+    hurt = {**s, "dout": s["dout"].clone()}
+    hurt["dout"][1, 41, 7] = bad
+    got = train(hurt)
+    for k in ("dx", "ddt", "dz", "dB", "dC"):
+        assert torch.equal(got[k][0], want[k][0]) and torch.equal(got[k][1, 42:], want[k][1, 42:]), k
+    state = s["state"].clone()
+    hurt = {**s, "x": s["x"].clone()}
+    hurt["x"][1, 41, 7] = bad
+    with torch.no_grad():
+        call(hurt, state=state)
+    other = s["state"].clone()
+    with torch.no_grad():
+        call(s, state=other)
+    assert torch.equal(state[0], other[0]) and torch.equal(state[1, 8:], other[1, 8:]) and not state[1, 7].isfinite().all()
+
+
+def test_odd_addresses_of_the_state(cuda):
+    for n in (16, 7):
+        s = inputs(3, 1, 33, n, torch.float32)
+        space = torch.zeros(3 * 33 * n + 1, device="cuda")
+        odd = space[1:].view(3, 33, n)
+        for l in (1, 20):
+            s = inputs(3, l, 33, n, torch.float32)
+            odd.copy_(s["state"])
+            state = s["state"].clone()
+            with torch.no_grad():
+                assert torch.equal(call(s, state=odd), call(s, state=state)) and torch.equal(odd, state) and space[0] == 0
+
+
 @pytest.mark.parametrize("dt", TYPES)
 @pytest.mark.parametrize("d,n", [(37, 16), (70, 24), (5, 3), (64, 64)])
 def test_pieces_are_the_whole(cuda, d, n, dt):

@@ -669,16 +669,16 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
       float hs[4] = {hv.x, hv.y, hv.z, hv.w}, as[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        hs[i] = __builtin_amdgcn_exp2f(s * (as[i] * kLog2e)) * hs[i] + u * to_f32(Bm[n + i]);
-        y += hs[i] * to_f32(Cm[n + i]);
+        hs[i] = fmaf(__builtin_amdgcn_exp2f(s * (as[i] * kLog2e)), hs[i], u * to_f32(Bm[n + i]));
+        y = fmaf(hs[i], to_f32(Cm[n + i]), y);
       }
       if (counts && at < all) *(float4*)(h + n) = make_float4(hs[0], hs[1], hs[2], hs[3]);
     }
-  } else {  // (in the same order)
+  } else {  // (the same operations in the same order)
     for (int first = 4 * q; first < A.N; first += 16)
       for (int n = first; n < min(first + 4, A.N); ++n) {
-        const float v = __builtin_amdgcn_exp2f(s * (a[n] * kLog2e)) * h[n] + u * to_f32(Bm[n]);
-        y += v * to_f32(Cm[n]);
+        const float v = fmaf(__builtin_amdgcn_exp2f(s * (a[n] * kLog2e)), h[n], u * to_f32(Bm[n]));
+        y = fmaf(v, to_f32(Cm[n]), y);
         if (counts && at < all) h[n] = v;
       }
   }

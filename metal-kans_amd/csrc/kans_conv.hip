@@ -200,11 +200,16 @@ __global__ __launch_bounds__(256) void k_conv_bwd(const ConvArgs A) {
           const float s = sigmoid(u);
           slope = s * (1.0f + u * (1.0f - s));
         }
-        const float v = t + g < p.len ? d[g][e] * slope : 0.0f, mine = t + g < p.t1 ? v : 0.0f;
-        du[W - 1 + g][e] = v;
-        dbias[e] += mine;
+        du[W - 1 + g][e] = t + g < p.len ? d[g][e] * slope : 0.0f;
+      }
+      if (t + g < min(p.t1, p.len)) {  // (not by zeros: the next tile's inputs may be infinite)
 #pragma unroll
-        for (int j = 0; j < W; ++j) dw[j][e] += mine * in[g + j][e];
+        for (int e = 0; e < V; ++e) {
+          const float v = du[W - 1 + g][e];
+          dbias[e] += v;
+#pragma unroll
+          for (int j = 0; j < W; ++j) dw[j][e] += v * in[g + j][e];
+        }
       }
       const int to = t + g - (W - 1);  // du[g + j] is that of step to + j
       if (dx && to >= p.t0 && to < p.t1) {

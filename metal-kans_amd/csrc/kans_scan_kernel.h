@@ -236,6 +236,15 @@ struct Steps {
     for (int m = 0; m < kCount; ++m) v[m] = fetch<T>(from, four(m));
   }
   __device__ __forceinline__ void write(Buffer to, int m, float v) const { put(to, four(m), from_f32<T>(v)); }
+  // Zeros in `steps` steps from the tile on (to the end of one), `left` as above.
+  __device__ __forceinline__ void clear(int left, int steps) {
+    for (; steps > 0; steps -= kTile, left -= kTile) {
+      const Buffer to = this->steps(left);
+#pragma unroll
+      for (int m = 0; m < kTile / 4; ++m) write(to, m, 0.0f);
+      move(1);
+    }
+  }
 };
 
 // The states of the workgroup's channels at a place of the padded layouts.
@@ -389,7 +398,8 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   read(l.t0);
   rows.write(bc[0]);
   __syncthreads();
-  for (int t = l.t0, turn = 0; t < l.t1; t += kTile, turn ^= 1) {
+  int t = l.t0;
+  for (int turn = 0; t < min(l.t1, l.len); t += kTile, turn ^= 1) {
     take_turns(t / kTile);
     float s[kM], u[kM], xs[kM], gate[kM];
     const int left = l.len - t - l.q;
@@ -438,6 +448,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
     rows.write(bc[turn ^ 1]);
     __syncthreads();
   }
+  if (!kEdges) out.clear(A.L - t, l.t1 - t);  // (the states stay as they are; the backward does not ask for them)
   if (kEdges) {
     put_states<kRegs>(h, states_at<kRegs>(A.edge, place, l, A.D, true), mine);
     total = quad_sum(total);
@@ -459,7 +470,9 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   __shared__ float bc[2][kTile * 2 * kPad];
   __shared__ float red[kEdges ? 1 : 2][4][kEdges ? 1 : kGroups * 64];
   const Lane l = lane_of(A);
-  const int tiles = (l.t1 - l.t0 + kTile - 1) / kTile, last = l.t0 + (tiles - 1) * kTile;
+  // the chunk's tiles, and the last one that the sequence reaches: behind it all gradients are zeros
+  const int all = (l.t1 - l.t0 + kTile - 1) / kTile, tiles = max(0, (min(l.t1, l.len) - l.t0 + kTile - 1) / kTile);
+  const int last = l.t0 + (tiles - 1) * kTile;
   const long full = (long)A.L * A.D;
   Steps<T, kTile> x(A.x, A.x_batch, A.x_row, l, last, A.D), dt(A.dt, A.dt_batch, A.dt_row, l, last, A.D);
   Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, last, A.D), dout(A.dout, full, A.D, l, last, A.D);
@@ -495,7 +508,15 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     rows.move(-1);
     saved -= (long)A.D * kPad;
   };
-  read(last, true);
+  if (!kEdges && tiles < all) {
+    Steps<T, kTile> behind[3] = {dx, ddt, dz};
+#pragma unroll
+    for (int i = 0; i < (kGated ? 3 : 2); ++i) {
+      behind[i].move(1);
+      behind[i].clear(A.L - last - kTile, (all - tiles) * kTile);
+    }
+  }
+  read(last, tiles > 0);
   rows.write(bc[0]);
   __syncthreads();
   for (int tile = tiles - 1, turn = 0; tile >= 0; --tile, turn ^= 1) {
@@ -614,7 +635,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     if (!kEdges) {
       // the sums over this workgroup's channels: [step][B or C][state]
       float* part = A.part_bc + (((long)l.block * A.B + l.b) * A.L + t) * 2 * kPad;
-      const int there = min(kTile, A.L - t) * 2 * kPad;
+      const int there = min(kTile, l.len - t) * 2 * kPad;  // (no others are added up)
 #pragma unroll
       for (int i = 0; i < (kTile * 2 * kPad + kThreads - 1) / kThreads; ++i) {
         const int at = i * kThreads + (int)threadIdx.x;
@@ -623,8 +644,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
         const int value = (kTile - 1 - j) * 2 * kRegs + which * kRegs + n % kRegs, v = value % 16, odd = v >> 2 & 1;
         // (where wave_sums leaves it)
         const int lane = (v & 8) + (v & 4) + (v & 2) * 8 + (v & 1) * 32 + (odd ? 3 - n / kRegs : n / kRegs), from = value / 16 * 64 + lane;
-        const float sum = (red[turn][0][from] + red[turn][1][from]) + (red[turn][2][from] + red[turn][3][from]);
-        part[at] = t + j < l.len ? sum : 0.0f;  // (an infinite state times no gradient is not zero)
+        part[at] = (red[turn][0][from] + red[turn][1][from]) + (red[turn][2][from] + red[turn][3][from]);
       }
     }
   }
@@ -693,18 +713,21 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
 }
 
 // ---- sums of the partial rows --------------------------------------------------------------------------
-// dB and dC: [blocks][rows][2][padded] to [rows][N] twice.
+// dB and dC: [blocks][B][L][2][padded] to [B][L][N] twice, zeros behind a sequence's length.
 template <typename T>
-__global__ __launch_bounds__(256) void k_scan_reduce(const float* part, int blocks, long rows, int padded, int N, T* dB, T* dC) {
+__global__ __launch_bounds__(256) void k_scan_reduce(const float* part, int blocks, long rows, int padded, int N, int L, const int64_t* lengths,
+                                                     T* dB, T* dC) {
   const long at = (long)blockIdx.x * 256 + threadIdx.x, all = rows * 2 * padded;
   if (at >= all) return;
-  float s = 0.0f;
-#pragma unroll 8
-  for (int k = 0; k < blocks; ++k) s += part[k * all + at];
   const int n = (int)(at % padded);
   if (n >= N) return;
+  const long row = at / (2 * padded);
+  float s = 0.0f;
+  if (!lengths || row % L < lengths[row / L])
+#pragma unroll 8
+    for (int k = 0; k < blocks; ++k) s += part[k * all + at];
   T* to = at / padded & 1 ? dC : dB;
-  if (to) to[at / (2 * padded) * N + n] = from_f32<T>(s);
+  if (to) to[row * N + n] = from_f32<T>(s);
 }
 
 template <typename T, int kRegs, bool kFull>
@@ -745,7 +768,7 @@ template <typename T>
 hipError_t reduce_scan(const ScanArgs& A, int padded, void* dB, void* dC, hipStream_t st) {
   const long rows = (long)A.B * A.L;
   hipLaunchKernelGGL(k_scan_reduce<T>, dim3((unsigned)((rows * 2 * padded + 255) / 256)), dim3(256), 0, st, A.part_bc,
-                     (A.D + kScanChannels - 1) / kScanChannels, rows, padded, A.N, (T*)dB, (T*)dC);
+                     (A.D + kScanChannels - 1) / kScanChannels, rows, padded, A.N, A.L, A.lengths, (T*)dB, (T*)dC);
   return hipGetLastError();
 }
 

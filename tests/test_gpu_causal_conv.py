@@ -148,6 +148,38 @@ def test_masked_places_are_not_looked_at(cuda, dt):
         assert torch.equal(state, zero) and torch.equal(state[0], s["state"][0])
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_infinities_stay_where_they_belong(cuda, bad):
+    """An input reaches the outputs of W steps of its channel, a gradient the inputs of W steps; sums only where a step that
+    counts meets it."""
+    import metal_kans as mk
+    s = inputs(2, 200, 20, 4, torch.float32, lengths=[200, 130])
+    y, grads = check(s, None)
+    for t, d in ((63, 7), (64, 18), (129, 19)):
+        x = s["x"].clone()
+        x[1, t, d] = bad
+        x.requires_grad_(True)
+        w = s["weight"].detach().requires_grad_(True)
+        got = mk.causal_conv(x, w, s["bias"], activation=None, lengths=s["lengths"])
+        same = torch.ones_like(got, dtype=torch.bool)
+        same[1, t:t + 4, d] = False
+        assert torch.equal(got[same], y[same]) and not got[1, t, d].isfinite()
+        dx, dw = torch.autograd.grad(got, (x, w), s["dy"])
+        assert torch.equal(dx, grads["x"])
+        keep = torch.arange(20, device="cuda") != d
+        assert torch.equal(dw[keep], grads["weight"][keep])
+        taps = min(4, 130 - t)     # steps t, t + 1, ... that count see it at the last, the last but one, ... tap
+        assert not dw[d, 4 - taps:].isfinite().any() and torch.equal(dw[d, :4 - taps], grads["weight"][d, :4 - taps])
+        if bad == float("inf"):    # (one term: no NaN)
+            assert dw[d, 4 - taps:].isinf().all()
+        dy = s["dy"].clone()
+        dy[1, t, d] = bad
+        dx, = torch.autograd.grad(mk.causal_conv(x, w, s["bias"], activation=None, lengths=s["lengths"]), x, dy)
+        same = torch.ones_like(dx, dtype=torch.bool)
+        same[1, t - 3:t + 1, d] = False
+        assert torch.equal(dx[same], grads["x"][same])
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_pieces_are_the_whole(cuda, dt):
     """A prompt in pieces, then single tokens."""

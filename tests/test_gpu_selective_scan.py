@@ -301,6 +301,20 @@ def test_infinities_stay_where_they_belong(cuda, n, bad):
     assert torch.equal(state[0], other[0]) and torch.equal(state[1, 8:], other[1, 8:]) and not state[1, 7].isfinite().all()
 
 
+def test_long_padding(cuda):
+    """Whole tiles and chunks behind the ends of the sequences."""
+    for dt, b, l, d, n, lengths in ((torch.float32, 4, 700, 20, 16, [3, 700, 0, 350]), (torch.bfloat16, 3, 129, 70, 24, [16, 1, 128]),
+                                    (torch.float16, 2, 64, 600, 64, [32, 0])):
+        check(inputs(b, l, d, n, dt, lengths=lengths))
+        s = inputs(b, l, d, n, dt, lengths=lengths)
+        used = [torch.full(shape, 7.0, device="cuda", dtype=dt) for shape in ((b, l, d), (b, l, n)) for _ in range(4)]
+        del used     # (memory that the results are likely to get holds no zeros)
+        got = train(s)
+        for i, end in enumerate(lengths):
+            for k in ("out", "dx", "ddt", "dz", "dB", "dC"):
+                assert not got[k][i, end:].any(), k
+
+
 def test_odd_addresses_of_the_state(cuda):
     for n in (16, 7):
         s = inputs(3, 1, 33, n, torch.float32)

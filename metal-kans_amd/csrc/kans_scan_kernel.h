@@ -217,16 +217,16 @@ __device__ __forceinline__ Lane lane_of(const ScanArgs& A) {
 template <typename T, int kTile>
 struct Steps {
   const char* tile;     // the sequence's and workgroup's first channel in the tile's first step
-  int row, width;       // bytes of a step, and of the channels from the first one on (0: no tensor)
+  int row, width;       // bytes of a step, and of the channels from the first one on
   unsigned at;          // the lane's place in four steps
   __device__ __forceinline__ Steps(const void* p, long batch, long row_, const Lane& l, int t, int D)
       : tile((const char*)p + (l.b * batch + l.c0 + t * row_) * (long)sizeof(T)), row((int)row_ * (int)sizeof(T)),
-        width(p ? (D - l.c0) * (int)sizeof(T) : 0),
+        width((D - l.c0) * (int)sizeof(T)),
         at(!l.on ? kNowhere : (unsigned)l.q * (unsigned)row + (unsigned)(l.in * (int)sizeof(T))) {}
   __device__ __forceinline__ void move(int tiles) { tile += (long)tiles * kTile * row; }
   __device__ __forceinline__ Buffer steps(int left) const {  // left: of the tensor from the tile's first step on
     const int there = min(left, kTile);
-    return buffer(tile, ((there - 1) * row + width) & (there > 0 && width > 0 ? -1 : 0));
+    return buffer(tile, ((there - 1) * row + width) & (there > 0 ? -1 : 0));
   }
   __device__ __forceinline__ unsigned four(int m) const { return at + (unsigned)(4 * m * row); }
   template <int kCount>
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     }
 #pragma unroll
     for (int i = 0; i < kRegs; ++i) h[i] = first[i];
-    const Buffer to_dx = dx.steps(A.L - t), to_ddt = ddt.steps(A.L - t), to_dz = dz.steps(kGated ? A.L - t : 0);
+    const Buffer to_dx = dx.steps(A.L - t), to_ddt = ddt.steps(A.L - t), to_dz = dz.steps(A.L - t);
     const float* lds = bc[turn] + group * kRegs;
     // the states of the tile again: before each step, and what the step leaves of them
     float before[kEdges ? 1 : kTile][kRegs], stay[kTile][kRegs];

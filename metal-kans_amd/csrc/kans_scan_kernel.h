@@ -42,17 +42,19 @@ __device__ __forceinline__ float quad_sums(const float (&v)[4]) {
 // partner in a mirrored row, or half of a row, holds the same states.
 __device__ __forceinline__ int states_of(int lane) { return lane & 4 ? 3 - (lane & 3) : lane & 3; }
 
-// The sums of 16 values over the 16 lanes with the same states: lane l gets that of value 8 b3 + 4 b2 + 2 b4 + b5, b its bits.  Half of the lanes that are added
-// take one value of a pair, half the other: sums with the mirrored row (and half row) are written to some banks of four lanes
-// only, two instructions a pair; the rows meet by swaps.  33 issue slots for 16 values, 47 by swaps and selections alone (a swap
-// takes two).  On the matrix pipe, 16 products of 16 x 16 x 4 in a chain, the backward took twice as long.
+// The sums of 16 values over the 16 lanes with the same states: lane l gets that of value 8 b3 + 4 b2 + 2 b4 + b5, b its bits.
+// Half of the lanes that are added take one value of a pair, half the other: sums with the mirrored row (and half row) are
+// written to some banks of four lanes only, two instructions a pair; the rows meet by swaps.  33 issue slots for 16 values, 47
+// by swaps and selections alone (a swap takes two).  On the matrix pipe, 16 products of 16 x 16 x 4 in a chain, the
+// backward took twice as long.
 typedef unsigned Pair __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float sum_of(Pair v) {
   const unsigned a = v.x, b = v.y;  // (a bit cast of v.y itself takes v.x)
   return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
 __device__ __forceinline__ float wave_sums(float (&v)[16]) {
-  // (a lane permute reads what is at least two instructions old, and five behind a change of the lanes that are on)
+  // (A lane permute reads what is at least two instructions old, and five behind a change of the lanes that are on.  Results are
+  // written while others are still to be read.)
   asm("s_nop 4\n"
       "v_add_f32_dpp %0, %0, %0 row_mirror row_mask:0xf bank_mask:0xf\n"
       "v_add_f32_dpp %1, %1, %1 row_mirror row_mask:0xf bank_mask:0xf\n"
@@ -79,7 +81,7 @@ __device__ __forceinline__ float wave_sums(float (&v)[16]) {
       "v_add_f32_dpp %2, %6, %6 row_half_mirror row_mask:0xf bank_mask:0xa\n"
       "v_add_f32_dpp %3, %7, %7 row_half_mirror row_mask:0xf bank_mask:0xa\n"
       "s_nop 1"
-      : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7])
+      : "+&v"(v[0]), "+&v"(v[1]), "+&v"(v[2]), "+&v"(v[3]), "+&v"(v[4]), "+&v"(v[5]), "+&v"(v[6]), "+&v"(v[7])
       : "v"(v[8]), "v"(v[9]), "v"(v[10]), "v"(v[11]), "v"(v[12]), "v"(v[13]), "v"(v[14]), "v"(v[15]));
   auto bits = [](float f) { return __builtin_bit_cast(unsigned, f); };
 #pragma unroll
@@ -213,7 +215,8 @@ __device__ __forceinline__ Lane lane_of(const ScanArgs& A) {
 }
 
 // A [B][L][channels] tensor, seen from a workgroup: lane q's values of the steps t + 4 m + q of a tile of kTile steps, zeros
-// behind the sequence's length and the last channel (so x and dout, whatever memory holds there).  The tile's buffer is made of a pointer that moves with it and the steps left, by the same few scalar instructions for all.
+// behind the sequence's length and the last channel, whatever memory holds there.  The tile's buffer is made of a pointer that
+// moves with it and the steps left, by the same few scalar instructions for all.
 template <typename T, int kTile>
 struct Steps {
   const char* tile;     // the sequence's and workgroup's first channel in the tile's first step

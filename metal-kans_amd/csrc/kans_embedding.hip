@@ -103,6 +103,7 @@ constexpr int kHeld = 4 * kRound;  // tokens that stay in registers between coun
 // 16384 tokens by their frequency in a language, 65536 in all: 22 -> 15 us.
 constexpr int kAlone = 256, kShared = 512;
 constexpr int kMaxRange = 8192;
+constexpr int kMaxPiece = 64;  // positions of a piece at most
 constexpr int kMaxFill = 256;  // rows of a workgroup that writes zeros, a wave's counts one a lane
 
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const GradArgs A) {
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(256) void k_embed_join(const GradArgs A) {
   const int c = column(i, S, A.D);
   // the run's first position in the piece and its length give the piece in which it ends
   int begin = end - 1;
-  for (int half = A.piece; half > 0; half >>= 1)
+  for (int half = kMaxPiece; half > 0; half >>= 1)  // (powers of two, whatever the piece: they add up to any distance)
     if (begin - half >= first && A.token[begin - half] == key) begin -= half;
   const int last = (begin + A.count[key] - 1) / A.piece;
   float s[S];
@@ -374,7 +375,7 @@ EmbedPlan plan_embed(int esize, long n, int D, int V) {
   p.range = (V + 255) / 256;
   p.range = std::min(p.range, kMaxRange);
   p.groups = (V + p.range - 1) / p.range;
-  p.piece = (int)std::min(64L, std::max(8L, (n + 511) / 512 + 7 & ~7L));
+  p.piece = (int)std::min((long)kMaxPiece, std::max(8L, (n + 511) / 512 + 7 & ~7L));
   p.pieces = (int)((n + p.piece - 1) / p.piece);
   const int step = 16 / esize;
   p.wide = D >= step;

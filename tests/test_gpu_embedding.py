@@ -77,6 +77,22 @@ def test_frequent_tokens(cuda, n, d, v, hot):
     check(*inputs(n, d, v, torch.float32, hot=hot), 0.5)
 
 
+@pytest.mark.parametrize("n,each", [(12288, 48), (12288, 24), (12000, 25), (20000, 80), (20000, 41), (5000, 16), (5000, 23), (40000, 64), (30000, 57)])
+def test_runs_of_every_place(cuda, n, each):
+    """Equal tokens in runs that begin and end anywhere in the pieces of the sorted order (of 8 to 64 positions, no powers of two
+    among them): whole numbers, exact; the memory that partial rows may come from holds no numbers."""
+    import metal_kans as mk
+    v = -(-n // each)
+    tokens = (torch.arange(n, device="cuda") // each)[torch.randperm(n, generator=torch.Generator("cuda").manual_seed(1), device="cuda")]
+    dout = (torch.arange(n * 20, device="cuda").view(n, 20) % 5 - 2).float()
+    want = torch.zeros(v, 20, device="cuda").index_add_(0, tokens, dout)
+    w = torch.zeros(v, 20, device="cuda", requires_grad=True)
+    out = mk.embedding(tokens, w)
+    used = [torch.full((1 << 20,), float("nan"), device="cuda") for _ in range(3)]
+    del used
+    assert torch.equal(torch.autograd.grad(out, w, dout)[0], want)
+
+
 def test_large_vocabulary(cuda):
     """Beyond 256 workgroups of 8192 tokens each."""
     check(*inputs(300, 8, (1 << 21) + 77, torch.bfloat16, hot=0.2), 1.0)

@@ -10,7 +10,7 @@
 // inputs in registers; a tile reads W - 1 steps of its neighbour again.  Sums over steps and sequences: a tile writes
 // one partial row for each tap and the bias, and a second kernel adds the rows in a fixed order.  The inputs of the next 8
 // (backward 4) steps are under way while those before are computed; with one step at a time the kernels waited for memory.
-// bf16 8 x 2048 x 4096, 4 taps: forward 54 us (268 MB, 5.0 TB/s), with single steps 100; backward 90 (455 MB, 5.1 TB/s) and
+// bf16 8 x 2048 x 4096, 4 taps: forward 55 us (268 MB, 4.9 TB/s), with single steps 100; backward 80 (455 MB, 5.7 TB/s) and
 // 143, its reduction 7.
 #include <hip/hip_runtime.h>
 

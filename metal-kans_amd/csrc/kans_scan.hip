@@ -15,8 +15,9 @@
 // the recurrence's own: product, exponential, product and two sums for each four states) and 95 backward (24 for the states again,
 // 32 for the gradients, 17 for the sums of dB and dC over the channels).  Four lanes share a channel: with one, a
 // wave would have 64 channels and there would be too few waves; with 16, sums over the states would cost as much as the
-// recurrence.  bf16 8 x 2048 x 4096, 16 states: forward 346 us, backward 917 (80 % of the issue slots taken at 2.2 GHz), of
-// which the bytes alone take 160 and 280; 1 x 8192 x 1024 fp16 forward 46 us and 33 for the chunks' edges.
+// recurrence.  bf16 8 x 2048 x 4096, 16 states: forward 327 us, backward 858 (83 and 87 % of the issue slots taken, at 2.2 GHz),
+// of which the bytes alone take 160 and 280; 1 x 8192 x 1024 fp16 forward 44 us and 32 for the chunks' edges.  What lies
+// behind a sequence's end is cleared, not computed.
 // A batch of B sequences and D channels has B D / 16 waves.  Where those are too few for the card the sequence is cut in chunks: a
 // first pass runs each from a state of zeros for its last state (the decay over a chunk is exp(A sum s)), k_scan_join adds
 // these up to the state before each chunk, and the scan runs the chunks beside each other.

@@ -350,7 +350,7 @@ __device__ __forceinline__ float here(float v) {
 }
 
 // Where a grid has no more than two workgroups a CU, the two waves of a SIMD come first by turns.  The older one always came first,
-// was done early and left the other alone, which cannot use all cycles: forward of bf16 8 x 2048 x 4096 386 -> 359 us.
+// was done early and left the other alone, which cannot use all cycles: forward of bf16 8 x 2048 x 4096 386 -> 359 us then.
 // (Larger grids fill the places themselves: 3 % slower with turns.)  Workgroups go over the card's 256 CUs in order.
 __device__ __forceinline__ void take_turns(int tile) {
   if (gridDim.x > 512) return;

@@ -6,6 +6,8 @@
 // steps lie in LDS in fp32, a lane reads its own states' there.  Sums over the states go through the quad, four steps at
 // a time, so that lane q ends with the sum of step 4 m + q.
 #pragma once
+#include <algorithm>
+
 #include "kans_scan.h"
 #include "kans_tile.h"
 
@@ -716,21 +718,24 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
 }
 
 // ---- sums of the partial rows --------------------------------------------------------------------------
-// dB and dC: [blocks][B][L][2][padded] to [B][L][N] twice, zeros behind a sequence's length.
+// dB and dC: [blocks][B][L][2][padded] to [B][L][N] twice, zeros behind a sequence's length.  (Every kReduceBlocks workgroups: a
+// grid holds fewer than 2^32 threads.)
+constexpr long kReduceBlocks = 1 << 20;
 template <typename T>
 __global__ __launch_bounds__(256) void k_scan_reduce(const float* part, int blocks, long rows, int padded, int N, int L, const int64_t* lengths,
                                                      T* dB, T* dC) {
-  const long at = (long)blockIdx.x * 256 + threadIdx.x, all = rows * 2 * padded;
-  if (at >= all) return;
-  const int n = (int)(at % padded);
-  if (n >= N) return;
-  const long row = at / (2 * padded);
-  float s = 0.0f;
-  if (!lengths || row % L < lengths[row / L])
+  const long all = rows * 2 * padded;
+  for (long at = (long)blockIdx.x * 256 + threadIdx.x; at < all; at += kReduceBlocks * 256) {
+    const int n = (int)(at % padded);
+    if (n >= N) continue;
+    const long row = at / (2 * padded);
+    float s = 0.0f;
+    if (!lengths || row % L < lengths[row / L])
 #pragma unroll 8
-    for (int k = 0; k < blocks; ++k) s += part[k * all + at];
-  T* to = at / padded & 1 ? dC : dB;
-  if (to) to[row * N + n] = from_f32<T>(s);
+      for (int k = 0; k < blocks; ++k) s += part[k * all + at];
+    T* to = at / padded & 1 ? dC : dB;
+    if (to) to[row * N + n] = from_f32<T>(s);
+  }
 }
 
 template <typename T, int kRegs, bool kFull>
@@ -770,7 +775,7 @@ hipError_t launch_scan(ScanPass pass, const ScanArgs& A, hipStream_t st) {
 template <typename T>
 hipError_t reduce_scan(const ScanArgs& A, int padded, void* dB, void* dC, hipStream_t st) {
   const long rows = (long)A.B * A.L;
-  hipLaunchKernelGGL(k_scan_reduce<T>, dim3((unsigned)((rows * 2 * padded + 255) / 256)), dim3(256), 0, st, A.part_bc,
+  hipLaunchKernelGGL(k_scan_reduce<T>, dim3((unsigned)std::min(kReduceBlocks, (rows * 2 * padded + 255) / 256)), dim3(256), 0, st, A.part_bc,
                      (A.D + kScanChannels - 1) / kScanChannels, rows, padded, A.N, A.L, A.lengths, (T*)dB, (T*)dC);
   return hipGetLastError();
 }

@@ -406,6 +406,26 @@ def test_far_steps(cuda):
         assert torch.equal(call(one, state=s["state"].clone()), call(same, state=s["state"].clone()))
 
 
+def test_more_sums_than_threads(cuda):
+    """Partial rows of B's and C's gradients that are more than 2^32 numbers: one channel that forgets at once, 64 states."""
+    steps, n = (1 << 25) + 100, 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x, dt, dout = (torch.randn(1, steps, 1, device="cuda", dtype=torch.bfloat16, generator=g) for _ in range(3))
+    dt.fill_(1.0)
+    wide = [torch.empty(1, steps, n, device="cuda", dtype=torch.bfloat16).normal_(generator=g).requires_grad_(True) for _ in range(2)]
+    A = torch.full((1, n), -1000.0, device="cuda")
+    import metal_kans as mk
+    out = mk.selective_scan(x, dt, A, wide[0], wide[1], softplus=False)
+    dB, dC = torch.autograd.grad(out, wide, dout)
+    # (h = x B in each step, so dB = C dout x and dC = dout x B: two products in fp32 and a rounding)
+    for first in (0, steps // 2, steps - (1 << 16)):
+        at = slice(first, first + (1 << 16))
+        both = dout[:, at].double() * x[:, at].double()
+        for got, other in ((dB, wide[1]), (dC, wide[0])):
+            want = both * other.detach()[:, at].double()
+            assert bool(((got[:, at].double() - want).abs() <= want.abs() * (2 ** -8 + 4 * 2 ** -24) + 2 ** -126).all())
+
+
 def test_nothing(cuda):
     for b, l in ((0, 5), (2, 0)):
         s = inputs(b, l, 12, 16, torch.float32)

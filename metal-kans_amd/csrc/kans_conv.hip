@@ -282,8 +282,8 @@ int check_conv(int dtype, int B, int L, int D, int W, long x_batch = 0, long x_r
   if (B < 0 || L < 0 || D <= 0) return kans_fail(KANS_ERR_ARG, "bad dims B=%d L=%d D=%d", B, L, D);
   if (x_batch < 0 || x_row < 0) return kans_fail(KANS_ERR_ARG, "negative strides");
   if (W < 1 || W > kMaxTaps) return kans_fail(KANS_ERR_UNSUPPORTED, "%d taps, 1 to %d", W, kMaxTaps);
-  // (a grid holds fewer than 2^32 threads along x)
-  if (L > (1 << 30) || plan_conv(B, L, D).threads >= 1L << 31)
+  // (a grid holds fewer than 2^32 threads along x; the sums' has 1024 for 64 channels)
+  if (L > (1 << 30) || D > (1 << 27) || plan_conv(B, L, D).threads >= 1L << 31)
     return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
   return 0;
 }

@@ -96,7 +96,8 @@ extern "C" int kans_dropout(int dtype, const void* x, void* y, long n, double p,
   if (n < 0) return kans_fail(KANS_ERR_ARG, "bad dims n=%ld", n);
   if (!(p >= 0.0 && p <= 1.0)) return kans_fail(KANS_ERR_ARG, "p must be in [0, 1]");
   if (n && (!x || !y)) return kans_fail(KANS_ERR_ARG, "null argument");
-  if (n >= 1L << 34) return kans_fail(KANS_ERR_UNSUPPORTED, "n=%ld, fewer than 2^34 elements", n);  // (2^32 threads of 4)
+  // (a grid holds fewer than 2^32 threads, of 4 elements, and 256 of them are a workgroup)
+  if (n > (1L << 34) - 1024) return kans_fail(KANS_ERR_UNSUPPORTED, "n=%ld, up to 2^34 - 1024 elements", n);
   std::lock_guard<std::mutex> lk(kans_mutex());
   int rc = kans_ensure_init();
   if (rc) return rc;

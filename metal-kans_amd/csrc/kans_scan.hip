@@ -124,14 +124,14 @@ int check_scan(int dtype, int B, int L, int D, int N) {
   if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return kans_fail(KANS_ERR_ARG, "dtype %d", dtype);
   if (B < 0 || L < 0 || D <= 0 || N <= 0) return kans_fail(KANS_ERR_ARG, "bad dims B=%d L=%d D=%d N=%d", B, L, D, N);
   if (N > kMaxStates) return kans_fail(KANS_ERR_UNSUPPORTED, "%d states, up to %d", N, kMaxStates);
-  // (a grid holds fewer than 2^32 threads along x, a channel four)
+  // (a grid holds fewer than 2^32 threads along x, a channel four; the kernels reach 16 steps by offsets below 2^30 and the
+  // outputs have D elements a step)
   const long blocks = ((long)D + kScanChannels - 1) / kScanChannels;
-  if (L > (1 << 30) || (long)B * blocks >= 1L << 22 || (long)B * L * 2 * kMaxStates >= 1L << 38)
+  if (L > (1 << 30) || D >= 1 << 23 || (long)B * blocks >= 1L << 22 || (long)B * L * 2 * kMaxStates >= 1L << 38)
     return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
   return 0;
 }
 
-// The kernels reach 16 steps of a tensor by offsets below 2^30.
 int check_rows(std::initializer_list<long> batches, std::initializer_list<long> rows) {
   for (long b : batches)
     if (b < 0) return kans_fail(KANS_ERR_ARG, "%ld elements between sequences", b);
@@ -173,7 +173,7 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
   int rc = check_scan(dtype, B, L, D, N);
   if (rc || B == 0 || L == 0) return rc;
   if (!x || !dt || !A || !Bm || !Cm || !out) return kans_fail(KANS_ERR_ARG, "null argument");
-  if ((rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0, D}))) return rc;
+  if ((rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, p.edges * (long)sizeof(float)))) return rc;
   std::lock_guard<std::mutex> lk(kans_mutex());
@@ -211,7 +211,7 @@ int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_
   const bool any = B > 0 && L > 0;
   if (any && (!x || !dt || !A || !Bm || !Cm || !saved || !dout || !dx || !ddt || (z && !dz))) return kans_fail(KANS_ERR_ARG, "null argument");
   if ((dskip && !skip) || (dz && !z) || (ddt_bias && !dt_bias)) return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
-  if (any && (rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0, D}))) return rc;
+  if (any && (rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, (p.edges + p.part_bc + p.part_par) * (long)sizeof(float)))) return rc;
   std::lock_guard<std::mutex> lk(kans_mutex());

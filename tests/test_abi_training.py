@@ -165,3 +165,12 @@ def test_selective_scan_refusals(lib):
     assert lib.kans_selective_scan_workspace(2, 5, 4, 16, 0) == 0
     assert lib.kans_selective_scan_workspace(1, 700, 4, 16, 0) > 0
     assert lib.kans_selective_scan_saved(2, 17, 4, 16) == 2 * 2 * 4 * 16 * 4
+
+
+def test_grids_end_below_2_32_threads(lib):
+    """Sizes whose launches would have 2^32 threads or more are refused before anything is launched."""
+    assert lib.kans_dropout(0, 64, 64, (1 << 34) - 1023, 0.5, 1, None, None, 0, None) == -5
+    for d in ((1 << 27) + 1, 1 << 28):
+        assert lib.kans_causal_conv_workspace(0, 1, 1, d, 4) == -5 and lib.kans_causal_conv_workspace(0, 0, 0, d, 4) == -5
+    for b, n in ((1, 1), (1, 0), (0, 5)):
+        assert lib.kans_selective_scan_workspace(b, n, 1 << 23, 64, 1) == -5

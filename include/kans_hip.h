@@ -417,14 +417,15 @@ int kans_embedding_backward(int dtype, const int64_t* tokens, const void* dout, 
 
 /* Dropout of n elements: y[i] = 0 where r[i] < p 2^32, else x[i] / (1 - p), with r[i] word i % 4 of Philox4x32-10 under the key
  * `seed` at the counter whose low 64 bits are i / 4 and high 64 bits `offset`.  The key is *seed_dev (device memory) where that is
- * not null; seed_used (device memory, may be null) receives the key, for the same call on y's gradient. */
+ * not null; seed_used (device memory, may be null) receives the key, for the same call on y's gradient.  y may be x; n up to
+ * 2^34 - 1024. */
 int kans_dropout(int dtype, const void* x, void* y, long n, double p, int64_t seed, const int64_t* seed_dev, int64_t* seed_used,
                  int64_t offset, void* stream);
 
 /* Short causal convolution along the sequence, channel by channel, over B sequences of L steps and D channels of `dtype`:
  *   u[t] = bias + sum_j w[d][j] x[t - W + 1 + j],  y[t] = silu ? u[t] sigmoid(u[t]) : u[t],
  * w [D][W], W from 1 to 8; bias [D] or null.  Channels lie side by side; x_batch and x_row are elements between sequences and
- * between steps of x, y is contiguous.  Inputs before the first step are `state` [B][W - 1][D] (null: zeros), which becomes the last
+ * between steps of x, y is contiguous and apart from x.  L up to 2^30, D to 2^27.  Inputs before the first step are `state` [B][W - 1][D] (null: zeros), which becomes the last
  * W - 1 inputs of each sequence.  lengths [B] (device memory; null: L each): steps from a sequence's length on give zeros
  * and are not looked at. */
 int kans_causal_conv_forward(int dtype, const void* x, long x_batch, long x_row, const void* w, const void* bias, void* state,
@@ -441,7 +442,7 @@ int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row
  *   s[t] = softplus(dt[t] + dt_bias) (softplus 0: dt[t] + dt_bias),
  *   h[t] = exp(s[t] A) h[t-1] + s[t] x[t] Bm[t],  out[t] = (Cm[t] . h[t] + skip x[t]) (z[t] sigmoid(z[t])),
  * all in fp32.  x, dt, z and out [B][L][D], Bm and Cm [B][L][N] are of `dtype`, channels (states) side by side, *_batch and *_row
- * elements between sequences and between steps, out contiguous; A [D][N], skip [D], dt_bias [D] and state [B][D][N] are
+ * elements between sequences and (fewer than 2^23) between steps, out contiguous and apart from the inputs, D below 2^23; A [D][N], skip [D], dt_bias [D] and state [B][D][N] are
  * fp32.  skip, z and dt_bias may be null.  state (null: zeros) is the state before the first step
  * and becomes the one behind the last.  lengths as above: steps from a sequence's length on give zeros and leave the state.
  * saved (null: not wanted) is filled for the backward, kans_selective_scan_saved bytes.  The workspaces (16-byte aligned

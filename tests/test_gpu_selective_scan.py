@@ -515,3 +515,25 @@ def test_machinery(cuda, l):
         torch.autograd.grad(out, s["x"], s["dout"])
     with pytest.raises(RuntimeError, match="no gradients"):
         call(s, state=state)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("l,d,n,lengths", [(15, 20, 16, [15, 15]), (16, 20, 16, [16, 13]), (33, 20, 30, [33, 2]), (50, 20, 64, [47, 50]),
+                                           (701, 40, 16, [701, 333]), (700, 9, 5, [1, 700])])
+def test_the_last_step_may_be_infinite(cuda, l, d, n, lengths, dt, bad):
+    """An infinite or NaN input of a sequence's last step is in the state behind it, which no step's decay meets: dA, dx and all that
+    belongs to other steps keep their bits."""
+    s = inputs(2, l, d, n, dt, lengths=lengths)
+    for b, end in enumerate(lengths):
+        s["x"][b, end - 1, 7] = 0.0
+    want = train(s)
+    for b, end in enumerate(lengths):
+        s["x"][b, end - 1, 7] = bad
+    got = train(s)
+    for k in ("dA", "dx"):
+        assert got[k].isfinite().all() and torch.equal(got[k], want[k]), k
+    for b, end in enumerate(lengths):
+        assert not got["out"][b, end - 1, 7].isfinite() and not got["dC"][b, end - 1].isfinite().any()
+        for k in ("out", "ddt", "dz", "dB", "dC"):
+            assert torch.equal(got[k][b, :end - 1], want[k][b, :end - 1]) and not got[k][b, end:].any(), k

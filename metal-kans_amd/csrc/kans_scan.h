@@ -3,6 +3,8 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
+
 #include "kans_api_internal.h"
 
 namespace kans {
@@ -29,6 +31,10 @@ struct ScanArgs {
 };
 
 constexpr int kScanChannels = 64;  // of a workgroup
+
+// exp(s A) is the hardware's exponential of (s log2(e)) A: A log2(e) would overflow for the largest A, and a step of size zero must
+// leave the state as it is.  Minus infinity counts as the lowest number for the same reason.
+__device__ __forceinline__ float decay_of(float a) { return a == -__builtin_inff() ? -FLT_MAX : a; }
 
 // Registers of a lane for the states, four lanes a channel; steps between two saved states.
 inline int scan_regs(int N) {

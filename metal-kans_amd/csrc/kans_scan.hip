@@ -38,7 +38,7 @@ __global__ __launch_bounds__(64) void k_scan_join(const ScanArgs A, int padded, 
   const long b = at / states, to = at - b * states, d = to / padded;
   const int n = (int)(to - d * padded);
   if (n >= A.N) return;  // (zeros throughout)
-  const float a2 = A.A[d * A.N + n] * 1.44269504088896340736f;
+  const float a = decay_of(A.A[d * A.N + n]);
   float h = !backward && A.state ? A.state[(b * A.D + d) * A.N + n] : 0.0f;
   constexpr int kAhead = 16;  // chunks whose values are under way together
   for (int first = 0; first < A.chunks; first += kAhead) {
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(64) void k_scan_join(const ScanArgs A, int padded, 
       const long place = b * A.chunks + (backward ? A.chunks - 1 - first - i : first + i);
       A.edge[place * A.D * padded + to] = h;
       // (in two halves: a chunk may let a small state grow by more than fp32 holds; and nothing times that is nothing)
-      const float half = __builtin_amdgcn_exp2f(0.5f * a2 * s[i]), grown = half * (half * h);
+      const float half = __builtin_amdgcn_exp2f(0.5f * kLog2e * s[i] * a), grown = half * (half * h);
       h = (h == 0.0f ? 0.0f : grown) + e[i];
     }
   }

@@ -15,7 +15,6 @@ namespace kans {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -335,13 +334,13 @@ struct There {
   __device__ __forceinline__ float operator()(int i, float v) const { return kFull || is[i] ? v : 0.0f; }
 };
 
-// A lane's A log2(e).
+// A lane's A.
 template <int kRegs>
-__device__ __forceinline__ void load_decays(float (&a2)[kRegs], const ScanArgs& A, const Lane& l, int group) {
+__device__ __forceinline__ void load_decays(float (&a)[kRegs], const ScanArgs& A, const Lane& l, int group) {
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) {
     const int n = group * kRegs + i;
-    a2[i] = n < A.N ? A.A[(long)l.row * A.N + n] * kLog2e : 0.0f;
+    a[i] = n < A.N ? decay_of(A.A[(long)l.row * A.N + n]) : 0.0f;
   }
 }
 
@@ -372,9 +371,9 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   Steps<T, kTile> z(A.z, A.z_batch, A.z_row, l, l.t0, A.D), out(A.out, (long)A.L * A.D, A.D, l, l.t0, A.D);
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const unsigned mine = (unsigned)(l.in * kPad + l.q * kRegs) * 4;
-  float a2[kRegs], h[kRegs];
+  float a[kRegs], h[kRegs];
   const There<kRegs, kFull> there(A, l.q);
-  load_decays<kRegs>(a2, A, l, l.q);
+  load_decays<kRegs>(a, A, l, l.q);
   const long place = (long)l.b * A.chunks + l.chunk;
   float* state = A.state ? A.state + ((long)l.b * A.D + l.row) * A.N : nullptr;
 #pragma unroll
@@ -406,17 +405,18 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
   int t = l.t0;
   for (int turn = 0; t < min(l.t1, l.len); t += kTile, turn ^= 1) {
     take_turns(t / kTile);
-    float s[kM], u[kM], xs[kM], gate[kM];
+    float s2[kM], u[kM], xs[kM], gate[kM];  // s2: the step size times log2(e)
     const int left = l.len - t - l.q;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
       const bool counts = 4 * m < left;
       const float v = to_f32(dv[m]) + bias, soft = here(softplus(v));
-      s[m] = counts ? (A.softplus ? soft : v) : 0.0f;  // (no step: the state stays)
+      const float s = counts ? (A.softplus ? soft : v) : 0.0f;  // (no step: the state stays)
+      s2[m] = s * kLog2e;
       xs[m] = to_f32(xv[m]);
-      u[m] = s[m] * xs[m];
+      u[m] = s * xs[m];
       gate[m] = 1.0f;
-      if (kEdges) total += s[m];
+      if (kEdges) total += s;
       else if (kGated) gate[m] = to_f32(zv[m]) * sigmoid(to_f32(zv[m]));
     }
     // (behind the chunk's last tile the reads are another chunk's, or nothing)
@@ -439,7 +439,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_fwd(const ScanArgs A) {
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < kRegs; ++i) {
-          h[i] = there(i, __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]) * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i]);
+          h[i] = there(i, __builtin_amdgcn_exp2f(of_lane<k>(s2[m]) * a[i]) * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i]);
           if (!kEdges) sum += h[i] * now.C[j - g * kAhead][i];
         }
         y[k] = sum;
@@ -488,9 +488,9 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
   const float bias = A.bias ? A.bias[l.row] : 0.0f, skip = A.skip ? A.skip[l.row] : 0.0f;
   const int group = states_of(threadIdx.x);  // of the lane's states
   const unsigned mine = (unsigned)(l.in * kPad + group * kRegs) * 4;
-  float a2[kRegs], carry[kRegs], dA[kRegs] = {}, dskip = 0.0f, dbias = 0.0f, total = 0.0f;
+  float a[kRegs], carry[kRegs], dA[kRegs] = {}, dskip = 0.0f, dbias = 0.0f, total = 0.0f;
   const There<kRegs, kFull> is_there(A, group);
-  load_decays<kRegs>(a2, A, l, group);
+  load_decays<kRegs>(a, A, l, group);
   const long place = (long)l.b * A.chunks + l.chunk;
 #pragma unroll
   for (int i = 0; i < kRegs; ++i) carry[i] = 0.0f;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
     const int t = l.t0 + tile * kTile;
     take_turns(tile);
     // dzs: dout times silu's slope, slope: the step size's
-    float s[kM], u[kM], xs[kM], dy[kM], dzs[kM], slope[kM], h[kRegs];
+    float s[kM], s2[kM], u[kM], xs[kM], dy[kM], dzs[kM], slope[kM], h[kRegs];
     const int left = l.len - t - l.q;
 #pragma unroll
     for (int m = 0; m < kM; ++m) {
@@ -540,6 +540,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
       float sig;
       const float soft = here(softplus(v, sig));
       s[m] = counts ? (A.softplus ? soft : v) : 0.0f;
+      s2[m] = s[m] * kLog2e;
       slope[m] = A.softplus ? here(sig) : 1.0f;  // (of the length's end on it meets zeros)
       xs[m] = to_f32(xv[m]);
       u[m] = s[m] * xs[m];
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           float sum = 0.0f;
 #pragma unroll
           for (int i = 0; i < kRegs; ++i) {
-            stay[j][i] = __builtin_amdgcn_exp2f(of_lane<k>(s[m]) * a2[i]);
+            stay[j][i] = __builtin_amdgcn_exp2f(of_lane<k>(s2[m]) * a[i]);
             if constexpr (!kEdges) {
               before[j][i] = h[i];
               h[i] = is_there(i, stay[j][i] * h[i] + of_lane<k>(u[m]) * now.B[j - g * kAhead][i]);
@@ -606,7 +607,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           if constexpr (!kEdges) {
             sB += gr[i] * now.B[j - g * kAhead][i];
             const float w = kWhole || j < l.len - t ? carry[i] * before[j][i] : 0.0f;
-            sA += w * a2[i];
+            sA += w * a[i];
             dA_tile[i] += w * of_lane<k>(s[m]);
           }
         }
@@ -622,7 +623,7 @@ __global__ __launch_bounds__(kThreads, kRegs <= 8 ? 2 : 1) void k_scan_bwd(const
           for (int i = 0; i < kRegs; ++i) h[i] = before[j][i];
           if constexpr (k == 0) __builtin_amdgcn_sched_barrier(0);
           if constexpr (k == 0) {
-            const float gB = quad_sums(of_b), gA = quad_sums(of_a) * kLn2;
+            const float gB = quad_sums(of_b), gA = quad_sums(of_a);
             const bool counts = 4 * m < left;
             const float ddtv = counts ? (xs[m] * gB + gA) * slope[m] : 0.0f;
             dskip += dy[m] * xs[m];
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
   const float x = to_f32(((const T*)A.x)[b * A.x_batch + c]);
   float s = to_f32(((const T*)A.dt)[b * A.dt_batch + c]) + (A.bias ? A.bias[c] : 0.0f);
   if (A.softplus) s = softplus(s);
-  const float u = s * x;
+  const float u = s * x, s2 = s * kLog2e;
   const T *Bm = (const T*)A.Bm + b * A.b_batch, *Cm = (const T*)A.Cm + b * A.c_batch;
   float* h = A.state + row * A.N;
   const float* a = A.A + (long)c * A.N;
@@ -697,7 +698,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
       float hs[4] = {hv.x, hv.y, hv.z, hv.w}, as[4] = {av.x, av.y, av.z, av.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        hs[i] = fmaf(__builtin_amdgcn_exp2f(s * (as[i] * kLog2e)), hs[i], u * to_f32(Bm[n + i]));
+        hs[i] = fmaf(__builtin_amdgcn_exp2f(s2 * decay_of(as[i])), hs[i], u * to_f32(Bm[n + i]));
         y = fmaf(hs[i], to_f32(Cm[n + i]), y);
       }
       if (counts && at < all) *(float4*)(h + n) = make_float4(hs[0], hs[1], hs[2], hs[3]);
@@ -705,7 +706,7 @@ __global__ __launch_bounds__(kThreads) void k_scan_step(const ScanArgs A) {
   } else {  // (the same operations in the same order)
     for (int first = 4 * q; first < A.N; first += 16)
       for (int n = first; n < min(first + 4, A.N); ++n) {
-        const float v = fmaf(__builtin_amdgcn_exp2f(s * (a[n] * kLog2e)), h[n], u * to_f32(Bm[n]));
+        const float v = fmaf(__builtin_amdgcn_exp2f(s2 * decay_of(a[n])), h[n], u * to_f32(Bm[n]));
         y = fmaf(v, to_f32(Cm[n]), y);
         if (counts && at < all) h[n] = v;
       }

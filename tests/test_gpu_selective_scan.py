@@ -537,3 +537,30 @@ def test_the_last_step_may_be_infinite(cuda, l, d, n, lengths, dt, bad):
         assert not got["out"][b, end - 1, 7].isfinite() and not got["dC"][b, end - 1].isfinite().any()
         for k in ("out", "ddt", "dz", "dB", "dC"):
             assert torch.equal(got[k][b, :end - 1], want[k][b, :end - 1]) and not got[k][b, end:].any(), k
+
+
+@pytest.mark.parametrize("l,lengths", [(1, None), (1, [0, 1]), (15, None), (40, [17, 0]), (333, None), (333, [100, 333])])
+def test_the_largest_decays(cuda, l, lengths):
+    """A of the type's lowest value: a step leaves nothing of the state, none (behind a length, or of size zero) all of it.
+    Minus infinity is the same for steps of any size."""
+    lowest = torch.finfo(torch.float32).min
+    for softplus in (True, False):
+        s = inputs(2, l, 20, 16, torch.float32, lengths=lengths, without=() if softplus else ("dt_bias",))
+        s["A"][3], s["A"][4], s["A"][5, ::2] = lowest, -2.5e38, lowest
+        if not softplus:
+            s["dt"] = s["dt"].abs()
+            s["dt"][0, ::3] = 0.0
+        got, want = train(s, softplus), reference(s, softplus)
+        for k in got:
+            if softplus or k != "ddt":   # (A times a state that a step of size zero leaves is beyond fp32)
+                near(got[k], want, k, torch.float32)
+        state = s["state"].clone()
+        with torch.no_grad():
+            out = call(s, softplus, state=state)
+            want = reference(s, softplus, state=True, backward=False)
+            near(out, want, "out", torch.float32)
+            near(state, want, "state", torch.float32)
+            if softplus:
+                again = s["state"].clone()
+                infinite = {**s, "A": torch.where(s["A"] < -2e38, float("-inf"), s["A"])}
+                assert torch.equal(call(infinite, state=again), out) and torch.equal(again, state)

@@ -442,7 +442,7 @@ int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row
  *   s[t] = softplus(dt[t] + dt_bias) (softplus 0: dt[t] + dt_bias),
  *   h[t] = exp(s[t] A) h[t-1] + s[t] x[t] Bm[t],  out[t] = (Cm[t] . h[t] + skip x[t]) (z[t] sigmoid(z[t])),
  * all in fp32.  x, dt, z and out [B][L][D], Bm and Cm [B][L][N] are of `dtype`, channels (states) side by side, *_batch and *_row
- * elements between sequences and (fewer than 2^23) between steps, out contiguous and apart from the inputs, D below 2^23; A [D][N], skip [D], dt_bias [D] and state [B][D][N] are
+ * elements between sequences and between steps (fewer than 2^23; 0, or no fewer than a step has), out contiguous and apart from the inputs, D below 2^23; A [D][N], skip [D], dt_bias [D] and state [B][D][N] are
  * fp32.  skip, z and dt_bias may be null.  state (null: zeros) is the state before the first step
  * and becomes the one behind the last.  lengths as above: steps from a sequence's length on give zeros and leave the state.
  * saved (null: not wanted) is filled for the backward, kans_selective_scan_saved bytes.  The workspaces (16-byte aligned

@@ -132,11 +132,19 @@ int check_scan(int dtype, int B, int L, int D, int N) {
   return 0;
 }
 
-int check_rows(std::initializer_list<long> batches, std::initializer_list<long> rows) {
-  for (long b : batches)
-    if (b < 0) return kans_fail(KANS_ERR_ARG, "%ld elements between sequences", b);
-  for (long r : rows)
-    if (r < 0 || r >= 1L << 23) return kans_fail(KANS_ERR_UNSUPPORTED, "%ld elements between steps, fewer than 2^23", r);
+// Elements between sequences and between the L steps of `width` channels or states.  (Steps in each other's memory would be read
+// behind a length, where a buffer's end is to give zeros.)
+struct Rows {
+  long batch, row;
+  int width;
+};
+int check_rows(int L, std::initializer_list<Rows> tensors) {
+  for (const Rows& t : tensors) {
+    if (t.batch < 0) return kans_fail(KANS_ERR_ARG, "%ld elements between sequences", t.batch);
+    if (t.row < 0 || t.row >= 1L << 23) return kans_fail(KANS_ERR_UNSUPPORTED, "%ld elements between steps, fewer than 2^23", t.row);
+    if (L > 1 && t.row > 0 && t.row < t.width)
+      return kans_fail(KANS_ERR_UNSUPPORTED, "%ld elements between steps of %d: 0, or at least these", t.row, t.width);
+  }
   return 0;
 }
 
@@ -173,7 +181,8 @@ int kans_selective_scan_forward(int dtype, const void* x, long x_batch, long x_r
   int rc = check_scan(dtype, B, L, D, N);
   if (rc || B == 0 || L == 0) return rc;
   if (!x || !dt || !A || !Bm || !Cm || !out) return kans_fail(KANS_ERR_ARG, "null argument");
-  if ((rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0}))) return rc;
+  if ((rc = check_rows(L, {{x_batch, x_row, D}, {dt_batch, dt_row, D}, {b_batch, b_row, N}, {c_batch, c_row, N},
+                          {z ? z_batch : 0, z ? z_row : 0, D}}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, p.edges * (long)sizeof(float)))) return rc;
   std::lock_guard<std::mutex> lk(kans_mutex());
@@ -211,7 +220,8 @@ int kans_selective_scan_backward(int dtype, const void* x, long x_batch, long x_
   const bool any = B > 0 && L > 0;
   if (any && (!x || !dt || !A || !Bm || !Cm || !saved || !dout || !dx || !ddt || (z && !dz))) return kans_fail(KANS_ERR_ARG, "null argument");
   if ((dskip && !skip) || (dz && !z) || (ddt_bias && !dt_bias)) return kans_fail(KANS_ERR_ARG, "gradient of an input that is not there");
-  if (any && (rc = check_rows({x_batch, dt_batch, b_batch, c_batch, z ? z_batch : 0}, {x_row, dt_row, b_row, c_row, z ? z_row : 0}))) return rc;
+  if (any && (rc = check_rows(L, {{x_batch, x_row, D}, {dt_batch, dt_row, D}, {b_batch, b_row, N}, {c_batch, c_row, N},
+                          {z ? z_batch : 0, z ? z_row : 0, D}}))) return rc;
   const ScanPlan p = plan_scan(B, L, D, N);
   if ((rc = check_workspace(workspace, workspace_bytes, (p.edges + p.part_bc + p.part_par) * (long)sizeof(float)))) return rc;
   std::lock_guard<std::mutex> lk(kans_mutex());

@@ -612,9 +612,10 @@ std::optional<Tensor> causal_conv(const Tensor& x, const Tensor& w, const std::o
 }
 
 // ---- selective_scan --------------------------------------------------------------------------------
-// (the scan's kernels take fewer than 2^23 elements between steps)
+// (the scan's kernels take fewer than 2^23 elements between steps, and steps that are the same or apart)
 Tensor with_steps(const Tensor& t) {
-  return (t.size(2) == 1 || t.stride(2) == 1) && (t.size(1) <= 1 || t.stride(1) < 1 << 23) ? t : t.contiguous();
+  const bool steps = t.size(1) <= 1 || t.stride(1) == 0 || (t.stride(1) >= t.size(2) && t.stride(1) < 1 << 23);
+  return (t.size(2) == 1 || t.stride(2) == 1) && steps ? t : t.contiguous();
 }
 
 struct Scan {

@@ -174,3 +174,19 @@ def test_grids_end_below_2_32_threads(lib):
         assert lib.kans_causal_conv_workspace(0, 1, 1, d, 4) == -5 and lib.kans_causal_conv_workspace(0, 0, 0, d, 4) == -5
     for b, n in ((1, 1), (1, 0), (0, 5)):
         assert lib.kans_selective_scan_workspace(b, n, 1 << 23, 64, 1) == -5
+
+
+def test_scan_refuses_steps_in_each_others_memory(lib):
+    def rows(x=4, dt=4, b=16, c=16, z=4, n=300):   # (more than one step without a workspace: nothing is launched)
+        return lib.kans_selective_scan_forward(0, 64, 20, x, 64, 20, dt, 64, 64, 80, b, 64, 80, c, None, 64, 20, z, None, 1, None, None, 64,
+                                               None, 2, n, 4, 16, None, 0, None)
+
+    def back(x=4, b=16):
+        return lib.kans_selective_scan_backward(0, 64, 20, x, 64, 20, 4, 64, 64, 80, b, 64, 80, 16, None, None, 0, 0, None, 1, None, 64, 64, 64,
+                                                64, 64, 64, 64, None, None, None, 2, 300, 4, 16, None, 0, None)
+    for good in (dict(), dict(x=0, b=0), dict(x=5, dt=9, z=100, b=17, c=(1 << 23) - 1)):
+        assert rows(**good) == -1, good
+    assert back() == -1 and back(x=0, b=0) == -1
+    for bad in (dict(x=1), dict(x=3), dict(dt=3), dict(b=15), dict(c=1), dict(z=2), dict(c=1 << 23)):
+        assert rows(**bad) == -5, bad
+    assert back(x=3) == -5 and back(b=15) == -5

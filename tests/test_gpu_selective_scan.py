@@ -564,3 +564,31 @@ def test_the_largest_decays(cuda, l, lengths):
                 again = s["state"].clone()
                 infinite = {**s, "A": torch.where(s["A"] < -2e38, float("-inf"), s["A"])}
                 assert torch.equal(call(infinite, state=again), out) and torch.equal(again, state)
+
+
+def test_steps_that_share_memory(cuda):
+    """Steps that lie in each other's memory, an infinite or NaN input among them: it stays with its own steps and channels, though
+    what lies behind a length is another step's channel."""
+    names = ("x", "B", "C")
+    for dt in TYPES:
+        for l, lengths in ((40, [21, 9]), (333, [100, 333]), (37, None)):
+            for name in names:
+                for bad in (float("inf"), float("nan")):
+                    s = inputs(2, l, 20, 16, dt, lengths=lengths)
+                    gen = torch.Generator("cuda").manual_seed(5)
+                    for k in ("x", "dt", "B", "C", "z"):
+                        width = s[k].shape[2]
+                        long = torch.randn(2, l + width, device="cuda", generator=gen).to(dt)
+                        if k == name:    # (the last step's last but two)
+                            for b in range(2):
+                                long[b, (lengths[b] if lengths else l) - 1 + width - 3] = bad
+                        s[k] = long.as_strided((2, l, width), (long.stride(0), 1, 1))
+                    apart = {k: v.contiguous() if k in ("x", "dt", "B", "C", "z") else v for k, v in s.items()}
+                    want, got = train(apart), train(s)
+                    for k in want:
+                        assert torch.equal(got[k].nan_to_num(7.0, 8.0, 9.0), want[k].nan_to_num(7.0, 8.0, 9.0)), (name, k)
+                    state, other = s["state"].clone(), s["state"].clone()
+                    with torch.no_grad():
+                        call(s, state=state)
+                        call(apart, state=other)
+                    assert torch.equal(state.nan_to_num(7.0, 8.0, 9.0), other.nan_to_num(7.0, 8.0, 9.0)), name

@@ -425,7 +425,8 @@ int kans_dropout(int dtype, const void* x, void* y, long n, double p, int64_t se
 /* Short causal convolution along the sequence, channel by channel, over B sequences of L steps and D channels of `dtype`:
  *   u[t] = bias + sum_j w[d][j] x[t - W + 1 + j],  y[t] = silu ? u[t] sigmoid(u[t]) : u[t],
  * w [D][W], W from 1 to 8; bias [D] or null.  Channels lie side by side; x_batch and x_row are elements between sequences and
- * between steps of x, y is contiguous and apart from x.  L up to 2^30, D to 2^27.  Inputs before the first step are `state` [B][W - 1][D] (null: zeros), which becomes the last
+ * between steps of x, y is contiguous and apart from x.  L up to 2^30, D to 2^27, and B ceil(L / 64) ceil(D / 4), for D below 4
+ * B ceil(L / 64) D, below 2^31.  Inputs before the first step are `state` [B][W - 1][D] (null: zeros), which becomes the last
  * W - 1 inputs of each sequence.  lengths [B] (device memory; null: L each): steps from a sequence's length on give zeros
  * and are not looked at. */
 int kans_causal_conv_forward(int dtype, const void* x, long x_batch, long x_row, const void* w, const void* bias, void* state,
@@ -442,9 +443,10 @@ int kans_causal_conv_backward(int dtype, const void* x, long x_batch, long x_row
  *   s[t] = softplus(dt[t] + dt_bias) (softplus 0: dt[t] + dt_bias),
  *   h[t] = exp(s[t] A) h[t-1] + s[t] x[t] Bm[t],  out[t] = (Cm[t] . h[t] + skip x[t]) (z[t] sigmoid(z[t])),
  * all in fp32.  x, dt, z and out [B][L][D], Bm and Cm [B][L][N] are of `dtype`, channels (states) side by side, *_batch and *_row
- * elements between sequences and between steps (fewer than 2^23; 0, or no fewer than a step has), out contiguous and apart from the inputs, D below 2^23; A [D][N], skip [D], dt_bias [D] and state [B][D][N] are
- * fp32.  skip, z and dt_bias may be null.  state (null: zeros) is the state before the first step
- * and becomes the one behind the last.  lengths as above: steps from a sequence's length on give zeros and leave the state.
+ * elements between sequences and between steps (fewer than 2^23; 0, or no fewer than a step has), out contiguous and apart
+ * from the inputs; D below 2^23, L up to 2^30, B ceil(D / 64) below 2^22 and B L below 2^31.  A [D][N], skip [D], dt_bias [D] and
+ * state [B][D][N] are fp32.  skip, z and dt_bias may be null.  state (null: zeros) is the state before the first step and
+ * becomes the one behind the last.  lengths as above: steps from a sequence's length on give zeros and leave the state.
  * saved (null: not wanted) is filled for the backward, kans_selective_scan_saved bytes.  The workspaces (16-byte aligned
  * device memory, kans_selective_scan_workspace bytes, which may be 0) are negative for refused sizes. */
 long kans_selective_scan_saved(int B, int L, int D, int N);

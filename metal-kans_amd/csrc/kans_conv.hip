@@ -265,12 +265,13 @@ struct ConvPlan {
   int tile, tiles, v, vecs;
   long threads;
 };
+constexpr int kTile = 64;
 // v: channels of a thread.
 ConvPlan plan_conv(int B, int L, int D) {
   ConvPlan p{};
   p.v = D < 4 ? 1 : 4;
   p.vecs = (D + p.v - 1) / p.v;
-  p.tile = 64;
+  p.tile = kTile;
   while (p.tile > 8 && (long)B * ((L + p.tile - 1) / p.tile) * p.vecs < 256L * 256) p.tile /= 2;
   p.tiles = (L + p.tile - 1) / p.tile;
   p.threads = (long)B * p.tiles * p.vecs;
@@ -282,8 +283,10 @@ int check_conv(int dtype, int B, int L, int D, int W, long x_batch = 0, long x_r
   if (B < 0 || L < 0 || D <= 0) return kans_fail(KANS_ERR_ARG, "bad dims B=%d L=%d D=%d", B, L, D);
   if (x_batch < 0 || x_row < 0) return kans_fail(KANS_ERR_ARG, "negative strides");
   if (W < 1 || W > kMaxTaps) return kans_fail(KANS_ERR_UNSUPPORTED, "%d taps, 1 to %d", W, kMaxTaps);
-  // (a grid holds fewer than 2^32 threads along x; the sums' has 1024 for 64 channels)
-  if (L > (1 << 30) || D > (1 << 27) || plan_conv(B, L, D).threads >= 1L << 31)
+  // (a grid holds fewer than 2^32 threads along x; the sums' has 1024 for 64 channels.  Tiles are shorter than kTile only where
+  // there are few threads.  By division: the product may pass 64 bits.)
+  const long rows = (long)B * ((L + (long)kTile - 1) / kTile), vecs = D < 4 ? D : (D + 3L) / 4;
+  if (L > (1 << 30) || D > (1 << 27) || rows > ((1L << 31) - 1) / vecs)
     return kans_fail(KANS_ERR_UNSUPPORTED, "B=%d L=%d D=%d fit no grid", B, L, D);
   return 0;
 }

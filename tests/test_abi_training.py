@@ -190,3 +190,19 @@ def test_scan_refuses_steps_in_each_others_memory(lib):
     for bad in (dict(x=1), dict(x=3), dict(dt=3), dict(b=15), dict(c=1), dict(z=2), dict(c=1 << 23)):
         assert rows(**bad) == -5, bad
     assert back(x=3) == -5 and back(b=15) == -5
+
+
+def test_conv_sizes_whose_product_passes_64_bits(lib):
+    """Threads counted modulo 2^64 would be few, or none."""
+    for b, l, d in ((1 << 24, 1 << 30, 1 << 18), (1 << 22, 1 << 27, 1 << 26), ((1 << 31) - 1, 1 << 30, 1 << 27), (1 << 30, 1 << 30, 1 << 20),
+                    ((1 << 31) - 1, 1, 1 << 20), (1 << 20, 1 << 30, 4)):
+        for dt in (0, 1, 2):
+            assert lib.kans_causal_conv_workspace(dt, b, l, d, 4) == -5, (b, l, d)
+            assert lib.kans_causal_conv_forward(dt, 64, 0, 0, 64, None, None, None, 1, 64, b, l, d, 4, None) == -5
+            assert lib.kans_causal_conv_backward(dt, 64, 0, 0, 64, None, None, 1, 64, 64, 64, None, b, l, d, 4, 64, 1 << 62, None) == -5
+    assert lib.kans_causal_conv_workspace(0, (1 << 31) - 1, 0, 1 << 27, 4) == 0    # (no steps, no work)
+    # the largest that are taken, and the first beyond: 2^31 threads, of 4 channels and up to 64 steps
+    assert lib.kans_causal_conv_workspace(0, 32, 1 << 30, 4, 4) > 0 and lib.kans_causal_conv_workspace(0, 127, 1 << 30, 4, 4) > 0
+    assert lib.kans_causal_conv_workspace(0, 128, 1 << 30, 4, 4) == -5
+    assert lib.kans_causal_conv_workspace(0, (1 << 31) - 1, 1, 4, 4) > 0
+    assert lib.kans_causal_conv_workspace(0, (1 << 31) - 1, 1, 8, 4) == -5

@@ -142,17 +142,40 @@ void no_tangents(std::initializer_list<const Tensor*> inputs, const char* what) 
 // A backward under capture hands its gradients to the streams of the nodes before it.  Where one of these is the default
 // stream -- an eager graph of the same leaf still lives and with it the node that collects the leaf's gradient -- the
 // capture is torn and the process ends at its end: refused here, while there is a call to name.
+bool capturing(c10::DeviceIndex device) {
+  const auto current = c10::hip::getCurrentHIPStream(device);
+  if (!current.stream()) return false;  // (the default stream is never under capture)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(current.stream(), &status) == hipSuccess && status != hipStreamCaptureStatusNone;
+}
+void refuse_default_stream(torch::autograd::Node* node, const char* what) {
+  const auto stream = node ? node->stream() : std::nullopt;
+  TORCH_CHECK(!stream || stream->id() != 0, what,
+              " under a graph capture: an autograd graph from outside of it, on the default stream, still holds an input; delete it first");
+}
+
+// In the forward: the nodes of the inputs as they are given.  (A copy in another layout has a node of its own.)
 void capturable(std::initializer_list<const Tensor*> inputs, const char* what) {
   for (const Tensor* t : inputs) {
     if (!t->defined() || !t->requires_grad()) continue;
-    const auto current = c10::hip::getCurrentHIPStream(t->get_device());
-    if (!current.stream()) return;  // (the default stream is never under capture)
-    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
-    const auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!stream || stream->id() != 0, what,
-                " under a graph capture: an autograd graph from outside of it, on the default stream, still holds an input; delete it first");
+    if (!capturing(t->get_device())) return;
+    refuse_default_stream((t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t)).get(), what);
+  }
+}
+
+// In the backward, before it hands anything on: all nodes that its gradients reach.
+void capturable_behind(const Tensor& grad, const char* what) {
+  if (!capturing(grad.get_device())) return;
+  const auto self = torch::autograd::get_current_node();
+  std::vector<torch::autograd::Node*> next{self.get()};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!next.empty()) {
+    torch::autograd::Node* const node = next.back();
+    next.pop_back();
+    if (!node || !seen.insert(node).second) continue;
+    if (node != self.get()) refuse_default_stream(node, what);
+    for (uint32_t i = 0; i < node->num_outputs(); ++i)
+      if (node->task_should_compute_output(i)) next.push_back(node->next_edge(i).function.get());
   }
 }
 
@@ -434,6 +457,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     at::NoGradGuard no_grad;
     if (!grads[0].defined()) return variable_list(4);
     no_tangents({&grads[0]}, "embedding's backward");
+    capturable_behind(grads[0], "embedding's backward");
     const auto s = ctx->get_saved_variables();
     const auto rest = ctx->saved_data["rest"].toIntVector();
     const Tensor dout = grads[0].contiguous(), &tokens = s[0];
@@ -461,7 +485,7 @@ std::optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, doub
   no_tangents({&w}, "embedding");
   const at::OptionalDeviceGuard device(w.device());
   if (!wants_grad({&w})) return EmbeddingFunction::call(t, w, scale, ignore);
-  capturable({&w}, "embedding");
+  capturable({&weight}, "embedding");
   return EmbeddingFunction::apply(t, w, scale, ignore)[0];
 }
 
@@ -491,6 +515,7 @@ struct DropoutFunction : torch::autograd::Function<DropoutFunction> {
     at::NoGradGuard no_grad;
     if (!grads[0].defined()) return variable_list(5);
     no_tangents({&grads[0]}, "dropout's backward");
+    capturable_behind(grads[0], "dropout's backward");
     const auto rest = ctx->saved_data["rest"].toIntVector();
     const Tensor dy = grads[0].contiguous();
     const at::OptionalDeviceGuard device(dy.device());
@@ -508,7 +533,7 @@ std::optional<Tensor> dropout(const Tensor& x, double p, int64_t seed, const std
   no_tangents({&in}, "dropout");
   const at::OptionalDeviceGuard device(in.device());
   if (!wants_grad({&in})) return DropoutFunction::call(in, p, seed, dev ? *dev : Tensor(), Tensor(), offset);
-  capturable({&in}, "dropout");
+  capturable({&x}, "dropout");
   return DropoutFunction::apply(in, p, seed, dev, offset)[0];
 }
 
@@ -571,6 +596,7 @@ struct ConvFunction : torch::autograd::Function<ConvFunction> {
     variable_list d(5);
     if (!grads[0].defined()) return d;
     no_tangents({&grads[0]}, "causal_conv's backward");
+    capturable_behind(grads[0], "causal_conv's backward");
     const auto s = ctx->get_saved_variables();
     const at::OptionalDeviceGuard device(s[0].device());
     const Conv c{s[0], s[1], s[2], s[3], ctx->saved_data["silu"].toBool()};
@@ -601,7 +627,8 @@ std::optional<Tensor> causal_conv(const Tensor& x, const Tensor& w, const std::o
   const at::OptionalDeviceGuard device(x.device());
   if (wants_grad({&c.x, &c.w, &c.bias})) {
     TORCH_CHECK(!state, "causal_conv with a state has no gradients: call it under torch.no_grad()");
-    capturable({&c.x, &c.w, &c.bias}, "causal_conv");
+    const Tensor b = given(bias);
+    capturable({&x, &w, &b}, "causal_conv");
     return ConvFunction::apply(c.x, c.w, maybe(c.bias), maybe(c.lengths), c.silu)[0];
   }
   TORCH_CHECK(!state || !(at::GradMode::is_enabled() && state->requires_grad()),
@@ -686,6 +713,7 @@ struct ScanFunction : torch::autograd::Function<ScanFunction> {
     variable_list d(10);
     if (!grads[0].defined()) return d;
     no_tangents({&grads[0]}, "selective_scan's backward");
+    capturable_behind(grads[0], "selective_scan's backward");
     const auto s = ctx->get_saved_variables();
     const at::OptionalDeviceGuard device(s[0].device());
     const Scan scan{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], ctx->saved_data["softplus"].toBool()};
@@ -724,7 +752,8 @@ std::optional<Tensor> selective_scan(const Tensor& x, const Tensor& dt, const Te
   const at::OptionalDeviceGuard device(x.device());
   if (wants_grad({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias})) {
     TORCH_CHECK(!state, "selective_scan with a state has no gradients: call it under torch.no_grad()");
-    capturable({&s.x, &s.dt, &s.A, &s.B, &s.C, &s.skip, &s.z, &s.bias}, "selective_scan");
+    const Tensor rest[] = {given(skip), given(z), given(bias)};
+    capturable({&x, &dt, &A, &B, &C, &rest[0], &rest[1], &rest[2]}, "selective_scan");
     return ScanFunction::apply(s.x, s.dt, s.A, s.B, s.C, maybe(s.skip), maybe(s.z), maybe(s.bias), maybe(s.lengths), softplus)[0];
   }
   TORCH_CHECK(!state || !(at::GradMode::is_enabled() && state->requires_grad()),

@@ -280,6 +280,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     const Tensor dy = grads.size() == 2 ? grads[0] : Tensor(), dh = grads.back();
     if (!dy.defined() && !dh.defined()) return d;
     no_tangents({&dy, &dh}, "residual_norm's backward");
+    capturable_behind(dy.defined() ? dy : dh, "residual_norm's backward");
     const Norm n{s[0], s[1], s[2], s[3], s[4], s[5], numbers[0], rest[0], (int)rest[1], numbers[1], (at::ScalarType)rest[2]};
     std::array<bool, 6> need;
     for (size_t i = 0, edge = 0; i < 6; ++i) need[i] = s[i].defined() && ctx->needs_input_grad(edge++);
@@ -404,6 +405,7 @@ struct XentFunction : torch::autograd::Function<XentFunction> {
     const auto s = ctx->get_saved_variables();
     const auto rest = ctx->saved_data["rest"].toIntVector();
     no_tangents({&grads[0]}, "linear_cross_entropy's backward");
+    capturable_behind(grads[0], "linear_cross_entropy's backward");
     const Xent x{s[0], s[1], s[2], rest[0], (int)rest[1]};
     const variable_list d = once(x.backward(s[3], grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1)), graph);
     return {d[0], d[1], Tensor(), Tensor(), Tensor()};

@@ -24,7 +24,10 @@ def operators():
     import metal_kans as mk
     tokens = torch.arange(30, device="cuda") % 20
     taps, dt, A, B = rnd(24, 4), rnd(2, 9, 24), -rnd(24, 8).abs(), rnd(2, 9, 8)
-    return {"embedding": ((20, 24), lambda w: mk.embedding(tokens, w)),
+    scale, table, target = rnd(24), rnd(50, 24), torch.arange(40, device="cuda")
+    return {"residual_norm": ((40, 24), lambda x: mk.residual_norm(x, pre_weight=scale)[1]),
+            "linear_cross_entropy": ((40, 24), lambda x: mk.linear_cross_entropy(x, table, target)),
+            "embedding": ((20, 24), lambda w: mk.embedding(tokens, w)),
             "dropout": ((40, 24), lambda x: mk.dropout(x, 0.3, 5)),
             "causal_conv": ((2, 9, 24), lambda x: mk.causal_conv(x, taps)),
             "selective_scan": ((2, 9, 24), lambda x: mk.selective_scan(x, dt, A, B, B))}
@@ -110,3 +113,46 @@ def test_gradients_that_are_not_asked_for(cuda):
     held = x * 3.0
     assert all(torch.equal(a, b) for a, b in zip(captured(step), want))
     del held
+
+
+@pytest.mark.parametrize("order", [True, False])
+@pytest.mark.parametrize("name", ["residual_norm", "linear_cross_entropy"])
+def test_norms_and_losses(cuda, name, order):
+    """Their forwards may be captured alone; their backwards refuse, whether or not a node stands between."""
+    shape, call = operators()[name]
+    x = leaf(shape, order)
+    for through in (call, lambda x: call((x * 2.0).neg())):
+        want = step_of(through, x)()
+        held = through(x)
+        with torch.no_grad():
+            assert torch.equal(captured(lambda: [through(x).detach()])[0], want[0])
+        torch.cuda.synchronize()
+        alone = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(alone):
+            out = through(x).detach()
+        alone.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[0])
+        with pytest.raises(RuntimeError, match=name + "'s backward under a graph capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                out = through(x)
+                torch.autograd.grad(out, x, torch.ones_like(out))
+        del held, out
+        assert all(torch.equal(a, b) for a, b in zip(captured(step_of(through, x)), want))
+
+
+def test_weights_of_norms_and_losses(cuda):
+    """The weights' gradients alone."""
+    import metal_kans as mk
+    x, w, target = rnd(40, 24), leaf((50, 24), True), torch.arange(40, device="cuda")
+    scale = leaf((1, 24), True)
+    calls = {"linear_cross_entropy": (w, lambda: mk.linear_cross_entropy(x, w, target)),
+             "residual_norm": (scale, lambda: mk.residual_norm(x, pre_weight=scale[0])[1])}
+    for name, (of, call) in calls.items():
+        held = of * 2.0
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match=name + "'s backward under a graph capture"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                out = call()
+                torch.autograd.grad(out, of, torch.ones_like(out))
+        del held, out

@@ -404,8 +404,8 @@ int kans_prefill_set_block_pairs(int on);
  * work enqueued on `stream`.
  * ======================================================================= */
 /* Rows of a table for the tokens of a batch: out[n] = scale * W[tokens[n]] (W [V][D], out [N][D] of `dtype`, rows contiguous,
- * any alignment).  Tokens equal to ignore_index give rows of zeros, others outside [0, V) rows of NaN.  N up to 2^23, D to
- * 2^16, V to 2^24. */
+ * any alignment).  Tokens equal to ignore_index give rows of zeros, others outside [0, V) rows of NaN.  scale is zero or a normal
+ * number of fp32, in which it multiplies.  N up to 2^23, D to 2^16, V to 2^24. */
 int kans_embedding_forward(int dtype, const int64_t* tokens, const void* W, long N, int D, int V, int64_t ignore_index, double scale,
                            void* out, void* stream);
 /* bytes of device memory (16-byte aligned) that the backward works in; negative for refused sizes */

@@ -18,6 +18,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "kans_api_internal.h"
@@ -389,7 +390,9 @@ EmbedPlan plan_embed(int esize, long n, int D, int V) {
 int check_embed(int dtype, long n, int D, int V, double scale) {
   if (dtype != DT_F32 && dtype != DT_F16 && dtype != DT_BF16) return kans_fail(KANS_ERR_ARG, "dtype %d", dtype);
   if (n < 0 || D <= 0 || V <= 0) return kans_fail(KANS_ERR_ARG, "bad dims N=%ld D=%d V=%d", n, D, V);
-  if (!std::isfinite(scale)) return kans_fail(KANS_ERR_ARG, "scale must be finite");
+  // (the kernels multiply in fp32: zeros would meet an infinite scale, and a scale below its normal numbers has lost digits)
+  if (!(scale == 0.0 || (std::fabs(scale) >= FLT_MIN && std::fabs(scale) <= FLT_MAX)))
+    return kans_fail(KANS_ERR_ARG, "scale must be zero or a normal number of fp32");
   // (a grid holds fewer than 2^32 threads along x)
   if (n > (1L << 23) || D > (1 << 16) || V > (1 << 24))
     return kans_fail(KANS_ERR_UNSUPPORTED, "N=%ld D=%d V=%d, up to 2^23 tokens, 2^16 columns and 2^24 rows", n, D, V);

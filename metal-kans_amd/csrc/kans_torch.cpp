@@ -15,6 +15,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <limits>
@@ -479,8 +480,9 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
 // None where the arguments do not fit together (the caller says why).
 std::optional<Tensor> embedding(const Tensor& tokens, const Tensor& weight, double scale, int64_t ignore) {
   not_traced("embedding");
-  if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0 || type_of(weight.scalar_type()) < 0 || !std::isfinite(scale) ||
-      tokens.scalar_type() != at::kLong || !weight.is_cuda() || tokens.device() != weight.device())
+  if (weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0 || type_of(weight.scalar_type()) < 0 ||
+      tokens.scalar_type() != at::kLong || !weight.is_cuda() || tokens.device() != weight.device() ||
+      !(scale == 0.0 || (std::fabs(scale) >= FLT_MIN && std::fabs(scale) <= FLT_MAX)))
     return {};
   TORCH_CHECK_VALUE(weight.size(0) <= INT_MAX && weight.size(1) <= INT_MAX, "weight has more than 2^31 rows or columns");
   const Tensor t = tokens.contiguous(), w = weight.contiguous();

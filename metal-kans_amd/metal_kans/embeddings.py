@@ -5,19 +5,19 @@ atomics, the same result on every run.
 """
 from __future__ import annotations
 
-import math
-
 import torch
 
 from ._torch_ops import load
+
+_LEAST, _MOST = 2.0 ** -126, (2.0 - 2.0 ** -23) * 2.0 ** 127  # of fp32's normal numbers
 
 
 def _refuse(tokens, weight, scale):
     """What is wrong with the arguments of a call."""
     if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"weight {tuple(weight.shape)} must be [V, D]")
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if scale != 0 and not _LEAST <= abs(scale) <= _MOST:
+        raise ValueError(f"scale must be zero or a normal number of fp32, got {scale}")
     if weight.dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise TypeError(f"weight is {weight.dtype}, must be fp32, fp16 or bf16")
     if tokens.dtype != torch.int64:
@@ -32,7 +32,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, ig
         tokens: [...] int64 on the GPU, rows in [0, V) or ``ignore_index`` (padding: a row of zeros, whose
             gradient is not looked at); any other value gives a row of NaN and takes no part in the gradient
         weight: the table [V, D], fp32, fp16 or bf16
-        scale: a number that every row is multiplied with
+        scale: a number that every row is multiplied with, in fp32 (zero, or from 2^-126 to below 2^128)
 
     Returns [..., D] in weight's type.  weight's gradient is dense: rows of tokens that are not there are zeros.
     """

@@ -206,3 +206,12 @@ def test_conv_sizes_whose_product_passes_64_bits(lib):
     assert lib.kans_causal_conv_workspace(0, 128, 1 << 30, 4, 4) == -5
     assert lib.kans_causal_conv_workspace(0, (1 << 31) - 1, 1, 4, 4) > 0
     assert lib.kans_causal_conv_workspace(0, (1 << 31) - 1, 1, 8, 4) == -5
+
+
+def test_embedding_scales(lib):
+    """Scales that fp32 holds with all their digits, and zero."""
+    for dt in (0, 1, 2):
+        for scale, code in ((0.0, 0), (-0.0, 0), (2.0 ** -126, 0), (-3.4e38, 0), (1e-40, -1), (-1e-300, -1), (3.5e38, -1), (1e300, -1),
+                            (float("nan"), -1), (float("-inf"), -1)):
+            assert lib.kans_embedding_forward(dt, None, 64, 0, 8, 5, -100, scale, 64, None) == code, scale
+            assert lib.kans_embedding_backward(dt, 64, 64, 4, 8, 5, -100, scale, 64, None, 0, None) == -1

@@ -154,3 +154,12 @@ def test_selective_scan_refuses(mk):
                        (dict(x=x.double(), dt=x.double(), B=B.double(), C=B.double()), TypeError), (dict(x=None), TypeError)):
         with pytest.raises(error):
             mk.selective_scan(**{**ok, **bad})
+
+
+def test_embedding_refuses_scales_beyond_fp32(mk):
+    t, w = torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4)
+    for scale in (1e39, -1e39, 1e-39, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="scale"):
+            mk.embedding(t, w, scale)
+    with pytest.raises(ValueError, match="one GPU"):
+        mk.embedding(t, w, 0.0)

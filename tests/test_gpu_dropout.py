@@ -187,3 +187,14 @@ def test_share_and_streams(cuda):
         c = mk.dropout(x, 0.5, 1, 0)
     side.synchronize()
     assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("p", [0.1, 0.5, 0.9])
+def test_words_that_all_differ(cuda, p):
+    """A seed and an offset of the digits of pi, whose halves are not alike, against the oracle that holds the published answers."""
+    import metal_kans as mk
+    from philox import words as published
+    seed, offset = 0x299f31d0a4093822, 0x0370734413198a2e
+    keep = torch.tensor([w >= round(p * 2 ** 32) for w in published(0, 1003, seed, offset)], device="cuda")
+    for dt in (torch.float32, torch.float16, torch.bfloat16):
+        assert torch.equal(mk.dropout(torch.ones(1003, device="cuda", dtype=dt), p, seed, offset) != 0, keep)

@@ -226,3 +226,27 @@ def test_gradient_is_the_difference(cuda):
             down[v, c] -= 1.0
             diff = ((mk.embedding(tokens, up, scale=1.5) - mk.embedding(tokens, down, scale=1.5)).double() * dout).sum() / 2
         assert abs(diff - dw[v, c]) <= 1e-4
+
+
+@pytest.mark.parametrize("v", [131072, 131073, 200003, 262144, 262145, 500009])
+@pytest.mark.parametrize("n,hot", [(3000, 0.3), (20000, 0.5), (20000, 1.0)])
+def test_frequent_tokens_of_large_tables(cuda, n, hot, v):
+    """Long lists of equal tokens on both sides of the ranges (of up to 512 tokens) that all waves of a workgroup place: whole numbers,
+    exact, and the sorted order of the positions through a sum that it changes."""
+    import metal_kans as mk
+    tokens, _, _ = inputs(n, 1, v, torch.float32, seed=v, hot=hot)
+    tokens[:7] = torch.tensor([0, v - 1, v // 2, v // 2 - 1, v // 2 + 1, v - 1, 511], device="cuda")
+    dout = (torch.arange(n * 12, device="cuda").view(n, 12) % 7 - 3).float()
+    w = torch.zeros(v, 12, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(mk.embedding(tokens, w), w, dout)
+    assert torch.equal(dw, torch.zeros(v, 12, device="cuda").index_add_(0, tokens, dout))
+    check(*inputs(n, 12, v, torch.float32, seed=v + 1, hot=hot), 0.5)
+
+
+def test_ends_of_a_large_vocabulary(cuda):
+    """Tokens of the 257th sorting workgroup, which has 77 of the table's, and of both ends of those before it."""
+    v = (1 << 21) + 77
+    tokens, w, dout = inputs(300, 8, v, torch.bfloat16)
+    tokens[:10] = torch.tensor([v - 1, v - 77, v - 78, v - 1, 0, 8191, 8192, 1 << 21, (1 << 21) - 8192, v - 40], device="cuda")
+    dw = check(tokens, w, dout, 1.0)
+    assert dw[v - 1].any() and dw[v - 77].any()

@@ -592,3 +592,12 @@ def test_steps_that_share_memory(cuda):
                         call(s, state=state)
                         call(apart, state=other)
                     assert torch.equal(state.nan_to_num(7.0, 8.0, 9.0), other.nan_to_num(7.0, 8.0, 9.0)), name
+
+
+# 4 ceil(D / 64) B waves: whole sequences from 1024 on, a grid above 512 workgroups in the second and the last
+@pytest.mark.parametrize("b,l,d,n,dt,lengths", [(4, 131, 4099, 4, torch.float32, [131, 70, 17, 0]), (9, 131, 4099, 3, torch.bfloat16, None),
+                                                (5, 203, 3300, 8, torch.float16, [203, 202, 96, 1, 150]), (4, 300, 4099, 2, torch.bfloat16, [300, 299, 129, 16]),
+                                                (17, 150, 2050, 16, torch.float32, [150 - 9 * i for i in range(17)])])
+def test_long_sequences_that_stay_whole(cuda, b, l, d, n, dt, lengths):
+    """Large batches are not cut in chunks: many tiles one after the other, ends in the middle of a sequence and of a tile."""
+    check(inputs(b, l, d, n, dt, lengths=lengths))

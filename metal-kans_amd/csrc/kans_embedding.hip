@@ -101,7 +101,8 @@ struct GradArgs {
 constexpr int kSortThreads = 1024, kWaves = kSortThreads / 64, kPer = 8, kRound = kSortThreads * kPer;  // tokens of a thread, of a round
 constexpr int kHeld = 4 * kRound;  // tokens that stay in registers between counting and placing
 // Lists of more entries than kAlone are placed by all waves, where their counters (of up to kShared tokens each) fit:
-// 16384 tokens by their frequency in a language, 65536 in all: 22 -> 15 us.
+// 16384 tokens by their frequency in a language, 65536 in all: 22 -> 15 us.  A range has V / 256 tokens, so that beyond 131072
+// rows one wave places every list: 16 us at 131072, 22 at 131073, 20 at 262144.
 constexpr int kAlone = 256, kShared = 512;
 constexpr int kMaxRange = 8192;
 constexpr int kMaxPiece = 64;  // positions of a piece at most

@@ -11,11 +11,11 @@
 // All of it in fp32; h does not leave the registers but for every 16th step (8th or 4th for many states), where the forward of a
 // training step keeps it: the backward runs through the 16 steps again and then back.
 //
-// The vector units bound it, not memory: a step of 16 channels and 16 states takes a wave 31 instructions forward (20 of them
-// the recurrence's own: product, exponential, product and two sums for each four states) and 95 backward (24 for the states again,
+// The vector units bound it, not memory: a step of 16 channels and 16 states takes a wave 32 instructions forward (20 of them
+// the recurrence's own: product, exponential, product and two sums for each four states) and 93 backward (24 for the states again,
 // 32 for the gradients, 17 for the sums of dB and dC over the channels).  Four lanes share a channel: with one, a
 // wave would have 64 channels and there would be too few waves; with 16, sums over the states would cost as much as the
-// recurrence.  bf16 8 x 2048 x 4096, 16 states: forward 327 us, backward 858 (83 and 87 % of the issue slots taken, at 2.2 GHz),
+// recurrence.  bf16 8 x 2048 x 4096, 16 states: forward 327 - 332 us, backward 858 - 877 (84 and 86 % of the issue slots taken, at 2.2 GHz),
 // of which the bytes alone take 160 and 280; 1 x 8192 x 1024 fp16 forward 44 us and 32 for the chunks' edges.  What lies
 // behind a sequence's end is cleared, not computed.
 // A batch of B sequences and D channels has B D / 16 waves.  Where those are too few for the card the sequence is cut in chunks: a

@@ -352,7 +352,11 @@ __device__ __forceinline__ float here(float v) {
 
 // Where a grid has no more than two workgroups a CU, the two waves of a SIMD come first by turns.  The older one always came first,
 // was done early and left the other alone, which cannot use all cycles: forward of bf16 8 x 2048 x 4096 386 -> 359 us then.
-// (Larger grids fill the places themselves: 3 % slower with turns.)  Workgroups go over the card's 256 CUs in order.
+// Workgroups go over the card's 256 CUs in order.  bf16, 1024 steps of 4096 channels, 16 states, us, without turns | with them:
+//   sequences  4 (256 workgroups)  5 (320)    8 (512)    9 (576)    16 (1024)
+//   forward    112 | 132           156 | 156  158 | 158  221 | 211  282 | 268
+//   both ways  396 | 423           592 | 566  616 | 583  880 | 876  1158 | 1125
+// (The border is that of the case measured first; those that these figures ask for are not drawn yet.)
 __device__ __forceinline__ void take_turns(int tile) {
   if (gridDim.x > 512) return;
   if ((tile ^ (int)(blockIdx.x >> 8)) & 1) __builtin_amdgcn_s_setprio(1);

@@ -58,7 +58,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         weight: [D, W], W from 1 to 8; the last tap is the step's own
         bias: [D]
         activation: "silu" (u sigmoid(u)) or None
-        state: [B, W - 1, D], contiguous: the inputs before the first step (None: zeros).  Afterwards it holds the last
+        state: [B, W - 1, D], contiguous, apart from x: the inputs before the first step (None: zeros).  Afterwards it holds the last
             W - 1 inputs of each sequence, for the next call.  Without gradients only.
         lengths: [B] int64 on the GPU, the steps of each sequence that count: the others give zeros (as do gradients
             there) and are not looked at, nor kept in the state
@@ -109,12 +109,12 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
         B, C: [batch, L, N] of x's type, shared by the channels
         D, dt_bias: [channels] fp32 (None: zeros)
         softplus: False takes dt + dt_bias as it is
-        state: [batch, channels, N] fp32, contiguous: the states before the first step (None: zeros).  Afterwards it
+        state: [batch, channels, N] fp32, contiguous, apart from the others: the states before the first step (None: zeros).  Afterwards it
             holds those behind each sequence's last step, for the next call.  Without gradients only.
         lengths: [batch] int64 on the GPU, the steps of each sequence that count: the others give zeros (as do
             gradients there), are not looked at and leave the state
 
-    Views whose channels (states) lie side by side are read as they are.  Returns [batch, L, channels] in x's
+    Views whose channels (states) lie side by side and whose steps do not overlap are read as they are.  Returns [batch, L, channels] in x's
     type; gradients reach x, dt, A, B, C, D, z and dt_bias, those of A, D and dt_bias in fp32.
     """
     out = load().selective_scan(x, dt, A, B, C, D, z, dt_bias, softplus, state, lengths)
